@@ -1,0 +1,136 @@
+// C entry points of softmax attention: checks of the arguments, the choice of the
+// kernel, and the document starts that training passes down.
+#include "dn_attn_fwd.h"
+
+namespace dn {
+namespace {
+
+constexpr int kScan = 1024;
+
+// One workgroup per row: starts[i] = the last j <= i whose id differs from its
+// predecessor's, as a running maximum over blocks of kScan tokens.
+__global__ __launch_bounds__(kScan) void k_doc_starts(const void* seg, int i64, int batched, int L, int32_t* starts) {
+  __shared__ int part[kScan / 64];
+  const int64_t row = (int64_t)blockIdx.x * L, base = batched ? row : 0;
+  auto id = [&](int i) { return i64 ? ((const int64_t*)seg)[base + i] : (int64_t)((const int32_t*)seg)[base + i]; };
+  int carry = 0;
+  for (int i0 = 0; i0 < L; i0 += kScan) {
+    const int i = i0 + threadIdx.x, l = threadIdx.x & 63, w = threadIdx.x >> 6;
+    int m = i < L && i > 0 && id(i) != id(i - 1) ? i : 0;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int x = __shfl_up(m, o);
+      if (l >= o) m = max(m, x);
+    }
+    if (l == 63) part[w] = m;
+    __syncthreads();
+    int all = carry;
+    for (int x = 0; x < kScan / 64; ++x) {
+      if (x < w) m = max(m, part[x]);
+      all = max(all, part[x]);
+    }
+    m = max(m, carry);
+    carry = all;
+    if (i < L) starts[row + i] = m;
+    __syncthreads();
+  }
+}
+
+int bad(const char* m) { return set_error(DN_E_INVALID, m); }
+bool wide(const void* p, const int64_t* s, int dtype, int n) {
+  const int64_t per = dtype == DN_F32 ? 4 : 8;
+  for (int i = 0; i < n; ++i)
+    if (s[i] % per) return false;
+  return ((uintptr_t)p & 15) == 0;
+}
+
+// checks that the entries share; NULL if all is well
+const char* shape_error(int64_t tokens, int Hq, int Hkv, int D, int dtype, float scale, int window) {
+  if (D != 64 && D != 128 && D != 256) return "head dimension must be 64, 128 or 256";
+  if (Hq <= 0 || Hkv <= 0 || Hq % Hkv) return "query heads must be a multiple of the key heads";
+  if (dtype != DN_F32 && dtype != DN_BF16 && dtype != DN_F16) return "attention dtype not supported";
+  if (!(scale == scale) || scale - scale != 0.f) return "scale must be finite";
+  if (window < 0) return "window must not be negative";
+  if (tokens * Hq >= ((int64_t)1 << 31)) return "too many query rows";
+  return nullptr;
+}
+
+int paged_params(const dn_paged_attention_args* a, AF& p) {
+  if (a == nullptr) return bad("null args");
+  if (a->abi_version != DN_ABI_VERSION) return set_error(DN_E_ABI, "dn_paged_attention_args built for another ABI version");
+  if (a->N < 0 || a->B < 0) return bad("bad attention sizes");
+  if (const char* m = shape_error(a->N, a->Hq, a->Hkv, a->D, a->dtype, a->scale, a->window)) return bad(m);
+  if (a->pages <= 0 || a->max_pages <= 0 || a->page_size <= 0 || (a->page_size & (a->page_size - 1)))
+    return bad("the cache needs pages of a power of two tokens");
+  if ((int64_t)a->max_pages * a->page_size >= ((int64_t)1 << 31)) return bad("a sequence must have fewer than 2^31 tokens");
+  if (a->N && !a->B) return bad("tokens without a sequence");
+  if (a->cu_seqlens == nullptr && a->B && a->N % a->B) return bad("without cu_seqlens every sequence has N / B new tokens");
+  if (a->N && (!a->q || !a->k_cache || !a->v_cache || !a->out || !a->page_table || !a->seq_lens)) return bad("missing tensor pointer");
+  if (!wide(a->q, a->q_strides, a->dtype, 3) || !wide(a->k_cache, a->kc_strides, a->dtype, 3) ||
+      !wide(a->v_cache, a->vc_strides, a->dtype, 3) || ((uintptr_t)a->out & 15))
+    return bad("attention rows must start on 16 bytes");
+  p.B = a->B; p.N = a->N; p.T = a->cu_seqlens ? 0 : a->B ? a->N / a->B : 0;
+  p.Hkv = a->Hkv; p.G = a->Hq / a->Hkv; p.window = a->window;
+  p.pages = a->pages; p.max_pages = a->max_pages;
+  while ((1 << p.shift) < a->page_size) ++p.shift;
+  p.sc = a->scale * kLog2e;
+  p.q = a->q; p.k = a->k_cache; p.v = a->v_cache; p.out = a->out; p.lse = a->lse;
+  p.cu = a->cu_seqlens; p.lens = a->seq_lens; p.pt = a->page_table; p.pts = a->page_table_stride;
+  for (int i = 0; i < 3; ++i) { p.qs[i] = a->q_strides[i]; p.ks[i] = a->kc_strides[i]; p.vs[i] = a->vc_strides[i]; }
+  return DN_OK;
+}
+
+}  // namespace
+}  // namespace dn
+
+using namespace dn;
+
+extern "C" size_t dn_paged_attention_workspace_size(const dn_paged_attention_args* a) {
+  AF p{};
+  if (paged_params(a, p) != DN_OK) return 0;
+  return 0;
+}
+
+extern "C" int dn_paged_attention(const dn_paged_attention_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+  AF p{};
+  if (const int rc = paged_params(a, p)) return rc;
+  if (p.N == 0) return DN_OK;
+  const hipError_t e = attn_many(p, a->D, a->dtype, true, (hipStream_t)stream);
+  return e == hipSuccess ? DN_OK : set_error(DN_E_LAUNCH, hipGetErrorString(e));
+}
+
+extern "C" int dn_document_starts(const void* seg, int32_t seg_dtype, int32_t batched, int32_t B, int32_t L, int32_t* starts, void* stream) {
+  if (B < 0 || L < 0 || (seg_dtype != DN_I32 && seg_dtype != DN_I64)) return bad("bad segment ids");
+  if (B == 0 || L == 0) return DN_OK;
+  if (!seg || !starts) return bad("missing tensor pointer");
+  hipLaunchKernelGGL(k_doc_starts, dim3(B), dim3(kScan), 0, (hipStream_t)stream, seg, seg_dtype == DN_I64, batched, L, starts);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? DN_OK : set_error(DN_E_LAUNCH, hipGetErrorString(e));
+}
+
+namespace {
+int attention_params(const dn_attention_args* a, AF& p) {
+  if (a == nullptr) return bad("null args");
+  if (a->abi_version != DN_ABI_VERSION) return set_error(DN_E_ABI, "dn_attention_args built for another ABI version");
+  if (a->B < 0 || a->L < 0) return bad("bad attention sizes");
+  if (const char* m = shape_error((int64_t)a->B * a->L, a->Hq, a->Hkv, a->D, a->dtype, a->scale, a->window)) return bad(m);
+  if (a->B && a->L && (!a->q || !a->k || !a->v || !a->out)) return bad("missing tensor pointer");
+  if (!wide(a->q, a->q_strides, a->dtype, 3) || !wide(a->k, a->k_strides, a->dtype, 3) || !wide(a->v, a->v_strides, a->dtype, 3) ||
+      ((uintptr_t)a->out & 15))
+    return bad("attention rows must start on 16 bytes");
+  p.B = a->B; p.T = a->L; p.N = a->B * a->L;
+  p.Hkv = a->Hkv; p.G = a->Hq / a->Hkv; p.window = a->window;
+  p.sc = a->scale * kLog2e;
+  p.q = a->q; p.k = a->k; p.v = a->v; p.out = a->out; p.lse = a->lse; p.start = a->starts;
+  for (int i = 0; i < 3; ++i) { p.qs[i] = a->q_strides[i]; p.ks[i] = a->k_strides[i]; p.vs[i] = a->v_strides[i]; }
+  return DN_OK;
+}
+}  // namespace
+
+extern "C" int dn_attention_fwd(const dn_attention_args* a, void* stream) {
+  AF p{};
+  if (const int rc = attention_params(a, p)) return rc;
+  if (p.N == 0) return DN_OK;
+  const hipError_t e = attn_many(p, a->D, a->dtype, false, (hipStream_t)stream);
+  return e == hipSuccess ? DN_OK : set_error(DN_E_LAUNCH, hipGetErrorString(e));
+}

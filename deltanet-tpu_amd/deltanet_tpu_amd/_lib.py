@@ -19,6 +19,7 @@ DN_ABI_VERSION = 2
 DN_F32, DN_BF16, DN_F16, DN_I32, DN_I64 = 0, 1, 2, 3, 4
 
 _c_i32 = ctypes.c_int32
+_c_i64 = ctypes.c_int64
 _c_ptr = ctypes.c_void_p
 
 
@@ -90,6 +91,67 @@ class BackwardArgs(ctypes.Structure):
     ]
 
 
+class RotaryArgs(ctypes.Structure):
+    """Mirror of ``dn_rotary_args``."""
+
+    _fields_ = [
+        ("abi_version", _c_i32),
+        ("B", _c_i32), ("L", _c_i32), ("Hq", _c_i32), ("Hk", _c_i32), ("D", _c_i32), ("R", _c_i32),
+        ("dtype", _c_i32), ("pos_dtype", _c_i32), ("interleaved", _c_i32), ("inverse", _c_i32), ("rows", _c_i32),
+        ("q", _c_ptr), ("k", _c_ptr), ("q_out", _c_ptr), ("k_out", _c_ptr), ("pos", _c_ptr), ("table", _c_ptr),
+        ("q_strides", _c_i64 * 3), ("k_strides", _c_i64 * 3), ("pos_strides", _c_i64 * 2),
+    ]
+
+
+class KvAppendArgs(ctypes.Structure):
+    """Mirror of ``dn_kv_append_args``."""
+
+    _fields_ = [
+        ("abi_version", _c_i32),
+        ("N", _c_i32), ("B", _c_i32), ("H", _c_i32), ("D", _c_i32), ("R", _c_i32),
+        ("dtype", _c_i32), ("cache_dtype", _c_i32), ("interleaved", _c_i32), ("rows", _c_i32),
+        ("pages", _c_i32), ("page_size", _c_i32), ("max_pages", _c_i32),
+        ("k", _c_ptr), ("v", _c_ptr), ("k_cache", _c_ptr), ("v_cache", _c_ptr), ("page_table", _c_ptr),
+        ("seq_lens", _c_ptr), ("cu_seqlens", _c_ptr), ("table", _c_ptr),
+        ("k_strides", _c_i64 * 3), ("v_strides", _c_i64 * 3), ("kc_strides", _c_i64 * 3), ("vc_strides", _c_i64 * 3),
+        ("page_table_stride", _c_i64),
+    ]
+
+
+class PagedAttentionArgs(ctypes.Structure):
+    """Mirror of ``dn_paged_attention_args``."""
+
+    _fields_ = [
+        ("abi_version", _c_i32),
+        ("N", _c_i32), ("B", _c_i32), ("Hq", _c_i32), ("Hkv", _c_i32), ("D", _c_i32),
+        ("dtype", _c_i32), ("window", _c_i32), ("pages", _c_i32), ("page_size", _c_i32), ("max_pages", _c_i32),
+        ("scale", ctypes.c_float),
+        ("q", _c_ptr), ("k_cache", _c_ptr), ("v_cache", _c_ptr), ("out", _c_ptr), ("lse", _c_ptr),
+        ("page_table", _c_ptr), ("seq_lens", _c_ptr), ("cu_seqlens", _c_ptr),
+        ("q_strides", _c_i64 * 3), ("kc_strides", _c_i64 * 3), ("vc_strides", _c_i64 * 3), ("page_table_stride", _c_i64),
+    ]
+
+
+class AttentionArgs(ctypes.Structure):
+    """Mirror of ``dn_attention_args``."""
+
+    _fields_ = [
+        ("abi_version", _c_i32),
+        ("B", _c_i32), ("L", _c_i32), ("Hq", _c_i32), ("Hkv", _c_i32), ("D", _c_i32),
+        ("dtype", _c_i32), ("window", _c_i32),
+        ("scale", ctypes.c_float),
+        ("q", _c_ptr), ("k", _c_ptr), ("v", _c_ptr), ("out", _c_ptr), ("lse", _c_ptr), ("starts", _c_ptr),
+        ("q_strides", _c_i64 * 3), ("k_strides", _c_i64 * 3), ("v_strides", _c_i64 * 3),
+    ]
+
+
+# The same blocks in one call (the order and alignment of the fields above).
+ROTARY_PACK = struct.Struct("@12i6P8q").pack
+KV_APPEND_PACK = struct.Struct("@13i8P13q").pack
+PAGED_ATTENTION_PACK = struct.Struct("@11if8P10q").pack
+ATTENTION_PACK = struct.Struct("@8if6P9q").pack
+
+
 EXPORTED_SYMBOLS = (
     "dn_prefill_workspace_size",
     "dn_prefill_fwd",
@@ -101,6 +163,12 @@ EXPORTED_SYMBOLS = (
     "dn_prefill_bwd_raw_workspace_size",
     "dn_prefill_bwd_raw",
     "dn_state_frob_cap",
+    "dn_rotary",
+    "dn_kv_append",
+    "dn_paged_attention_workspace_size",
+    "dn_paged_attention",
+    "dn_document_starts",
+    "dn_attention_fwd",
     "dn_last_error",
     "dn_abi_version",
     "dn_profile_begin",
@@ -125,6 +193,29 @@ def packed_decode():
         many.argtypes, many.restype = [ctypes.c_char_p, _c_i32, _c_ptr], ctypes.c_int
         _packed = one, many
     return _packed
+
+
+_packed_calls = {}
+_PACKED = {   # argument types behind the packed argument block, and the result's
+    "dn_rotary": ([_c_ptr], ctypes.c_int),
+    "dn_kv_append": ([_c_ptr], ctypes.c_int),
+    "dn_paged_attention_workspace_size": ([], ctypes.c_size_t),
+    "dn_paged_attention": ([_c_ptr, ctypes.c_size_t, _c_ptr], ctypes.c_int),
+    "dn_attention_fwd": ([_c_ptr], ctypes.c_int),
+}
+
+
+def packed_call(name):
+    """An entry point of the loaded library that takes its argument block as
+    packed bytes."""
+    f = _packed_calls.get(name)
+    if f is None:
+        lib = load_library()
+        f = getattr(ctypes.CDLL(lib._name, handle=lib._handle), name)
+        args, f.restype = _PACKED[name]
+        f.argtypes = [ctypes.c_char_p, *args]
+        _packed_calls[name] = f
+    return f
 
 
 def load_library(path: str | None = None) -> ctypes.CDLL:
@@ -159,6 +250,8 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
         lib.dn_prefill_bwd_raw.restype = ctypes.c_int
         lib.dn_state_frob_cap.argtypes = [_c_ptr, ctypes.c_int64, _c_i32, _c_i32, ctypes.c_float, _c_ptr]
         lib.dn_state_frob_cap.restype = ctypes.c_int
+        lib.dn_document_starts.argtypes = [_c_ptr, _c_i32, _c_i32, _c_i32, _c_i32, _c_ptr, _c_ptr]
+        lib.dn_document_starts.restype = ctypes.c_int
         lib.dn_last_error.argtypes = []
         lib.dn_last_error.restype = ctypes.c_char_p
         lib.dn_abi_version.argtypes = []

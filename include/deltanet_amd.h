@@ -237,6 +237,133 @@ int dn_prefill_bwd_raw(const dn_prefill_args* a, const void* d_out, const void* 
  * gdn2.py:2180-2188 / 2224-2226 / 2236-2238). */
 int dn_state_frob_cap(float* state, int64_t nmat, int32_t rows, int32_t cols, float tau, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * The softmax-attention layers of a hybrid model (no counterpart in the
+ * reference, which has the delta-rule layers alone): rotary positions, a paged
+ * key/value cache, attention over it, and causal attention in training.
+ *
+ * Strides are in elements; channels (the last axis) are always contiguous.
+ * A cache is (pages, page_size, Hkv, D) with any strides of the first three
+ * axes; page_table (B, max_pages) int32 holds the page of each page_size tokens
+ * of a sequence.  seq_lens (B) int32 counts a sequence's tokens, the new ones
+ * included.  cu_seqlens (B + 1) int32 is where each sequence's new tokens start
+ * among the N of the call; NULL gives every sequence N / B of them.  All of
+ * these are device arrays, never read by the host.
+ * ------------------------------------------------------------------------- */
+
+/* Rotation of the first R channels of every head of q and k by the angles of
+ * the token's position: with (c, s) = table[pos][i], table[pos][R/2 + i] the
+ * pair (x_i, x_{i+R/2}) -- interleaved: (x_{2i}, x_{2i+1}) -- becomes
+ * (x c - y s, y c + x s).  `inverse` turns back (s -> -s), which is also the
+ * gradient.  A position outside [0, rows) gives NaN in the rotated channels. */
+typedef struct dn_rotary_args {
+  int32_t abi_version;
+  int32_t B, L, Hq, Hk, D, R;   /* R even, <= D; Hk = 0: no k                    */
+  int32_t dtype;                /* DN_F32 / DN_BF16 / DN_F16, all tensors        */
+  int32_t pos_dtype;            /* DN_I32 / DN_I64                               */
+  int32_t interleaved, inverse;
+  int32_t rows;                 /* positions that the table covers               */
+  const void* q;                /* (B,L,Hq,D), strides q_strides                 */
+  const void* k;                /* (B,L,Hk,D), strides k_strides                 */
+  void* q_out;                  /* (B,L,Hq,D) dense                              */
+  void* k_out;                  /* (B,L,Hk,D) dense                              */
+  const void* pos;              /* (B,L), strides pos_strides (0: shared)        */
+  const float* table;           /* (rows, R): cos in the first half, sin after   */
+  int64_t q_strides[3];         /* batch, token, head                            */
+  int64_t k_strides[3];
+  int64_t pos_strides[2];       /* batch, token                                  */
+} dn_rotary_args;
+
+int dn_rotary(const dn_rotary_args* a, void* stream);
+
+/* Stores the new tokens' keys, rotated by their positions, and values in a
+ * paged cache.  New token i of sequence b, n_b of them, has position
+ * seq_lens[b] - n_b + i.  A token whose position is negative or past the page
+ * table, or whose page is outside the cache, is not stored.  Elements are
+ * rounded to the cache's type (nearest even). */
+typedef struct dn_kv_append_args {
+  int32_t abi_version;
+  int32_t N, B, H, D, R;        /* new tokens in all, sequences, key/value heads; R = 0: not rotated */
+  int32_t dtype, cache_dtype;   /* DN_F32 / DN_BF16 / DN_F16                     */
+  int32_t interleaved, rows;    /* as in dn_rotary_args                          */
+  int32_t pages, page_size, max_pages;   /* page_size a power of two             */
+  const void* k;                /* (N,H,D) or (B,N/B,H,D), strides k_strides     */
+  const void* v;
+  void* k_cache;                /* (pages,page_size,H,D), strides kc_strides     */
+  void* v_cache;
+  const int32_t* page_table;    /* (B,max_pages), row stride page_table_stride   */
+  const int32_t* seq_lens;
+  const int32_t* cu_seqlens;
+  const float* table;           /* (rows, R); NULL if R = 0                      */
+  int64_t k_strides[3];         /* batch (unused with cu_seqlens), token, head   */
+  int64_t v_strides[3];
+  int64_t kc_strides[3];        /* page, token, head                             */
+  int64_t vc_strides[3];
+  int64_t page_table_stride;
+} dn_kv_append_args;
+
+int dn_kv_append(const dn_kv_append_args* a, void* stream);
+
+/* Attention of new tokens over a paged cache: out_i = sum_j softmax_j(scale q_i
+ * k_j) v_j over the positions j <= position of i, and with `window` > 0 only the
+ * last `window` of them.  Positions, pages and sequences as in dn_kv_append_args
+ * (the new tokens' keys and values are in the cache already); query head h reads
+ * key head h / (Hq / Hkv).  A query without a key (a position below 0) gets zeros
+ * and lse -inf.  Page numbers outside the cache are read as its nearest page and
+ * seq_lens past the page table as its end.  Nothing that a query must not see
+ * reaches it, infinities and NaNs included. */
+typedef struct dn_paged_attention_args {
+  int32_t abi_version;
+  int32_t N, B, Hq, Hkv, D;     /* D: 64, 128 or 256                             */
+  int32_t dtype;                /* DN_F32 / DN_BF16 / DN_F16, all tensors        */
+  int32_t window;               /* 0: every key up to the query                  */
+  int32_t pages, page_size, max_pages;
+  float scale;
+  const void* q;                /* (N,Hq,D) or (B,N/B,Hq,D), strides q_strides   */
+  const void* k_cache;
+  const void* v_cache;
+  void* out;                    /* (N,Hq,D) dense                                */
+  float* lse;                   /* NULL or (N,Hq): log of the sum of exponentials */
+  const int32_t* page_table;
+  const int32_t* seq_lens;
+  const int32_t* cu_seqlens;
+  int64_t q_strides[3];         /* batch (unused with cu_seqlens), token, head   */
+  int64_t kc_strides[3];        /* page, token, head                             */
+  int64_t vc_strides[3];
+  int64_t page_table_stride;
+} dn_paged_attention_args;
+
+/* Bytes of device workspace dn_paged_attention needs (0: none). */
+size_t dn_paged_attention_workspace_size(const dn_paged_attention_args* a);
+int dn_paged_attention(const dn_paged_attention_args* a, void* workspace, size_t workspace_bytes, void* stream);
+
+/* First token of each token's document: starts (B,L) int32 from segment ids
+ * (B,L) (batched) or (L,) int32 / int64, where a document is a run of equal ids
+ * (an id that comes again starts another one). */
+int dn_document_starts(const void* seg, int32_t seg_dtype, int32_t batched, int32_t B, int32_t L, int32_t* starts, void* stream);
+
+/* Causal attention of whole rows, and its gradient.  Query i sees the keys j <= i
+ * from starts[i] on (NULL: from 0), and with `window` > 0 only the last `window`
+ * of them. */
+typedef struct dn_attention_args {
+  int32_t abi_version;
+  int32_t B, L, Hq, Hkv, D;     /* D: 64, 128 or 256                             */
+  int32_t dtype;                /* DN_F32 / DN_BF16 / DN_F16, all tensors        */
+  int32_t window;
+  float scale;
+  const void* q;                /* (B,L,Hq,D), strides q_strides                 */
+  const void* k;                /* (B,L,Hkv,D)                                   */
+  const void* v;
+  void* out;                    /* (B,L,Hq,D) dense                              */
+  float* lse;                   /* (B,L,Hq); forward: NULL if not wanted         */
+  const int32_t* starts;        /* NULL or (B,L), nondecreasing, 0 <= starts[i] <= i */
+  int64_t q_strides[3];         /* batch, token, head                            */
+  int64_t k_strides[3];
+  int64_t v_strides[3];
+} dn_attention_args;
+
+int dn_attention_fwd(const dn_attention_args* a, void* stream);
+
 /* Kernel timing instrumentation (no counterpart in the reference; for
  * benchmarks and profilers).  Between dn_profile_begin() and dn_profile_end()
  * every dn_prefill_fwd call (from any thread of the process) records HIP events on its
