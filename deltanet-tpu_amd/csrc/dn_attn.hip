@@ -134,3 +134,24 @@ extern "C" int dn_attention_fwd(const dn_attention_args* a, void* stream) {
   const hipError_t e = attn_many(p, a->D, a->dtype, false, (hipStream_t)stream);
   return e == hipSuccess ? DN_OK : set_error(DN_E_LAUNCH, hipGetErrorString(e));
 }
+
+extern "C" size_t dn_attention_bwd_workspace_size(const dn_attention_args* a) {
+  AF p{};
+  if (attention_params(a, p) != DN_OK) return 0;
+  return (((size_t)p.N * a->Hq * sizeof(float) + 255) / 256 + 1) * 256;
+}
+
+extern "C" int dn_attention_bwd(const dn_attention_args* a, const void* d_out, void* dq, void* dk, void* dv, void* workspace,
+                                size_t workspace_bytes, void* stream) {
+  AB p{};
+  if (const int rc = attention_params(a, p.f)) return rc;
+  if (p.f.N == 0) return DN_OK;
+  if (!a->lse || !d_out || !dq || !dk || !dv) return bad("missing tensor pointer");
+  if (((uintptr_t)d_out | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15) return bad("attention rows must start on 16 bytes");
+  if (!workspace || workspace_bytes < dn_attention_bwd_workspace_size(a)) return set_error(DN_E_WORKSPACE, "workspace missing or too small");
+  p.scale = a->scale;
+  p.d_out = d_out; p.dq = dq; p.dk = dk; p.dv = dv;
+  p.delta = (float*)(((uintptr_t)workspace + 255) & ~(uintptr_t)255);
+  const hipError_t e = attn_backward(p, a->D, a->dtype, (hipStream_t)stream);
+  return e == hipSuccess ? DN_OK : set_error(DN_E_LAUNCH, hipGetErrorString(e));
+}

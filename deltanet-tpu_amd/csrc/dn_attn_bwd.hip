@@ -1,0 +1,409 @@
+// Gradient of causal softmax attention.
+//
+// With P = exp(scale S - lse) and delta = rowsum(dO O):
+//   dV = P^T dO,  dP = dO V^T,  dS = P (dP - delta),  dQ = scale dS K,  dK = scale dS^T Q.
+// Probabilities are recomputed from lse.  Two kernels, so that every sum runs in
+// one place in a fixed order: by keys (dK, dV; a workgroup walks over the query
+// rows of all heads of its group, which is the sum over them too) and by query
+// rows (dQ).  That is seven products for the five of a single pass, whose third
+// output would have to be added up in memory.
+#include "dn_attn_fwd.h"
+
+namespace dn {
+namespace {
+
+// delta = sum of d_out * out over a row's channels: D/8 lanes per row
+template <class T, int D>
+__global__ __launch_bounds__(256) void k_attn_delta(const AB p, int64_t rows) {
+  constexpr int per = D / 8;
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, row = id / per;
+  float s = 0.f;
+  if (row < rows) {
+    typedef T V __attribute__((ext_vector_type(8)));
+    const V a = reinterpret_cast<const V*>(p.d_out)[id], b = reinterpret_cast<const V*>(p.f.out)[id];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s += (float)a[e] * (float)b[e];
+  }
+#pragma unroll
+  for (int o = 1; o < per; o <<= 1) s += __shfl_xor(s, o);
+  if (row < rows && id % per == 0) p.delta[row] = s;
+}
+
+// Query rows are (token, head of the group), token first.
+template <class T> struct QRows {
+  const T *q, *g;       // q and d_out of the sequence and key head
+  int64_t qt, qh, gt, gh;
+  int G, last;
+  __device__ __forceinline__ const T* query(int row) const {
+    row = min(row, last);
+    const int t = row / G;
+    return q + t * qt + (row - t * G) * qh;
+  }
+  __device__ __forceinline__ const T* grad(int row) const {
+    row = min(row, last);
+    const int t = row / G;
+    return g + t * gt + (row - t * G) * gh;
+  }
+};
+
+// The last token whose document starts at or before key k1 (starts is
+// nondecreasing and starts[k1] <= k1), by all lanes of a wave.
+__device__ __forceinline__ int last_token(const int32_t* starts, int T, int k1) {
+  int lo = k1, hi = T;   // starts[lo] <= k1, hi: T or the first known above
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 64) / 65;
+    const int t = lo + (lane_id() + 1) * step;
+    const unsigned long long in = __ballot(t < hi && starts[min(t, T - 1)] <= k1);
+    const int n = __popcll(in);
+    const int nlo = lo + n * step;
+    hi = min(hi, nlo + step);
+    lo = nlo;
+  }
+  return lo;
+}
+
+// dK and dV of 16 NK NW keys of one key head.
+template <class T, int D, int NK, int NW, int BQ>
+__global__ __launch_bounds__(64 * NW) void k_attn_dkv(const AB p) {
+  using TL = Tile<T, D>;
+  using F = typename At<T>::F;
+  constexpr int BN = 16 * NK * NW, NS = D / 32, NC = D / 16, NT = 64 * NW;
+  __shared__ __align__(16) T lds[4 * BQ * D];    // [2][q, d_out][BQ][D]
+  __shared__ __align__(16) float ls[2][BQ], de[2][BQ];   // lse * log2(e) and delta per row
+  __shared__ __align__(16) int tk[2][BQ], lw[2][BQ];     // token and first visible key per row
+  const AF& f = p.f;
+
+  const int l = lane_id(), r = l & 15, q = l >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // batch row and head innermost; the first keys, which most queries see, first
+  const int groups = f.B * f.Hkv, gi = blockIdx.x % groups;
+  const int b = gi / f.Hkv, h = gi % f.Hkv, k0 = (int)(blockIdx.x / groups) * BN;
+  const int k1 = min(k0 + BN, f.T) - 1;
+  const int32_t* starts = f.start ? f.start + (int64_t)b * f.T : nullptr;
+
+  int t1 = f.T - 1;   // the last token that sees one of the keys
+  if (f.window) t1 = (int)min((int64_t)t1, (int64_t)k1 + f.window - 1);
+  if (starts) t1 = min(t1, __builtin_amdgcn_readfirstlane(last_token(starts, f.T, k1)));
+
+  const int key = k0 + (w * NK) * 16 + r;
+  F kf[NK][NS], vf[NK][NS];
+#pragma unroll
+  for (int i = 0; i < NK; ++i) {
+    const int64_t t = min(key + 16 * i, f.T - 1);
+    const T* kp = (const T*)f.k + b * f.ks[0] + t * f.ks[1] + h * f.ks[2];
+    const T* vp = (const T*)f.v + b * f.vs[0] + t * f.vs[1] + h * f.vs[2];
+#pragma unroll
+    for (int c = 0; c < NS; ++c) {
+      kf[i][c] = *reinterpret_cast<const F*>(kp + 32 * c + 8 * q);
+      vf[i][c] = *reinterpret_cast<const F*>(vp + 32 * c + 8 * q);
+    }
+  }
+
+  const int Hq = f.Hkv * f.G;
+  QRows<T> rows;
+  rows.q = (const T*)f.q + b * f.qs[0] + (int64_t)h * f.G * f.qs[2];
+  rows.qt = f.qs[1]; rows.qh = f.qs[2];
+  rows.g = (const T*)p.d_out + ((int64_t)b * f.T * Hq + h * f.G) * D;
+  rows.gt = (int64_t)Hq * D; rows.gh = D;
+  rows.G = f.G; rows.last = f.T * f.G - 1;
+  const int r0 = k0 * f.G / BQ, r1 = (t1 * f.G + f.G - 1) / BQ + 1;   // tiles of query rows
+
+  f32x4 dk[NK][NC], dv[NK][NC];
+#pragma unroll
+  for (int i = 0; i < NK; ++i)
+#pragma unroll
+    for (int c = 0; c < NC; ++c) dk[i][c] = dv[i][c] = zero4();
+
+  float m_ls = 0.f, m_de = 0.f;
+  int m_tk = 0, m_lw = 0, m_hi = 0;   // m_hi: first visible key of the tile's last row
+  auto fetch = [&](int j) {
+    T* t = lds + (j & 1) * 2 * BQ * D;
+    TL::template load<BQ, NT>(t, threadIdx.x, [&](int x) { return rows.query(j * BQ + x); });
+    TL::template load<BQ, NT>(t + BQ * D, threadIdx.x, [&](int x) { return rows.grad(j * BQ + x); });
+    auto low = [&](int t) {
+      int x = f.window ? max(t - f.window + 1, 0) : 0;
+      return starts ? max(x, starts[t]) : x;
+    };
+    if (threadIdx.x < BQ) {
+      const int row = j * BQ + threadIdx.x, c = min(row, rows.last), tok = c / f.G;
+      const int64_t at = ((int64_t)b * f.T + tok) * Hq + h * f.G + (c - tok * f.G);
+      m_ls = f.lse[at] * kLog2e;
+      m_de = p.delta[at];
+      m_tk = row <= rows.last ? tok : -1;   // a row past the last one sees no key
+      m_lw = low(tok);
+    }
+    m_hi = low(min(j * BQ + BQ - 1, rows.last) / f.G);
+  };
+  bool odd = false;
+  if (r0 < r1) fetch(r0);
+#pragma unroll 1
+  for (int j = r0; j < r1; ++j) {
+    if (threadIdx.x < BQ) {
+      ls[j & 1][threadIdx.x] = m_ls;
+      de[j & 1][threadIdx.x] = m_de;
+      tk[j & 1][threadIdx.x] = m_tk;
+      lw[j & 1][threadIdx.x] = m_lw;
+    }
+    const bool masked = j * BQ / f.G < k1 || m_hi > k0 || j * BQ + BQ - 1 > rows.last;
+    loads_barrier();
+    if (j + 1 < r1) fetch(j + 1);
+    const T* qt = lds + (j & 1) * 2 * BQ * D;
+    const T* gt = qt + BQ * D;
+#pragma unroll 1
+    for (int u = 0; u < BQ; u += 32) {
+      f32x4 s[NK][2], dp[NK][2];
+#pragma unroll
+      for (int i = 0; i < NK; ++i) s[i][0] = s[i][1] = dp[i][0] = dp[i][1] = zero4();
+#pragma unroll
+      for (int c = 0; c < NS; ++c)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const F qf = TL::row8(qt, u + 16 * e + r, c, q);
+          const F gf = TL::row8(gt, u + 16 * e + r, c, q);
+#pragma unroll
+          for (int i = 0; i < NK; ++i) {
+            At<T>::mma(s[i][e], qf, kf[i][c]);
+            At<T>::mma(dp[i][e], gf, vf[i][c]);
+          }
+        }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int at = u + 16 * e + 4 * q;
+        const f32x4 lse = *reinterpret_cast<const f32x4*>(&ls[j & 1][at]);
+        const f32x4 del = *reinterpret_cast<const f32x4*>(&de[j & 1][at]);
+#pragma unroll
+        for (int i = 0; i < NK; ++i)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const float pr = fast_exp2(__builtin_fmaf(s[i][e][x], f.sc, -lse[x]));
+            s[i][e][x] = pr;
+            dp[i][e][x] = pr * (dp[i][e][x] - del[x]);
+          }
+        if (masked) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int t = tk[j & 1][at + x], lo = lw[j & 1][at + x];
+#pragma unroll
+            for (int i = 0; i < NK; ++i) {
+              const bool see = key + 16 * i <= t && key + 16 * i >= lo;
+              s[i][e][x] = see ? s[i][e][x] : 0.f;
+              dp[i][e][x] = see ? dp[i][e][x] : 0.f;
+            }
+          }
+        }
+      }
+      F pf[NK], df[NK];
+#pragma unroll
+      for (int i = 0; i < NK; ++i) {
+        pf[i] = frag8<T>(s[i][0], s[i][1]);
+        df[i] = frag8<T>(dp[i][0], dp[i][1]);
+      }
+      const bool bad = masked && (TL::odd32(qt + u * D) || TL::odd32(gt + u * D));
+      odd |= bad;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        F gf = TL::col8(gt, u, 16 * c, r, q);
+        F qf = TL::col8(qt, u, 16 * c, r, q);
+        if (bad) {
+          gf = finite8<T>(gf);
+          qf = finite8<T>(qf);
+        }
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+          At<T>::mma(dv[i][c], gf, pf[i]);
+          At<T>::mma(dk[i][c], qf, df[i]);
+        }
+      }
+    }
+  }
+
+#pragma unroll
+  for (int i = 0; i < NK; ++i) {
+    const int t = key + 16 * i;
+    if (t >= f.T) continue;
+    const int64_t at = (((int64_t)b * f.T + t) * f.Hkv + h) * D;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      float x[4], y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[e] = dk[i][c][e] * p.scale;
+        y[e] = dv[i][c][e];
+      }
+      if (odd) {   // what the queries that see this key had left out of dV (dK of such a query is NaN by its scores)
+#pragma unroll 1
+        for (int row = max(r0 * BQ, t * f.G); row <= min(r1 * BQ - 1, rows.last); ++row) {
+          const int tok = row / f.G;
+          int lo = f.window ? max(tok - f.window + 1, 0) : 0;
+          if (starts) lo = max(lo, starts[tok]);
+          const int j = row / BQ, tl = min(j * BQ + BQ - 1, rows.last) / f.G;
+          int hi = f.window ? max(tl - f.window + 1, 0) : 0;
+          if (starts) hi = max(hi, starts[tl]);
+          if (t < lo || !(j * BQ / f.G < k1 || hi > k0 || j * BQ + BQ - 1 > rows.last)) continue;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float z = (float)rows.grad(row)[16 * c + 4 * q + e];
+            if (!__builtin_isfinite(z)) y[e] += z;
+          }
+        }
+      }
+      st4<T>((T*)p.dk + at + 16 * c + 4 * q, x);
+      st4<T>((T*)p.dv + at + 16 * c + 4 * q, y);
+    }
+  }
+}
+
+// dQ of 16 NQ NW query rows: the forward's walk over the keys.
+template <class T, int D, int NQ, int NW, int BN>
+__global__ __launch_bounds__(64 * NW) void k_attn_dq(const AB p) {
+  using TL = Tile<T, D>;
+  using F = typename At<T>::F;
+  constexpr int BM = 16 * NQ * NW, NS = D / 32, NC = D / 16, NT = 64 * NW;
+  __shared__ __align__(16) T lds[4 * BN * D];   // [2][K, V][BN][D]
+  const AF& f = p.f;
+
+  const int l = lane_id(), r = l & 15, q = l >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int groups = f.B * f.Hkv, gi = blockIdx.x % groups, tiles = gridDim.x / groups;
+  const int b = gi / f.Hkv, h = gi % f.Hkv, row0 = (tiles - 1 - (int)(blockIdx.x / groups)) * BM;
+  const int nrow = f.T * f.G, row1 = min(row0 + BM, nrow);
+  const int p0 = row0 / f.G, p1 = (row1 - 1) / f.G;
+  const int32_t* starts = f.start ? f.start + (int64_t)b * f.T : nullptr;
+  const int Hq = f.Hkv * f.G;
+
+  F qf[NQ][NS], gf[NQ][NS];
+  int pos[NQ], low[NQ];
+  float ls[NQ], de[NQ];
+#pragma unroll
+  for (int i = 0; i < NQ; ++i) {
+    const int row = min(row0 + (w * NQ + i) * 16 + r, nrow - 1);
+    const int t = row / f.G, g = row - t * f.G;
+    const int64_t at = ((int64_t)b * f.T + t) * Hq + h * f.G + g;
+    const T* qp = (const T*)f.q + b * f.qs[0] + t * f.qs[1] + (h * f.G + g) * f.qs[2];
+    const T* gp = (const T*)p.d_out + at * D;
+#pragma unroll
+    for (int c = 0; c < NS; ++c) {
+      qf[i][c] = *reinterpret_cast<const F*>(qp + 32 * c + 8 * q);
+      gf[i][c] = *reinterpret_cast<const F*>(gp + 32 * c + 8 * q);
+    }
+    ls[i] = f.lse[at] * kLog2e;
+    de[i] = p.delta[at];
+    pos[i] = t;
+    low[i] = f.window ? t - f.window + 1 : 0;
+    if (starts) low[i] = max(low[i], starts[t]);
+  }
+  int lo0 = f.window ? max(p0 - f.window + 1, 0) : 0, lo1 = f.window ? p1 - f.window + 1 : 0;
+  if (starts) {
+    lo0 = max(lo0, starts[p0]);
+    lo1 = max(lo1, starts[p1]);
+  }
+  const int j0 = lo0 / BN, j1 = p1 / BN + 1;
+
+  Rows<T, false> kr{}, vr{};
+  kr.base = (const T*)f.k + b * f.ks[0] + h * f.ks[2];
+  vr.base = (const T*)f.v + b * f.vs[0] + h * f.vs[2];
+  kr.token = f.ks[1]; vr.token = f.vs[1];
+  kr.last = vr.last = p1;
+
+  f32x4 dq[NQ][NC];
+#pragma unroll
+  for (int i = 0; i < NQ; ++i)
+#pragma unroll
+    for (int c = 0; c < NC; ++c) dq[i][c] = zero4();
+
+  auto fetch = [&](int j) {
+    T* t = lds + (j & 1) * 2 * BN * D;
+    TL::template load<BN, NT>(t, threadIdx.x, [&](int x) { return kr(j * BN + x); });
+    TL::template load<BN, NT>(t + BN * D, threadIdx.x, [&](int x) { return vr(j * BN + x); });
+  };
+  fetch(j0);
+#pragma unroll 1
+  for (int j = j0; j < j1; ++j) {
+    loads_barrier();
+    if (j + 1 < j1) fetch(j + 1);
+    const T* kt = lds + (j & 1) * 2 * BN * D;
+    const T* vt = kt + BN * D;
+    const bool masked = j * BN + BN - 1 > p0 || j * BN < lo1;
+#pragma unroll 1
+    for (int u = 0; u < BN; u += 32) {
+      f32x4 s[NQ][2], dp[NQ][2];
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) s[i][0] = s[i][1] = dp[i][0] = dp[i][1] = zero4();
+#pragma unroll
+      for (int c = 0; c < NS; ++c)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const F kf = TL::row8(kt, u + 16 * e + r, c, q);
+          const F vf = TL::row8(vt, u + 16 * e + r, c, q);
+#pragma unroll
+          for (int i = 0; i < NQ; ++i) {
+            At<T>::mma(s[i][e], kf, qf[i][c]);
+            At<T>::mma(dp[i][e], vf, gf[i][c]);
+          }
+        }
+      F df[NQ];
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const float pr = fast_exp2(__builtin_fmaf(s[i][e][x], f.sc, -ls[i]));
+            dp[i][e][x] = pr * (dp[i][e][x] - de[i]);
+            if (masked) {
+              const int key = j * BN + u + 16 * e + 4 * q + x;
+              dp[i][e][x] = key <= pos[i] && key >= low[i] ? dp[i][e][x] : 0.f;
+            }
+          }
+        df[i] = frag8<T>(dp[i][0], dp[i][1]);
+      }
+      const bool bad = masked && TL::odd32(kt + u * D);   // (a query that sees such a key is NaN by its scores)
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        F kf = TL::col8(kt, u, 16 * c, r, q);
+        if (bad) kf = finite8<T>(kf);
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) At<T>::mma(dq[i][c], kf, df[i]);
+      }
+    }
+  }
+
+#pragma unroll
+  for (int i = 0; i < NQ; ++i) {
+    const int row = row0 + (w * NQ + i) * 16 + r;
+    if (row >= nrow) continue;
+    const int t = row / f.G, g = row - t * f.G;
+    T* op = (T*)p.dq + (((int64_t)b * f.T + t) * Hq + h * f.G + g) * D;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const float x[4] = {dq[i][c][0] * p.scale, dq[i][c][1] * p.scale, dq[i][c][2] * p.scale, dq[i][c][3] * p.scale};
+      st4<T>(op + 16 * c + 4 * q, x);
+    }
+  }
+}
+
+template <class T, int D> hipError_t run(const AB& p, hipStream_t st) {
+  constexpr bool f32 = sizeof(T) == 4;
+  constexpr int NW = 4, BT = f32 ? 32 : 64;
+  constexpr int NK = D == 256 || (f32 && D == 128) ? 1 : 2, NQ = f32 && D == 256 ? 1 : 2;
+  const AF& f = p.f;
+  const int64_t rows = (int64_t)f.N * f.Hkv * f.G, groups = (int64_t)f.B * f.Hkv;
+  hipLaunchKernelGGL((k_attn_delta<T, D>), dim3((unsigned)((rows * (D / 8) + 255) / 256)), dim3(256), 0, st, p, rows);
+  const int64_t kt = ((int64_t)f.T + 16 * NK * NW - 1) / (16 * NK * NW);
+  hipLaunchKernelGGL((k_attn_dkv<T, D, NK, NW, BT>), dim3((unsigned)(kt * groups)), dim3(64 * NW), 0, st, p);
+  const int64_t qt = ((int64_t)f.T * f.G + 16 * NQ * NW - 1) / (16 * NQ * NW);
+  hipLaunchKernelGGL((k_attn_dq<T, D, NQ, NW, BT>), dim3((unsigned)(qt * groups)), dim3(64 * NW), 0, st, p);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t attn_backward(const AB& p, int D, int dtype, hipStream_t st) {
+  auto go = [&](auto z) {
+    using T = decltype(z);
+    return D == 64 ? run<T, 64>(p, st) : D == 128 ? run<T, 128>(p, st) : run<T, 256>(p, st);
+  };
+  return dtype == DN_BF16 ? go((bf16)0.f) : dtype == DN_F16 ? go((f16)0.f) : go(0.f);
+}
+
+}  // namespace dn

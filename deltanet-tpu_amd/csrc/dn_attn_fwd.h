@@ -22,6 +22,20 @@ struct AF {
   int64_t pts;
 };
 
+// Rows of K or V in memory: contiguous, or through a page table.
+template <class T, bool PAGED> struct Rows {
+  const T* base;       // the head's first channel of token 0 (of page 0)
+  int64_t token, page;
+  const int32_t* pt;
+  int shift, pages, last;   // last: the last token that may be read
+  __device__ __forceinline__ const T* operator()(int t) const {
+    t = min(t, last);
+    if constexpr (!PAGED) return base + t * token;
+    const int pg = min(max(pt[t >> shift], 0), pages - 1);
+    return base + pg * page + (t & ((1 << shift) - 1)) * token;
+  }
+};
+
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLazy = 8.f;   // a running maximum may lag behind by a factor 2^8
 
@@ -71,5 +85,16 @@ __device__ __forceinline__ bool find_tile(const AF& p, int tile, int BM, Seq& s)
 // Attention over many rows per sequence (training, prompts): head dimension and
 // type checked by the caller.
 hipError_t attn_many(const AF& p, int D, int dtype, bool paged, hipStream_t st);
+
+// The gradient (contiguous rows): p with out, lse and start of the forward, d_out
+// dense, the three gradients dense, delta (tokens, Hkv G) floats of scratch.
+struct AB {
+  AF f;
+  float scale;
+  const void* d_out;
+  void *dq, *dk, *dv;
+  float* delta;
+};
+hipError_t attn_backward(const AB& p, int D, int dtype, hipStream_t st);
 
 }  // namespace dn

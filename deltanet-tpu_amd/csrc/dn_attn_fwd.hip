@@ -4,20 +4,6 @@
 namespace dn {
 namespace {
 
-// Rows of K or V in memory: contiguous, or through a page table.
-template <class T, bool PAGED> struct Rows {
-  const T* base;       // the head's first channel of token 0 (of page 0)
-  int64_t token, page;
-  const int32_t* pt;
-  int shift, pages, last;   // last: the last token that may be read
-  __device__ __forceinline__ const T* operator()(int t) const {
-    t = min(t, last);
-    if constexpr (!PAGED) return base + t * token;
-    const int pg = min(max(pt[t >> shift], 0), pages - 1);
-    return base + pg * page + (t & ((1 << shift) - 1)) * token;
-  }
-};
-
 // One workgroup: NW waves of 16 NQ query rows each over one head's keys.
 template <class T, int D, int NQ, int NW, int BN, bool PAGED>
 __global__ __launch_bounds__(64 * NW) void k_attn(const AF p) {

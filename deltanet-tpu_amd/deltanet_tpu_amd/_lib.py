@@ -169,6 +169,8 @@ EXPORTED_SYMBOLS = (
     "dn_paged_attention",
     "dn_document_starts",
     "dn_attention_fwd",
+    "dn_attention_bwd_workspace_size",
+    "dn_attention_bwd",
     "dn_last_error",
     "dn_abi_version",
     "dn_profile_begin",
@@ -202,6 +204,8 @@ _PACKED = {   # argument types behind the packed argument block, and the result'
     "dn_paged_attention_workspace_size": ([], ctypes.c_size_t),
     "dn_paged_attention": ([_c_ptr, ctypes.c_size_t, _c_ptr], ctypes.c_int),
     "dn_attention_fwd": ([_c_ptr], ctypes.c_int),
+    "dn_attention_bwd_workspace_size": ([], ctypes.c_size_t),
+    "dn_attention_bwd": ([_c_ptr] * 5 + [ctypes.c_size_t, _c_ptr], ctypes.c_int),
 }
 
 

@@ -411,6 +411,36 @@ def _attention_forward(q, k, v, starts, scale, window, want_lse):
     return out, lse
 
 
+class _AttentionFn(torch.autograd.Function):
+    """Causal attention under autograd: the forward keeps the log of each row's sum
+    of exponentials, from which the backward recomputes the probabilities."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, starts, scale, window):
+        out, lse = _attention_forward(q, k, v, starts, scale, window, True)
+        ctx.save_for_backward(q, k, v, out, lse, starts)
+        ctx.meta = scale, window
+        ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
+        return out, lse
+
+    @staticmethod
+    def backward(ctx, d_out, _):
+        q, k, v, out, lse, starts = ctx.saved_tensors
+        scale, window = ctx.meta
+        if d_out is None:
+            return (None,) * 6
+        d_out = d_out.contiguous()
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        if q.numel():
+            block = _attention_block(q, k, v, out, lse, starts, scale, window)
+            need = _lib.packed_call("dn_attention_bwd_workspace_size")(block)
+            ws = torch.empty((need,), dtype=torch.uint8, device=q.device)
+            _call("dn_attention_bwd", q.get_device(), block, d_out.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                  ws.data_ptr(), need)
+        return dq, dk, dv, None, None, None
+
+
 def causal_attention(q, k, v, *, segment_ids=None, cu_seqlens=None, scale=None, window=None, return_lse: bool = False):
     """Causal softmax attention of whole rows.
 
@@ -420,7 +450,9 @@ def causal_attention(q, k, v, *, segment_ids=None, cu_seqlens=None, scale=None, 
     to itself, or the last ``window`` of them.  scale: 1 / sqrt(D) unless given.
     Sums and softmax statistics in float32.  Returns the output in q's shape and
     type, and with ``return_lse`` also the log of the sum of exponentials (B, L, Hq)
-    in float32.
+    in float32.  Differentiable in q, k and v (not through the lse); gradients come
+    in the inputs' type, those of k and v summed over the heads that share them, and
+    are the same bits every time.
     """
     if q.ndim != 4:
         raise ValueError(f"Query tensor q must be 4D (B, L, Hq, D), got shape {tuple(q.shape)}.")
@@ -435,5 +467,8 @@ def causal_attention(q, k, v, *, segment_ids=None, cu_seqlens=None, scale=None, 
     dev = _require_gpu(q, k, v, segment_ids if isinstance(segment_ids, torch.Tensor) else None)
     starts = _document_starts(segment_ids, cu_seqlens, B, L, dev)
     q, k, v = _rows16(q), _rows16(k), _rows16(v)
-    out, lse = _attention_forward(q, k, v, starts, scale, window, return_lse)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        out, lse = _AttentionFn.apply(q, k, v, starts, scale, window)
+    else:
+        out, lse = _attention_forward(q, k, v, starts, scale, window, return_lse)
     return (out, lse) if return_lse else out

@@ -364,6 +364,15 @@ typedef struct dn_attention_args {
 
 int dn_attention_fwd(const dn_attention_args* a, void* stream);
 
+/* Gradients of sum(out * d_out): `a` is the forward's block with out and lse as it
+ * wrote them; d_out (B,L,Hq,D) dense; dq (B,L,Hq,D), dk and dv (B,L,Hkv,D) dense,
+ * written (not accumulated) in the inputs' type.  Two passes recompute the
+ * probabilities from lse: dk and dv by keys, dq by queries, each output summed in
+ * a fixed order (no atomics: the same bits every time). */
+size_t dn_attention_bwd_workspace_size(const dn_attention_args* a);
+int dn_attention_bwd(const dn_attention_args* a, const void* d_out, void* dq, void* dk, void* dv,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
 /* Kernel timing instrumentation (no counterpart in the reference; for
  * benchmarks and profilers).  Between dn_profile_begin() and dn_profile_end()
  * every dn_prefill_fwd call (from any thread of the process) records HIP events on its

@@ -97,3 +97,26 @@ def rotate_tolerance(x, dt, R):
     a = x[..., :R].abs()
     top = a.amax(-1, keepdim=True) * 2.0 if R else 0.0
     return top * (2.0 ** -23 + ROUND[dt] * 1.01) + TINY[dt]
+
+
+def attend_grad(q, k, v, do, vis, scale, dt):
+    """One head: (dq, dk, dv, tolerances of the three) from the formulas
+    dV = P^T dO, dS = P (dO V^T - rowsum(dO O)), dQ = scale dS K, dK = scale dS^T Q.
+
+    Roundings to the type: P and dS before their products, the output that
+    rowsum(dO O) reads (as far off as its tolerance), the results.
+    """
+    s = torch.where(vis, (q @ k.T) * scale, -math.inf)
+    p = torch.exp(s - torch.logsumexp(s, 1, keepdim=True))
+    out = p @ v
+    u, f = ROUND[dt], f32_error(q, k, scale, s)
+    r = 0.0 if dt == "f32" else u
+    dp = do @ v.T
+    ds = p * (dp - (do * out).sum(1, keepdim=True))
+    off = (do.abs() * tolerance(q, k, v, p, out, s, scale, dt)).sum(1, keepdim=True)
+    f32 = f * (do.abs() @ v.abs().T + (do * out).abs().sum(1, keepdim=True))
+    eds = 1.05 * (r * ds.abs() + p * (off + f32)) + f * ds.abs() + (0.0 if dt == "f32" else TINY[dt])
+    ep = 1.05 * r * p + f * p + (0.0 if dt == "f32" else TINY[dt])
+    dq, dk, dv = scale * ds @ k, scale * ds.T @ q, p.T @ do
+    sc = abs(scale)
+    return dq, dk, dv, sc * eds @ k.abs() + 1.05 * u * dq.abs() + TINY[dt], sc * eds.T @ q.abs(), ep.T @ do.abs()
