@@ -87,15 +87,22 @@ using namespace dn;
 
 extern "C" size_t dn_paged_attention_workspace_size(const dn_paged_attention_args* a) {
   AF p{};
-  if (paged_params(a, p) != DN_OK) return 0;
-  return 0;
+  if (paged_params(a, p) != DN_OK || p.N == 0 || !attn_few_takes(p)) return 0;
+  return attn_few_bytes(p, a->D) + 256;
 }
 
 extern "C" int dn_paged_attention(const dn_paged_attention_args* a, void* workspace, size_t workspace_bytes, void* stream) {
   AF p{};
   if (const int rc = paged_params(a, p)) return rc;
   if (p.N == 0) return DN_OK;
-  const hipError_t e = attn_many(p, a->D, a->dtype, true, (hipStream_t)stream);
+  hipError_t e;
+  if (attn_few_takes(p)) {
+    if (!workspace || workspace_bytes < attn_few_bytes(p, a->D) + 256) return set_error(DN_E_WORKSPACE, "workspace missing or too small");
+    p.part = (float*)(((uintptr_t)workspace + 255) & ~(uintptr_t)255);
+    e = attn_few(p, a->D, a->dtype, (hipStream_t)stream);
+  } else {
+    e = attn_many(p, a->D, a->dtype, true, (hipStream_t)stream);
+  }
   return e == hipSuccess ? DN_OK : set_error(DN_E_LAUNCH, hipGetErrorString(e));
 }
 

@@ -16,6 +16,7 @@ struct AF {
   const void *q, *k, *v;
   void* out;                 // dense (tokens, Hkv G, D)
   float* lse;                // NULL or (tokens, Hkv G)
+  float* part;               // partial results (dn_attn_few.hip)
   const int32_t *cu, *lens, *pt;
   const int32_t* start;      // contiguous: NULL or the first token of each token's document (B, T)
   int64_t qs[3], ks[3], vs[3];   // batch or page, token, head
@@ -82,9 +83,132 @@ __device__ __forceinline__ bool find_tile(const AF& p, int tile, int BM, Seq& s)
   return false;
 }
 
+// A sequence of a paged call: its first new token among all, new tokens, tokens in all.
+struct Span { int c0, n, len; };
+__device__ __forceinline__ Span span_of(const AF& p, int b) {
+  Span s;
+  s.c0 = b * p.T;
+  s.n = p.T;
+  if (p.cu) {
+    s.c0 = min(max(p.cu[b], 0), p.N);
+    s.n = min(max(p.cu[b + 1], s.c0), p.N) - s.c0;
+  }
+  s.len = min(max(p.lens[b], 0), p.max_pages << p.shift);
+  return s;
+}
+
+// Keys [lo, hi) that rows [row0, row1) of a sequence see between them, in units.
+__device__ __forceinline__ void units_of(const AF& p, const Span& s, int row0, int row1, int unit, int& u0, int& u1) {
+  const int off = s.len - s.n, p0 = off + row0 / p.G, p1 = off + (row1 - 1) / p.G;
+  u0 = p.window ? max(p0 - p.window + 1, 0) / unit : 0;
+  u1 = p1 < 0 ? u0 : p1 / unit + 1;
+  u1 = max(u1, u0 + 1);   // a tile without keys is work too: it writes zeros
+}
+
+// The work of a paged call split evenly over the workgroups.  Its tasks are (b,
+// key head, tile of BM rows), in that order, each of as many units as `unit`
+// tokens its rows see; workgroup w of W takes the units [w C / W, (w+1) C / W) of
+// the C in all, wherever tasks begin and end in them.  Lengths are known on the
+// device alone, so every workgroup adds them up itself.
+struct Task {
+  Span s;
+  int b, h, m;
+  int64_t first;   // its first unit
+  int units;
+};
+// units of sequence b, one head
+__device__ __forceinline__ int64_t head_units(const AF& p, const Span& s, int BM, int unit) {
+  const int rows = s.n * p.G;
+  int64_t c = 0;
+  for (int r = 0; r < rows; r += BM) {
+    int u0, u1;
+    units_of(p, s, r, min(r + BM, rows), unit, u0, u1);
+    c += u1 - u0;
+  }
+  return c;
+}
+__device__ __forceinline__ int64_t shfl_up64(int64_t x, int o) {
+  const int lo = __shfl_up((int)(uint32_t)x, o), hi = __shfl_up((int)(x >> 32), o);
+  return ((int64_t)hi << 32) | (uint32_t)lo;
+}
+__device__ __forceinline__ int64_t shfl64(int64_t x, int l) {
+  const int lo = __shfl((int)(uint32_t)x, l), hi = __shfl((int)(x >> 32), l);
+  return ((int64_t)hi << 32) | (uint32_t)lo;
+}
+// inclusive prefix sum over a wave
+__device__ __forceinline__ int64_t scan64(int64_t x) {
+  const int l = lane_id();
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t y = shfl_up64(x, o);
+    if (l >= o) x += y;
+  }
+  return x;
+}
+// all units of the call, by a wave
+__device__ __forceinline__ int64_t all_units(const AF& p, int BM, int unit) {
+  int64_t c = 0;
+  for (int b = lane_id(); b < p.B; b += 64) c += head_units(p, span_of(p, b), BM, unit) * p.Hkv;
+  return shfl64(scan64(c), 63);
+}
+// the task that holds unit u < C (of task number u of the tasks, if by_task), by a wave
+template <bool BY_TASK>
+__device__ __forceinline__ bool find_task(const AF& p, int64_t u, int BM, int unit, Task& t) {
+  int64_t before = 0, ubefore = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
+    const int b = b0 + lane_id();
+    Span s{0, 0, 0};
+    if (b < p.B) s = span_of(p, b);
+    const int64_t mine = b < p.B ? head_units(p, s, BM, unit) * p.Hkv : 0;
+    const int64_t us = scan64(mine);
+    const int64_t tasks = (int64_t)((s.n * p.G + BM - 1) / BM) * p.Hkv;
+    const int64_t sum = BY_TASK ? scan64(tasks) : us;
+    const unsigned long long hit = __ballot(before + sum > u);
+    if (hit) {
+      const int w = __builtin_ctzll(hit);
+      t.b = b0 + w;
+      t.s.c0 = __builtin_amdgcn_readfirstlane(__shfl(s.c0, w));
+      t.s.n = __builtin_amdgcn_readfirstlane(__shfl(s.n, w));
+      t.s.len = __builtin_amdgcn_readfirstlane(__shfl(s.len, w));
+      const int64_t per = shfl64(mine, w) / p.Hkv;   // units of a head
+      const int rows = t.s.n * p.G, tiles = (rows + BM - 1) / BM;
+      t.first = ubefore + shfl64(us - mine, w);
+      if (BY_TASK) {
+        const int64_t k = u - before - shfl64(sum - tasks, w);
+        t.h = (int)(k / tiles);
+        t.m = (int)(k % tiles);
+      } else {
+        t.h = (int)((u - t.first) / per);
+        t.m = 0;
+      }
+      t.first += t.h * per;
+      for (int m = 0;; ++m) {   // (one tile in all but ragged calls)
+        int u0, u1;
+        units_of(p, t.s, m * BM, min((m + 1) * BM, rows), unit, u0, u1);
+        t.units = u1 - u0;
+        if (BY_TASK ? m == t.m : u < t.first + t.units) {
+          t.m = m;
+          break;
+        }
+        t.first += t.units;
+      }
+      return true;
+    }
+    before += shfl64(sum, 63);
+    ubefore += shfl64(us, 63);
+  }
+  return false;
+}
+
 // Attention over many rows per sequence (training, prompts): head dimension and
 // type checked by the caller.
 hipError_t attn_many(const AF& p, int D, int dtype, bool paged, hipStream_t st);
+
+// Attention of few rows per sequence over a paged cache, the keys split over the
+// workgroups: whether the call is one of these, the bytes it needs, the launches.
+bool attn_few_takes(const AF& p);
+size_t attn_few_bytes(const AF& p, int D);
+hipError_t attn_few(const AF& p, int D, int dtype, hipStream_t st);
 
 // The gradient (contiguous rows): p with out, lse and start of the forward, d_out
 // dense, the three gradients dense, delta (tokens, Hkv G) floats of scratch.

@@ -12,7 +12,8 @@ REPO_ROOT = os.path.dirname(PKG_ROOT)
 CSRC = os.path.join(PKG_ROOT, "csrc")
 INCLUDE = os.path.join(REPO_ROOT, "include")
 SOURCES = ("dn_prefill.hip", "dn_prefill_long.hip", "dn_backward.hip", "dn_decode.hip",
-           "dn_rotary.hip", "dn_attn.hip", "dn_attn_fwd.hip", "dn_attn_bwd.hip")
+           "dn_rotary.hip", "dn_attn.hip", "dn_attn_fwd.hip", "dn_attn_few.hip",
+           "dn_attn_bwd.hip")
 OUT = os.path.join(HERE, "libdeltanet_amd.so")
 
 
