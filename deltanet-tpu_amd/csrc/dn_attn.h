@@ -13,10 +13,13 @@
 // {4q .. 4q+3, 16+4q .. 16+4q+3}.  Its A operand, V^T in that order, comes out
 // of row-major LDS by two transposing reads.
 //
-// LDS tiles are rows of D elements whose 16-byte pieces are permuted within
-// each 128 bytes by the row number: the row reads of a slab, the transposing
-// reads of 4 rows, and the direct loads that fill the tile all spread over the
-// banks.
+// LDS tiles are slabs of 32 channels, each ROWS rows of them: the 16 rows of an
+// operand are 1 KB in a row, which a wave reads without a bank conflict, and
+// slabs, tiles of 16 rows and steps of 32 are constant offsets from one address.
+// The halves of a row change places in every other four rows, for the
+// transposing reads' sake: they take half a row of 4 rows at a time.
+// (Rows of all D channels with permuted 16-byte pieces read as fast, but each
+// slab needs an address register of its own: 37 spilled registers at D = 128.)
 #pragma once
 #include "dn_common.h"
 
@@ -88,74 +91,91 @@ __device__ __forceinline__ void loads_barrier() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
-// A tile of rows of D elements in LDS.
-template <class T, int D> struct Tile {
+// A tile of ROWS rows of D elements in LDS, a multiple of 32 rows.
+template <class T, int D, int ROWS> struct Tile {
   using F = typename At<T>::F;
-  static constexpr int kPer = 16 / sizeof(T);       // elements of a 16-byte piece
-  static constexpr int kPieces = D / kPer;          // pieces of a row
-  static __device__ __forceinline__ int swz(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
+  static constexpr int kPer = 16 / sizeof(T);     // elements of a 16-byte piece
+  static constexpr int kPieces = 32 / kPer;       // pieces of a row of a slab
+  static constexpr int kLoad = 64 / kPieces;      // rows that a wave's load fills
+  static constexpr int kSlab = ROWS * 32;
+  static __device__ __forceinline__ int piece(int row, int x) { return x ^ (((row >> 2) & 1) * (kPieces / 2)); }
+  static __device__ __forceinline__ int at(int row, int x) { return row * 32 + piece(row, x) * kPer; }   // piece x of a slab's row
 
   // channels 32 s + 8q .. + 7 of a row
   static __device__ __forceinline__ F row8(const T* t, int row, int s, int q) {
-    const T* p = t + row * D;
+    const T* p = t + s * kSlab;
     if constexpr (sizeof(T) == 2) {
-      return *reinterpret_cast<const F*>(p + (((4 * s + q) ^ swz(row)) * 8));
+      return *reinterpret_cast<const F*>(p + at(row, q));
     } else {
-      const f32x4 a = *reinterpret_cast<const f32x4*>(p + ((8 * s + 2 * q) ^ swz(row)) * 4);
-      const f32x4 b = *reinterpret_cast<const f32x4*>(p + ((8 * s + 2 * q + 1) ^ swz(row)) * 4);
+      const f32x4 a = *reinterpret_cast<const f32x4*>(p + at(row, 2 * q));
+      const f32x4 b = *reinterpret_cast<const f32x4*>(p + at(row, 2 * q) + 4);
       return F{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     }
   }
 
-  // channel c0 + r of rows row0 + {4q .. 4q+3, 16+4q .. 16+4q+3}
-  static __device__ __forceinline__ F col8(const T* t, int row0, int c0, int r, int q) {
+  // channel 16 c + r of rows {4q .. 4q+3, 16+4q .. 16+4q+3}
+  static __device__ __forceinline__ F col8(const T* t, int c, int r, int q) {
+    const T* p = t + (c >> 1) * kSlab;
     if constexpr (sizeof(T) == 2) {
       typedef short s4 __attribute__((ext_vector_type(4)));
       typedef short s8 __attribute__((ext_vector_type(8)));
-      const int row = row0 + 4 * q + (r >> 2);   // (row0 is a multiple of 16: both halves have the row's permutation)
-      const T* p = t + row * D + (((c0 >> 3) + ((r & 3) >> 1)) ^ swz(row)) * 8 + (r & 1) * 4;
+      const int row = 4 * q + (r >> 2);
+      p += at(row, 2 * (c & 1) + ((r & 3) >> 1)) + (r & 1) * 4;
       const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)p);
-      const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(p + 16 * D));
+      const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(p + 16 * 32));
       return __builtin_bit_cast(F, (s8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}));
     } else {
       F f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = at(t, row0 + pi_k(q, e), c0 + r);
+      for (int e = 0; e < 8; ++e) {
+        const int row = pi_k(q, e), ch = 16 * (c & 1) + r;
+        f[e] = p[at(row, ch / kPer) + ch % kPer];
+      }
       return f;
     }
-  }
-
-  static __device__ __forceinline__ T at(const T* t, int row, int c) {
-    return t[row * D + ((c / kPer) ^ swz(row)) * kPer + c % kPer];
   }
 
   // Whether any of 32 rows has an infinity or a NaN.
   static __device__ __forceinline__ bool odd32(const T* t) {
     typedef uint32_t u4 __attribute__((ext_vector_type(4)));
     uint32_t bad = 0;
-    const u4* p = reinterpret_cast<const u4*>(t);
-#pragma unroll 4
-    for (int i = lane_id(); i < 32 * kPieces; i += 64) {
-      const u4 x = p[i];
+#pragma unroll 1
+    for (int s = 0; s < D / 32; ++s) {
+      const u4* p = reinterpret_cast<const u4*>(t + s * kSlab);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) bad |= (x[e] & At<T>::kExp) + At<T>::kOne;
+      for (int i = 0; i < 32 * kPieces / 64; ++i) {
+        const u4 x = p[i * 64 + lane_id()];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) bad |= (x[e] & At<T>::kExp) + At<T>::kOne;
+      }
     }
     return __any((bad & At<T>::kTop) != 0);
   }
 
-  // Starts the loads of ROWS rows into t by NT threads; at(row) is a row's
-  // first channel in memory.  A wave's load fills 1 KB of LDS in lane order,
-  // each lane from its own address.
-  template <int ROWS, int NT, class At_> static __device__ __forceinline__ void load(T* t, int tid, At_ at) {
-    constexpr int n = ROWS * kPieces / NT;
-    static_assert(n * NT == ROWS * kPieces, "whole loads");
+  // Starts wave w's part (of NW) of the loads of all rows into t; at(row) is a
+  // row's first channel in memory.  A load fills 1 KB of LDS in lane order, each
+  // lane from its own address; a lane has the same row in all of them.
+  template <int NW, class Row> static __device__ __forceinline__ void load(T* t, int w, Row at) {
+    constexpr int groups = ROWS / kLoad, n = groups * (D / 32) / NW;
+    static_assert(n * NW == groups * (D / 32) && (NW % groups == 0 || groups % NW == 0), "whole loads");
+    const int l = lane_id();
+    if constexpr (NW % groups == 0) {
+      const int g = w % groups, row = g * kLoad + l / kPieces;
+      const T* s = at(row) + piece(row, l % kPieces) * kPer;
 #pragma unroll
-    for (int i = 0; i < n; ++i) {
-      const int c = i * NT + tid, row = c / kPieces, piece = (c % kPieces) ^ swz(row);
-      const T* s = at(row) + piece * kPer;
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)s,
-                                       (__attribute__((address_space(3))) void*)(t + (i * NT + (tid & ~63)) * kPer), 16, 0, 0);
+      for (int i = 0; i < n; ++i) copy(s + (w / groups + i * (NW / groups)) * 32, t + (w / groups + i * (NW / groups)) * kSlab + g * kLoad * 32);
+    } else {
+#pragma unroll
+      for (int j = 0; j < groups / NW; ++j) {
+        const int g = w + j * NW, row = g * kLoad + l / kPieces;
+        const T* s = at(row) + piece(row, l % kPieces) * kPer;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) copy(s + i * 32, t + i * kSlab + g * kLoad * 32);
+      }
     }
+  }
+  static __device__ __forceinline__ void copy(const T* s, T* d) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)s, (__attribute__((address_space(3))) void*)d, 16, 0, 0);
   }
 };
 

@@ -65,9 +65,9 @@ __device__ __forceinline__ int last_token(const int32_t* starts, int T, int k1) 
 // dK and dV of 16 NK NW keys of one key head.
 template <class T, int D, int NK, int NW, int BQ>
 __global__ __launch_bounds__(64 * NW) void k_attn_dkv(const AB p) {
-  using TL = Tile<T, D>;
+  using TL = Tile<T, D, BQ>;
   using F = typename At<T>::F;
-  constexpr int BN = 16 * NK * NW, NS = D / 32, NC = D / 16, NT = 64 * NW;
+  constexpr int BN = 16 * NK * NW, NS = D / 32, NC = D / 16;
   __shared__ __align__(16) T lds[4 * BQ * D];    // [2][q, d_out][BQ][D]
   __shared__ __align__(16) float ls[2][BQ], de[2][BQ];   // lse * log2(e) and delta per row
   __shared__ __align__(16) int tk[2][BQ], lw[2][BQ];     // token and first visible key per row
@@ -118,8 +118,8 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dkv(const AB p) {
   int m_tk = 0, m_lw = 0, m_hi = 0;   // m_hi: first visible key of the tile's last row
   auto fetch = [&](int j) {
     T* t = lds + (j & 1) * 2 * BQ * D;
-    TL::template load<BQ, NT>(t, threadIdx.x, [&](int x) { return rows.query(j * BQ + x); });
-    TL::template load<BQ, NT>(t + BQ * D, threadIdx.x, [&](int x) { return rows.grad(j * BQ + x); });
+    TL::template load<NW>(t, w, [&](int x) { return rows.query(j * BQ + x); });
+    TL::template load<NW>(t + BQ * D, w, [&](int x) { return rows.grad(j * BQ + x); });
     auto low = [&](int t) {
       int x = f.window ? max(t - f.window + 1, 0) : 0;
       return starts ? max(x, starts[t]) : x;
@@ -198,12 +198,12 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dkv(const AB p) {
         pf[i] = frag8<T>(s[i][0], s[i][1]);
         df[i] = frag8<T>(dp[i][0], dp[i][1]);
       }
-      const bool bad = masked && (TL::odd32(qt + u * D) || TL::odd32(gt + u * D));
+      const bool bad = masked && (TL::odd32(qt + u * 32) || TL::odd32(gt + u * 32));
       odd |= bad;
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        F gf = TL::col8(gt, u, 16 * c, r, q);
-        F qf = TL::col8(qt, u, 16 * c, r, q);
+        F gf = TL::col8(gt + u * 32, c, r, q);
+        F qf = TL::col8(qt + u * 32, c, r, q);
         if (bad) {
           gf = finite8<T>(gf);
           qf = finite8<T>(qf);
@@ -256,9 +256,9 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dkv(const AB p) {
 // dQ of 16 NQ NW query rows: the forward's walk over the keys.
 template <class T, int D, int NQ, int NW, int BN>
 __global__ __launch_bounds__(64 * NW) void k_attn_dq(const AB p) {
-  using TL = Tile<T, D>;
+  using TL = Tile<T, D, BN>;
   using F = typename At<T>::F;
-  constexpr int BM = 16 * NQ * NW, NS = D / 32, NC = D / 16, NT = 64 * NW;
+  constexpr int BM = 16 * NQ * NW, NS = D / 32, NC = D / 16;
   __shared__ __align__(16) T lds[4 * BN * D];   // [2][K, V][BN][D]
   const AF& f = p.f;
 
@@ -313,8 +313,8 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dq(const AB p) {
 
   auto fetch = [&](int j) {
     T* t = lds + (j & 1) * 2 * BN * D;
-    TL::template load<BN, NT>(t, threadIdx.x, [&](int x) { return kr(j * BN + x); });
-    TL::template load<BN, NT>(t + BN * D, threadIdx.x, [&](int x) { return vr(j * BN + x); });
+    TL::template load<NW>(t, w, [&](int x) { return kr(j * BN + x); });
+    TL::template load<NW>(t + BN * D, w, [&](int x) { return vr(j * BN + x); });
   };
   fetch(j0);
 #pragma unroll 1
@@ -357,10 +357,10 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dq(const AB p) {
           }
         df[i] = frag8<T>(dp[i][0], dp[i][1]);
       }
-      const bool bad = masked && TL::odd32(kt + u * D);   // (a query that sees such a key is NaN by its scores)
+      const bool bad = masked && TL::odd32(kt + u * 32);   // (a query that sees such a key is NaN by its scores)
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        F kf = TL::col8(kt, u, 16 * c, r, q);
+        F kf = TL::col8(kt + u * 32, c, r, q);
         if (bad) kf = finite8<T>(kf);
 #pragma unroll
         for (int i = 0; i < NQ; ++i) At<T>::mma(dq[i][c], kf, df[i]);

@@ -22,10 +22,10 @@ template <int D, int BM> constexpr int64_t slot_floats() { return (int64_t)BM * 
 
 template <class T, int D, int NQ>
 __global__ __launch_bounds__(64 * kWaves) void k_attn_few(const AF p) {
-  using TL = Tile<T, D>;
+  using TL = Tile<T, D, 32>;
   using F = typename At<T>::F;
   typedef uint32_t U4 __attribute__((ext_vector_type(4)));
-  constexpr int BM = 16 * NQ, NS = D / 32, NC = D / 16, NV = 32 * TL::kPieces / 64;   // NV: 16-byte loads of a wave's 32 value rows
+  constexpr int BM = 16 * NQ, NS = D / 32, NC = D / 16, NG = 32 / TL::kLoad, NV = NG * NS;   // NV: loads of a wave's 32 value rows, NG groups of rows by slabs
   // values of a wave's 32 keys; at a task's end the waves' sums
   constexpr int kV = 32 * D * (int)sizeof(T), kO = BM * D * 4;
   __shared__ __align__(16) char smem[kWaves * (kV > kO ? kV : kO)];
@@ -94,11 +94,12 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_few(const AF p) {
         for (int c = 0; c < NS; ++c) kf[e][c] = *reinterpret_cast<const F*>(s + 32 * c + 8 * q);
       }
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int c = i * 64 + l, row = c / TL::kPieces, piece = c % TL::kPieces, e = i >= NV / 2;
+      for (int g = 0; g < NG; ++g) {
+        const int row = g * TL::kLoad + l / TL::kPieces, e = g >= NG / 2;
         const int a = key + 16 * e, base = min(a, last & ~15), rel = min(row & 15, last - base);
-        const T* s = vb + (e ? pg1 : pg0) * p.vs[0] + (int64_t)((base & mask) + rel) * p.vs[1] + piece * TL::kPer;
-        vr[i] = *reinterpret_cast<const U4*>(s);
+        const T* s = vb + (e ? pg1 : pg0) * p.vs[0] + (int64_t)((base & mask) + rel) * p.vs[1] + l % TL::kPieces * TL::kPer;
+#pragma unroll
+        for (int c = 0; c < NS; ++c) vr[g * NS + c] = *reinterpret_cast<const U4*>(s + 32 * c);
       }
     };
     fetch(j0);
@@ -118,10 +119,10 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_few(const AF p) {
 #pragma unroll
           for (int i = 0; i < NQ; ++i) At<T>::mma(sc[i][e], kf[e][c], qf[i][c]);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int c = i * 64 + l, row = c / TL::kPieces, piece = (c % TL::kPieces) ^ TL::swz(row);
-        *reinterpret_cast<U4*>(vt + row * D + piece * TL::kPer) = vr[i];
-      }
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int c = 0; c < NS; ++c)
+          *reinterpret_cast<U4*>(vt + c * TL::kSlab + TL::at(g * TL::kLoad + l / TL::kPieces, l % TL::kPieces)) = vr[g * NS + c];
       if (j + 1 < j1) {
         fetch(j + 1);
         pg0 = page_of((j + 2) * kUnit + 32 * w);
@@ -174,7 +175,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_few(const AF p) {
       odd |= bad;
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        F vf = TL::col8(vt, 0, 16 * c, r, q);
+        F vf = TL::col8(vt, c, r, q);
         if (bad) vf = finite8<T>(vf);
 #pragma unroll
         for (int i = 0; i < NQ; ++i) At<T>::mma(o[i][c], vf, pf[i]);

@@ -1,4 +1,6 @@
 // Forward softmax attention over many rows: training and prompts.
+#include <type_traits>
+
 #include "dn_attn_fwd.h"
 
 namespace dn {
@@ -6,10 +8,10 @@ namespace {
 
 // One workgroup: NW waves of 16 NQ query rows each over one head's keys.
 template <class T, int D, int NQ, int NW, int BN, bool PAGED>
-__global__ __launch_bounds__(64 * NW) void k_attn(const AF p) {
-  using TL = Tile<T, D>;
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn(const AF p) {
+  using TL = Tile<T, D, BN>;
   using F = typename At<T>::F;
-  constexpr int BM = 16 * NQ * NW, NS = D / 32, NC = D / 16, NT = 64 * NW;
+  constexpr int BM = 16 * NQ * NW, NS = D / 32, NC = D / 16;
   __shared__ __align__(16) T lds[4 * BN * D];   // [2][K, V][BN][D]
 
   const int l = lane_id(), r = l & 15, q = l >> 4;
@@ -62,98 +64,127 @@ __global__ __launch_bounds__(64 * NW) void k_attn(const AF p) {
   kr.pages = vr.pages = p.pages;
   kr.last = vr.last = max(p1, 0);   // rows past it repeat it: finite unless a query that sees it is not
 
+  // The exponents' reference is a query's score with itself, which it always sees:
+  // no maximum has to be known while the sums run.  Sums of exponentials up to
+  // 2^kRange above it are as exact as any in a type with float32's range; the
+  // rare row that goes beyond is found at the end, and the tile done again with
+  // the maxima that are known then.
+  constexpr float kRange = std::is_same<T, f16>::value ? 15.f : 60.f, kShift = std::is_same<T, f16>::value ? 6.f : 0.f;
   f32x4 o[NQ][NC];
-  float mx[NQ], sum[NQ];
+  float mx[NQ], top[NQ], sum[NQ];
 #pragma unroll
   for (int i = 0; i < NQ; ++i) {
-    mx[i] = -INFINITY;
-    sum[i] = 0.f;
+    const T* kp = kr(max(pos[i], 0));
+    float x = 0.f;
 #pragma unroll
-    for (int c = 0; c < NC; ++c) o[i][c] = zero4();
+    for (int c = 0; c < NS; ++c) {
+      const F kf = *reinterpret_cast<const F*>(kp + 32 * c + 8 * q);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x += (float)kf[e] * (float)qf[i][c][e];
+    }
+    mx[i] = pos[i] < 0 ? 0.f : sum_q(x) * p.sc + kShift;
   }
-
   auto fetch = [&](int j) {
     T* t = lds + (j & 1) * 2 * BN * D;
-    TL::template load<BN, NT>(t, threadIdx.x, [&](int x) { return kr(j * BN + x); });
-    TL::template load<BN, NT>(t + BN * D, threadIdx.x, [&](int x) { return vr(j * BN + x); });
+    TL::template load<NW>(t, w, [&](int x) { return kr(j * BN + x); });
+    TL::template load<NW>(t + BN * D, w, [&](int x) { return vr(j * BN + x); });
   };
-  if (j0 < j1) fetch(j0);
   bool odd = false;   // infinities or NaNs in a masked tile were left out
-#pragma unroll 1
-  for (int j = j0; j < j1; ++j) {
-    loads_barrier();   // tile j is there, tile j - 1 is no longer read
-    if (j + 1 < j1) fetch(j + 1);
-    const T* kt = lds + (j & 1) * 2 * BN * D;
-    const T* vt = kt + BN * D;
-    const bool masked = j * BN + BN - 1 > p0 || j * BN < lo1;
-#pragma unroll 1
-    for (int u = 0; u < BN; u += 32) {
-      f32x4 sc[NQ][2];
+  // 32 keys of a tile; MASKED: some query must not see some of them.  At D = 256
+  // the first values are read under the exponentials and the others VB operands
+  // ahead, in this order (1006 us for 2 x 4096 tokens over 8192); at 128 the
+  // compiler's own order is better (601 against 668 us for 2 x 8192).
+  constexpr int VB = D == 256 ? 4 : NC, NB = NC / VB;
+  auto in_order = [] {
+    if constexpr (D == 256) __builtin_amdgcn_sched_barrier(0);
+  };
+  auto step = [&](auto masked, const T* kt, const T* vt, int key0) {
+    constexpr bool MASKED = decltype(masked)::value;
+    f32x4 sc[NQ][2];
 #pragma unroll
-      for (int i = 0; i < NQ; ++i) sc[i][0] = sc[i][1] = zero4();
+    for (int i = 0; i < NQ; ++i) sc[i][0] = sc[i][1] = zero4();
 #pragma unroll
-      for (int c = 0; c < NS; ++c)
+    for (int c = 0; c < NS; ++c)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const F kf = TL::row8(kt, u + 16 * e + r, c, q);
+      for (int e = 0; e < 2; ++e) {
+        const F kf = TL::row8(kt, 16 * e + r, c, q);
 #pragma unroll
-          for (int i = 0; i < NQ; ++i) At<T>::mma(sc[i][e], kf, qf[i][c]);
-        }
-      F pf[NQ];
-      bool grow = false;
-      float mt[NQ];
-#pragma unroll
-      for (int i = 0; i < NQ; ++i) {
-        if (masked) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const int key = j * BN + u + 16 * e + 4 * q + x;
-              sc[i][e][x] = key <= pos[i] && key >= low[i] ? sc[i][e][x] : -INFINITY;
-            }
-        }
-        float m = fmaxf(fmaxf(fmaxf(sc[i][0][0], sc[i][0][1]), fmaxf(sc[i][0][2], sc[i][0][3])),
-                        fmaxf(fmaxf(sc[i][1][0], sc[i][1][1]), fmaxf(sc[i][1][2], sc[i][1][3])));
-        mt[i] = max_q(m) * p.sc;
-        grow |= mt[i] > mx[i] + kLazy;
+        for (int i = 0; i < NQ; ++i) At<T>::mma(sc[i][e], kf, qf[i][c]);
       }
-      if (__any(grow)) {
+    F vf[2][VB];
+    auto values = [&](int n) {
 #pragma unroll
-        for (int i = 0; i < NQ; ++i) {
-          const float m = fmaxf(mx[i], mt[i]);
-          const float f = m == -INFINITY ? 1.f : fast_exp2(mx[i] - m);
-          mx[i] = m;
-          sum[i] *= f;
+      for (int c = 0; c < VB; ++c) vf[n & 1][c] = TL::col8(vt, n * VB + c, r, q);
+    };
+    in_order();
+    values(0);
+    in_order();
+    F pf[NQ];
 #pragma unroll
-          for (int c = 0; c < NC; ++c) {
-            o[i][c] *= f;
-            __builtin_amdgcn_sched_barrier(0);
+    for (int i = 0; i < NQ; ++i) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          if (MASKED) {
+            const int key = key0 + 16 * e + 4 * q + x;
+            sc[i][e][x] = key <= pos[i] && key >= low[i] ? sc[i][e][x] : -INFINITY;
           }
+          top[i] = fmaxf(top[i], sc[i][e][x]);
+          sc[i][e][x] = fast_exp2(__builtin_fmaf(sc[i][e][x], p.sc, -mx[i]));
+          sum[i] += sc[i][e][x];
         }
+      pf[i] = frag8<T>(sc[i][0], sc[i][1]);
+    }
+    const bool bad = MASKED && TL::odd32(vt);
+    if (MASKED) odd |= bad;
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      if (n + 1 < NB) values(n + 1);
+      in_order();
+      if (MASKED && bad) {
+#pragma unroll
+        for (int c = 0; c < VB; ++c) vf[n & 1][c] = finite8<T>(vf[n & 1][c]);
       }
 #pragma unroll
-      for (int i = 0; i < NQ; ++i) {
-        const float m = mx[i] == -INFINITY ? 0.f : mx[i];
+      for (int c = 0; c < VB; ++c)
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
+        for (int i = 0; i < NQ; ++i) At<T>::mma(o[i][n * VB + c], vf[n & 1][c], pf[i]);
+    }
+  };
+#pragma unroll 1
+  for (int pass = 0;; ++pass) {
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            sc[i][e][x] = fast_exp2(__builtin_fmaf(sc[i][e][x], p.sc, -m));
-            sum[i] += sc[i][e][x];
-          }
-        pf[i] = frag8<T>(sc[i][0], sc[i][1]);
-      }
-      const bool bad = masked && TL::odd32(vt + u * D);
-      odd |= bad;
+    for (int i = 0; i < NQ; ++i) {
+      top[i] = -INFINITY;
+      sum[i] = 0.f;
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        F vf = TL::col8(vt, u, 16 * c, r, q);
-        if (bad) vf = finite8<T>(vf);
+      for (int c = 0; c < NC; ++c) o[i][c] = zero4();
+    }
+    if (j0 < j1) fetch(j0);
+#pragma unroll 1
+    for (int j = j0; j < j1; ++j) {
+      loads_barrier();   // tile j is there, tile j - 1 is no longer read
+      if (j + 1 < j1) fetch(j + 1);
+      const T* kt = lds + (j & 1) * 2 * BN * D;
+      const T* vt = kt + BN * D;
+      if (j * BN + BN - 1 > p0 || j * BN < lo1) {
+#pragma unroll 1
+        for (int u = 0; u < BN; u += 32) step(std::true_type{}, kt + u * 32, vt + u * 32, j * BN + u);
+      } else {
 #pragma unroll
-        for (int i = 0; i < NQ; ++i) At<T>::mma(o[i][c], vf, pf[i]);
+        for (int u = 0; u < BN; u += 32) step(std::false_type{}, kt + u * 32, vt + u * 32, j * BN + u);
       }
     }
+    bool over = false;
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+      top[i] = max_q(top[i]) * p.sc;
+      over |= top[i] > mx[i] + kRange;
+    }
+    if (pass == 1 || !__syncthreads_or(over)) break;
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) mx[i] = top[i] > mx[i] + kRange ? top[i] : mx[i];   // (the other rows keep their bits)
   }
 
 #pragma unroll
@@ -187,7 +218,13 @@ __global__ __launch_bounds__(64 * NW) void k_attn(const AF p) {
 }
 
 template <class T, int D, bool PAGED> hipError_t run(const AF& p, hipStream_t st) {
-  constexpr int NQ = sizeof(T) == 4 ? 2 : 2, NW = 4, BN = sizeof(T) == 4 ? 32 : 64;
+  // 32 query rows per wave read each LDS operand for two products; at D = 256
+  // their sums leave no room for two waves on a SIMD, and 16 rows are faster.
+  // D = 128: four waves, two workgroups on a CU (601 us at 2 x 8192; eight waves
+  // around one copy of the keys 666, 64 rows per wave 869, 16 rows 793).  D = 256:
+  // eight waves of 16 rows (1006 us; 32 rows 1687, four waves and tiles of 32 keys
+  // 1103).
+  constexpr int NQ = sizeof(T) == 4 || D < 256 ? 2 : 1, NW = sizeof(T) == 4 || D < 256 ? 4 : 8, BN = sizeof(T) == 4 ? 32 : 64;
   constexpr int BM = 16 * NQ * NW;
   // rows are whole tiles per sequence: at most one more tile each
   const int64_t tiles = p.cu ? (int64_t)p.N * p.G / BM + p.B : (int64_t)p.B * (((int64_t)p.T * p.G + BM - 1) / BM);

@@ -119,6 +119,31 @@ def test_rows_hidden_infinities(dev, dt, odd):
     assert torch.equal(out[0, ~hit], base[0, ~hit])
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_rows_scores_far_above_the_own(dev, dt, D):
+    """Queries whose score with themselves is far below another one's: by the
+    thousand (the kernel's range of exponents does not reach), and growing from
+    tile to tile; other rows of the tile keep their bits."""
+    B, L, H = 1, 400, 2
+    q, k, v = (_rows(s, B, L, H, D, dt=dt) for s in (1, 2, 3))
+    base = causal_attention(q.to(dev), k.to(dev), v.to(dev))
+    k2, q2 = k.clone(), q.clone()
+    for at, size in ((3, 40.0), (70, 80.0), (200, 160.0)):   # keys along one axis, ever longer
+        k2[0, at] = 0
+        k2[0, at, :, 0] = size
+    q2[0, 100:110, :, 0], q2[0, 300:310, :, 0] = 50.0, 100.0
+    out, lse = causal_attention(q2.to(dev), k2.to(dev), v.to(dev), return_lse=True)
+    _check_rows(out, None, q2, k2, v, dt)
+    assert torch.equal(out[0, :3], base[0, :3])
+    # the same keys, with and without rows that go beyond the range
+    plain = causal_attention(q.to(dev), k2.to(dev), v.to(dev))
+    same = torch.ones(L, dtype=torch.bool)
+    same[100:110] = same[300:310] = False
+    if dt != "f16":   # (float16's range is narrow enough for other rows to go beyond it as well)
+        assert torch.equal(out[0, same], plain[0, same])
+
+
 # ---------------------------------------------------------------------------
 # paged
 # ---------------------------------------------------------------------------
