@@ -142,10 +142,13 @@ extern "C" int dn_attention_fwd(const dn_attention_args* a, void* stream) {
   return e == hipSuccess ? DN_OK : set_error(DN_E_LAUNCH, hipGetErrorString(e));
 }
 
+static size_t delta_bytes(const AF& p) { return ((size_t)p.N * p.Hkv * p.G * sizeof(float) + 255) / 256 * 256; }
+
 extern "C" size_t dn_attention_bwd_workspace_size(const dn_attention_args* a) {
   AF p{};
   if (attention_params(a, p) != DN_OK) return 0;
-  return (((size_t)p.N * a->Hq * sizeof(float) + 255) / 256 + 1) * 256;
+  if (p.N == 0) return 0;
+  return delta_bytes(p) + attn_backward_part_bytes(p, a->D, a->dtype) + 256;
 }
 
 extern "C" int dn_attention_bwd(const dn_attention_args* a, const void* d_out, void* dq, void* dk, void* dv, void* workspace,
@@ -159,6 +162,7 @@ extern "C" int dn_attention_bwd(const dn_attention_args* a, const void* d_out, v
   p.scale = a->scale;
   p.d_out = d_out; p.dq = dq; p.dk = dk; p.dv = dv;
   p.delta = (float*)(((uintptr_t)workspace + 255) & ~(uintptr_t)255);
+  p.part = (float*)((char*)p.delta + delta_bytes(p.f));
   const hipError_t e = attn_backward(p, a->D, a->dtype, (hipStream_t)stream);
   return e == hipSuccess ? DN_OK : set_error(DN_E_LAUNCH, hipGetErrorString(e));
 }

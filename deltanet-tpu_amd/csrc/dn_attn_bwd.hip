@@ -7,6 +7,8 @@
 // rows of all heads of its group, which is the sum over them too) and by query
 // rows (dQ).  That is seven products for the five of a single pass, whose third
 // output would have to be added up in memory.
+#include <type_traits>
+
 #include "dn_attn_fwd.h"
 
 namespace dn {
@@ -62,9 +64,11 @@ __device__ __forceinline__ int last_token(const int32_t* starts, int T, int k1) 
   return lo;
 }
 
-// dK and dV of 16 NK NW keys of one key head.
+// dK and dV of 16 NK NW keys of one key head: every S-th tile of query rows from
+// the blockIdx.y-th on, of S = gridDim.y.  With S > 1 the sums go to p.part, as
+// floats, and are added up by k_attn_dkv_sum.
 template <class T, int D, int NK, int NW, int BQ>
-__global__ __launch_bounds__(64 * NW) void k_attn_dkv(const AB p) {
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && D < 256 ? 2 : 1) void k_attn_dkv(const AB p) {
   using TL = Tile<T, D, BQ>;
   using F = typename At<T>::F;
   constexpr int BN = 16 * NK * NW, NS = D / 32, NC = D / 16;
@@ -106,7 +110,8 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dkv(const AB p) {
   rows.g = (const T*)p.d_out + ((int64_t)b * f.T * Hq + h * f.G) * D;
   rows.gt = (int64_t)Hq * D; rows.gh = D;
   rows.G = f.G; rows.last = f.T * f.G - 1;
-  const int r0 = k0 * f.G / BQ, r1 = (t1 * f.G + f.G - 1) / BQ + 1;   // tiles of query rows
+  const int S = gridDim.y;
+  const int r0 = k0 * f.G / BQ + blockIdx.y, r1 = (t1 * f.G + f.G - 1) / BQ + 1;   // tiles of query rows, by S
 
   f32x4 dk[NK][NC], dv[NK][NC];
 #pragma unroll
@@ -116,8 +121,8 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dkv(const AB p) {
 
   float m_ls = 0.f, m_de = 0.f;
   int m_tk = 0, m_lw = 0, m_hi = 0;   // m_hi: first visible key of the tile's last row
-  auto fetch = [&](int j) {
-    T* t = lds + (j & 1) * 2 * BQ * D;
+  auto fetch = [&](int j, int buf) {
+    T* t = lds + buf * 2 * BQ * D;
     TL::template load<NW>(t, w, [&](int x) { return rows.query(j * BQ + x); });
     TL::template load<NW>(t + BQ * D, w, [&](int x) { return rows.grad(j * BQ + x); });
     auto low = [&](int t) {
@@ -135,85 +140,103 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dkv(const AB p) {
     m_hi = low(min(j * BQ + BQ - 1, rows.last) / f.G);
   };
   bool odd = false;
-  if (r0 < r1) fetch(r0);
+  // 32 query rows of a tile; MASKED: some of them must not see some key
+  auto step = [&](auto mask, const T* qt, const T* gt, int buf, int u) {
+    constexpr bool MASKED = decltype(mask)::value;
+    f32x4 s[NK][2], dp[NK][2];
+#pragma unroll
+    for (int i = 0; i < NK; ++i) s[i][0] = s[i][1] = dp[i][0] = dp[i][1] = zero4();
+#pragma unroll
+    for (int c = 0; c < NS; ++c)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const F qf = TL::row8(qt, 16 * e + r, c, q);
+        const F gf = TL::row8(gt, 16 * e + r, c, q);
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+          At<T>::mma(s[i][e], qf, kf[i][c]);
+          At<T>::mma(dp[i][e], gf, vf[i][c]);
+        }
+      }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int at = u + 16 * e + 4 * q;
+      const f32x4 lse = *reinterpret_cast<const f32x4*>(&ls[buf][at]);
+      const f32x4 del = *reinterpret_cast<const f32x4*>(&de[buf][at]);
+#pragma unroll
+      for (int i = 0; i < NK; ++i)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const float pr = fast_exp2(__builtin_fmaf(s[i][e][x], f.sc, -lse[x]));
+          s[i][e][x] = pr;
+          dp[i][e][x] = pr * (dp[i][e][x] - del[x]);
+        }
+      if (MASKED) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int t = tk[buf][at + x], lo = lw[buf][at + x];
+#pragma unroll
+          for (int i = 0; i < NK; ++i) {
+            const bool see = key + 16 * i <= t && key + 16 * i >= lo;
+            s[i][e][x] = see ? s[i][e][x] : 0.f;
+            dp[i][e][x] = see ? dp[i][e][x] : 0.f;
+          }
+        }
+      }
+    }
+    F pf[NK], df[NK];
+#pragma unroll
+    for (int i = 0; i < NK; ++i) {
+      pf[i] = frag8<T>(s[i][0], s[i][1]);
+      df[i] = frag8<T>(dp[i][0], dp[i][1]);
+    }
+    const bool bad = MASKED && (TL::odd32(qt) || TL::odd32(gt));
+    if (MASKED) odd |= bad;
+#pragma unroll
+    for (int n = 0; n < NC; n += 4) {
+      F gc[4], qc[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        gc[c] = TL::col8(gt, n + c, r, q);
+        qc[c] = TL::col8(qt, n + c, r, q);
+      }
+      if (MASKED && bad) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          gc[c] = finite8<T>(gc[c]);
+          qc[c] = finite8<T>(qc[c]);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+          At<T>::mma(dv[i][n + c], gc[c], pf[i]);
+          At<T>::mma(dk[i][n + c], qc[c], df[i]);
+        }
+    }
+  };
+  if (r0 < r1) fetch(r0, 0);
+  int buf = 0;
 #pragma unroll 1
-  for (int j = r0; j < r1; ++j) {
+  for (int j = r0; j < r1; j += S, buf ^= 1) {
     if (threadIdx.x < BQ) {
-      ls[j & 1][threadIdx.x] = m_ls;
-      de[j & 1][threadIdx.x] = m_de;
-      tk[j & 1][threadIdx.x] = m_tk;
-      lw[j & 1][threadIdx.x] = m_lw;
+      ls[buf][threadIdx.x] = m_ls;
+      de[buf][threadIdx.x] = m_de;
+      tk[buf][threadIdx.x] = m_tk;
+      lw[buf][threadIdx.x] = m_lw;
     }
     const bool masked = j * BQ / f.G < k1 || m_hi > k0 || j * BQ + BQ - 1 > rows.last;
     loads_barrier();
-    if (j + 1 < r1) fetch(j + 1);
-    const T* qt = lds + (j & 1) * 2 * BQ * D;
+    if (j + S < r1) fetch(j + S, buf ^ 1);
+    const T* qt = lds + buf * 2 * BQ * D;
     const T* gt = qt + BQ * D;
+    if (masked) {
 #pragma unroll 1
-    for (int u = 0; u < BQ; u += 32) {
-      f32x4 s[NK][2], dp[NK][2];
+      for (int u = 0; u < BQ; u += 32) step(std::true_type{}, qt + u * 32, gt + u * 32, buf, u);
+    } else {
 #pragma unroll
-      for (int i = 0; i < NK; ++i) s[i][0] = s[i][1] = dp[i][0] = dp[i][1] = zero4();
-#pragma unroll
-      for (int c = 0; c < NS; ++c)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const F qf = TL::row8(qt, u + 16 * e + r, c, q);
-          const F gf = TL::row8(gt, u + 16 * e + r, c, q);
-#pragma unroll
-          for (int i = 0; i < NK; ++i) {
-            At<T>::mma(s[i][e], qf, kf[i][c]);
-            At<T>::mma(dp[i][e], gf, vf[i][c]);
-          }
-        }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int at = u + 16 * e + 4 * q;
-        const f32x4 lse = *reinterpret_cast<const f32x4*>(&ls[j & 1][at]);
-        const f32x4 del = *reinterpret_cast<const f32x4*>(&de[j & 1][at]);
-#pragma unroll
-        for (int i = 0; i < NK; ++i)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const float pr = fast_exp2(__builtin_fmaf(s[i][e][x], f.sc, -lse[x]));
-            s[i][e][x] = pr;
-            dp[i][e][x] = pr * (dp[i][e][x] - del[x]);
-          }
-        if (masked) {
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int t = tk[j & 1][at + x], lo = lw[j & 1][at + x];
-#pragma unroll
-            for (int i = 0; i < NK; ++i) {
-              const bool see = key + 16 * i <= t && key + 16 * i >= lo;
-              s[i][e][x] = see ? s[i][e][x] : 0.f;
-              dp[i][e][x] = see ? dp[i][e][x] : 0.f;
-            }
-          }
-        }
-      }
-      F pf[NK], df[NK];
-#pragma unroll
-      for (int i = 0; i < NK; ++i) {
-        pf[i] = frag8<T>(s[i][0], s[i][1]);
-        df[i] = frag8<T>(dp[i][0], dp[i][1]);
-      }
-      const bool bad = masked && (TL::odd32(qt + u * 32) || TL::odd32(gt + u * 32));
-      odd |= bad;
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        F gf = TL::col8(gt + u * 32, c, r, q);
-        F qf = TL::col8(qt + u * 32, c, r, q);
-        if (bad) {
-          gf = finite8<T>(gf);
-          qf = finite8<T>(qf);
-        }
-#pragma unroll
-        for (int i = 0; i < NK; ++i) {
-          At<T>::mma(dv[i][c], gf, pf[i]);
-          At<T>::mma(dk[i][c], qf, df[i]);
-        }
-      }
+      for (int u = 0; u < BQ; u += 32) step(std::false_type{}, qt + u * 32, gt + u * 32, buf, u);
     }
   }
 
@@ -227,13 +250,14 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dkv(const AB p) {
       float x[4], y[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        x[e] = dk[i][c][e] * p.scale;
+        x[e] = dk[i][c][e];
         y[e] = dv[i][c][e];
       }
       if (odd) {   // what the queries that see this key had left out of dV (dK of such a query is NaN by its scores)
 #pragma unroll 1
-        for (int row = max(r0 * BQ, t * f.G); row <= min(r1 * BQ - 1, rows.last); ++row) {
+        for (int row = r0 * BQ; row <= min(r1 * BQ - 1, rows.last); ++row) {
           const int tok = row / f.G;
+          if ((row / BQ - r0) % S || tok < t) continue;
           int lo = f.window ? max(tok - f.window + 1, 0) : 0;
           if (starts) lo = max(lo, starts[tok]);
           const int j = row / BQ, tl = min(j * BQ + BQ - 1, rows.last) / f.G;
@@ -247,15 +271,37 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dkv(const AB p) {
           }
         }
       }
-      st4<T>((T*)p.dk + at + 16 * c + 4 * q, x);
-      st4<T>((T*)p.dv + at + 16 * c + 4 * q, y);
+      if (S == 1) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] *= p.scale;
+        st4<T>((T*)p.dk + at + 16 * c + 4 * q, x);
+        st4<T>((T*)p.dv + at + 16 * c + 4 * q, y);
+      } else {
+        const int64_t n = (int64_t)f.N * f.Hkv * D;
+        float* part = p.part + (int64_t)blockIdx.y * 2 * n + at + 16 * c + 4 * q;
+        st4<float>(part, x);
+        st4<float>(part + n, y);
+      }
     }
   }
 }
 
+// dK and dV from S parts of each, in their order: 4 elements per thread.
+template <class T>
+__global__ __launch_bounds__(256) void k_attn_dkv_sum(const AB p, int64_t n, int S) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= 2 * n) return;
+  f32x4 a = *reinterpret_cast<const f32x4*>(p.part + i);
+#pragma unroll 4
+  for (int s = 1; s < S; ++s) a += *reinterpret_cast<const f32x4*>(p.part + s * 2 * n + i);
+  const float f = i < n ? p.scale : 1.f;
+  const float x[4] = {a[0] * f, a[1] * f, a[2] * f, a[3] * f};
+  st4<T>((i < n ? (T*)p.dk + i : (T*)p.dv + (i - n)), x);
+}
+
 // dQ of 16 NQ NW query rows: the forward's walk over the keys.
 template <class T, int D, int NQ, int NW, int BN>
-__global__ __launch_bounds__(64 * NW) void k_attn_dq(const AB p) {
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(const AB p) {
   using TL = Tile<T, D, BN>;
   using F = typename At<T>::F;
   constexpr int BM = 16 * NQ * NW, NS = D / 32, NC = D / 16;
@@ -316,6 +362,56 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dq(const AB p) {
     TL::template load<NW>(t, w, [&](int x) { return kr(j * BN + x); });
     TL::template load<NW>(t + BN * D, w, [&](int x) { return vr(j * BN + x); });
   };
+  // 32 keys of a tile; MASKED: some query must not see some of them
+  auto step = [&](auto mask, const T* kt, const T* vt, int key0) {
+    constexpr bool MASKED = decltype(mask)::value;
+    f32x4 s[NQ][2], dp[NQ][2];
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) s[i][0] = s[i][1] = dp[i][0] = dp[i][1] = zero4();
+#pragma unroll
+    for (int c = 0; c < NS; ++c)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const F kf = TL::row8(kt, 16 * e + r, c, q);
+        const F vf = TL::row8(vt, 16 * e + r, c, q);
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+          At<T>::mma(s[i][e], kf, qf[i][c]);
+          At<T>::mma(dp[i][e], vf, gf[i][c]);
+        }
+      }
+    F df[NQ];
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const float pr = fast_exp2(__builtin_fmaf(s[i][e][x], f.sc, -ls[i]));
+          dp[i][e][x] = pr * (dp[i][e][x] - de[i]);
+          if (MASKED) {
+            const int key = key0 + 16 * e + 4 * q + x;
+            dp[i][e][x] = key <= pos[i] && key >= low[i] ? dp[i][e][x] : 0.f;
+          }
+        }
+      df[i] = frag8<T>(dp[i][0], dp[i][1]);
+    }
+    const bool bad = MASKED && TL::odd32(kt);   // (a query that sees such a key is NaN by its scores)
+#pragma unroll
+    for (int n = 0; n < NC; n += 4) {
+      F kc[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) kc[c] = TL::col8(kt, n + c, r, q);
+      if (MASKED && bad) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) kc[c] = finite8<T>(kc[c]);
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) At<T>::mma(dq[i][n + c], kc[c], df[i]);
+    }
+  };
   fetch(j0);
 #pragma unroll 1
   for (int j = j0; j < j1; ++j) {
@@ -323,48 +419,12 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dq(const AB p) {
     if (j + 1 < j1) fetch(j + 1);
     const T* kt = lds + (j & 1) * 2 * BN * D;
     const T* vt = kt + BN * D;
-    const bool masked = j * BN + BN - 1 > p0 || j * BN < lo1;
+    if (j * BN + BN - 1 > p0 || j * BN < lo1) {
 #pragma unroll 1
-    for (int u = 0; u < BN; u += 32) {
-      f32x4 s[NQ][2], dp[NQ][2];
+      for (int u = 0; u < BN; u += 32) step(std::true_type{}, kt + u * 32, vt + u * 32, j * BN + u);
+    } else {
 #pragma unroll
-      for (int i = 0; i < NQ; ++i) s[i][0] = s[i][1] = dp[i][0] = dp[i][1] = zero4();
-#pragma unroll
-      for (int c = 0; c < NS; ++c)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const F kf = TL::row8(kt, u + 16 * e + r, c, q);
-          const F vf = TL::row8(vt, u + 16 * e + r, c, q);
-#pragma unroll
-          for (int i = 0; i < NQ; ++i) {
-            At<T>::mma(s[i][e], kf, qf[i][c]);
-            At<T>::mma(dp[i][e], vf, gf[i][c]);
-          }
-        }
-      F df[NQ];
-#pragma unroll
-      for (int i = 0; i < NQ; ++i) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const float pr = fast_exp2(__builtin_fmaf(s[i][e][x], f.sc, -ls[i]));
-            dp[i][e][x] = pr * (dp[i][e][x] - de[i]);
-            if (masked) {
-              const int key = j * BN + u + 16 * e + 4 * q + x;
-              dp[i][e][x] = key <= pos[i] && key >= low[i] ? dp[i][e][x] : 0.f;
-            }
-          }
-        df[i] = frag8<T>(dp[i][0], dp[i][1]);
-      }
-      const bool bad = masked && TL::odd32(kt + u * 32);   // (a query that sees such a key is NaN by its scores)
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        F kf = TL::col8(kt + u * 32, c, r, q);
-        if (bad) kf = finite8<T>(kf);
-#pragma unroll
-        for (int i = 0; i < NQ; ++i) At<T>::mma(dq[i][c], kf, df[i]);
-      }
+      for (int u = 0; u < BN; u += 32) step(std::false_type{}, kt + u * 32, vt + u * 32, j * BN + u);
     }
   }
 
@@ -382,28 +442,64 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dq(const AB p) {
   }
 }
 
+template <class T, int D> struct Shape {
+  // dkv: 16 keys per wave and two waves on a SIMD (2 x 8192 tokens, D 128: 1467 us,
+  // 32 keys and one wave 1690); at D = 256 the sums of 16 keys alone take 128
+  // registers.  dq: 32 rows (767 us; 16 rows 797); 16 at D = 256 (87 us at 2048
+  // tokens, 32 rows 107).
+  static constexpr bool f32 = sizeof(T) == 4;
+  static constexpr int NW = 4, BT = f32 ? 32 : 64;
+  static constexpr int NK = f32 && D == 64 ? 2 : 1, NQ = D == 256 ? 1 : 2;
+  static constexpr int keys = 16 * NK * NW, rows = 16 * NQ * NW;
+};
+
+// Parts of the walk over query rows, so that dkv fills the card (kFill workgroups),
+// none shorter than two tiles of rows.
+constexpr int64_t kFill = 512;
+template <class T, int D> int splits(const AF& f) {
+  using Sh = Shape<T, D>;
+  const int64_t wg = ((int64_t)f.T + Sh::keys - 1) / Sh::keys * f.B * f.Hkv;
+  const int64_t tiles = ((int64_t)f.T * f.G + Sh::BT - 1) / Sh::BT;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({kFill / wg, tiles / 2, 8}));
+}
+
 template <class T, int D> hipError_t run(const AB& p, hipStream_t st) {
-  constexpr bool f32 = sizeof(T) == 4;
-  constexpr int NW = 4, BT = f32 ? 32 : 64;
-  constexpr int NK = D == 256 || (f32 && D == 128) ? 1 : 2, NQ = f32 && D == 256 ? 1 : 2;
+  using Sh = Shape<T, D>;
+  constexpr int NW = Sh::NW;
   const AF& f = p.f;
   const int64_t rows = (int64_t)f.N * f.Hkv * f.G, groups = (int64_t)f.B * f.Hkv;
   hipLaunchKernelGGL((k_attn_delta<T, D>), dim3((unsigned)((rows * (D / 8) + 255) / 256)), dim3(256), 0, st, p, rows);
-  const int64_t kt = ((int64_t)f.T + 16 * NK * NW - 1) / (16 * NK * NW);
-  hipLaunchKernelGGL((k_attn_dkv<T, D, NK, NW, BT>), dim3((unsigned)(kt * groups)), dim3(64 * NW), 0, st, p);
-  const int64_t qt = ((int64_t)f.T * f.G + 16 * NQ * NW - 1) / (16 * NQ * NW);
-  hipLaunchKernelGGL((k_attn_dq<T, D, NQ, NW, BT>), dim3((unsigned)(qt * groups)), dim3(64 * NW), 0, st, p);
+  const int S = splits<T, D>(f);
+  const int64_t kt = ((int64_t)f.T + Sh::keys - 1) / Sh::keys;
+  hipLaunchKernelGGL((k_attn_dkv<T, D, Sh::NK, NW, Sh::BT>), dim3((unsigned)(kt * groups), S), dim3(64 * NW), 0, st, p);
+  if (S > 1) {
+    const int64_t n = (int64_t)f.N * f.Hkv * D;
+    hipLaunchKernelGGL((k_attn_dkv_sum<T>), dim3((unsigned)((2 * n / 4 + 255) / 256)), dim3(256), 0, st, p, n, S);
+  }
+  const int64_t qt = ((int64_t)f.T * f.G + Sh::rows - 1) / Sh::rows;
+  hipLaunchKernelGGL((k_attn_dq<T, D, Sh::NQ, NW, Sh::BT>), dim3((unsigned)(qt * groups)), dim3(64 * NW), 0, st, p);
   return hipGetLastError();
+}
+
+// f(T, D) for a type and head dimension
+template <class F> auto choose(int D, int dtype, F f) {
+  auto go = [&](auto z) {
+    if (D == 64) return f(z, std::integral_constant<int, 64>{});
+    if (D == 128) return f(z, std::integral_constant<int, 128>{});
+    return f(z, std::integral_constant<int, 256>{});
+  };
+  return dtype == DN_BF16 ? go((bf16)0.f) : dtype == DN_F16 ? go((f16)0.f) : go(0.f);
 }
 
 }  // namespace
 
+size_t attn_backward_part_bytes(const AF& f, int D, int dtype) {
+  const int S = choose(D, dtype, [&](auto z, auto d) { return splits<decltype(z), decltype(d)::value>(f); });
+  return S > 1 ? (size_t)S * 2 * f.N * f.Hkv * D * sizeof(float) : 0;
+}
+
 hipError_t attn_backward(const AB& p, int D, int dtype, hipStream_t st) {
-  auto go = [&](auto z) {
-    using T = decltype(z);
-    return D == 64 ? run<T, 64>(p, st) : D == 128 ? run<T, 128>(p, st) : run<T, 256>(p, st);
-  };
-  return dtype == DN_BF16 ? go((bf16)0.f) : dtype == DN_F16 ? go((f16)0.f) : go(0.f);
+  return choose(D, dtype, [&](auto z, auto d) { return run<decltype(z), decltype(d)::value>(p, st); });
 }
 
 }  // namespace dn

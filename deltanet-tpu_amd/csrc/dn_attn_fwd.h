@@ -218,7 +218,9 @@ struct AB {
   const void* d_out;
   void *dq, *dk, *dv;
   float* delta;
+  float* part;   // attn_backward_part_bytes
 };
+size_t attn_backward_part_bytes(const AF& f, int D, int dtype);
 hipError_t attn_backward(const AB& p, int D, int dtype, hipStream_t st);
 
 }  // namespace dn
