@@ -123,12 +123,12 @@ int attention_params(const dn_attention_args* a, AF& p) {
   if (const char* m = shape_error((int64_t)a->B * a->L, a->Hq, a->Hkv, a->D, a->dtype, a->scale, a->window)) return bad(m);
   if (a->B && a->L && (!a->q || !a->k || !a->v || !a->out)) return bad("missing tensor pointer");
   if (!wide(a->q, a->q_strides, a->dtype, 3) || !wide(a->k, a->k_strides, a->dtype, 3) || !wide(a->v, a->v_strides, a->dtype, 3) ||
-      ((uintptr_t)a->out & 15))
+      (((uintptr_t)a->out | (uintptr_t)a->out_low) & 15))
     return bad("attention rows must start on 16 bytes");
   p.B = a->B; p.T = a->L; p.N = a->B * a->L;
   p.Hkv = a->Hkv; p.G = a->Hq / a->Hkv; p.window = a->window;
   p.sc = a->scale * kLog2e;
-  p.q = a->q; p.k = a->k; p.v = a->v; p.out = a->out; p.lse = a->lse; p.start = a->starts;
+  p.q = a->q; p.k = a->k; p.v = a->v; p.out = a->out; p.low = a->out_low; p.lse = a->lse; p.start = a->starts;
   for (int i = 0; i < 3; ++i) { p.qs[i] = a->q_strides[i]; p.ks[i] = a->k_strides[i]; p.vs[i] = a->v_strides[i]; }
   return DN_OK;
 }

@@ -14,7 +14,7 @@
 namespace dn {
 namespace {
 
-// delta = sum of d_out * out over a row's channels: D/8 lanes per row
+// delta = sum of d_out * (out + out_low) over a row's channels: D/8 lanes per row
 template <class T, int D>
 __global__ __launch_bounds__(256) void k_attn_delta(const AB p, int64_t rows) {
   constexpr int per = D / 8;
@@ -25,6 +25,11 @@ __global__ __launch_bounds__(256) void k_attn_delta(const AB p, int64_t rows) {
     const V a = reinterpret_cast<const V*>(p.d_out)[id], b = reinterpret_cast<const V*>(p.f.out)[id];
 #pragma unroll
     for (int e = 0; e < 8; ++e) s += (float)a[e] * (float)b[e];
+    if (p.f.low) {
+      const V c = reinterpret_cast<const V*>(p.f.low)[id];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s += (float)a[e] * (float)c[e];
+    }
   }
 #pragma unroll
   for (int o = 1; o < per; o <<= 1) s += __shfl_xor(s, o);

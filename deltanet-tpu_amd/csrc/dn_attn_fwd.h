@@ -15,6 +15,7 @@ struct AF {
   float sc;                  // scale * log2(e)
   const void *q, *k, *v;
   void* out;                 // dense (tokens, Hkv G, D)
+  void* low;                 // NULL or as out: what its rounding cut off
   float* lse;                // NULL or (tokens, Hkv G)
   float* part;               // partial results (dn_attn_few.hip)
   const int32_t *cu, *lens, *pt;

@@ -212,6 +212,11 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn(const 
         }
       }
       st4<T>(op + 16 * c + 4 * q, x);
+      if (!PAGED && p.low) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] -= (float)(T)x[e];
+        st4<T>((T*)p.low + at * D + 16 * c + 4 * q, x);
+      }
     }
     if (p.lse && q == 0) p.lse[at] = z == 0.f ? -INFINITY : kLn2 * (mx[i] + __log2f(z));
   }

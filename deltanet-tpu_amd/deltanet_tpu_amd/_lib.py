@@ -140,7 +140,7 @@ class AttentionArgs(ctypes.Structure):
         ("B", _c_i32), ("L", _c_i32), ("Hq", _c_i32), ("Hkv", _c_i32), ("D", _c_i32),
         ("dtype", _c_i32), ("window", _c_i32),
         ("scale", ctypes.c_float),
-        ("q", _c_ptr), ("k", _c_ptr), ("v", _c_ptr), ("out", _c_ptr), ("lse", _c_ptr), ("starts", _c_ptr),
+        ("q", _c_ptr), ("k", _c_ptr), ("v", _c_ptr), ("out", _c_ptr), ("out_low", _c_ptr), ("lse", _c_ptr), ("starts", _c_ptr),
         ("q_strides", _c_i64 * 3), ("k_strides", _c_i64 * 3), ("v_strides", _c_i64 * 3),
     ]
 
@@ -149,7 +149,7 @@ class AttentionArgs(ctypes.Structure):
 ROTARY_PACK = struct.Struct("@12i6P8q").pack
 KV_APPEND_PACK = struct.Struct("@13i8P13q").pack
 PAGED_ATTENTION_PACK = struct.Struct("@11if8P10q").pack
-ATTENTION_PACK = struct.Struct("@8if6P9q").pack
+ATTENTION_PACK = struct.Struct("@8if7P9q").pack
 
 
 EXPORTED_SYMBOLS = (

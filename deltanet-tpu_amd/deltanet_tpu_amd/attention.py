@@ -394,31 +394,33 @@ def _document_starts(segment_ids, cu_seqlens, B, L, dev):
     return starts
 
 
-def _attention_block(q, k, v, out, lse, starts, scale, window):
+def _attention_block(q, k, v, out, low, lse, starts, scale, window):
     B, L, Hq, D = q.shape
     qs, ks, vs = q.stride(), k.stride(), v.stride()
     return _lib.ATTENTION_PACK(
         _lib.DN_ABI_VERSION, B, L, Hq, k.shape[2], D, _DT[q.dtype], window or 0, scale, q.data_ptr(), k.data_ptr(),
-        v.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), 0 if starts is None else starts.data_ptr(),
+        v.data_ptr(), out.data_ptr(), 0 if low is None else low.data_ptr(), 0 if lse is None else lse.data_ptr(), 0 if starts is None else starts.data_ptr(),
         qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2])
 
 
-def _attention_forward(q, k, v, starts, scale, window, want_lse):
+def _attention_forward(q, k, v, starts, scale, window, want_lse, want_low=False):
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    low = torch.empty(q.shape, dtype=q.dtype, device=q.device) if want_low else None
     lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device) if want_lse else None
     if q.numel():
-        _call("dn_attention_fwd", q.get_device(), _attention_block(q, k, v, out, lse, starts, scale, window))
-    return out, lse
+        _call("dn_attention_fwd", q.get_device(), _attention_block(q, k, v, out, low, lse, starts, scale, window))
+    return out, low, lse
 
 
 class _AttentionFn(torch.autograd.Function):
     """Causal attention under autograd: the forward keeps the log of each row's sum
-    of exponentials, from which the backward recomputes the probabilities."""
+    of exponentials, from which the backward recomputes the probabilities, and what
+    rounding cut off the output, which the backward's row sums read with it."""
 
     @staticmethod
     def forward(ctx, q, k, v, starts, scale, window):
-        out, lse = _attention_forward(q, k, v, starts, scale, window, True)
-        ctx.save_for_backward(q, k, v, out, lse, starts)
+        out, low, lse = _attention_forward(q, k, v, starts, scale, window, True, q.dtype is not torch.float32)
+        ctx.save_for_backward(q, k, v, out, low, lse, starts)
         ctx.meta = scale, window
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
@@ -426,14 +428,14 @@ class _AttentionFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, d_out, _):
-        q, k, v, out, lse, starts = ctx.saved_tensors
+        q, k, v, out, low, lse, starts = ctx.saved_tensors
         scale, window = ctx.meta
         if d_out is None:
             return (None,) * 6
         d_out = d_out.contiguous()
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
         if q.numel():
-            block = _attention_block(q, k, v, out, lse, starts, scale, window)
+            block = _attention_block(q, k, v, out, low, lse, starts, scale, window)
             need = _lib.packed_call("dn_attention_bwd_workspace_size")(block)
             ws = torch.empty((need,), dtype=torch.uint8, device=q.device)
             _call("dn_attention_bwd", q.get_device(), block, d_out.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
@@ -470,5 +472,5 @@ def causal_attention(q, k, v, *, segment_ids=None, cu_seqlens=None, scale=None, 
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out, lse = _AttentionFn.apply(q, k, v, starts, scale, window)
     else:
-        out, lse = _attention_forward(q, k, v, starts, scale, window, return_lse)
+        out, _, lse = _attention_forward(q, k, v, starts, scale, window, return_lse)
     return (out, lse) if return_lse else out
