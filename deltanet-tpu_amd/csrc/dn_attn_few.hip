@@ -15,7 +15,7 @@ namespace {
 constexpr int kWaves = 4, kUnit = 32 * kWaves;
 constexpr int kGroups = 512;   // workgroups of a launch: two per CU
 
-__host__ __device__ __forceinline__ int64_t first_unit(int64_t w, int64_t W, int64_t C) { return w * C / W; }
+__device__ __forceinline__ int first_unit(int w, int W, int C) { return (int)((int64_t)w * C / W); }
 
 // A partial result: BM rows of D sums, then BM maxima, then BM sums of exponentials.
 template <int D, int BM> constexpr int64_t slot_floats() { return (int64_t)BM * (D + 2); }
@@ -34,20 +34,20 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_few(const AF p) {
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   T* vt = reinterpret_cast<T*>(smem + w * kV);
 
-  const int64_t C = all_units(p, BM, kUnit);
-  const int64_t W = min((int64_t)gridDim.x, C);   // each has a unit at least
-  if (blockIdx.x >= W) return;
-  int64_t u = first_unit(blockIdx.x, W, C);
-  const int64_t uend = first_unit(blockIdx.x + 1, W, C);
+  const Plan plan(p, BM, kUnit);
+  const int W = min((int)gridDim.x, plan.C);   // each has a unit at least
+  if ((int)blockIdx.x >= W) return;
+  int u = first_unit(blockIdx.x, W, plan.C);
+  const int uend = first_unit(blockIdx.x + 1, W, plan.C);
 #pragma unroll 1
   while (u < uend) {
     Task t;
-    if (!find_task<false>(p, u, BM, kUnit, t)) break;
+    if (!plan.of_unit(u, t)) break;
     const int rows = t.s.n * p.G, row0 = t.m * BM, row1 = min(row0 + BM, rows);
     const int off = t.s.len - t.s.n, p0 = off + row0 / p.G, p1 = off + (row1 - 1) / p.G;
     int k0, k1;
     units_of(p, t.s, row0, row1, kUnit, k0, k1);
-    const int skip = (int)(u - t.first), take = (int)min((int64_t)(t.units - skip), uend - u);
+    const int skip = u - t.first, take = min(t.units - skip, uend - u);
     const int j0 = k0 + skip, j1 = j0 + take;   // units of this piece
     const int last = max(p1, 0);
     const int lo1 = p.window ? p1 - p.window + 1 : 0;
@@ -254,40 +254,59 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_few(const AF p) {
   }
 }
 
-// Joins the parts of the task blockIdx.x if more than one workgroup had some.
+// Joins the parts of a query row if more than one workgroup had some: D/4 threads
+// per part, 1024/D parts at a time.
 template <class T, int D, int BM>
 __global__ __launch_bounds__(256) void k_attn_join(const AF p, int groups) {
+  constexpr int NP = 1024 / D;
+  __shared__ float ps[NP][D + 4];
   Task t;
-  const int64_t C = all_units(p, BM, kUnit), W = min((int64_t)groups, C);
-  if (!find_task<true>(p, blockIdx.x, BM, kUnit, t)) return;
+  int row;
+  const int Hq = p.Hkv * p.G, i = blockIdx.x / Hq, hq = blockIdx.x - i * Hq;
+  const Plan plan(p, BM, kUnit);
+  const int W = min(groups, plan.C);
+  if (!plan.of_row(i, hq, t, row)) return;
   // the workgroup that has unit u: the last w with w C / W <= u
-  auto owner = [&](int64_t u) { return ((u + 1) * W + C - 1) / C - 1; };
-  const int64_t w0 = owner(t.first), w1 = owner(t.first + t.units - 1);
+  auto owner = [&](int u) { return (int)((((int64_t)u + 1) * W + plan.C - 1) / plan.C) - 1; };
+  const int w0 = owner(t.first), w1 = owner(t.first + t.units - 1);
   if (w0 == w1) return;
-  const int row0 = t.m * BM, nrow = min(t.s.n * p.G - row0, BM);
-  auto slot = [&](int64_t w) { return p.part + (2 * w + (w == w0 ? 1 : 0)) * slot_floats<D, BM>(); };
-  for (int x = threadIdx.x; x < nrow * (D / 4); x += 256) {
-    const int row = x / (D / 4), ch = x % (D / 4);
-    float m = -INFINITY;
-    for (int64_t w = w0; w <= w1; ++w) m = fmaxf(m, slot(w)[BM * D + row]);
-    f32x4 a = zero4();
-    float z = 0.f;
+  row -= t.m * BM;
+  const int ch = threadIdx.x % (D / 4), part = threadIdx.x / (D / 4);
+  f32x4 a = zero4();
+  float m = -INFINITY, z = 0.f;
 #pragma unroll 4
-    for (int64_t w = w0; w <= w1; ++w) {
-      const float* s = slot(w);
-      const float mw = s[BM * D + row];
-      const float f = mw == -INFINITY ? 0.f : fast_exp2(mw - m);
-      const f32x4 y = *reinterpret_cast<const f32x4*>(s + row * D + 4 * ch);
-      if (f != 0.f) a += f * y;
-      z += f * s[BM * D + BM + row];
-    }
-    const int tk = (row0 + row) / p.G, g = row0 + row - tk * p.G;
-    const int64_t at = (int64_t)(t.s.c0 + tk) * p.Hkv * p.G + t.h * p.G + g;
-    const float f = z == 0.f ? 0.f : 1.f / z;
-    const float y[4] = {a[0] * f, a[1] * f, a[2] * f, a[3] * f};
-    st4<T>((T*)p.out + at * D + 4 * ch, y);
-    if (p.lse && ch == 0) p.lse[at] = z == 0.f ? -INFINITY : kLn2 * (m + __log2f(z));
+  for (int w = w0 + part; w <= w1; w += NP) {
+    const float* s = p.part + (2 * (int64_t)w + (w == w0 ? 1 : 0)) * slot_floats<D, BM>();
+    const f32x4 y = *reinterpret_cast<const f32x4*>(s + row * D + 4 * ch);
+    const float mw = s[BM * D + row], zw = s[BM * D + BM + row];
+    const float n = fmaxf(m, mw);
+    const float f = m == -INFINITY ? 0.f : fast_exp2(m - n), g = mw == -INFINITY ? 0.f : fast_exp2(mw - n);
+    if (f != 1.f) a *= f;
+    if (g != 0.f) a += g * y;
+    z = z * f + g * zw;
+    m = n;
   }
+  *reinterpret_cast<f32x4*>(&ps[part][4 * ch]) = a;
+  if (ch == 0) {
+    ps[part][D] = m;
+    ps[part][D + 1] = z;
+  }
+  __syncthreads();
+  if (part) return;
+#pragma unroll
+  for (int k = 1; k < NP; ++k) {
+    const float mw = ps[k][D], n = fmaxf(m, mw);
+    const float f = m == -INFINITY ? 0.f : fast_exp2(m - n), g = mw == -INFINITY ? 0.f : fast_exp2(mw - n);
+    const f32x4 y = *reinterpret_cast<const f32x4*>(&ps[k][4 * ch]);
+    if (f != 1.f) a *= f;
+    if (g != 0.f) a += g * y;
+    z = z * f + g * ps[k][D + 1];
+    m = n;
+  }
+  const float f = z == 0.f ? 0.f : 1.f / z;
+  const float y[4] = {a[0] * f, a[1] * f, a[2] * f, a[3] * f};
+  st4<T>((T*)p.out + (int64_t)blockIdx.x * D + 4 * ch, y);
+  if (p.lse && ch == 0) p.lse[blockIdx.x] = z == 0.f ? -INFINITY : kLn2 * (m + __log2f(z));
 }
 
 int row_tile(const AF& p) { return (int64_t)p.N * p.G <= (int64_t)16 * p.B ? 16 : 32; }
@@ -296,26 +315,24 @@ int64_t most_tasks(const AF& p) {
   return (p.cu ? (int64_t)p.N * p.G / BM + p.B : (int64_t)p.B * ((p.T * p.G + BM - 1) / BM)) * p.Hkv;
 }
 // No more workgroups than there can be units.
-int64_t groups_of(const AF& p) {
-  const int64_t per = (((int64_t)p.max_pages << p.shift) + kUnit - 1) / kUnit;
-  return std::min<int64_t>(kGroups, most_tasks(p) * per);
-}
+int64_t most_units(const AF& p) { return most_tasks(p) * ((((int64_t)p.max_pages << p.shift) + kUnit - 1) / kUnit); }
+int64_t groups_of(const AF& p) { return std::min<int64_t>(kGroups, most_units(p)); }
 
 template <class T, int D> hipError_t run(const AF& p, hipStream_t st) {
-  const unsigned W = (unsigned)groups_of(p), tasks = (unsigned)most_tasks(p);
+  const unsigned W = (unsigned)groups_of(p), rows = (unsigned)p.N * p.Hkv * p.G;
   if (row_tile(p) == 16) {
     hipLaunchKernelGGL((k_attn_few<T, D, 1>), dim3(W), dim3(64 * kWaves), 0, st, p);
-    if (W > 1) hipLaunchKernelGGL((k_attn_join<T, D, 16>), dim3(tasks), dim3(256), 0, st, p, (int)W);
+    if (W > 1) hipLaunchKernelGGL((k_attn_join<T, D, 16>), dim3(rows), dim3(256), 0, st, p, (int)W);
   } else {
     hipLaunchKernelGGL((k_attn_few<T, D, 2>), dim3(W), dim3(64 * kWaves), 0, st, p);
-    if (W > 1) hipLaunchKernelGGL((k_attn_join<T, D, 32>), dim3(tasks), dim3(256), 0, st, p, (int)W);
+    if (W > 1) hipLaunchKernelGGL((k_attn_join<T, D, 32>), dim3(rows), dim3(256), 0, st, p, (int)W);
   }
   return hipGetLastError();
 }
 
 }  // namespace
 
-bool attn_few_takes(const AF& p) { return p.shift >= 4 && (int64_t)p.N * p.G <= (int64_t)32 * p.B; }
+bool attn_few_takes(const AF& p) { return p.shift >= 4 && (int64_t)p.N * p.G <= (int64_t)32 * p.B && most_units(p) < (1 << 30); }
 
 size_t attn_few_bytes(const AF& p, int D) { return (size_t)groups_of(p) * 2 * row_tile(p) * (D + 2) * sizeof(float); }
 

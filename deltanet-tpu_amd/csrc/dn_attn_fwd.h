@@ -110,96 +110,110 @@ __device__ __forceinline__ void units_of(const AF& p, const Span& s, int row0, i
 // key head, tile of BM rows), in that order, each of as many units as `unit`
 // tokens its rows see; workgroup w of W takes the units [w C / W, (w+1) C / W) of
 // the C in all, wherever tasks begin and end in them.  Lengths are known on the
-// device alone, so every workgroup adds them up itself.
+// device alone, so every wave adds them up itself, a sequence per lane (the first
+// 64 once for all its questions).
 struct Task {
   Span s;
   int b, h, m;
-  int64_t first;   // its first unit
+  int first;   // its first unit
   int units;
 };
-// units of sequence b, one head
-__device__ __forceinline__ int64_t head_units(const AF& p, const Span& s, int BM, int unit) {
-  const int rows = s.n * p.G;
-  int64_t c = 0;
-  for (int r = 0; r < rows; r += BM) {
-    int u0, u1;
-    units_of(p, s, r, min(r + BM, rows), unit, u0, u1);
-    c += u1 - u0;
-  }
-  return c;
-}
-__device__ __forceinline__ int64_t shfl_up64(int64_t x, int o) {
-  const int lo = __shfl_up((int)(uint32_t)x, o), hi = __shfl_up((int)(x >> 32), o);
-  return ((int64_t)hi << 32) | (uint32_t)lo;
-}
-__device__ __forceinline__ int64_t shfl64(int64_t x, int l) {
-  const int lo = __shfl((int)(uint32_t)x, l), hi = __shfl((int)(x >> 32), l);
-  return ((int64_t)hi << 32) | (uint32_t)lo;
-}
-// inclusive prefix sum over a wave
-__device__ __forceinline__ int64_t scan64(int64_t x) {
+__device__ __forceinline__ int scan(int x) {   // inclusive, over a wave
   const int l = lane_id();
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const int64_t y = shfl_up64(x, o);
+    const int y = __shfl_up(x, o);
     if (l >= o) x += y;
   }
   return x;
 }
-// all units of the call, by a wave
-__device__ __forceinline__ int64_t all_units(const AF& p, int BM, int unit) {
-  int64_t c = 0;
-  for (int b = lane_id(); b < p.B; b += 64) c += head_units(p, span_of(p, b), BM, unit) * p.Hkv;
-  return shfl64(scan64(c), 63);
-}
-// the task that holds unit u < C (of task number u of the tasks, if by_task), by a wave
-template <bool BY_TASK>
-__device__ __forceinline__ bool find_task(const AF& p, int64_t u, int BM, int unit, Task& t) {
-  int64_t before = 0, ubefore = 0;
-  for (int b0 = 0; b0 < p.B; b0 += 64) {
-    const int b = b0 + lane_id();
-    Span s{0, 0, 0};
-    if (b < p.B) s = span_of(p, b);
-    const int64_t mine = b < p.B ? head_units(p, s, BM, unit) * p.Hkv : 0;
-    const int64_t us = scan64(mine);
-    const int64_t tasks = (int64_t)((s.n * p.G + BM - 1) / BM) * p.Hkv;
-    const int64_t sum = BY_TASK ? scan64(tasks) : us;
-    const unsigned long long hit = __ballot(before + sum > u);
-    if (hit) {
-      const int w = __builtin_ctzll(hit);
-      t.b = b0 + w;
-      t.s.c0 = __builtin_amdgcn_readfirstlane(__shfl(s.c0, w));
-      t.s.n = __builtin_amdgcn_readfirstlane(__shfl(s.n, w));
-      t.s.len = __builtin_amdgcn_readfirstlane(__shfl(s.len, w));
-      const int64_t per = shfl64(mine, w) / p.Hkv;   // units of a head
-      const int rows = t.s.n * p.G, tiles = (rows + BM - 1) / BM;
-      t.first = ubefore + shfl64(us - mine, w);
-      if (BY_TASK) {
-        const int64_t k = u - before - shfl64(sum - tasks, w);
-        t.h = (int)(k / tiles);
-        t.m = (int)(k % tiles);
-      } else {
-        t.h = (int)((u - t.first) / per);
-        t.m = 0;
-      }
-      t.first += t.h * per;
-      for (int m = 0;; ++m) {   // (one tile in all but ragged calls)
-        int u0, u1;
-        units_of(p, t.s, m * BM, min((m + 1) * BM, rows), unit, u0, u1);
-        t.units = u1 - u0;
-        if (BY_TASK ? m == t.m : u < t.first + t.units) {
-          t.m = m;
-          break;
-        }
-        t.first += t.units;
-      }
-      return true;
+struct Plan {
+  const AF& p;
+  int BM, unit;
+  Span s0;       // of sequence `lane`
+  int mine0, sum0;   // its units over all heads, and with those before it
+  int C;         // units of the call
+  __device__ __forceinline__ Plan(const AF& p_, int BM_, int unit_) : p(p_), BM(BM_), unit(unit_) {
+    load(0, s0, mine0);
+    sum0 = scan(mine0);
+    C = __builtin_amdgcn_readfirstlane(__shfl(sum0, 63));
+    for (int b0 = 64; b0 < p.B; b0 += 64) {
+      Span s;
+      int mine;
+      load(b0, s, mine);
+      C += __builtin_amdgcn_readfirstlane(__shfl(scan(mine), 63));
     }
-    before += shfl64(sum, 63);
-    ubefore += shfl64(us, 63);
   }
-  return false;
-}
+  __device__ __forceinline__ void load(int b0, Span& s, int& mine) const {
+    const int b = b0 + lane_id();
+    s = {0, 0, 0};
+    mine = 0;
+    if (b >= p.B) return;
+    s = span_of(p, b);
+    const int rows = s.n * p.G;
+    for (int r = 0; r < rows; r += BM) {
+      int u0, u1;
+      units_of(p, s, r, min(r + BM, rows), unit, u0, u1);
+      mine += u1 - u0;
+    }
+    mine *= p.Hkv;
+  }
+  // The sequence whose lane says so in hit(span, units before and with it), its
+  // span and the units before it.
+  template <class Hit> __device__ __forceinline__ bool find(Hit hit, Task& t, int& per) const {
+    Span s = s0;
+    int mine = mine0, sum = sum0, before = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+      if (b0) {
+        before += __builtin_amdgcn_readfirstlane(__shfl(sum, 63));
+        load(b0, s, mine);
+        sum = scan(mine);
+      }
+      const unsigned long long in = __ballot(mine > 0 && hit(s, before + sum));
+      if (in) {
+        const int w = __builtin_ctzll(in);
+        t.b = b0 + w;
+        t.s.c0 = __builtin_amdgcn_readfirstlane(__shfl(s.c0, w));
+        t.s.n = __builtin_amdgcn_readfirstlane(__shfl(s.n, w));
+        t.s.len = __builtin_amdgcn_readfirstlane(__shfl(s.len, w));
+        per = __builtin_amdgcn_readfirstlane(__shfl(mine, w)) / p.Hkv;
+        t.first = before + __builtin_amdgcn_readfirstlane(__shfl(sum - mine, w));
+        return true;
+      }
+    }
+    return false;
+  }
+  __device__ __forceinline__ int tile_units(const Task& t, int m) const {
+    int u0, u1;
+    const int rows = t.s.n * p.G;
+    units_of(p, t.s, m * BM, min((m + 1) * BM, rows), unit, u0, u1);
+    return u1 - u0;
+  }
+  // the task that holds unit u < C
+  __device__ __forceinline__ bool of_unit(int u, Task& t) const {
+    int per;
+    if (!find([&](const Span&, int sum) { return sum > u; }, t, per)) return false;
+    t.h = (u - t.first) / per;
+    t.first += t.h * per;
+    for (t.m = 0;; ++t.m) {   // (one tile in all but ragged calls)
+      t.units = tile_units(t, t.m);
+      if (u < t.first + t.units) return true;
+      t.first += t.units;
+    }
+  }
+  // the task of new token i's row for query head hq, and the row
+  __device__ __forceinline__ bool of_row(int i, int hq, Task& t, int& row) const {
+    int per;
+    if (!find([&](const Span& s, int) { return s.c0 + s.n > i && s.c0 <= i; }, t, per)) return false;
+    t.h = hq / p.G;
+    row = (i - t.s.c0) * p.G + hq - t.h * p.G;
+    t.m = row / BM;
+    t.first += t.h * per;
+    for (int m = 0; m < t.m; ++m) t.first += tile_units(t, m);
+    t.units = tile_units(t, t.m);
+    return true;
+  }
+};
 
 // Attention over many rows per sequence (training, prompts): head dimension and
 // type checked by the caller.
