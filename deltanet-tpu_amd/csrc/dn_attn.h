@@ -156,15 +156,12 @@ template <class T, int D, int ROWS> struct Tile {
   // row's first channel in memory.  A load fills 1 KB of LDS in lane order, each
   // lane from its own address; a lane has the same row in all of them.
   template <int NW, class Row> static __device__ __forceinline__ void load(T* t, int w, Row at) {
-    constexpr int groups = ROWS / kLoad, n = groups * (D / 32) / NW;
-    static_assert(n * NW == groups * (D / 32) && (NW % groups == 0 || groups % NW == 0), "whole loads");
-    const int l = lane_id();
+    constexpr int groups = ROWS / kLoad;
+    static_assert(groups * (D / 32) % NW == 0 && (NW % groups == 0 || groups % NW == 0), "whole loads");
     if constexpr (NW % groups == 0) {
-      const int g = w % groups, row = g * kLoad + l / kPieces;
-      const T* s = at(row) + piece(row, l % kPieces) * kPer;
-#pragma unroll
-      for (int i = 0; i < n; ++i) copy(s + (w / groups + i * (NW / groups)) * 32, t + (w / groups + i * (NW / groups)) * kSlab + g * kLoad * 32);
+      load_part<NW, 0, 1>(t, w, source<NW>(w, at));
     } else {
+      const int l = lane_id();
 #pragma unroll
       for (int j = 0; j < groups / NW; ++j) {
         const int g = w + j * NW, row = g * kLoad + l / kPieces;
@@ -172,6 +169,21 @@ template <class T, int D, int ROWS> struct Tile {
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) copy(s + i * 32, t + i * kSlab + g * kLoad * 32);
       }
+    }
+  }
+  // The same in parts, for NW a multiple of the groups of rows: where the lane
+  // reads, and part PART of PARTS of the wave's loads.
+  template <int NW, class Row> static __device__ __forceinline__ const T* source(int w, Row at) {
+    const int row = w % (ROWS / kLoad) * kLoad + lane_id() / kPieces;
+    return at(row) + piece(row, lane_id() % kPieces) * kPer;
+  }
+  template <int NW, int PART, int PARTS> static __device__ __forceinline__ void load_part(T* t, int w, const T* s) {
+    constexpr int groups = ROWS / kLoad, n = groups * (D / 32) / NW;
+    static_assert(NW % groups == 0 && n * NW == groups * (D / 32), "whole loads");
+#pragma unroll
+    for (int i = n * PART / PARTS; i < n * (PART + 1) / PARTS; ++i) {
+      const int slab = w / groups + i * (NW / groups);
+      copy(s + slab * 32, t + slab * kSlab + w % groups * kLoad * 32);
     }
   }
   static __device__ __forceinline__ void copy(const T* s, T* d) {

@@ -84,10 +84,29 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn(const 
     }
     mx[i] = pos[i] < 0 ? 0.f : sum_q(x) * p.sc + kShift;
   }
-  auto fetch = [&](int j) {
-    T* t = lds + (j & 1) * 2 * BN * D;
-    TL::template load<NW>(t, w, [&](int x) { return kr(j * BN + x); });
-    TL::template load<NW>(t + BN * D, w, [&](int x) { return vr(j * BN + x); });
+  // At D = 256 a tile's loads go out in four parts between the products of the
+  // tile before it: all at once they fill the memory queue, and the waves wait to
+  // issue (600 to 1600 of 5700 clocks per tile; 893 us for 2 x 4096 tokens over
+  // 8192, 1008 otherwise).  At 128 that costs registers that are not there (773 us
+  // for 2 x 8192, 580 otherwise).
+  constexpr bool SPREAD = D == 256 && BN == 64;
+  const T *ks = nullptr, *vs = nullptr;
+  T* to = nullptr;
+  auto aim = [&](int j) {
+    ks = TL::template source<NW>(w, [&](int x) { return kr(j * BN + x); });
+    vs = TL::template source<NW>(w, [&](int x) { return vr(j * BN + x); });
+    to = lds + (j & 1) * 2 * BN * D;
+  };
+  auto fetch = [&](auto part) {
+    constexpr int P = decltype(part)::value;
+    if constexpr (P < 2) TL::template load_part<NW, P, 2>(to, w, ks);
+    else TL::template load_part<NW, P - 2, 2>(to + BN * D, w, vs);
+  };
+  auto fetch_all = [&] {
+    fetch(std::integral_constant<int, 0>{});
+    fetch(std::integral_constant<int, 1>{});
+    fetch(std::integral_constant<int, 2>{});
+    fetch(std::integral_constant<int, 3>{});
   };
   bool odd = false;   // infinities or NaNs in a masked tile were left out
   // 32 keys of a tile; MASKED: some query must not see some of them.  At D = 256
@@ -98,7 +117,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn(const 
   auto in_order = [] {
     if constexpr (D == 256) __builtin_amdgcn_sched_barrier(0);
   };
-  auto step = [&](auto masked, const T* kt, const T* vt, int key0) {
+  auto step = [&](auto masked, auto between, const T* kt, const T* vt, int key0) {
     constexpr bool MASKED = decltype(masked)::value;
     f32x4 sc[NQ][2];
 #pragma unroll
@@ -136,6 +155,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn(const 
         }
       pf[i] = frag8<T>(sc[i][0], sc[i][1]);
     }
+    between();
     const bool bad = MASKED && TL::odd32(vt);
     if (MASKED) odd |= bad;
 #pragma unroll
@@ -161,19 +181,30 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn(const 
 #pragma unroll
       for (int c = 0; c < NC; ++c) o[i][c] = zero4();
     }
-    if (j0 < j1) fetch(j0);
+    if (j0 < j1) {
+      aim(j0);
+      fetch_all();
+    }
 #pragma unroll 1
     for (int j = j0; j < j1; ++j) {
       loads_barrier();   // tile j is there, tile j - 1 is no longer read
-      if (j + 1 < j1) fetch(j + 1);
+      const bool more = j + 1 < j1;
+      if (more) aim(j + 1);
+      if (!SPREAD && more) fetch_all();
       const T* kt = lds + (j & 1) * 2 * BN * D;
       const T* vt = kt + BN * D;
       if (j * BN + BN - 1 > p0 || j * BN < lo1) {
+        if (SPREAD && more) fetch_all();
 #pragma unroll 1
-        for (int u = 0; u < BN; u += 32) step(std::true_type{}, kt + u * 32, vt + u * 32, j * BN + u);
+        for (int u = 0; u < BN; u += 32) step(std::true_type{}, [] {}, kt + u * 32, vt + u * 32, j * BN + u);
+      } else if constexpr (SPREAD) {
+        if (more) fetch(std::integral_constant<int, 0>{});
+        step(std::false_type{}, [&] { if (more) fetch(std::integral_constant<int, 1>{}); }, kt, vt, j * BN);
+        if (more) fetch(std::integral_constant<int, 2>{});
+        step(std::false_type{}, [&] { if (more) fetch(std::integral_constant<int, 3>{}); }, kt + 32 * 32, vt + 32 * 32, j * BN + 32);
       } else {
 #pragma unroll
-        for (int u = 0; u < BN; u += 32) step(std::false_type{}, kt + u * 32, vt + u * 32, j * BN + u);
+        for (int u = 0; u < BN; u += 32) step(std::false_type{}, [] {}, kt + u * 32, vt + u * 32, j * BN + u);
       }
     }
     bool over = false;
