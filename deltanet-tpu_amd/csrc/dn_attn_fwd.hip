@@ -6,16 +6,20 @@
 namespace dn {
 namespace {
 
-// One workgroup: NW waves of 16 NQ query rows each over one head's keys.
-template <class T, int D, int NQ, int NW, int BN, bool PAGED>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn(const AF p) {
+// One workgroup: NW waves of 16 NQ query rows each over one head's keys, KG times:
+// with KG = 2 a second set of waves takes every other tile of keys, and the sums,
+// which have the same reference, are added at the end.
+template <class T, int D, int NQ, int NW, int KG, int BN, bool PAGED>
+__global__ __launch_bounds__(64 * NW * KG, sizeof(T) == 2 ? 2 : 1) void k_attn(const AF p) {
   using TL = Tile<T, D, BN>;
   using F = typename At<T>::F;
   constexpr int BM = 16 * NQ * NW, NS = D / 32, NC = D / 16;
-  __shared__ __align__(16) T lds[4 * BN * D];   // [2][K, V][BN][D]
+  __shared__ __align__(16) T smem[KG * 4 * BN * D];   // [KG][2][K, V][BN][D]; at the end the other waves' sums
+  __shared__ float s_top[KG][BM], s_sum[KG][BM];
 
   const int l = lane_id(), r = l & 15, q = l >> 4;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave % NW, kg = wave / NW;
+  T* lds = smem + kg * 4 * BN * D;
 
   // head innermost, then the tiles of all sequences, the last (longest) first
   const int nt = gridDim.x / p.Hkv;
@@ -95,7 +99,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn(const 
   auto aim = [&](int j) {
     ks = TL::template source<NW>(w, [&](int x) { return kr(j * BN + x); });
     vs = TL::template source<NW>(w, [&](int x) { return vr(j * BN + x); });
-    to = lds + (j & 1) * 2 * BN * D;
+    to = lds + ((j - j0) / KG & 1) * 2 * BN * D;
   };
   auto fetch = [&](auto part) {
     constexpr int P = decltype(part)::value;
@@ -181,17 +185,19 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn(const 
 #pragma unroll
       for (int c = 0; c < NC; ++c) o[i][c] = zero4();
     }
-    if (j0 < j1) {
-      aim(j0);
+    if (j0 + kg < j1) {
+      aim(j0 + kg);
       fetch_all();
     }
 #pragma unroll 1
-    for (int j = j0; j < j1; ++j) {
-      loads_barrier();   // tile j is there, tile j - 1 is no longer read
-      const bool more = j + 1 < j1;
-      if (more) aim(j + 1);
+    for (int jj = j0; jj < j1; jj += KG) {
+      loads_barrier();   // the tiles are there, those before them no longer read
+      const int j = jj + kg;
+      if (KG > 1 && j >= j1) continue;
+      const bool more = j + KG < j1;
+      if (more) aim(j + KG);
       if (!SPREAD && more) fetch_all();
-      const T* kt = lds + (j & 1) * 2 * BN * D;
+      const T* kt = lds + ((j - j0) / KG & 1) * 2 * BN * D;
       const T* vt = kt + BN * D;
       if (j * BN + BN - 1 > p0 || j * BN < lo1) {
         if (SPREAD && more) fetch_all();
@@ -212,16 +218,46 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn(const 
     for (int i = 0; i < NQ; ++i) {
       top[i] = max_q(top[i]) * p.sc;
       over |= top[i] > mx[i] + kRange;
+      if (KG > 1 && q == 0) s_top[kg][(w * NQ + i) * 16 + r] = top[i];
     }
     if (pass == 1 || !__syncthreads_or(over)) break;
 #pragma unroll
-    for (int i = 0; i < NQ; ++i) mx[i] = top[i] > mx[i] + kRange ? top[i] : mx[i];   // (the other rows keep their bits)
+    for (int i = 0; i < NQ; ++i) {
+#pragma unroll
+      for (int g = 0; g < KG; ++g)
+        if (KG > 1) top[i] = fmaxf(top[i], s_top[g][(w * NQ + i) * 16 + r]);
+      mx[i] = top[i] > mx[i] + kRange ? top[i] : mx[i];   // (the other rows keep their bits)
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < NQ; ++i) sum[i] = sum_q(sum[i]);
+  if constexpr (KG > 1) {   // (2: the second set hands its sums over)
+    static_assert(KG == 2 && BM * D * 4 <= sizeof(smem), "room for one set of sums");
+    f32x4* os = reinterpret_cast<f32x4*>(smem) + w * NQ * NC * 64 + l;
+    odd = __syncthreads_or(odd);   // (and nobody reads a tile any more)
+    if (kg) {
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) {
+        if (q == 0) s_sum[1][(w * NQ + i) * 16 + r] = sum[i];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) os[(i * NC + c) * 64] = o[i][c];
+      }
+    }
+    __syncthreads();
+    if (kg) return;
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+      sum[i] += s_sum[1][(w * NQ + i) * 16 + r];
+#pragma unroll
+      for (int c = 0; c < NC; ++c) o[i][c] += os[(i * NC + c) * 64];
+    }
   }
 
 #pragma unroll
   for (int i = 0; i < NQ; ++i) {
     const int row = row0 + (w * NQ + i) * 16 + r;
-    const float z = sum_q(sum[i]);
+    const float z = sum[i];
     if (row >= rows) continue;
     const int t = row / p.G, g = row - t * p.G;
     const int64_t at = (int64_t)(s.c0 + t) * p.Hkv * p.G + h * p.G + g;
@@ -253,18 +289,34 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn(const 
   }
 }
 
+// rows are whole tiles per sequence: at most one more tile each
+int64_t tiles_of(const AF& p, int BM) {
+  return p.cu ? (int64_t)p.N * p.G / BM + p.B : (int64_t)p.B * (((int64_t)p.T * p.G + BM - 1) / BM);
+}
+
 template <class T, int D, bool PAGED> hipError_t run(const AF& p, hipStream_t st) {
   // 32 query rows per wave read each LDS operand for two products; at D = 256
   // their sums leave no room for two waves on a SIMD, and 16 rows are faster.
   // D = 128: four waves, two workgroups on a CU (601 us at 2 x 8192; eight waves
   // around one copy of the keys 666, 64 rows per wave 869, 16 rows 793).  D = 256:
-  // eight waves of 16 rows (1006 us; 32 rows 1687, four waves and tiles of 32 keys
-  // 1103).
-  constexpr int NQ = sizeof(T) == 4 || D < 256 ? 2 : 1, NW = sizeof(T) == 4 || D < 256 ? 4 : 8, BN = sizeof(T) == 4 ? 32 : 64;
-  constexpr int BM = 16 * NQ * NW;
-  // rows are whole tiles per sequence: at most one more tile each
-  const int64_t tiles = p.cu ? (int64_t)p.N * p.G / BM + p.B : (int64_t)p.B * (((int64_t)p.T * p.G + BM - 1) / BM);
-  hipLaunchKernelGGL((k_attn<T, D, NQ, NW, BN, PAGED>), dim3((unsigned)(tiles * p.Hkv)), dim3(64 * NW), 0, st, p);
+  // eight waves of 16 rows (1006 us for 2 x 4096 over 8192; 32 rows 1687, four waves
+  // and tiles of 32 keys 1103).
+  constexpr bool f32 = sizeof(T) == 4;
+  constexpr int NQ = f32 || D < 256 ? 2 : 1, NW = f32 || D < 256 ? 4 : 8, BN = f32 ? 32 : 64;
+  const int64_t tiles = tiles_of(p, 16 * NQ * NW) * p.Hkv;
+  // With few tiles of a long walk over the keys the longest walk is what takes the
+  // time: tiles of 64 rows, two sets of waves on every other tile of keys.  us, this
+  // form / the other, 16 query and 4 key heads: bf16 D = 128 20 / 30 (1024 tokens, 128
+  // tiles), 39 / 53 (2048, 256 tiles), 82 / 80 (3104, 388), but 23 / 20 (4 x 512, 256);
+  // D = 256 37 / 43, 74 / 81, 160 / 119, 41 / 31; float32 D = 128 179 / 317 (2048), 416 /
+  // 475 (3104), 206 / 285 (4 x 1024, 512), 85 / 87 (4 x 512).
+  const int64_t walk = std::min<int64_t>(PAGED ? (int64_t)p.max_pages << p.shift : p.T, p.window ? p.window : INT64_MAX);
+  if (f32 ? tiles <= 512 : tiles <= 128 || (tiles <= 256 && walk >= 1024)) {
+    constexpr int SQ = 1, SW = 4, SG = f32 && D == 256 ? 1 : 2, SN = f32 || D == 256 ? 32 : 64;
+    hipLaunchKernelGGL((k_attn<T, D, SQ, SW, SG, SN, PAGED>), dim3((unsigned)(tiles_of(p, 16 * SQ * SW) * p.Hkv)), dim3(64 * SW * SG), 0, st, p);
+  } else {
+    hipLaunchKernelGGL((k_attn<T, D, NQ, NW, 1, BN, PAGED>), dim3((unsigned)tiles), dim3(64 * NW), 0, st, p);
+  }
   return hipGetLastError();
 }
 
