@@ -25,16 +25,35 @@ __all__ = ["rotary_table", "apply_rotary", "paged_kv_append", "paged_attention",
 _INT = {torch.int32: _lib.DN_I32, torch.int64: _lib.DN_I64}
 
 
+_current = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_calls = _lib._packed_calls
+
+
 def _call(name, dev, block, *args):
     """An entry point on the current stream of GPU `dev`."""
-    f = _lib.packed_call(name)
-    if dev == torch.cuda.current_device():
+    f = _calls.get(name) or _lib.packed_call(name)
+    if dev == _current():
         rc = f(block, *args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
             rc = f(block, *args, _raw_stream(dev))
     if rc:
         _lib.check(rc, name)
+
+
+def _on_gpu(*ts):
+    """The index of the GPU that all of them (None aside) are on; the message of
+    ``_require_gpu`` otherwise."""
+    try:
+        dev = ts[0].get_device()
+        for t in ts:
+            if t is not None and t.get_device() != dev:
+                dev = -1
+        if dev >= 0:
+            return dev
+    except AttributeError:
+        pass
+    return _require_gpu(*ts).index
 
 
 def _dense_channels(t):
@@ -114,12 +133,12 @@ def _check_table(table, D):
 
 def _rotary_launch(q, k, pos, ps, table, interleaved, inverse):
     B, L, Hq, D = q.shape
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    q_out = q.new_empty(q.shape)
     sq = q.stride()
     if k is None:
         Hk, sk, kp, ko, k_out = 0, (0, 0, 0), 0, 0, None
     else:
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        k_out = k.new_empty(k.shape)
         Hk, sk, kp, ko = k.shape[2], k.stride(), k.data_ptr(), k_out.data_ptr()
     block = _lib.ROTARY_PACK(_lib.DN_ABI_VERSION, B, L, Hq, Hk, D, table.shape[1], _DT[q.dtype], _INT[pos.dtype],
                              1 if interleaved else 0, 1 if inverse else 0, table.shape[0], q.data_ptr(), kp, q_out.data_ptr(),
@@ -174,7 +193,7 @@ def apply_rotary(q, k, positions, table, *, interleaved: bool = False):
     _check_table(table, q.shape[-1])
     if positions.dtype not in _INT:
         raise ValueError(f"positions must be int32 or int64, got {positions.dtype}.")
-    _require_gpu(q, k, positions, table)
+    _on_gpu(q, k, positions, table)
     lead = q.shape[:-2]
     if positions.shape == lead:
         ps = positions.stride()
@@ -200,11 +219,16 @@ def apply_rotary(q, k, positions, table, *, interleaved: bool = False):
 # paged cache
 # ---------------------------------------------------------------------------
 
-def _check_cache(name, c):
-    if c.ndim != 4 or c.dtype not in _DT:
-        raise ValueError(f"{name} must be a float32, bfloat16 or float16 tensor (pages, page_size, Hkv, D), got {c.dtype} {tuple(c.shape)}.")
-    if c.stride(-1) != 1:
-        raise ValueError(f"{name} must have contiguous channels, got strides {c.stride()}.")
+def _check_caches(k_cache, v_cache):
+    shape = k_cache.shape
+    for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if c.ndim != 4 or c.dtype not in _DT:
+            raise ValueError(f"{name} must be a float32, bfloat16 or float16 tensor (pages, page_size, Hkv, D), got {c.dtype} {tuple(c.shape)}.")
+        if c.stride(-1) != 1:
+            raise ValueError(f"{name} must have contiguous channels, got strides {c.stride()}.")
+    if v_cache.shape != shape or v_cache.dtype is not k_cache.dtype:
+        raise ValueError(f"v_cache {tuple(v_cache.shape)} {v_cache.dtype} must match k_cache {tuple(shape)} {k_cache.dtype}.")
+    return shape
 
 
 def _check_pages(page_table, seq_lens, cu_seqlens, x, name):
@@ -246,18 +270,14 @@ def paged_kv_append(k, v, k_cache, v_cache, page_table, seq_lens, *, cu_seqlens=
     position outside ``table`` stores NaN in the rotated channels.  Pages that are
     written must not be shared.  Returns (k_cache, v_cache).
     """
-    _check_cache("k_cache", k_cache)
-    _check_cache("v_cache", v_cache)
-    if v_cache.shape != k_cache.shape or v_cache.dtype is not k_cache.dtype:
-        raise ValueError(f"v_cache {tuple(v_cache.shape)} {v_cache.dtype} must match k_cache {tuple(k_cache.shape)} {k_cache.dtype}.")
-    pages, page, H, D = k_cache.shape
+    pages, page, H, D = _check_caches(k_cache, v_cache)
     if page < 1 or page & (page - 1):
         raise ValueError(f"page_size must be a power of two, got {page}.")
     if k.dtype not in _DT or v.dtype is not k.dtype or v.shape != k.shape:
         raise ValueError(f"k and v must be of one shape and float32, bfloat16 or float16, got {tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}.")
     if k.shape[-2:] != (H, D):
         raise ValueError(f"k {tuple(k.shape)} must have the cache's heads and channels ({H}, {D}).")
-    _require_gpu(k, v, k_cache, v_cache, page_table, seq_lens, cu_seqlens, table)
+    dev = _on_gpu(k, v, k_cache, v_cache, page_table, seq_lens, cu_seqlens, table)
     k, v = _dense_channels(k), _dense_channels(v)
     B, N, ksb, kst = _check_pages(page_table, seq_lens, cu_seqlens, k, "k")
     R = _check_table(table, D) if table is not None else 0
@@ -271,7 +291,7 @@ def paged_kv_append(k, v, k_cache, v_cache, page_table, seq_lens, *, cu_seqlens=
             page_table.data_ptr(), seq_lens.data_ptr(), 0 if cu_seqlens is None else cu_seqlens.data_ptr(),
             table.data_ptr() if R else 0, ksb, kst, k.stride(-2), vs[0], vs[0] if v.ndim == 3 else vs[1], vs[-2],
             kcs[0], kcs[1], kcs[2], vcs[0], vcs[1], vcs[2], page_table.stride(0))
-        _call("dn_kv_append", k.get_device(), block)
+        _call("dn_kv_append", dev, block)
     return k_cache, v_cache
 
 
@@ -281,8 +301,8 @@ def paged_kv_append(k, v, k_cache, v_cache, page_table, seq_lens, *, cu_seqlens=
 
 def _rows16(t):
     """A tensor whose rows of channels start on 16 bytes, as the kernels read them."""
-    per = 16 // t.element_size()
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % per == 0 for s in t.stride()[:-1]):
+    s, per = t.stride(), 16 // t.element_size()
+    if s[-1] == 1 and t.data_ptr() % 16 == 0 and not any(x % per for x in s[:-1]):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -322,16 +342,12 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, *, cu_seqlens=Non
     the output in q's shape and type, and with ``return_lse`` also the log of the
     sum of exponentials (float32, q's shape without D).
     """
-    _check_cache("k_cache", k_cache)
-    _check_cache("v_cache", v_cache)
-    if v_cache.shape != k_cache.shape or v_cache.dtype is not k_cache.dtype:
-        raise ValueError(f"v_cache {tuple(v_cache.shape)} {v_cache.dtype} must match k_cache {tuple(k_cache.shape)} {k_cache.dtype}.")
-    pages, page, Hkv, D = k_cache.shape
+    pages, page, Hkv, D = _check_caches(k_cache, v_cache)
     if page < 1 or page & (page - 1) or pages < 1:
         raise ValueError(f"page_size must be a power of two and the cache have a page, got {tuple(k_cache.shape)}.")
     if q.dtype is not k_cache.dtype or q.shape[-1] != D:
         raise ValueError(f"q {tuple(q.shape)} {q.dtype} must have the cache's channels and type ({D}, {k_cache.dtype}).")
-    _require_gpu(q, k_cache, v_cache, page_table, seq_lens, cu_seqlens)
+    dev = _on_gpu(q, k_cache, v_cache, page_table, seq_lens, cu_seqlens)
     if torch.is_grad_enabled() and q.requires_grad:
         raise ValueError("paged_attention is not differentiable; use causal_attention for training.")
     q = _rows16(q)
@@ -341,7 +357,7 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, *, cu_seqlens=Non
     kcs, vcs = k_cache.stride(), v_cache.stride()
     if page_table.shape[1] < 1:
         raise ValueError("page_table must have a column.")
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = q.new_empty(q.shape)
     lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device) if return_lse else None
     block = _lib.PAGED_ATTENTION_PACK(
         _lib.DN_ABI_VERSION, N, B, Hq, Hkv, D, _DT[q.dtype], window or 0, pages, page, page_table.shape[1], scale,
@@ -349,15 +365,15 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, *, cu_seqlens=Non
         page_table.data_ptr(), seq_lens.data_ptr(), 0 if cu_seqlens is None else cu_seqlens.data_ptr(),
         qsb, qst, q.stride(-2), kcs[0], kcs[1], kcs[2], vcs[0], vcs[1], vcs[2], page_table.stride(0))
     if N:
-        need = _lib.packed_call("dn_paged_attention_workspace_size")(block)
-        ws = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None
-        _call("dn_paged_attention", q.get_device(), block, 0 if ws is None else ws.data_ptr(), need)
+        need = (_calls.get("dn_paged_attention_workspace_size") or _lib.packed_call("dn_paged_attention_workspace_size"))(block)
+        ws = q.new_empty(-(-need // q.element_size())) if need else None
+        _call("dn_paged_attention", dev, block, 0 if ws is None else ws.data_ptr(), need)
     return (out, lse) if return_lse else out
 
 
 def _document_starts(segment_ids, cu_seqlens, B, L, dev):
-    """(B, L) int32 first token of each token's document, or None for one document
-    (checks and messages as in ``chunk_gdn2``)."""
+    """(B, L) int32 first token of each token's document (checks and messages as in
+    ``chunk_gdn2``)."""
     if segment_ids is not None and cu_seqlens is not None:
         raise ValueError("Cannot pass both segment_ids and cu_seqlens; specify at most one.")
     if segment_ids is not None:
@@ -374,7 +390,7 @@ def _document_starts(segment_ids, cu_seqlens, B, L, dev):
             raise ValueError(f"segment_ids must be 1D (L,) or 2D (B, L), got rank {seg.ndim} with shape {tuple(seg.shape)}.")
         if seg.dtype not in _INT:
             seg = seg.to(torch.int64)
-    elif cu_seqlens is not None:
+    else:
         cu = cu_seqlens.detach().cpu().numpy() if isinstance(cu_seqlens, torch.Tensor) else np.asarray(cu_seqlens)
         if len(cu) == 0 or int(cu[0]) != 0:
             raise ValueError(f"cu_seqlens[0] must be 0, got {cu[0] if len(cu) else 'empty'}.")
@@ -384,8 +400,6 @@ def _document_starts(segment_ids, cu_seqlens, B, L, dev):
         if len(lens) > 0 and np.any(lens <= 0):
             raise ValueError(f"cu_seqlens must be strictly monotonically increasing, got {cu_seqlens}.")
         seg = torch.from_numpy(np.repeat(np.arange(len(lens), dtype=np.int32), lens))
-    else:
-        return None
     seg = seg.to(dev).contiguous()
     starts = torch.empty((B, L), dtype=torch.int32, device=dev)
     with torch.cuda.device(dev):
@@ -404,8 +418,8 @@ def _attention_block(q, k, v, out, low, lse, starts, scale, window):
 
 
 def _attention_forward(q, k, v, starts, scale, window, want_lse, want_low=False):
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    low = torch.empty(q.shape, dtype=q.dtype, device=q.device) if want_low else None
+    out = q.new_empty(q.shape)
+    low = q.new_empty(q.shape) if want_low else None
     lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device) if want_lse else None
     if q.numel():
         _call("dn_attention_fwd", q.get_device(), _attention_block(q, k, v, out, low, lse, starts, scale, window))
@@ -433,11 +447,11 @@ class _AttentionFn(torch.autograd.Function):
         if d_out is None:
             return (None,) * 6
         d_out = d_out.contiguous()
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
         if q.numel():
             block = _attention_block(q, k, v, out, low, lse, starts, scale, window)
             need = _lib.packed_call("dn_attention_bwd_workspace_size")(block)
-            ws = torch.empty((need,), dtype=torch.uint8, device=q.device)
+            ws = q.new_empty(-(-need // q.element_size()))
             _call("dn_attention_bwd", q.get_device(), block, d_out.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                   ws.data_ptr(), need)
         return dq, dk, dv, None, None, None
@@ -466,8 +480,10 @@ def causal_attention(q, k, v, *, segment_ids=None, cu_seqlens=None, scale=None, 
     if k.dtype is not q.dtype or v.dtype is not q.dtype:
         raise ValueError(f"q, k and v must be of one type, got {q.dtype}, {k.dtype} and {v.dtype}.")
     scale = _attention_common(D, Hq, k.shape[2], q.dtype, scale, window)
-    dev = _require_gpu(q, k, v, segment_ids if isinstance(segment_ids, torch.Tensor) else None)
-    starts = _document_starts(segment_ids, cu_seqlens, B, L, dev)
+    _on_gpu(q, k, v, segment_ids if isinstance(segment_ids, torch.Tensor) else None)
+    starts = None
+    if segment_ids is not None or cu_seqlens is not None:
+        starts = _document_starts(segment_ids, cu_seqlens, B, L, q.device)
     q, k, v = _rows16(q), _rows16(k), _rows16(v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out, lse = _AttentionFn.apply(q, k, v, starts, scale, window)
