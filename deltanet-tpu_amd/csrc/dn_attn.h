@@ -85,6 +85,11 @@ __device__ __forceinline__ float sum_q(float x) {
   return a + b;
 }
 
+// A use of a loaded value in front of a loop: the wait for it lands here.  Left to
+// its first use inside the loop, the wait is for every load in flight there, in
+// every trip, the next tile's just started ones included.
+template <class V> __device__ __forceinline__ void settle(V& x) { asm volatile("" : "+v"(x)); }
+
 // Waits for this wave's direct loads into LDS, then for everyone's.  (A barrier
 // alone does not cover them.)
 __device__ __forceinline__ void loads_barrier() {
@@ -186,8 +191,14 @@ template <class T, int D, int ROWS> struct Tile {
       copy(s + slab * 32, t + slab * kSlab + w % groups * kLoad * 32);
     }
   }
+  // 64 lanes x 16 bytes from s (each lane's own) to the 1 KB of LDS at d.  Written
+  // out because the compiler takes any LDS read after its builtin for a read of
+  // what that writes and waits for it, the next tile's loads in front of this
+  // tile's products; here loads_barrier() is the wait.  No register is written,
+  // and the compiler's own counts of loads in flight only err to the safe side.
   static __device__ __forceinline__ void copy(const T* s, T* d) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)s, (__attribute__((address_space(3))) void*)d, 16, 0, 0);
+    const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)d);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(s) : "m0");
   }
 };
 

@@ -70,7 +70,8 @@ int paged_params(const dn_paged_attention_args* a, AF& p) {
       !wide(a->v_cache, a->vc_strides, a->dtype, 3) || ((uintptr_t)a->out & 15))
     return bad("attention rows must start on 16 bytes");
   p.B = a->B; p.N = a->N; p.T = a->cu_seqlens ? 0 : a->B ? a->N / a->B : 0;
-  p.Hkv = a->Hkv; p.G = a->Hq / a->Hkv; p.window = a->window;
+  set_heads(p, a->Hq, a->Hkv);
+  p.window = a->window;
   p.pages = a->pages; p.max_pages = a->max_pages;
   while ((1 << p.shift) < a->page_size) ++p.shift;
   p.sc = a->scale * kLog2e;
@@ -126,7 +127,8 @@ int attention_params(const dn_attention_args* a, AF& p) {
       (((uintptr_t)a->out | (uintptr_t)a->out_low) & 15))
     return bad("attention rows must start on 16 bytes");
   p.B = a->B; p.T = a->L; p.N = a->B * a->L;
-  p.Hkv = a->Hkv; p.G = a->Hq / a->Hkv; p.window = a->window;
+  set_heads(p, a->Hq, a->Hkv);
+  p.window = a->window;
   p.sc = a->scale * kLog2e;
   p.q = a->q; p.k = a->k; p.v = a->v; p.out = a->out; p.low = a->out_low; p.lse = a->lse; p.start = a->starts;
   for (int i = 0; i < 3; ++i) { p.qs[i] = a->q_strides[i]; p.ks[i] = a->k_strides[i]; p.vs[i] = a->v_strides[i]; }

@@ -41,14 +41,15 @@ template <class T> struct QRows {
   const T *q, *g;       // q and d_out of the sequence and key head
   int64_t qt, qh, gt, gh;
   int G, last;
+  const AF* f;
   __device__ __forceinline__ const T* query(int row) const {
     row = min(row, last);
-    const int t = row / G;
+    const int t = over_g(*f, row);
     return q + t * qt + (row - t * G) * qh;
   }
   __device__ __forceinline__ const T* grad(int row) const {
     row = min(row, last);
-    const int t = row / G;
+    const int t = over_g(*f, row);
     return g + t * gt + (row - t * G) * gh;
   }
 };
@@ -69,21 +70,30 @@ __device__ __forceinline__ int last_token(const int32_t* starts, int T, int k1) 
   return lo;
 }
 
-// dK and dV of 16 NK NW keys of one key head: every S-th tile of query rows from
-// the blockIdx.y-th on, of S = gridDim.y.  With S > 1 the sums go to p.part, as
+// dK and dV of 64 NK keys of one key head: every S-th tile of query rows from the
+// blockIdx.y-th on, of S = gridDim.y.  (From the last tile down, all workgroups of a
+// head reading the same rows at a time, is slower: 1658 against 1542 us at 2 x 8192,
+// though fewer reads go past L2.)  With S > 1 the sums go to p.part, as
 // floats, and are added up by k_attn_dkv_sum.
-template <class T, int D, int NK, int NW, int BQ>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && D < 256 ? 2 : 1) void k_attn_dkv(const AB p) {
+//
+// 16 NK keys belong to two waves of one SIMD: one forms S and P and sums up dV,
+// the other dP and dS, for which it takes P from the first through LDS, and dK.
+// Each holds half of the operands and sums that one wave would (two waves fit on
+// a SIMD) and reads half of the tiles' LDS.
+template <class T, int D, int NK, int BQ, int RS>
+__global__ __launch_bounds__(512, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(const AB p) {
   using TL = Tile<T, D, BQ>;
   using F = typename At<T>::F;
-  constexpr int BN = 16 * NK * NW, NS = D / 32, NC = D / 16;
+  constexpr int NW = 8, BN = 64 * NK, NS = D / 32, NC = D / 16, NE = RS / 16;   // RS: query rows of a step
   __shared__ __align__(16) T lds[4 * BQ * D];    // [2][q, d_out][BQ][D]
+  __shared__ __align__(16) f32x4 px[2][4][NK * NE * 64];  // P of a step, by its parity and the pair, as accumulators
   __shared__ __align__(16) float ls[2][BQ], de[2][BQ];   // lse * log2(e) and delta per row
   __shared__ __align__(16) int tk[2][BQ], lw[2][BQ];     // token and first visible key per row
   const AF& f = p.f;
 
   const int l = lane_id(), r = l & 15, q = l >> 4;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), pair = wave & 3;
+  const bool first = wave < 4;   // S, P, dV; the others dP, dS, dK
   // batch row and head innermost; the first keys, which most queries see, first
   const int groups = f.B * f.Hkv, gi = blockIdx.x % groups;
   const int b = gi / f.Hkv, h = gi % f.Hkv, k0 = (int)(blockIdx.x / groups) * BN;
@@ -94,18 +104,14 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && D < 256 ? 2 : 1) void k_
   if (f.window) t1 = (int)min((int64_t)t1, (int64_t)k1 + f.window - 1);
   if (starts) t1 = min(t1, __builtin_amdgcn_readfirstlane(last_token(starts, f.T, k1)));
 
-  const int key = k0 + (w * NK) * 16 + r;
-  F kf[NK][NS], vf[NK][NS];
+  const int key = k0 + pair * NK * 16 + r;
+  F own[NK][NS];   // K or V
 #pragma unroll
   for (int i = 0; i < NK; ++i) {
     const int64_t t = min(key + 16 * i, f.T - 1);
-    const T* kp = (const T*)f.k + b * f.ks[0] + t * f.ks[1] + h * f.ks[2];
-    const T* vp = (const T*)f.v + b * f.vs[0] + t * f.vs[1] + h * f.vs[2];
+    const T* s = first ? (const T*)f.k + b * f.ks[0] + t * f.ks[1] + h * f.ks[2] : (const T*)f.v + b * f.vs[0] + t * f.vs[1] + h * f.vs[2];
 #pragma unroll
-    for (int c = 0; c < NS; ++c) {
-      kf[i][c] = *reinterpret_cast<const F*>(kp + 32 * c + 8 * q);
-      vf[i][c] = *reinterpret_cast<const F*>(vp + 32 * c + 8 * q);
-    }
+    for (int c = 0; c < NS; ++c) own[i][c] = *reinterpret_cast<const F*>(s + 32 * c + 8 * q);
   }
 
   const int Hq = f.Hkv * f.G;
@@ -114,111 +120,113 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && D < 256 ? 2 : 1) void k_
   rows.qt = f.qs[1]; rows.qh = f.qs[2];
   rows.g = (const T*)p.d_out + ((int64_t)b * f.T * Hq + h * f.G) * D;
   rows.gt = (int64_t)Hq * D; rows.gh = D;
-  rows.G = f.G; rows.last = f.T * f.G - 1;
+  rows.G = f.G; rows.last = f.T * f.G - 1; rows.f = &f;
   const int S = gridDim.y;
   const int r0 = k0 * f.G / BQ + blockIdx.y, r1 = (t1 * f.G + f.G - 1) / BQ + 1;   // tiles of query rows, by S
 
-  f32x4 dk[NK][NC], dv[NK][NC];
+  f32x4 acc[NK][NC];   // dV or dK, transposed
 #pragma unroll
   for (int i = 0; i < NK; ++i)
 #pragma unroll
-    for (int c = 0; c < NC; ++c) dk[i][c] = dv[i][c] = zero4();
+    for (int c = 0; c < NC; ++c) acc[i][c] = zero4();
 
+#pragma unroll
+  for (int i = 0; i < NK; ++i)
+#pragma unroll
+    for (int c = 0; c < NS; ++c) settle(own[i][c]);
   float m_ls = 0.f, m_de = 0.f;
   int m_tk = 0, m_lw = 0, m_hi = 0;   // m_hi: first visible key of the tile's last row
   auto fetch = [&](int j, int buf) {
     T* t = lds + buf * 2 * BQ * D;
-    TL::template load<NW>(t, w, [&](int x) { return rows.query(j * BQ + x); });
-    TL::template load<NW>(t + BQ * D, w, [&](int x) { return rows.grad(j * BQ + x); });
+    TL::template load<NW>(t, wave, [&](int x) { return rows.query(j * BQ + x); });
+    TL::template load<NW>(t + BQ * D, wave, [&](int x) { return rows.grad(j * BQ + x); });
     auto low = [&](int t) {
       int x = f.window ? max(t - f.window + 1, 0) : 0;
       return starts ? max(x, starts[t]) : x;
     };
     if (threadIdx.x < BQ) {
-      const int row = j * BQ + threadIdx.x, c = min(row, rows.last), tok = c / f.G;
+      const int row = j * BQ + threadIdx.x, c = min(row, rows.last), tok = over_g(f, c);
       const int64_t at = ((int64_t)b * f.T + tok) * Hq + h * f.G + (c - tok * f.G);
       m_ls = f.lse[at] * kLog2e;
       m_de = p.delta[at];
       m_tk = row <= rows.last ? tok : -1;   // a row past the last one sees no key
       m_lw = low(tok);
     }
-    m_hi = low(min(j * BQ + BQ - 1, rows.last) / f.G);
+    m_hi = low(over_g(f, min(j * BQ + BQ - 1, rows.last)));
   };
   bool odd = false;
-  // 32 query rows of a tile; MASKED: some of them must not see some key
-  auto step = [&](auto mask, const T* qt, const T* gt, int buf, int u) {
+  // RS query rows of a tile; MASKED: some of them must not see some key.  Both
+  // waves multiply rows x by their own operand and rows y, transposed, by the result.
+  auto step = [&](auto mask, const T* x, const T* y, int buf, int u) {
     constexpr bool MASKED = decltype(mask)::value;
-    f32x4 s[NK][2], dp[NK][2];
+    f32x4 s[NK][NE];
 #pragma unroll
-    for (int i = 0; i < NK; ++i) s[i][0] = s[i][1] = dp[i][0] = dp[i][1] = zero4();
+    for (int i = 0; i < NK; ++i)
+#pragma unroll
+      for (int e = 0; e < NE; ++e) s[i][e] = zero4();
 #pragma unroll
     for (int c = 0; c < NS; ++c)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const F qf = TL::row8(qt, 16 * e + r, c, q);
-        const F gf = TL::row8(gt, 16 * e + r, c, q);
+      for (int e = 0; e < NE; ++e) {
+        const F xf = TL::row8(x, 16 * e + r, c, q);
+#pragma unroll
+        for (int i = 0; i < NK; ++i) At<T>::mma(s[i][e], xf, own[i][c]);
+      }
+    f32x4* ex = px[RS == BQ ? buf : u / RS & 1][pair] + l;
+    if (first) {
+#pragma unroll
+      for (int e = 0; e < NE; ++e) {
+        const int at = u + 16 * e + 4 * q;
+        const f32x4 lse = *reinterpret_cast<const f32x4*>(&ls[buf][at]);
 #pragma unroll
         for (int i = 0; i < NK; ++i) {
-          At<T>::mma(s[i][e], qf, kf[i][c]);
-          At<T>::mma(dp[i][e], gf, vf[i][c]);
+#pragma unroll
+          for (int z = 0; z < 4; ++z) {
+            s[i][e][z] = fast_exp2(__builtin_fmaf(s[i][e][z], f.sc, -lse[z]));
+            if (MASKED) s[i][e][z] = key + 16 * i <= tk[buf][at + z] && key + 16 * i >= lw[buf][at + z] ? s[i][e][z] : 0.f;
+          }
+          ex[(i * NE + e) * 64] = s[i][e];
         }
       }
+    }
+    lds_barrier();
+    if (!first) {
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int at = u + 16 * e + 4 * q;
-      const f32x4 lse = *reinterpret_cast<const f32x4*>(&ls[buf][at]);
-      const f32x4 del = *reinterpret_cast<const f32x4*>(&de[buf][at]);
+      for (int e = 0; e < NE; ++e) {
+        const f32x4 del = *reinterpret_cast<const f32x4*>(&de[buf][u + 16 * e + 4 * q]);
 #pragma unroll
-      for (int i = 0; i < NK; ++i)
+        for (int i = 0; i < NK; ++i) {
+          const f32x4 pr = ex[(i * NE + e) * 64];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const float pr = fast_exp2(__builtin_fmaf(s[i][e][x], f.sc, -lse[x]));
-          s[i][e][x] = pr;
-          dp[i][e][x] = pr * (dp[i][e][x] - del[x]);
-        }
-      if (MASKED) {
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int t = tk[buf][at + x], lo = lw[buf][at + x];
-#pragma unroll
-          for (int i = 0; i < NK; ++i) {
-            const bool see = key + 16 * i <= t && key + 16 * i >= lo;
-            s[i][e][x] = see ? s[i][e][x] : 0.f;
-            dp[i][e][x] = see ? dp[i][e][x] : 0.f;
+          for (int z = 0; z < 4; ++z) {
+            const float d = pr[z] * (s[i][e][z] - del[z]);
+            s[i][e][z] = MASKED && pr[z] == 0.f ? 0.f : d;   // (hidden rows of d_out may hold anything)
           }
         }
       }
     }
-    F pf[NK], df[NK];
 #pragma unroll
-    for (int i = 0; i < NK; ++i) {
-      pf[i] = frag8<T>(s[i][0], s[i][1]);
-      df[i] = frag8<T>(dp[i][0], dp[i][1]);
-    }
-    const bool bad = MASKED && (TL::odd32(qt) || TL::odd32(gt));
-    if (MASKED) odd |= bad;
+    for (int o = 0; o < RS; o += 32) {
+      F sf[NK];
 #pragma unroll
-    for (int n = 0; n < NC; n += 4) {
-      F gc[4], qc[4];
+      for (int i = 0; i < NK; ++i) sf[i] = frag8<T>(s[i][o / 16], s[i][o / 16 + 1]);
+      const T* yo = y + o * 32;
+      const bool bad = MASKED && TL::odd32(yo);
+      if (MASKED) odd |= bad;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        gc[c] = TL::col8(gt, n + c, r, q);
-        qc[c] = TL::col8(qt, n + c, r, q);
-      }
-      if (MASKED && bad) {
+      for (int n = 0; n < NC; n += 4) {
+        F yc[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          gc[c] = finite8<T>(gc[c]);
-          qc[c] = finite8<T>(qc[c]);
+        for (int c = 0; c < 4; ++c) yc[c] = TL::col8(yo, n + c, r, q);
+        if (MASKED && bad) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) yc[c] = finite8<T>(yc[c]);
         }
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < NK; ++i) At<T>::mma(acc[i][n + c], yc[c], sf[i]);
       }
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int i = 0; i < NK; ++i) {
-          At<T>::mma(dv[i][n + c], gc[c], pf[i]);
-          At<T>::mma(dk[i][n + c], qc[c], df[i]);
-        }
     }
   };
   if (r0 < r1) fetch(r0, 0);
@@ -231,20 +239,23 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && D < 256 ? 2 : 1) void k_
       tk[buf][threadIdx.x] = m_tk;
       lw[buf][threadIdx.x] = m_lw;
     }
-    const bool masked = j * BQ / f.G < k1 || m_hi > k0 || j * BQ + BQ - 1 > rows.last;
+    const bool masked = over_g(f, j * BQ) < k1 || m_hi > k0 || j * BQ + BQ - 1 > rows.last;
     loads_barrier();
     if (j + S < r1) fetch(j + S, buf ^ 1);
-    const T* qt = lds + buf * 2 * BQ * D;
-    const T* gt = qt + BQ * D;
+    const T* x = lds + buf * 2 * BQ * D + (first ? 0 : BQ * D);
+    const T* y = lds + buf * 2 * BQ * D + (first ? BQ * D : 0);
     if (masked) {
 #pragma unroll 1
-      for (int u = 0; u < BQ; u += 32) step(std::true_type{}, qt + u * 32, gt + u * 32, buf, u);
+      for (int u = 0; u < BQ; u += RS) step(std::true_type{}, x + u * 32, y + u * 32, buf, u);
     } else {
 #pragma unroll
-      for (int u = 0; u < BQ; u += 32) step(std::false_type{}, qt + u * 32, gt + u * 32, buf, u);
+      for (int u = 0; u < BQ; u += RS) step(std::false_type{}, x + u * 32, y + u * 32, buf, u);
     }
   }
 
+  const int64_t n = (int64_t)f.N * f.Hkv * D;
+  T* const dst = (T*)(first ? p.dv : p.dk);
+  float* const part = p.part + ((int64_t)blockIdx.y * 2 + (first ? 1 : 0)) * n;
 #pragma unroll
   for (int i = 0; i < NK; ++i) {
     const int t = key + 16 * i;
@@ -252,40 +263,31 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && D < 256 ? 2 : 1) void k_
     const int64_t at = (((int64_t)b * f.T + t) * f.Hkv + h) * D;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      float x[4], y[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[e] = dk[i][c][e];
-        y[e] = dv[i][c][e];
-      }
-      if (odd) {   // what the queries that see this key had left out of dV (dK of such a query is NaN by its scores)
+      float x[4] = {acc[i][c][0], acc[i][c][1], acc[i][c][2], acc[i][c][3]};
+      if (first && odd) {   // what the queries that see this key had left out of dV (dK of such a query is NaN by its scores)
 #pragma unroll 1
         for (int row = r0 * BQ; row <= min(r1 * BQ - 1, rows.last); ++row) {
-          const int tok = row / f.G;
+          const int tok = over_g(f, row);
           if ((row / BQ - r0) % S || tok < t) continue;
           int lo = f.window ? max(tok - f.window + 1, 0) : 0;
           if (starts) lo = max(lo, starts[tok]);
-          const int j = row / BQ, tl = min(j * BQ + BQ - 1, rows.last) / f.G;
+          const int j = row / BQ, tl = over_g(f, min(j * BQ + BQ - 1, rows.last));
           int hi = f.window ? max(tl - f.window + 1, 0) : 0;
           if (starts) hi = max(hi, starts[tl]);
-          if (t < lo || !(j * BQ / f.G < k1 || hi > k0 || j * BQ + BQ - 1 > rows.last)) continue;
+          if (t < lo || !(over_g(f, j * BQ) < k1 || hi > k0 || j * BQ + BQ - 1 > rows.last)) continue;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float z = (float)rows.grad(row)[16 * c + 4 * q + e];
-            if (!__builtin_isfinite(z)) y[e] += z;
+            if (!__builtin_isfinite(z)) x[e] += z;
           }
         }
       }
       if (S == 1) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] *= p.scale;
-        st4<T>((T*)p.dk + at + 16 * c + 4 * q, x);
-        st4<T>((T*)p.dv + at + 16 * c + 4 * q, y);
+        for (int e = 0; e < 4; ++e) x[e] = first ? x[e] : x[e] * p.scale;
+        st4<T>(dst + at + 16 * c + 4 * q, x);
       } else {
-        const int64_t n = (int64_t)f.N * f.Hkv * D;
-        float* part = p.part + (int64_t)blockIdx.y * 2 * n + at + 16 * c + 4 * q;
-        st4<float>(part, x);
-        st4<float>(part + n, y);
+        st4<float>(part + at + 16 * c + 4 * q, x);
       }
     }
   }
@@ -318,7 +320,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(con
   const int groups = f.B * f.Hkv, gi = blockIdx.x % groups, tiles = gridDim.x / groups;
   const int b = gi / f.Hkv, h = gi % f.Hkv, row0 = (tiles - 1 - (int)(blockIdx.x / groups)) * BM;
   const int nrow = f.T * f.G, row1 = min(row0 + BM, nrow);
-  const int p0 = row0 / f.G, p1 = (row1 - 1) / f.G;
+  const int p0 = over_g(f, row0), p1 = over_g(f, row1 - 1);
   const int32_t* starts = f.start ? f.start + (int64_t)b * f.T : nullptr;
   const int Hq = f.Hkv * f.G;
 
@@ -328,7 +330,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(con
 #pragma unroll
   for (int i = 0; i < NQ; ++i) {
     const int row = min(row0 + (w * NQ + i) * 16 + r, nrow - 1);
-    const int t = row / f.G, g = row - t * f.G;
+    const int t = over_g(f, row), g = row - t * f.G;
     const int64_t at = ((int64_t)b * f.T + t) * Hq + h * f.G + g;
     const T* qp = (const T*)f.q + b * f.qs[0] + t * f.qs[1] + (h * f.G + g) * f.qs[2];
     const T* gp = (const T*)p.d_out + at * D;
@@ -342,6 +344,17 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(con
     pos[i] = t;
     low[i] = f.window ? t - f.window + 1 : 0;
     if (starts) low[i] = max(low[i], starts[t]);
+  }
+#pragma unroll
+  for (int i = 0; i < NQ; ++i) {
+#pragma unroll
+    for (int c = 0; c < NS; ++c) {
+      settle(qf[i][c]);
+      settle(gf[i][c]);
+    }
+    settle(ls[i]);
+    settle(de[i]);
+    settle(low[i]);
   }
   int lo0 = f.window ? max(p0 - f.window + 1, 0) : 0, lo1 = f.window ? p1 - f.window + 1 : 0;
   if (starts) {
@@ -437,7 +450,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(con
   for (int i = 0; i < NQ; ++i) {
     const int row = row0 + (w * NQ + i) * 16 + r;
     if (row >= nrow) continue;
-    const int t = row / f.G, g = row - t * f.G;
+    const int t = over_g(f, row), g = row - t * f.G;
     T* op = (T*)p.dq + (((int64_t)b * f.T + t) * Hq + h * f.G + g) * D;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
@@ -448,14 +461,12 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(con
 }
 
 template <class T, int D> struct Shape {
-  // dkv: 16 keys per wave and two waves on a SIMD (2 x 8192 tokens, D 128: 1467 us,
-  // 32 keys and one wave 1690); at D = 256 the sums of 16 keys alone take 128
-  // registers.  dq: 32 rows (767 us; 16 rows 797); 16 at D = 256 (87 us at 2048
-  // tokens, 32 rows 107).
   static constexpr bool f32 = sizeof(T) == 4;
-  static constexpr int NW = 4, BT = f32 ? 32 : 64;
-  static constexpr int NK = f32 && D == 64 ? 2 : 1, NQ = D == 256 ? 1 : 2;
-  static constexpr int keys = 16 * NK * NW, rows = 16 * NQ * NW;
+  static constexpr int BT = f32 ? 32 : 64;   // rows of a tile in LDS
+  static constexpr int NK = !f32 && D < 256 ? 2 : 1, keys = 64 * NK, RS = 32;
+  // dq: 32 rows per wave (767 us at 2 x 8192 tokens, D 128; 16 rows 797); 16 at
+  // D = 256 (87 us at 2048 tokens, 32 rows 107)
+  static constexpr int NW = 4, NQ = D == 256 ? 1 : 2;
 };
 
 // Parts of the walk over query rows, so that dkv fills the card (kFill workgroups),
@@ -476,13 +487,17 @@ template <class T, int D> hipError_t run(const AB& p, hipStream_t st) {
   hipLaunchKernelGGL((k_attn_delta<T, D>), dim3((unsigned)((rows * (D / 8) + 255) / 256)), dim3(256), 0, st, p, rows);
   const int S = splits<T, D>(f);
   const int64_t kt = ((int64_t)f.T + Sh::keys - 1) / Sh::keys;
-  hipLaunchKernelGGL((k_attn_dkv<T, D, Sh::NK, NW, Sh::BT>), dim3((unsigned)(kt * groups), S), dim3(64 * NW), 0, st, p);
+  hipLaunchKernelGGL((k_attn_dkv<T, D, Sh::NK, Sh::BT, Sh::RS>), dim3((unsigned)(kt * groups), S), dim3(512), 0, st, p);
   if (S > 1) {
     const int64_t n = (int64_t)f.N * f.Hkv * D;
     hipLaunchKernelGGL((k_attn_dkv_sum<T>), dim3((unsigned)((2 * n / 4 + 255) / 256)), dim3(256), 0, st, p, n, S);
   }
-  const int64_t qt = ((int64_t)f.T * f.G + Sh::rows - 1) / Sh::rows;
-  hipLaunchKernelGGL((k_attn_dq<T, D, Sh::NQ, NW, Sh::BT>), dim3((unsigned)(qt * groups)), dim3(64 * NW), 0, st, p);
+  // half the rows per wave where that is needed to fill the card
+  const int64_t nrow = (int64_t)f.T * f.G, qt = (nrow + 16 * Sh::NQ * NW - 1) / (16 * Sh::NQ * NW);
+  if (Sh::NQ == 2 && qt * groups <= kFill)
+    hipLaunchKernelGGL((k_attn_dq<T, D, 1, NW, Sh::BT>), dim3((unsigned)((nrow + 16 * NW - 1) / (16 * NW) * groups)), dim3(64 * NW), 0, st, p);
+  else
+    hipLaunchKernelGGL((k_attn_dq<T, D, Sh::NQ, NW, Sh::BT>), dim3((unsigned)(qt * groups)), dim3(64 * NW), 0, st, p);
   return hipGetLastError();
 }
 

@@ -44,7 +44,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_few(const AF p) {
     Task t;
     if (!plan.of_unit(u, t)) break;
     const int rows = t.s.n * p.G, row0 = t.m * BM, row1 = min(row0 + BM, rows);
-    const int off = t.s.len - t.s.n, p0 = off + row0 / p.G, p1 = off + (row1 - 1) / p.G;
+    const int off = t.s.len - t.s.n, p0 = off + over_g(p, row0), p1 = off + over_g(p, row1 - 1);
     int k0, k1;
     units_of(p, t.s, row0, row1, kUnit, k0, k1);
     const int skip = u - t.first, take = min(t.units - skip, uend - u);
@@ -57,7 +57,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_few(const AF p) {
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
       const int row = min(row0 + i * 16 + r, rows - 1);
-      const int tk = row / p.G, g = row - tk * p.G;
+      const int tk = over_g(p, row), g = row - tk * p.G;
       const T* qp = (const T*)p.q + (p.cu ? (int64_t)(t.s.c0 + tk) * p.qs[1] : t.b * p.qs[0] + tk * p.qs[1]) + (t.h * p.G + g) * p.qs[2];
 #pragma unroll
       for (int c = 0; c < NS; ++c) qf[i][c] = *reinterpret_cast<const F*>(qp + 32 * c + 8 * q);
@@ -65,6 +65,10 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_few(const AF p) {
       low[i] = p.window ? pos[i] - p.window + 1 : 0;
     }
 
+#pragma unroll
+    for (int i = 0; i < NQ; ++i)
+#pragma unroll
+      for (int c = 0; c < NS; ++c) settle(qf[i][c]);
     f32x4 o[NQ][NC];
     float mx[NQ], sum[NQ];
 #pragma unroll
@@ -235,7 +239,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_few(const AF p) {
         z += f * wl[k][row];
       }
       if (whole) {
-        const int tk = (row0 + row) / p.G, g = row0 + row - tk * p.G;
+        const int tk = over_g(p, row0 + row), g = row0 + row - tk * p.G;
         const int64_t at = (int64_t)(t.s.c0 + tk) * p.Hkv * p.G + t.h * p.G + g;
         const float f = z == 0.f ? 0.f : 1.f / z;
         const float y[4] = {a[0] * f, a[1] * f, a[2] * f, a[3] * f};

@@ -10,6 +10,7 @@ namespace dn {
 struct AF {
   int B, N, T;               // sequences; new tokens in all; per sequence (0: cu)
   int Hkv, G;                // query heads = Hkv * G, query head h reads key head h / G
+  uint32_t gm; int gs;       // division by G (set_heads)
   int window;                // keys that a query sees, itself the last; 0: all
   int shift, pages, max_pages;
   float sc;                  // scale * log2(e)
@@ -37,6 +38,21 @@ template <class T, bool PAGED> struct Rows {
     return base + pg * page + (t & ((1 << shift) - 1)) * token;
   }
 };
+
+// row / G for 0 <= row < 2^31: with 2^k >= G and M = ceil(2^(31+k) / G), row M is
+// less than 2^(31+k) / G off, so the shift gives the quotient.  (The compiler's
+// division is 30 instructions, and rows are found by it in every tile.)
+__device__ __forceinline__ int over_g(const AF& p, int row) {
+  return p.gs < 0 ? row : (int)(__umulhi((uint32_t)row, p.gm) >> p.gs);
+}
+inline void set_heads(AF& p, int Hq, int Hkv) {
+  p.Hkv = Hkv;
+  p.G = Hq / Hkv;
+  int k = 0;
+  while ((1 << k) < p.G) ++k;
+  p.gs = k - 1;   // G = 1: no division
+  p.gm = k ? (uint32_t)((((uint64_t)1 << (31 + k)) + p.G - 1) / p.G) : 0;
+}
 
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLazy = 8.f;   // a running maximum may lag behind by a factor 2^8
@@ -100,7 +116,7 @@ __device__ __forceinline__ Span span_of(const AF& p, int b) {
 
 // Keys [lo, hi) that rows [row0, row1) of a sequence see between them, in units.
 __device__ __forceinline__ void units_of(const AF& p, const Span& s, int row0, int row1, int unit, int& u0, int& u1) {
-  const int off = s.len - s.n, p0 = off + row0 / p.G, p1 = off + (row1 - 1) / p.G;
+  const int off = s.len - s.n, p0 = off + over_g(p, row0), p1 = off + over_g(p, row1 - 1);
   u0 = p.window ? max(p0 - p.window + 1, 0) / unit : 0;
   u1 = p1 < 0 ? u0 : p1 / unit + 1;
   u1 = max(u1, u0 + 1);   // a tile without keys is work too: it writes zeros
@@ -205,7 +221,7 @@ struct Plan {
   __device__ __forceinline__ bool of_row(int i, int hq, Task& t, int& row) const {
     int per;
     if (!find([&](const Span& s, int) { return s.c0 + s.n > i && s.c0 <= i; }, t, per)) return false;
-    t.h = hq / p.G;
+    t.h = over_g(p, hq);
     row = (i - t.s.c0) * p.G + hq - t.h * p.G;
     t.m = row / BM;
     t.first += t.h * per;

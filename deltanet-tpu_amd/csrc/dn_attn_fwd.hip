@@ -35,7 +35,7 @@ __global__ __launch_bounds__(64 * NW * KG, sizeof(T) == 2 ? 2 : 1) void k_attn(c
   const int off = len - s.n;                       // position of the first new token
   const int rows = s.n * p.G, row0 = s.m * BM;
   const int row1 = min(row0 + BM, rows);           // the tile's rows
-  const int p0 = off + row0 / p.G, p1 = off + (row1 - 1) / p.G;   // their positions
+  const int p0 = off + over_g(p, row0), p1 = off + over_g(p, row1 - 1);   // their positions
 
   // queries: row -> token row / G, head h G + row % G
   F qf[NQ][NS];
@@ -43,7 +43,7 @@ __global__ __launch_bounds__(64 * NW * KG, sizeof(T) == 2 ? 2 : 1) void k_attn(c
 #pragma unroll
   for (int i = 0; i < NQ; ++i) {
     const int row = min(row0 + (w * NQ + i) * 16 + r, rows - 1);
-    const int t = row / p.G, g = row - t * p.G;
+    const int t = over_g(p, row), g = row - t * p.G;
     const T* qp = (const T*)p.q + (p.cu ? (int64_t)(s.c0 + t) * p.qs[1] : s.b * p.qs[0] + t * p.qs[1]) + (h * p.G + g) * p.qs[2];
 #pragma unroll
     for (int c = 0; c < NS; ++c) qf[i][c] = *reinterpret_cast<const F*>(qp + 32 * c + 8 * q);
@@ -176,6 +176,9 @@ __global__ __launch_bounds__(64 * NW * KG, sizeof(T) == 2 ? 2 : 1) void k_attn(c
         for (int i = 0; i < NQ; ++i) At<T>::mma(o[i][n * VB + c], vf[n & 1][c], pf[i]);
     }
   };
+  // the waits for the queries land here and not, for all loads in flight there, in
+  // every trip of the loop (registers pinned by settle() instead: 1041 us for 987)
+  __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
 #pragma unroll 1
   for (int pass = 0;; ++pass) {
 #pragma unroll
@@ -259,7 +262,7 @@ __global__ __launch_bounds__(64 * NW * KG, sizeof(T) == 2 ? 2 : 1) void k_attn(c
     const int row = row0 + (w * NQ + i) * 16 + r;
     const float z = sum[i];
     if (row >= rows) continue;
-    const int t = row / p.G, g = row - t * p.G;
+    const int t = over_g(p, row), g = row - t * p.G;
     const int64_t at = (int64_t)(s.c0 + t) * p.Hkv * p.G + h * p.G + g;
     const float f = z == 0.f ? 0.f : 1.f / z;
     T* op = (T*)p.out + at * D;
