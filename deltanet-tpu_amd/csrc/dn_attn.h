@@ -96,6 +96,23 @@ __device__ __forceinline__ void loads_barrier() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
+// N batches of operands out of LDS: read(b), then use(b).  AHEAD: each batch is
+// read while the products of the one before it run, the order held against the
+// compiler, which elsewhere reads an operand, waits for it (130 clocks) and uses
+// it, one after another.  It takes registers for two batches; where those are not
+// there the compiler's order is the better one.
+template <int N, bool AHEAD, class Read, class Use> __device__ __forceinline__ void batches(Read read, Use use) {
+  if (AHEAD) read(0);
+#pragma unroll
+  for (int b = 0; b < N; ++b) {
+    if (!AHEAD) read(b);
+    if (AHEAD && b + 1 < N) read(b + 1);
+    if (AHEAD) __builtin_amdgcn_sched_barrier(0);
+    use(b);
+    if (AHEAD) __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
 // A tile of ROWS rows of D elements in LDS, a multiple of 32 rows.
 template <class T, int D, int ROWS> struct Tile {
   using F = typename At<T>::F;

@@ -80,11 +80,11 @@ __device__ __forceinline__ int last_token(const int32_t* starts, int T, int k1) 
 // the other dP and dS, for which it takes P from the first through LDS, and dK.
 // Each holds half of the operands and sums that one wave would (two waves fit on
 // a SIMD) and reads half of the tiles' LDS.
-template <class T, int D, int NK, int BQ, int RS>
+template <class T, int D, int NK, int BQ>
 __global__ __launch_bounds__(512, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(const AB p) {
   using TL = Tile<T, D, BQ>;
   using F = typename At<T>::F;
-  constexpr int NW = 8, BN = 64 * NK, NS = D / 32, NC = D / 16, NE = RS / 16;   // RS: query rows of a step
+  constexpr int NW = 8, BN = 64 * NK, NS = D / 32, NC = D / 16, RS = 32, NE = RS / 16;   // RS: query rows of a step
   __shared__ __align__(16) T lds[4 * BQ * D];    // [2][q, d_out][BQ][D]
   __shared__ __align__(16) f32x4 px[2][4][NK * NE * 64];  // P of a step, by its parity and the pair, as accumulators
   __shared__ __align__(16) float ls[2][BQ], de[2][BQ];   // lse * log2(e) and delta per row
@@ -155,79 +155,102 @@ __global__ __launch_bounds__(512, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(const 
     m_hi = low(over_g(f, min(j * BQ + BQ - 1, rows.last)));
   };
   bool odd = false;
-  // RS query rows of a tile; MASKED: some of them must not see some key.  Both
-  // waves multiply rows x by their own operand and rows y, transposed, by the result.
-  auto step = [&](auto mask, const T* x, const T* y, int buf, int u) {
-    constexpr bool MASKED = decltype(mask)::value;
-    f32x4 s[NK][NE];
+  // The parts of a step of RS query rows.  Both waves multiply rows x by their own
+  // operand (forward) and rows y, transposed, by the result (back).
+  using Acc = f32x4[NK][NE];
+  auto forward = [&](Acc& s, const T* x) {
 #pragma unroll
     for (int i = 0; i < NK; ++i)
 #pragma unroll
       for (int e = 0; e < NE; ++e) s[i][e] = zero4();
+    constexpr int B = NS < 4 ? NS : 4;   // slabs of a batch
+    F xf[2][B][NE];
+    batches<NS / B, true>([&](int b) {
 #pragma unroll
-    for (int c = 0; c < NS; ++c)
+      for (int c = 0; c < B; ++c)
 #pragma unroll
-      for (int e = 0; e < NE; ++e) {
-        const F xf = TL::row8(x, 16 * e + r, c, q);
+        for (int e = 0; e < NE; ++e) xf[b & 1][c][e] = TL::row8(x, 16 * e + r, b * B + c, q);
+    }, [&](int b) {
 #pragma unroll
-        for (int i = 0; i < NK; ++i) At<T>::mma(s[i][e], xf, own[i][c]);
-      }
-    f32x4* ex = px[RS == BQ ? buf : u / RS & 1][pair] + l;
-    if (first) {
+      for (int c = 0; c < B; ++c)
 #pragma unroll
-      for (int e = 0; e < NE; ++e) {
-        const int at = u + 16 * e + 4 * q;
-        const f32x4 lse = *reinterpret_cast<const f32x4*>(&ls[buf][at]);
+        for (int e = 0; e < NE; ++e)
 #pragma unroll
-        for (int i = 0; i < NK; ++i) {
+          for (int i = 0; i < NK; ++i) At<T>::mma(s[i][e], xf[b & 1][c][e], own[i][b * B + c]);
+    });
+  };
+  // S to P, and to the other wave; MASKED: some of the rows must not see some key
+  auto probabilities = [&](auto mask, Acc& s, int buf, int u) {
+    constexpr bool MASKED = decltype(mask)::value;
+    f32x4* ex = px[u / RS & 1][pair] + l;
 #pragma unroll
-          for (int z = 0; z < 4; ++z) {
-            s[i][e][z] = fast_exp2(__builtin_fmaf(s[i][e][z], f.sc, -lse[z]));
-            if (MASKED) s[i][e][z] = key + 16 * i <= tk[buf][at + z] && key + 16 * i >= lw[buf][at + z] ? s[i][e][z] : 0.f;
-          }
-          ex[(i * NE + e) * 64] = s[i][e];
+    for (int e = 0; e < NE; ++e) {
+      const int at = u + 16 * e + 4 * q;
+      const f32x4 lse = *reinterpret_cast<const f32x4*>(&ls[buf][at]);
+#pragma unroll
+      for (int i = 0; i < NK; ++i) {
+#pragma unroll
+        for (int z = 0; z < 4; ++z) {
+          s[i][e][z] = fast_exp2(__builtin_fmaf(s[i][e][z], f.sc, -lse[z]));
+          if (MASKED) s[i][e][z] = key + 16 * i <= tk[buf][at + z] && key + 16 * i >= lw[buf][at + z] ? s[i][e][z] : 0.f;
         }
+        ex[(i * NE + e) * 64] = s[i][e];
       }
     }
+  };
+  auto take = [&](Acc& pr, int u) {
+    const f32x4* ex = px[u / RS & 1][pair] + l;
+#pragma unroll
+    for (int e = 0; e < NE; ++e)
+#pragma unroll
+      for (int i = 0; i < NK; ++i) pr[i][e] = ex[(i * NE + e) * 64];
+  };
+  // dP to dS
+  auto differences = [&](auto mask, Acc& s, const Acc& pr, int buf, int u) {
+    constexpr bool MASKED = decltype(mask)::value;
+#pragma unroll
+    for (int e = 0; e < NE; ++e) {
+      const f32x4 del = *reinterpret_cast<const f32x4*>(&de[buf][u + 16 * e + 4 * q]);
+#pragma unroll
+      for (int i = 0; i < NK; ++i)
+#pragma unroll
+        for (int z = 0; z < 4; ++z) {
+          const float d = pr[i][e][z] * (s[i][e][z] - del[z]);
+          s[i][e][z] = MASKED && pr[i][e][z] == 0.f ? 0.f : d;   // (hidden rows of d_out may hold anything)
+        }
+    }
+  };
+  auto back = [&](auto mask, const Acc& s, const T* y) {
+    constexpr bool MASKED = decltype(mask)::value;
+    F sf[NK], yc[2][4];
+#pragma unroll
+    for (int i = 0; i < NK; ++i) sf[i] = frag8<T>(s[i][0], s[i][1]);
+    const bool bad = MASKED && TL::odd32(y);
+    if (MASKED) odd |= bad;
+    batches<NC / 4, true>([&](int b) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) yc[b & 1][c] = TL::col8(y, b * 4 + c, r, q);
+    }, [&](int b) {
+      if (MASKED && bad) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) yc[b & 1][c] = finite8<T>(yc[b & 1][c]);
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int i = 0; i < NK; ++i) At<T>::mma(acc[i][b * 4 + c], yc[b & 1][c], sf[i]);
+    });
+  };
+  auto step = [&](auto mask, const T* x, const T* y, int buf, int u) {
+    Acc s, pr;
+    forward(s, x);
+    if (first) probabilities(mask, s, buf, u);
     lds_barrier();
     if (!first) {
-#pragma unroll
-      for (int e = 0; e < NE; ++e) {
-        const f32x4 del = *reinterpret_cast<const f32x4*>(&de[buf][u + 16 * e + 4 * q]);
-#pragma unroll
-        for (int i = 0; i < NK; ++i) {
-          const f32x4 pr = ex[(i * NE + e) * 64];
-#pragma unroll
-          for (int z = 0; z < 4; ++z) {
-            const float d = pr[z] * (s[i][e][z] - del[z]);
-            s[i][e][z] = MASKED && pr[z] == 0.f ? 0.f : d;   // (hidden rows of d_out may hold anything)
-          }
-        }
-      }
+      take(pr, u);
+      differences(mask, s, pr, buf, u);
     }
-#pragma unroll
-    for (int o = 0; o < RS; o += 32) {
-      F sf[NK];
-#pragma unroll
-      for (int i = 0; i < NK; ++i) sf[i] = frag8<T>(s[i][o / 16], s[i][o / 16 + 1]);
-      const T* yo = y + o * 32;
-      const bool bad = MASKED && TL::odd32(yo);
-      if (MASKED) odd |= bad;
-#pragma unroll
-      for (int n = 0; n < NC; n += 4) {
-        F yc[4];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) yc[c] = TL::col8(yo, n + c, r, q);
-        if (MASKED && bad) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) yc[c] = finite8<T>(yc[c]);
-        }
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int i = 0; i < NK; ++i) At<T>::mma(acc[i][n + c], yc[c], sf[i]);
-      }
-    }
+    back(mask, s, y);
   };
   if (r0 < r1) fetch(r0, 0);
   int buf = 0;
@@ -386,18 +409,41 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(con
     f32x4 s[NQ][2], dp[NQ][2];
 #pragma unroll
     for (int i = 0; i < NQ; ++i) s[i][0] = s[i][1] = dp[i][0] = dp[i][1] = zero4();
+    if constexpr (D == 256) {
+      F kf[2][2][2], vf[2][2][2];
+      batches<NS / 2, true>([&](int b) {
 #pragma unroll
-    for (int c = 0; c < NS; ++c)
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const F kf = TL::row8(kt, 16 * e + r, c, q);
-        const F vf = TL::row8(vt, 16 * e + r, c, q);
+          for (int e = 0; e < 2; ++e) {
+            kf[b & 1][c][e] = TL::row8(kt, 16 * e + r, b * 2 + c, q);
+            vf[b & 1][c][e] = TL::row8(vt, 16 * e + r, b * 2 + c, q);
+          }
+      }, [&](int b) {
 #pragma unroll
-        for (int i = 0; i < NQ; ++i) {
-          At<T>::mma(s[i][e], kf, qf[i][c]);
-          At<T>::mma(dp[i][e], vf, gf[i][c]);
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int i = 0; i < NQ; ++i) {
+              At<T>::mma(s[i][e], kf[b & 1][c][e], qf[i][b * 2 + c]);
+              At<T>::mma(dp[i][e], vf[b & 1][c][e], gf[i][b * 2 + c]);
+            }
+      });
+    } else {
+#pragma unroll
+      for (int c = 0; c < NS; ++c)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const F kf = TL::row8(kt, 16 * e + r, c, q);
+          const F vf = TL::row8(vt, 16 * e + r, c, q);
+#pragma unroll
+          for (int i = 0; i < NQ; ++i) {
+            At<T>::mma(s[i][e], kf, qf[i][c]);
+            At<T>::mma(dp[i][e], vf, gf[i][c]);
+          }
         }
-      }
+    }
     F df[NQ];
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
@@ -415,20 +461,20 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(con
       df[i] = frag8<T>(dp[i][0], dp[i][1]);
     }
     const bool bad = MASKED && TL::odd32(kt);   // (a query that sees such a key is NaN by its scores)
+    F kc[2][4];
+    batches<NC / 4, D == 256>([&](int b) {
 #pragma unroll
-    for (int n = 0; n < NC; n += 4) {
-      F kc[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) kc[c] = TL::col8(kt, n + c, r, q);
+      for (int c = 0; c < 4; ++c) kc[b & 1][c] = TL::col8(kt, b * 4 + c, r, q);
+    }, [&](int b) {
       if (MASKED && bad) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) kc[c] = finite8<T>(kc[c]);
+        for (int c = 0; c < 4; ++c) kc[b & 1][c] = finite8<T>(kc[b & 1][c]);
       }
 #pragma unroll
       for (int c = 0; c < 4; ++c)
 #pragma unroll
-        for (int i = 0; i < NQ; ++i) At<T>::mma(dq[i][n + c], kc[c], df[i]);
-    }
+        for (int i = 0; i < NQ; ++i) At<T>::mma(dq[i][b * 4 + c], kc[b & 1][c], df[i]);
+    });
   };
   fetch(j0);
 #pragma unroll 1
@@ -463,7 +509,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(con
 template <class T, int D> struct Shape {
   static constexpr bool f32 = sizeof(T) == 4;
   static constexpr int BT = f32 ? 32 : 64;   // rows of a tile in LDS
-  static constexpr int NK = !f32 && D < 256 ? 2 : 1, keys = 64 * NK, RS = 32;
+  static constexpr int NK = !f32 && D < 256 ? 2 : 1, keys = 64 * NK;
   // dq: 32 rows per wave (767 us at 2 x 8192 tokens, D 128; 16 rows 797); 16 at
   // D = 256 (87 us at 2048 tokens, 32 rows 107)
   static constexpr int NW = 4, NQ = D == 256 ? 1 : 2;
@@ -487,7 +533,7 @@ template <class T, int D> hipError_t run(const AB& p, hipStream_t st) {
   hipLaunchKernelGGL((k_attn_delta<T, D>), dim3((unsigned)((rows * (D / 8) + 255) / 256)), dim3(256), 0, st, p, rows);
   const int S = splits<T, D>(f);
   const int64_t kt = ((int64_t)f.T + Sh::keys - 1) / Sh::keys;
-  hipLaunchKernelGGL((k_attn_dkv<T, D, Sh::NK, Sh::BT, Sh::RS>), dim3((unsigned)(kt * groups), S), dim3(512), 0, st, p);
+  hipLaunchKernelGGL((k_attn_dkv<T, D, Sh::NK, Sh::BT>), dim3((unsigned)(kt * groups), S), dim3(512), 0, st, p);
   if (S > 1) {
     const int64_t n = (int64_t)f.N * f.Hkv * D;
     hipLaunchKernelGGL((k_attn_dkv_sum<T>), dim3((unsigned)((2 * n / 4 + 255) / 256)), dim3(256), 0, st, p, n, S);
