@@ -1,4 +1,14 @@
 // Forward softmax attention over many rows: training and prompts.
+//
+// One pass over the keys per tile of query rows (rows of a key head's whole group,
+// token first, so that a tile of keys is read once for all of them): S^T = K Q^T,
+// exponentials against a reference that is known before the loop, O^T += V^T P^T,
+// everything in registers but the tiles of keys and values, which direct loads
+// bring into LDS a tile ahead.  Bound by the matrix units and what keeps them
+// waiting, LDS reads and the exponentials of two waves per SIMD: 46 % of the
+// matrix units' time at 2 x 8192 tokens, D = 128 (550 to 580 us, 970 TFLOP/s), 41 %
+// at D = 256 (prompts of 4096 over 4096 cached: 900 us, 915 TFLOP/s), where each LDS
+// operand serves 16 rows, not 32.  A library product reaches 1414 TFLOP/s here.
 #include <type_traits>
 
 #include "dn_attn_fwd.h"
@@ -91,7 +101,7 @@ __global__ __launch_bounds__(64 * NW * KG, sizeof(T) == 2 ? 2 : 1) void k_attn(c
   // At D = 256 a tile's loads go out in four parts between the products of the
   // tile before it: all at once they fill the memory queue, and the waves wait to
   // issue (600 to 1600 of 5700 clocks per tile; 893 us for 2 x 4096 tokens over
-  // 8192, 1008 otherwise).  At 128 that costs registers that are not there (773 us
+  // 4096 cached, 1008 otherwise).  At 128 that costs registers that are not there (773 us
   // for 2 x 8192, 580 otherwise).
   constexpr bool SPREAD = D == 256 && BN == 64;
   const T *ks = nullptr, *vs = nullptr;
@@ -115,7 +125,7 @@ __global__ __launch_bounds__(64 * NW * KG, sizeof(T) == 2 ? 2 : 1) void k_attn(c
   bool odd = false;   // infinities or NaNs in a masked tile were left out
   // 32 keys of a tile; MASKED: some query must not see some of them.  At D = 256
   // the first values are read under the exponentials and the others VB operands
-  // ahead, in this order (1006 us for 2 x 4096 tokens over 8192); at 128 the
+  // ahead, in this order (1006 against 1066 us for 2 x 4096 tokens over 4096 cached); at 128 the
   // compiler's own order is better (601 against 668 us for 2 x 8192).
   constexpr int VB = D == 256 ? 4 : NC, NB = NC / VB;
   auto in_order = [] {
@@ -302,8 +312,8 @@ template <class T, int D, bool PAGED> hipError_t run(const AF& p, hipStream_t st
   // their sums leave no room for two waves on a SIMD, and 16 rows are faster.
   // D = 128: four waves, two workgroups on a CU (601 us at 2 x 8192; eight waves
   // around one copy of the keys 666, 64 rows per wave 869, 16 rows 793).  D = 256:
-  // eight waves of 16 rows (1006 us for 2 x 4096 over 8192; 32 rows 1687, four waves
-  // and tiles of 32 keys 1103).
+  // eight waves of 16 rows (1006 us for 2 x 4096 over 4096 cached; 32 rows 1687, four
+  // waves and tiles of 32 keys 1103).
   constexpr bool f32 = sizeof(T) == 4;
   constexpr int NQ = f32 || D < 256 ? 2 : 1, NW = f32 || D < 256 ? 4 : 8, BN = f32 ? 32 : 64;
   const int64_t tiles = tiles_of(p, 16 * NQ * NW) * p.Hkv;

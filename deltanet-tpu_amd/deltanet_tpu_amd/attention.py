@@ -16,6 +16,7 @@ import math
 
 import numpy as np
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .gdn2 import _DT, _is_integer_dtype, _raw_stream, _require_gpu
@@ -160,6 +161,7 @@ class _RotaryFn(torch.autograd.Function):
         return (q_out, k_out) if k is not None else q_out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, *grads):
         pos, table = ctx.saved_tensors
         ps, interleaved = ctx.meta
@@ -355,6 +357,8 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, *, cu_seqlens=Non
     Hq = q.shape[-2]
     scale = _attention_common(D, Hq, Hkv, q.dtype, scale, window)
     kcs, vcs = k_cache.stride(), v_cache.stride()
+    if (k_cache.data_ptr() | v_cache.data_ptr() | (kcs[0] | kcs[1] | kcs[2] | vcs[0] | vcs[1] | vcs[2]) * q.element_size()) & 15:
+        raise ValueError(f"cache rows must start on 16 bytes, got strides {kcs} and {vcs}.")
     if page_table.shape[1] < 1:
         raise ValueError("page_table must have a column.")
     out = q.new_empty(q.shape)
@@ -441,6 +445,7 @@ class _AttentionFn(torch.autograd.Function):
         return out, lse
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, d_out, _):
         q, k, v, out, low, lse, starts = ctx.saved_tensors
         scale, window = ctx.meta
