@@ -7,6 +7,11 @@
 // rows of all heads of its group, which is the sum over them too) and by query
 // rows (dQ).  That is seven products for the five of a single pass, whose third
 // output would have to be added up in memory.
+//
+// Bound as the forward is, by the matrix units and the waits on LDS and barriers.
+// 2 x 8192 tokens, D = 128, in us and share of the matrix units' time: by keys 1344
+// to 1440, 38 % (half of its reads miss the L2s); by rows 740 to 790, 52 %; delta 30,
+// 201 MB at 6.6 TB/s.  2048 tokens in documents, D = 256: 117 + 12, 80, delta 9.
 #include <type_traits>
 
 #include "dn_attn_fwd.h"
@@ -79,7 +84,8 @@ __device__ __forceinline__ int last_token(const int32_t* starts, int T, int k1) 
 // 16 NK keys belong to two waves of one SIMD: one forms S and P and sums up dV,
 // the other dP and dS, for which it takes P from the first through LDS, and dK.
 // Each holds half of the operands and sums that one wave would (two waves fit on
-// a SIMD) and reads half of the tiles' LDS.
+// a SIMD) and reads half of the tiles' LDS: against one wave for all of it 116 and
+// 137 us at D = 256 (2048 tokens).
 template <class T, int D, int NK, int BQ>
 __global__ __launch_bounds__(512, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(const AB p) {
   using TL = Tile<T, D, BQ>;
@@ -511,12 +517,13 @@ template <class T, int D> struct Shape {
   static constexpr int BT = f32 ? 32 : 64;   // rows of a tile in LDS
   static constexpr int NK = !f32 && D < 256 ? 2 : 1, keys = 64 * NK;
   // dq: 32 rows per wave (767 us at 2 x 8192 tokens, D 128; 16 rows 797); 16 at
-  // D = 256 (87 us at 2048 tokens, 32 rows 107)
+  // D = 256 (80 us at 2048 tokens; 32 rows 107 against 87 then)
   static constexpr int NW = 4, NQ = D == 256 ? 1 : 2;
 };
 
 // Parts of the walk over query rows, so that dkv fills the card (kFill workgroups),
-// none shorter than two tiles of rows.
+// none shorter than two tiles of rows: 140 us with the sum in place of 272 at 2048
+// tokens, D = 256.
 constexpr int64_t kFill = 512;
 template <class T, int D> int splits(const AF& f) {
   using Sh = Shape<T, D>;
@@ -538,7 +545,8 @@ template <class T, int D> hipError_t run(const AB& p, hipStream_t st) {
     const int64_t n = (int64_t)f.N * f.Hkv * D;
     hipLaunchKernelGGL((k_attn_dkv_sum<T>), dim3((unsigned)((2 * n / 4 + 255) / 256)), dim3(256), 0, st, p, n, S);
   }
-  // half the rows per wave where that is needed to fill the card
+  // half the rows per wave where that is needed to fill the card: 25 us in place of
+  // 39 at 2 x 300 tokens, float32
   const int64_t nrow = (int64_t)f.T * f.G, qt = (nrow + 16 * Sh::NQ * NW - 1) / (16 * Sh::NQ * NW);
   if (Sh::NQ == 2 && qt * groups <= kFill)
     hipLaunchKernelGGL((k_attn_dq<T, D, 1, NW, Sh::BT>), dim3((unsigned)((nrow + 16 * NW - 1) / (16 * NW) * groups)), dim3(64 * NW), 0, st, p);

@@ -7,6 +7,11 @@
 // of its own to read them transposed, and keeps its own running maximum and sums.
 // The waves' results are joined in LDS; a task that several workgroups hold parts
 // of is joined by a second launch, in the order of its keys.
+//
+// 64 sequences of up to 16384 tokens (2.2 GB of keys and values, D = 128): 409 + 9 us,
+// 5.4 TB/s, where a copy reaches 5.2; 32 drafts of up to 5 tokens (283 MB, D = 256):
+// 63 to 68 + 6 us; one token over 1000: 10 + 5 us, the chain of lengths, page table,
+// keys, products and the join.
 #include "dn_attn_fwd.h"
 
 namespace dn {
@@ -336,6 +341,11 @@ template <class T, int D> hipError_t run(const AF& p, hipStream_t st) {
 
 }  // namespace
 
+// Up to 32 rows per sequence and head on average (two operands of 16), so that a
+// workgroup's one read of the keys serves all rows: 5 tokens of 32 sequences take 73
+// us in place of 1231 with the kernel of many rows, one token over 1000 20 in place
+// of 73.  Pages of at least 16 tokens: a wave reads its keys as two halves of 16
+// that each lie in one page.
 bool attn_few_takes(const AF& p) { return p.shift >= 4 && (int64_t)p.N * p.G <= (int64_t)32 * p.B && most_units(p) < (1 << 30); }
 
 size_t attn_few_bytes(const AF& p, int D) { return (size_t)groups_of(p) * 2 * row_tile(p) * (D + 2) * sizeof(float); }

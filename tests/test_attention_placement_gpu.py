@@ -144,3 +144,19 @@ def test_decode_step_in_a_graph(dev):
         torch.cuda.synchronize()
         assert torch.equal(out, want), t
         assert torch.equal(graph_caches[0], eager[0]) and torch.equal(graph_caches[1], eager[1])
+
+
+def test_refusals_of_cuda_tensors(dev):
+    """A cache whose rows do not start on 16 bytes, and a gradient of a gradient."""
+    q = torch.randn(1, 2, 64, device=dev, dtype=torch.bfloat16)
+    pt = torch.zeros(1, 1, device=dev, dtype=torch.int32)
+    lens = torch.ones(1, device=dev, dtype=torch.int32)
+    odd = torch.randn(2, 16, 1, 68, device=dev, dtype=torch.bfloat16)[..., :64]
+    ok = torch.randn(2, 16, 1, 64, device=dev, dtype=torch.bfloat16)
+    for kc, vc in ((odd, ok), (ok, odd)):
+        with pytest.raises(ValueError, match="16 bytes"):
+            paged_attention(q, kc, vc, pt, lens)
+    x = torch.randn(1, 5, 2, 64, device=dev, requires_grad=True)
+    y, = torch.autograd.grad(causal_attention(x, x, x).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        y.sum().backward()
