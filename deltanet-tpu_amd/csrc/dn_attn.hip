@@ -88,7 +88,7 @@ using namespace dn;
 
 extern "C" size_t dn_paged_attention_workspace_size(const dn_paged_attention_args* a) {
   AF p{};
-  if (paged_params(a, p) != DN_OK || p.N == 0 || !attn_few_takes(p)) return 0;
+  if (paged_params(a, p) != DN_OK || p.N == 0 || !attn_few_takes(p, a->D, a->dtype)) return 0;
   return attn_few_bytes(p, a->D) + 256;
 }
 
@@ -97,7 +97,7 @@ extern "C" int dn_paged_attention(const dn_paged_attention_args* a, void* worksp
   if (const int rc = paged_params(a, p)) return rc;
   if (p.N == 0) return DN_OK;
   hipError_t e;
-  if (attn_few_takes(p)) {
+  if (attn_few_takes(p, a->D, a->dtype)) {
     if (!workspace || workspace_bytes < attn_few_bytes(p, a->D) + 256) return set_error(DN_E_WORKSPACE, "workspace missing or too small");
     p.part = (float*)(((uintptr_t)workspace + 255) & ~(uintptr_t)255);
     e = attn_few(p, a->D, a->dtype, (hipStream_t)stream);

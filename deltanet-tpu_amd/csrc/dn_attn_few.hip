@@ -1,4 +1,5 @@
-// Attention of few query rows over a paged cache: single tokens and drafts.
+// Attention of few query rows over a paged cache: single tokens, drafts and chunks
+// of a few sequences over a long one.
 //
 // Bound by reading the keys and values once.  A workgroup takes an even share of
 // all sequences' keys (Task), its four waves 32 keys each of a unit of 128, with
@@ -341,12 +342,34 @@ template <class T, int D> hipError_t run(const AF& p, hipStream_t st) {
 
 }  // namespace
 
-// Up to 32 rows per sequence and head on average (two operands of 16), so that a
-// workgroup's one read of the keys serves all rows: 5 tokens of 32 sequences take 73
-// us in place of 1231 with the kernel of many rows, one token over 1000 20 in place
-// of 73.  Pages of at least 16 tokens: a wave reads its keys as two halves of 16
-// that each lie in one page.
-bool attn_few_takes(const AF& p) { return p.shift >= 4 && (int64_t)p.N * p.G <= (int64_t)32 * p.B && most_units(p) < (1 << 30); }
+// This kernel reads the keys once per 16 or 32 rows and spreads them over the card
+// at the cost of a join; that of many rows reads them once per 64 or 128 rows, by
+// one workgroup.  It is the length of that one walk (the page table's width, or the
+// window) against the tiles of rows that share the card here which decides.  us, this
+// kernel / the other, tokens cached, 8 key heads at D = 128 and 4 at D = 256:
+// - tiles of 16 rows, one token, 16 bits: 1 sequence 17 / 13 (512), 17 / 17 (1024),
+//   18 / 50 (4096); 64 sequences 53 / 45 (1024), 109 / 110 (2048), 196 / 209 (4096),
+//   and less than half of it when lengths differ;
+// - tiles of 32, 16 bits: D = 128 16 tiles 19 / 30 (2048), 64 38 / 30 (2048), 56 / 98
+//   (8192), 128 95 / 101 (8192), 146 / 191 (16384), 256 183 / 112 (8192), 333 / 282
+//   (16384); D = 256 64 tiles 65 / 55 (2048), 119 / 194 (8192), 128 242 / 194 (8192);
+// - float32, whose products take the time: D = 128 128 tiles 60 / 46 (512), 94 / 159
+//   (2048), 512 804 / 615 (8192), but with up to 32 rows of a sequence, which fill half
+//   of the other's tile, 440 / 641 (512 tiles, 4096); D = 256 64 tiles 73 / 91 (512),
+//   818 / 1376 (8192), 128 1545 / 1366 (8192).
+// Pages of 16 tokens at least: 16 keys of a wave's 32 lie in one page.
+bool attn_few_takes(const AF& p, int D, int dtype) {
+  if (p.shift < 4 || most_units(p) >= (1 << 30)) return false;
+  const int64_t walk = std::min<int64_t>((int64_t)p.max_pages << p.shift, p.window ? p.window : INT64_MAX);
+  const int64_t tiles = most_tasks(p);
+  if (dtype == DN_F32) {
+    if (walk < 256) return false;
+    if (row_tile(p) == 16 || (D < 256 && (int64_t)p.N * p.G <= (int64_t)32 * p.B)) return true;
+    return tiles <= (D == 256 ? 64 : 256) && walk >= 8 * tiles;
+  }
+  if (row_tile(p) == 16) return walk >= (tiles <= 128 ? 1024 : 4096);
+  return tiles <= (D == 256 ? 64 : 128) && walk >= std::max<int64_t>(1024, 64 * tiles);
+}
 
 size_t attn_few_bytes(const AF& p, int D) { return (size_t)groups_of(p) * 2 * row_tile(p) * (D + 2) * sizeof(float); }
 

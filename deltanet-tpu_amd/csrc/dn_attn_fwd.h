@@ -235,9 +235,9 @@ struct Plan {
 // type checked by the caller.
 hipError_t attn_many(const AF& p, int D, int dtype, bool paged, hipStream_t st);
 
-// Attention of few rows per sequence over a paged cache, the keys split over the
+// Attention of few rows over a paged cache, the keys split over the
 // workgroups: whether the call is one of these, the bytes it needs, the launches.
-bool attn_few_takes(const AF& p);
+bool attn_few_takes(const AF& p, int D, int dtype);
 size_t attn_few_bytes(const AF& p, int D);
 hipError_t attn_few(const AF& p, int D, int dtype, hipStream_t st);
 

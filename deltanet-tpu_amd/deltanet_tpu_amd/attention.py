@@ -430,6 +430,18 @@ def _attention_forward(q, k, v, starts, scale, window, want_lse, want_low=False)
     return out, low, lse
 
 
+class _NoSecond(torch.autograd.Function):
+    """Gradients that depend on d_out, q, k and v, whose own gradient is refused."""
+
+    @staticmethod
+    def forward(ctx, dq, dk, dv, d_out, q, k, v):
+        return dq, dk, dv
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("causal_attention is once_differentiable: the gradient of its gradient is not implemented.")
+
+
 class _AttentionFn(torch.autograd.Function):
     """Causal attention under autograd: the forward keeps the log of each row's sum
     of exponentials, from which the backward recomputes the probabilities, and what
@@ -445,7 +457,6 @@ class _AttentionFn(torch.autograd.Function):
         return out, lse
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, d_out, _):
         q, k, v, out, low, lse, starts = ctx.saved_tensors
         scale, window = ctx.meta
@@ -459,6 +470,8 @@ class _AttentionFn(torch.autograd.Function):
             ws = q.new_empty(-(-need // q.element_size()))
             _call("dn_attention_bwd", q.get_device(), block, d_out.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                   ws.data_ptr(), need)
+        if torch.is_grad_enabled():   # create_graph
+            dq, dk, dv = _NoSecond.apply(dq, dk, dv, d_out, q, k, v)
         return dq, dk, dv, None, None, None
 
 

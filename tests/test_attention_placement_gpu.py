@@ -160,3 +160,59 @@ def test_refusals_of_cuda_tensors(dev):
     y, = torch.autograd.grad(causal_attention(x, x, x).sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         y.sum().backward()
+
+
+def _wide(pt, page, tokens=16384):
+    """The page table with columns that no sequence uses: rules go by its width."""
+    more = torch.full((pt.shape[0], tokens // page - pt.shape[1]), 1 << 30, dtype=torch.int32, device=pt.device)
+    return torch.cat([pt, more], 1)
+
+
+@pytest.mark.parametrize("new,lens", [([1], [1]), ([1], [1000]), ([1] * 9, [3, 2000, 16, 17, 129, 700, 1, 2, 33]), ([5, 5, 5], [5, 60, 300]),
+                                      ([2, 3], [0, 1]), ([70], [1500]), ([300], [300]), ([9, 0, 40], [2000, 7, 40]), ([0, 0], [4, 0])])
+@pytest.mark.parametrize("dt,Hq,Hkv,D,page,hf", [("bf16", 8, 2, 128, 16, False), ("bf16", 4, 1, 256, 64, True), ("f16", 3, 3, 64, 128, False),
+                                                 ("f32", 4, 2, 128, 32, False), ("f32", 2, 1, 256, 64, True), ("f16", 16, 1, 256, 16, False)])
+def test_wide_page_tables(dev, new, lens, dt, Hq, Hkv, D, page, hf):
+    """The keys of tokens, drafts and chunks split over the card."""
+    kc, vc, pt, sl, cu, ks, vs = _paged(17, new, lens, Hkv, D, page, dt, dev, hf)
+    q = _rows(18, sum(new), Hq, D, dt=dt)
+    out, lse = paged_attention(q.to(dev), kc, vc, _wide(pt, page), sl, cu_seqlens=cu, return_lse=True)
+    _check_paged(out, lse, q, ks, vs, new, lens, dt)
+
+
+@pytest.mark.parametrize("dt,window", [("bf16", 1024), ("bf16", 4100), ("f32", 256), ("f32", 300)])
+@pytest.mark.parametrize("new,lens", [([1, 2, 1], [1400, 300, 1100]), ([50], [1500])])
+def test_wide_page_tables_windows(dev, dt, window, new, lens):
+    kc, vc, pt, sl, cu, ks, vs = _paged(19, new, lens, 1, 128, 16, dt, dev)
+    q = _rows(20, sum(new), 4, 128, dt=dt)
+    out = paged_attention(q.to(dev), kc, vc, _wide(pt, 16), sl, cu_seqlens=cu, window=window, scale=0.2)
+    _check_paged(out, None, q, ks, vs, new, lens, dt, window, 0.2)
+
+
+@pytest.mark.parametrize("odd", [math.nan, math.inf])
+def test_wide_page_tables_hidden_infinities(dev, odd):
+    """Later tokens of the same call that are not finite do not reach earlier ones."""
+    kc, vc, pt, sl, cu, ks, vs = _paged(21, [20], [150], 1, 128, 16, "bf16", dev, junk=odd)
+    pt = _wide(pt, 16)
+    q = _rows(22, 20, 4, 128).to(dev)
+    base = paged_attention(q, kc, vc, pt, sl, cu_seqlens=cu)
+    vc[int(pt[0, 140 // 16]), 140 % 16] = odd   # the 11th new token
+    out = paged_attention(q, kc, vc, pt, sl, cu_seqlens=cu)
+    assert torch.equal(out[:10], base[:10])
+    assert not torch.isfinite(out[10:]).any()
+
+
+@pytest.mark.parametrize("kind", ["decode", "ragged", "long-among-short"])
+def test_wide_page_tables_of_many_sequences(dev, kind):
+    g = torch.Generator().manual_seed(1)
+    B = 150
+    lens = torch.randint(1, 90, (B,), generator=g).tolist()
+    lens[77] = 1500
+    new = [1] * B if kind != "ragged" else [int(x) % 4 for x in torch.randint(0, 100, (B,), generator=g)]
+    if kind == "long-among-short":
+        new[77] = 60
+    lens = [max(n, m) for n, m in zip(lens, new)]
+    kc, vc, pt, sl, cu, ks, vs = _paged(23, new, lens, 1, 64, 16, "bf16", dev)
+    q = _rows(24, sum(new), 4, 64)
+    out, lse = paged_attention(q.to(dev), kc, vc, _wide(pt, 16), sl, cu_seqlens=cu, return_lse=True)
+    _check_paged(out, lse, q, ks, vs, new, lens, "bf16")

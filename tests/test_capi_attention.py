@@ -63,7 +63,7 @@ def test_c_entries_refuse_before_any_launch():
     assert P("dn_kv_append")(bytes(a), None) == -1 and b"N / B" in err()
     a.N = 4
     assert P("dn_kv_append")(bytes(a), None) == -1 and b"missing" in err()
-    p = _set(_lib.PagedAttentionArgs(), abi_version=_lib.DN_ABI_VERSION, N=2, B=2, Hq=4, Hkv=2, D=96, dtype=1, pages=1, page_size=16, max_pages=4, scale=1.0)
+    p = _set(_lib.PagedAttentionArgs(), abi_version=_lib.DN_ABI_VERSION, N=2, B=2, Hq=4, Hkv=2, D=96, dtype=1, pages=1, page_size=16, max_pages=64, scale=1.0)
     call = lambda: P("dn_paged_attention")(bytes(p), None, 0, None)
     size = lambda: P("dn_paged_attention_workspace_size")(bytes(p))
     assert call() == -1 and b"head dimension" in err() and size() == 0
