@@ -16,7 +16,6 @@ import math
 
 import numpy as np
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .gdn2 import _DT, _is_integer_dtype, _raw_stream, _require_gpu
@@ -153,24 +152,29 @@ class _RotaryFn(torch.autograd.Function):
     rotation with the sines negated."""
 
     @staticmethod
-    def forward(ctx, q, k, pos, ps, table, interleaved):
+    def forward(ctx, q, k, pos, ps, table, interleaved, inverse):
         ctx.save_for_backward(pos, table)
-        ctx.meta = ps, interleaved
+        ctx.meta = ps, interleaved, inverse
         ctx.set_materialize_grads(False)
-        q_out, k_out = _rotary_launch(q, k, pos, ps, table, interleaved, False)
+        q_out, k_out = _rotary_launch(q, k, pos, ps, table, interleaved, inverse)
         return (q_out, k_out) if k is not None else q_out
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, *grads):
+    def backward(ctx, dq, dk=None):
         pos, table = ctx.saved_tensors
-        ps, interleaved = ctx.meta
-        given = [_dense_channels(g) for g in grads if g is not None]
-        turned = iter(())
-        if given:
-            turned = iter(_rotary_launch(given[0], given[1] if len(given) > 1 else None, pos, ps, table, interleaved, True))
-        dq, dk = (None if g is None else next(turned) for g in (*grads, None)[:2])
-        return dq, dk, None, None, None, None
+        ps, interleaved, inverse = ctx.meta
+        given = [_dense_channels(g) for g in (dq, dk) if g is not None]
+        if not given:
+            return (None,) * 7
+        a, b = given[0], given[1] if len(given) > 1 else None
+        if torch.is_grad_enabled():   # create_graph: the rotation of the gradients is differentiable in turn
+            turned = _RotaryFn.apply(a, b, pos, ps, table, interleaved, not inverse)
+            turned = turned if b is not None else (turned, None)
+        else:
+            turned = _rotary_launch(a, b, pos, ps, table, interleaved, not inverse)
+        if dq is None:
+            turned = None, turned[0]
+        return turned[0], turned[1], None, None, None, None, None
 
 
 def apply_rotary(q, k, positions, table, *, interleaved: bool = False):
@@ -183,7 +187,7 @@ def apply_rotary(q, k, positions, table, *, interleaved: bool = False):
     or (L,) for every row alike, (N,) for rank 3.  table: from ``rotary_table``.
     Pairs are (i, i + R/2), or (2i, 2i + 1) with ``interleaved``.  A position
     outside the table gives NaN in the rotated channels.  Products in float32,
-    one rounding.  Differentiable in q and k.  Returns (q', k') with k' None if k
+    one rounding.  Differentiable in q and k, any number of times.  Returns (q', k') with k' None if k
     is None; the results are contiguous.
     """
     if q.ndim not in (3, 4):
@@ -208,7 +212,7 @@ def apply_rotary(q, k, positions, table, *, interleaved: bool = False):
         q, k, ps = q[None], None if k is None else k[None], (0, ps[-1])
     q, k = _dense_channels(q), None if k is None else _dense_channels(k)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        r = _RotaryFn.apply(q, k, positions, ps, table, bool(interleaved))
+        r = _RotaryFn.apply(q, k, positions, ps, table, bool(interleaved), False)
         q_out, k_out = r if k is not None else (r, None)
     else:
         q_out, k_out = _rotary_launch(q, k, positions, ps, table, interleaved, False)

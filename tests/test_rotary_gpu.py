@@ -187,3 +187,27 @@ def test_append_uniform_and_out_of_range(dev):
     one = torch.randn(B, H, D, device=dev).to(torch.bfloat16)
     paged_kv_append(one, one, kc, vc, pt, torch.tensor([1, 1, 1], dtype=torch.int32, device=dev))
     assert torch.equal(kc[[0, 2, 3], 0], one) and torch.equal(vc[[0, 2, 3], 0], one)
+
+
+@pytest.mark.parametrize("parts", ["q", "k", "both", "q alone"])
+def test_rotary_gradient_of_some_and_of_the_gradient(dev, parts):
+    """A gradient of one result only, and the gradient of the gradient: the rotation
+    is linear, so that this is the rotation of what is put in again, to the bit."""
+    table = rotary_table(16, 32, device=dev)
+    pos = torch.arange(5, device=dev)
+    q = torch.randn(2, 5, 3, 64, device=dev, requires_grad=True)
+    k = None if parts == "q alone" else torch.randn(2, 5, 1, 64, device=dev, requires_grad=True)
+    yq, yk = apply_rotary(q, k, pos, table)
+    wq = torch.randn_like(q).requires_grad_(True)
+    wk = None if k is None else torch.randn_like(k).requires_grad_(True)
+    loss = (yq * wq).sum() if parts != "k" else 0.0
+    if parts in ("k", "both"):
+        loss = loss + (yk * wk).sum()
+    ins = [x for x, on in ((q, parts != "k"), (k, parts in ("k", "both"))) if on]
+    ws = [x for x, on in ((wq, parts != "k"), (wk, parts in ("k", "both"))) if on]
+    grads = torch.autograd.grad(loss, ins, create_graph=True)
+    # sum of grad * c, c given: its gradient in w is the rotation of c
+    cs = [torch.randn_like(x) for x in ins]
+    second = torch.autograd.grad(sum((g * c).sum() for g, c in zip(grads, cs)), ws)
+    for c, got in zip(cs, second):
+        assert torch.equal(got, apply_rotary(c, None, pos, table)[0])
