@@ -13,6 +13,8 @@
 // 5.4 TB/s, where a copy reaches 5.2; 32 drafts of up to 5 tokens (283 MB, D = 256):
 // 63 to 68 + 6 us; one token over 1000: 10 + 5 us, the chain of lengths, page table,
 // keys, products and the join.
+#include <type_traits>
+
 #include "dn_attn_fwd.h"
 
 namespace dn {
@@ -31,6 +33,9 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_few(const AF p) {
   using TL = Tile<T, D, 32>;
   using F = typename At<T>::F;
   typedef uint32_t U4 __attribute__((ext_vector_type(4)));
+  // float16: a running maximum's probability is 2^7 to 2^15, not 1 to 2^8, so that
+  // those far below it keep their bits (half a step is 2^-25)
+  constexpr float kLift = std::is_same<T, f16>::value ? 7.f : 0.f;
   constexpr int BM = 16 * NQ, NS = D / 32, NC = D / 16, NG = 32 / TL::kLoad, NV = NG * NS;   // NV: loads of a wave's 32 value rows, NG groups of rows by slabs
   // values of a wave's 32 keys; at a task's end the waves' sums
   constexpr int kV = 32 * D * (int)sizeof(T), kO = BM * D * 4;
@@ -155,7 +160,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_few(const AF p) {
         }
         const float m = fmaxf(fmaxf(fmaxf(sc[i][0][0], sc[i][0][1]), fmaxf(sc[i][0][2], sc[i][0][3])),
                               fmaxf(fmaxf(sc[i][1][0], sc[i][1][1]), fmaxf(sc[i][1][2], sc[i][1][3])));
-        mt[i] = max_q(m) * p.sc;
+        mt[i] = max_q(m) * p.sc - kLift;
         grow |= mt[i] > mx[i] + kLazy;
       }
       if (__any(grow)) {

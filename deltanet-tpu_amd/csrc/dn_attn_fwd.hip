@@ -82,8 +82,13 @@ __global__ __launch_bounds__(64 * NW * KG, sizeof(T) == 2 ? 2 : 1) void k_attn(c
   // no maximum has to be known while the sums run.  Sums of exponentials up to
   // 2^kRange above it are as exact as any in a type with float32's range; the
   // rare row that goes beyond is found at the end, and the tile done again with
-  // the maxima that are known then.
-  constexpr float kRange = std::is_same<T, f16>::value ? 15.f : 60.f, kShift = std::is_same<T, f16>::value ? 6.f : 0.f;
+  // the maxima that are known then.  float16 probabilities lose bits below 2^-14,
+  // half a step of theirs being 2^-25: the own key's is 2^4 there, so that they are
+  // right to 2^-29 of the largest whatever the other scores are, and a row's
+  // maximum may be 2^11 above its own score (7.6 in the exponent of e) before its
+  // tile is done again, with 2^14 at the maximum.
+  constexpr bool F16 = std::is_same<T, f16>::value;
+  constexpr float kRange = F16 ? 15.f : 60.f, kOwn = F16 ? 4.f : 0.f, kTop = F16 ? 14.f : 0.f;
   f32x4 o[NQ][NC];
   float mx[NQ], top[NQ], sum[NQ];
 #pragma unroll
@@ -96,7 +101,7 @@ __global__ __launch_bounds__(64 * NW * KG, sizeof(T) == 2 ? 2 : 1) void k_attn(c
 #pragma unroll
       for (int e = 0; e < 8; ++e) x += (float)kf[e] * (float)qf[i][c][e];
     }
-    mx[i] = pos[i] < 0 ? 0.f : sum_q(x) * p.sc + kShift;
+    mx[i] = pos[i] < 0 ? 0.f : sum_q(x) * p.sc - kOwn;
   }
   // At D = 256 a tile's loads go out in four parts between the products of the
   // tile before it: all at once they fill the memory queue, and the waves wait to
@@ -239,7 +244,7 @@ __global__ __launch_bounds__(64 * NW * KG, sizeof(T) == 2 ? 2 : 1) void k_attn(c
 #pragma unroll
       for (int g = 0; g < KG; ++g)
         if (KG > 1) top[i] = fmaxf(top[i], s_top[g][(w * NQ + i) * 16 + r]);
-      mx[i] = top[i] > mx[i] + kRange ? top[i] : mx[i];   // (the other rows keep their bits)
+      mx[i] = top[i] > mx[i] + kRange ? top[i] - kTop : mx[i];   // (the other rows keep their bits)
     }
     __syncthreads();
   }
