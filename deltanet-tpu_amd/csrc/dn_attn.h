@@ -231,4 +231,13 @@ template <class T> __device__ __forceinline__ typename At<T>::F finite8(const ty
   return f;
 }
 
+// an operand with its signs changed
+template <class T> __device__ __forceinline__ typename At<T>::F minus8(const typename At<T>::F& a) {
+  typedef uint32_t U __attribute__((ext_vector_type(2 * sizeof(T))));
+  U u = __builtin_bit_cast(U, a);
+#pragma unroll
+  for (int i = 0; i < 2 * (int)sizeof(T); ++i) u[i] ^= At<T>::kTop;
+  return __builtin_bit_cast(typename At<T>::F, u);
+}
+
 }  // namespace dn

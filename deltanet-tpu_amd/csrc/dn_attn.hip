@@ -49,7 +49,8 @@ const char* shape_error(int64_t tokens, int Hq, int Hkv, int D, int dtype, float
   if (D != 64 && D != 128 && D != 256) return "head dimension must be 64, 128 or 256";
   if (Hq <= 0 || Hkv <= 0 || Hq % Hkv) return "query heads must be a multiple of the key heads";
   if (dtype != DN_F32 && dtype != DN_BF16 && dtype != DN_F16) return "attention dtype not supported";
-  if (!(scale == scale) || scale - scale != 0.f) return "scale must be finite";
+  const float e = scale * kLog2e;
+  if (!(e - e == 0.f)) return "scale must be finite";
   if (window < 0) return "window must not be negative";
   if (tokens * Hq >= ((int64_t)1 << 31)) return "too many query rows";
   return nullptr;

@@ -45,6 +45,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_few(const AF p) {
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   T* vt = reinterpret_cast<T*>(smem + w * kV);
 
+  const float scale = exponent_scale(p);
   const Plan plan(p, BM, kUnit);
   const int W = min((int)gridDim.x, plan.C);   // each has a unit at least
   if ((int)blockIdx.x >= W) return;
@@ -72,6 +73,9 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_few(const AF p) {
       const T* qp = (const T*)p.q + (p.cu ? (int64_t)(t.s.c0 + tk) * p.qs[1] : t.b * p.qs[0] + tk * p.qs[1]) + (t.h * p.G + g) * p.qs[2];
 #pragma unroll
       for (int c = 0; c < NS; ++c) qf[i][c] = *reinterpret_cast<const F*>(qp + 32 * c + 8 * q);
+      if (p.sc < 0.f)
+#pragma unroll
+        for (int c = 0; c < NS; ++c) qf[i][c] = minus8<T>(qf[i][c]);
       pos[i] = off + tk;
       low[i] = p.window ? pos[i] - p.window + 1 : 0;
     }
@@ -160,7 +164,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_few(const AF p) {
         }
         const float m = fmaxf(fmaxf(fmaxf(sc[i][0][0], sc[i][0][1]), fmaxf(sc[i][0][2], sc[i][0][3])),
                               fmaxf(fmaxf(sc[i][1][0], sc[i][1][1]), fmaxf(sc[i][1][2], sc[i][1][3])));
-        mt[i] = max_q(m) * p.sc - kLift;
+        mt[i] = max_q(m) * scale - kLift;
         grow |= mt[i] > mx[i] + kLazy;
       }
       if (__any(grow)) {
@@ -181,7 +185,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_few(const AF p) {
         for (int e = 0; e < 2; ++e)
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            sc[i][e][x] = fast_exp2(__builtin_fmaf(sc[i][e][x], p.sc, -m));
+            sc[i][e][x] = fast_exp2(__builtin_fmaf(sc[i][e][x], scale, -m));
             sum[i] += sc[i][e][x];
           }
         pf[i] = frag8<T>(sc[i][0], sc[i][1]);

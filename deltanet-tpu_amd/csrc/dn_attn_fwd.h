@@ -13,7 +13,7 @@ struct AF {
   uint32_t gm; int gs;       // division by G (set_heads)
   int window;                // keys that a query sees, itself the last; 0: all
   int shift, pages, max_pages;
-  float sc;                  // scale * log2(e)
+  float sc;                  // scale * log2(e), any sign
   const void *q, *k, *v;
   void* out;                 // dense (tokens, Hkv G, D)
   void* low;                 // NULL or as out: what its rounding cut off
@@ -53,6 +53,13 @@ inline void set_heads(AF& p, int Hq, int Hkv) {
   p.gs = k - 1;   // G = 1: no division
   p.gm = k ? (uint32_t)((((uint64_t)1 << (31 + k)) + p.G - 1) / p.G) : 0;
 }
+
+// What a forward kernel multiplies scores by, positive: it hides a score as -inf
+// before it scales it and takes maxima of scores that are not scaled.  The sign of
+// a negative scale goes into the queries where they are loaded (exactly), and 0
+// becomes the least normal number: -inf stays -inf, and exponents of scores up to
+// 2^100 are 0 to 2^-26.
+__device__ __forceinline__ float exponent_scale(const AF& p) { return fmaxf(fabsf(p.sc), 0x1p-126f); }
 
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLazy = 8.f;   // a running maximum may lag behind by a factor 2^8

@@ -47,6 +47,7 @@ __global__ __launch_bounds__(64 * NW * KG, sizeof(T) == 2 ? 2 : 1) void k_attn(c
   const int row1 = min(row0 + BM, rows);           // the tile's rows
   const int p0 = off + over_g(p, row0), p1 = off + over_g(p, row1 - 1);   // their positions
 
+  const float scale = exponent_scale(p);
   // queries: row -> token row / G, head h G + row % G
   F qf[NQ][NS];
   int pos[NQ], low[NQ];
@@ -57,6 +58,9 @@ __global__ __launch_bounds__(64 * NW * KG, sizeof(T) == 2 ? 2 : 1) void k_attn(c
     const T* qp = (const T*)p.q + (p.cu ? (int64_t)(s.c0 + t) * p.qs[1] : s.b * p.qs[0] + t * p.qs[1]) + (h * p.G + g) * p.qs[2];
 #pragma unroll
     for (int c = 0; c < NS; ++c) qf[i][c] = *reinterpret_cast<const F*>(qp + 32 * c + 8 * q);
+    if (p.sc < 0.f)
+#pragma unroll
+      for (int c = 0; c < NS; ++c) qf[i][c] = minus8<T>(qf[i][c]);
     pos[i] = off + t;
     low[i] = p.window ? pos[i] - p.window + 1 : 0;
     if (!PAGED && p.start) low[i] = max(low[i], p.start[s.b * p.T + t]);
@@ -101,7 +105,7 @@ __global__ __launch_bounds__(64 * NW * KG, sizeof(T) == 2 ? 2 : 1) void k_attn(c
 #pragma unroll
       for (int e = 0; e < 8; ++e) x += (float)kf[e] * (float)qf[i][c][e];
     }
-    mx[i] = pos[i] < 0 ? 0.f : sum_q(x) * p.sc - kOwn;
+    mx[i] = pos[i] < 0 ? 0.f : sum_q(x) * scale - kOwn;
   }
   // At D = 256 a tile's loads go out in four parts between the products of the
   // tile before it: all at once they fill the memory queue, and the waves wait to
@@ -169,7 +173,7 @@ __global__ __launch_bounds__(64 * NW * KG, sizeof(T) == 2 ? 2 : 1) void k_attn(c
             sc[i][e][x] = key <= pos[i] && key >= low[i] ? sc[i][e][x] : -INFINITY;
           }
           top[i] = fmaxf(top[i], sc[i][e][x]);
-          sc[i][e][x] = fast_exp2(__builtin_fmaf(sc[i][e][x], p.sc, -mx[i]));
+          sc[i][e][x] = fast_exp2(__builtin_fmaf(sc[i][e][x], scale, -mx[i]));
           sum[i] += sc[i][e][x];
         }
       pf[i] = frag8<T>(sc[i][0], sc[i][1]);
@@ -234,7 +238,7 @@ __global__ __launch_bounds__(64 * NW * KG, sizeof(T) == 2 ? 2 : 1) void k_attn(c
     bool over = false;
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
-      top[i] = max_q(top[i]) * p.sc;
+      top[i] = max_q(top[i]) * scale;
       over |= top[i] > mx[i] + kRange;
       if (KG > 1 && q == 0) s_top[kg][(w * NQ + i) * 16 + r] = top[i];
     }

@@ -328,8 +328,8 @@ def _attention_common(D, Hq, Hkv, dtype, scale, window):
         scale = float(scale)
     except (TypeError, ValueError) as e:
         raise ValueError(f"scale must be convertible to a concrete float, got {type(scale)}: {e}")
-    if not math.isfinite(scale):
-        raise ValueError(f"scale must be finite, got {scale}.")
+    if not abs(scale) <= 2.0 ** 127:   # (its product with log2(e) is a float32)
+        raise ValueError(f"scale must be finite in float32, got {scale}.")
     return scale
 
 
@@ -343,8 +343,8 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, *, cu_seqlens=Non
     sequence, or (B, T, Hq, D); D 64, 128 or 256; the cache's type.  Caches,
     page_table and seq_lens as in ``paged_kv_append``; query head h reads key head
     h // (Hq // Hkv).  A query at position p sees positions 0 .. p, or the last
-    ``window`` of them.  scale: 1 / sqrt(D) unless given.  Sums and softmax
-    statistics in float32.  A query without a key gets zeros (lse -inf).  Returns
+    ``window`` of them.  scale: any finite number, 1 / sqrt(D) unless given.  Sums and
+    softmax statistics in float32.  A query without a key gets zeros (lse -inf).  Returns
     the output in q's shape and type, and with ``return_lse`` also the log of the
     sum of exponentials (float32, q's shape without D).
     """
@@ -485,12 +485,12 @@ def causal_attention(q, k, v, *, segment_ids=None, cu_seqlens=None, scale=None, 
     q: (B, L, Hq, D); k, v: (B, L, Hkv, D) with Hkv dividing Hq; one of float32,
     bfloat16 and float16; D 64, 128 or 256.  Documents by ``segment_ids`` or
     ``cu_seqlens`` as in ``chunk_gdn2``: token i sees the tokens of its document up
-    to itself, or the last ``window`` of them.  scale: 1 / sqrt(D) unless given.
-    Sums and softmax statistics in float32.  Returns the output in q's shape and
-    type, and with ``return_lse`` also the log of the sum of exponentials (B, L, Hq)
-    in float32.  Differentiable in q, k and v (not through the lse); gradients come
-    in the inputs' type, those of k and v summed over the heads that share them, and
-    are the same bits every time.
+    to itself, or the last ``window`` of them.  scale: any finite number,
+    1 / sqrt(D) unless given.  Sums and softmax statistics in float32.  Returns the
+    output in q's shape and type, and with ``return_lse`` also the log of the sum of
+    exponentials (B, L, Hq) in float32.  Differentiable in q, k and v (not through the
+    lse); gradients come in the inputs' type, those of k and v summed over the heads
+    that share them, and are the same bits every time.
     """
     if q.ndim != 4:
         raise ValueError(f"Query tensor q must be 4D (B, L, Hq, D), got shape {tuple(q.shape)}.")
