@@ -86,13 +86,15 @@ __global__ __launch_bounds__(64 * NW * KG, sizeof(T) == 2 ? 2 : 1) void k_attn(c
   // no maximum has to be known while the sums run.  Sums of exponentials up to
   // 2^kRange above it are as exact as any in a type with float32's range; the
   // rare row that goes beyond is found at the end, and the tile done again with
-  // the maxima that are known then.  float16 probabilities lose bits below 2^-14,
-  // half a step of theirs being 2^-25: the own key's is 2^4 there, so that they are
-  // right to 2^-29 of the largest whatever the other scores are, and a row's
-  // maximum may be 2^11 above its own score (7.6 in the exponent of e) before its
-  // tile is done again, with 2^14 at the maximum.
+  // the maxima that are known then.
+  // float16 has no such range, and loses bits below 2^-14: there the own key starts
+  // at 2^6, and a row whose largest gets to 2^15 has its reference raised on the way
+  // (raise_reference), and what is summed scaled down, so that the largest is 2^8.
+  // Half a step, 2^-25, is 2^-31 of a row's largest at most.  (2 x 8192 tokens at
+  // D = 128: 594 us, bf16 530; no such check but the own key at 2^-6, as far as the
+  // range allows without one, 545 with half of the probabilities' bits gone.)
   constexpr bool F16 = std::is_same<T, f16>::value;
-  constexpr float kRange = F16 ? 15.f : 60.f, kOwn = F16 ? 4.f : 0.f, kTop = F16 ? 14.f : 0.f;
+  constexpr float kRange = F16 ? 15.f : 60.f, kOwn = F16 ? 6.f : 0.f, kRaised = 8.f;
   f32x4 o[NQ][NC];
   float mx[NQ], top[NQ], sum[NQ];
 #pragma unroll
@@ -105,7 +107,8 @@ __global__ __launch_bounds__(64 * NW * KG, sizeof(T) == 2 ? 2 : 1) void k_attn(c
 #pragma unroll
       for (int e = 0; e < 8; ++e) x += (float)kf[e] * (float)qf[i][c][e];
     }
-    mx[i] = pos[i] < 0 ? 0.f : sum_q(x) * scale - kOwn;
+    const float own = sum_q(x) * scale;
+    mx[i] = pos[i] < 0 || own == -INFINITY ? 0.f : own - kOwn;
   }
   // At D = 256 a tile's loads go out in four parts between the products of the
   // tile before it: all at once they fill the memory queue, and the waves wait to
@@ -130,6 +133,23 @@ __global__ __launch_bounds__(64 * NW * KG, sizeof(T) == 2 ? 2 : 1) void k_attn(c
     fetch(std::integral_constant<int, 1>{});
     fetch(std::integral_constant<int, 2>{});
     fetch(std::integral_constant<int, 3>{});
+  };
+  auto raise_reference = [&] {
+    bool over = false;
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) over |= __builtin_fmaf(top[i], scale, -mx[i]) > kRange;
+    if (__builtin_expect(__any(over), 0)) {
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) {
+        const float t = max_q(top[i]) * scale;
+        const float m = t > mx[i] + kRange ? t - kRaised : mx[i];
+        const float f = fast_exp2(mx[i] - m);
+        mx[i] = m;
+        sum[i] *= f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) o[i][c] *= f;
+      }
+    }
   };
   bool odd = false;   // infinities or NaNs in a masked tile were left out
   // 32 keys of a tile; MASKED: some query must not see some of them.  At D = 256
@@ -163,7 +183,7 @@ __global__ __launch_bounds__(64 * NW * KG, sizeof(T) == 2 ? 2 : 1) void k_attn(c
     in_order();
     F pf[NQ];
 #pragma unroll
-    for (int i = 0; i < NQ; ++i) {
+    for (int i = 0; i < NQ; ++i)
 #pragma unroll
       for (int e = 0; e < 2; ++e)
 #pragma unroll
@@ -173,6 +193,14 @@ __global__ __launch_bounds__(64 * NW * KG, sizeof(T) == 2 ? 2 : 1) void k_attn(c
             sc[i][e][x] = key <= pos[i] && key >= low[i] ? sc[i][e][x] : -INFINITY;
           }
           top[i] = fmaxf(top[i], sc[i][e][x]);
+        }
+    if constexpr (F16) raise_reference();
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
           sc[i][e][x] = fast_exp2(__builtin_fmaf(sc[i][e][x], scale, -mx[i]));
           sum[i] += sc[i][e][x];
         }
@@ -240,20 +268,35 @@ __global__ __launch_bounds__(64 * NW * KG, sizeof(T) == 2 ? 2 : 1) void k_attn(c
     for (int i = 0; i < NQ; ++i) {
       top[i] = max_q(top[i]) * scale;
       over |= top[i] > mx[i] + kRange;
-      if (KG > 1 && q == 0) s_top[kg][(w * NQ + i) * 16 + r] = top[i];
+      if (!F16 && KG > 1 && q == 0) s_top[kg][(w * NQ + i) * 16 + r] = top[i];
     }
-    if (pass == 1 || !__syncthreads_or(over)) break;
+    if (F16 || pass == 1 || !__syncthreads_or(over)) break;
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
 #pragma unroll
       for (int g = 0; g < KG; ++g)
         if (KG > 1) top[i] = fmaxf(top[i], s_top[g][(w * NQ + i) * 16 + r]);
-      mx[i] = top[i] > mx[i] + kRange ? top[i] - kTop : mx[i];   // (the other rows keep their bits)
+      mx[i] = top[i] > mx[i] + kRange ? top[i] : mx[i];   // (the other rows keep their bits)
     }
     __syncthreads();
   }
 #pragma unroll
   for (int i = 0; i < NQ; ++i) sum[i] = sum_q(sum[i]);
+  if constexpr (F16 && KG > 1) {   // one reference for both sets of waves
+#pragma unroll
+    for (int i = 0; i < NQ; ++i)
+      if (q == 0) s_top[kg][(w * NQ + i) * 16 + r] = mx[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+      const float m = fmaxf(mx[i], s_top[kg ^ 1][(w * NQ + i) * 16 + r]);
+      const float f = fast_exp2(mx[i] - m);
+      mx[i] = m;
+      sum[i] *= f;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) o[i][c] *= f;
+    }
+  }
   if constexpr (KG > 1) {   // (2: the second set hands its sums over)
     static_assert(KG == 2 && BM * D * 4 <= sizeof(smem), "room for one set of sums");
     f32x4* os = reinterpret_cast<f32x4*>(smem) + w * NQ * NC * 64 + l;
@@ -283,7 +326,7 @@ __global__ __launch_bounds__(64 * NW * KG, sizeof(T) == 2 ? 2 : 1) void k_attn(c
     if (row >= rows) continue;
     const int t = over_g(p, row), g = row - t * p.G;
     const int64_t at = (int64_t)(s.c0 + t) * p.Hkv * p.G + h * p.G + g;
-    const float f = z == 0.f ? 0.f : 1.f / z;
+    const float f = pos[i] < 0 ? 0.f : 1.f / z;   // (a sum of 0 over keys that are seen is no number)
     T* op = (T*)p.out + at * D;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {

@@ -56,3 +56,24 @@ def test_paged_one_key_above_many(dev, page, new, other):
         c[pt[0, :L // page].long()] = x.view(L // page, page, Hkv, D).to(dev)
     out = paged_attention(q[-new:].to(dev), kc, vc, pt, sl, cu_seqlens=cu)
     _last(q, k, v, out[-1])
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("D", [64, 256])
+def test_rows_own_score_of_minus_infinity(dev, dt, D):
+    """A key that no query can choose, among them its own: it has no weight, and a
+    query that sees nothing else has no result."""
+    L, H, at = 300, 2, 200
+    q, k, v = (_rows(s, 1, L, H, D, dt=dt) for s in (1, 2, 3))
+    q[..., 0] = 1.0
+    shut = k.clone()
+    for i in (at, 150):
+        shut[0, i, :, 0] = -math.inf
+    seg = torch.tensor([0] * 150 + [1] * 150)
+    out = causal_attention(q.to(dev), shut.to(dev), v.to(dev), segment_ids=seg.to(dev))
+    vis = A.visible(L, L, 0, A.starts_of(seg.tolist()))
+    vis[:, [150, at]] = False
+    for h in range(H):
+        ref, _, tol = A.attend(q[0, :, h].double(), k[0, :, h].double(), v[0, :, h].double(), vis, 1.0 / math.sqrt(D), dt)
+        ref[150] = math.nan
+        _near(out[0, :, h], ref, tol, f"head {h}")
