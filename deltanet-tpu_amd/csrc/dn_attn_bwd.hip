@@ -19,6 +19,45 @@
 namespace dn {
 namespace {
 
+// float16 holds 2^-14 to 2^15 with all of its bits; probabilities of long rows and
+// score gradients of small cotangents lie below.  Probabilities carry 2^14
+// (kProb16, in the exponent that makes them).  Score gradients carry a power of two
+// per query (dQ) or key (dK): their largest so far is 2^7 to 2^15 with it, and when
+// one gets larger the power is lowered, and the sums made with it are too.
+// 2 x 8192 tokens, D = 128: 2310 us for the whole gradient, 2070 without (the check
+// splits what the compiler would interleave; the power in dQ's exponents and delta
+// in dP's accumulators, which saves as many instructions as this adds, spills: 2400).
+constexpr float kProb16 = 14.f, kFirst16 = 0x1p100f;
+template <int N, int NC> __device__ __forceinline__ void fit16(f32x4 (&d)[N][2], f32x4 (&acc)[N][NC], float (&power)[N]) {
+  float top[N];
+  bool over = false;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    top[i] = 0.f;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int z = 0; z < 4; ++z) top[i] = fmaxf(top[i], fabsf(d[i][e][z]));
+    over |= top[i] * power[i] > 0x1p15f;
+  }
+  if (__any(over)) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float m = max_q(top[i]);
+      const bool lower = m * power[i] > 0x1p15f && m < INFINITY;
+      const float next = lower ? __builtin_ldexpf(1.f, 8 - __builtin_amdgcn_frexp_expf(m)) : power[i];
+      const float f = next / power[i];
+      power[i] = next;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) acc[i][c] *= f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) d[i][e] *= power[i];
+}
+
 // delta = sum of d_out * (out + out_low) over a row's channels: D/8 lanes per row
 template <class T, int D>
 __global__ __launch_bounds__(256) void k_attn_delta(const AB p, int64_t rows) {
@@ -91,6 +130,7 @@ __global__ __launch_bounds__(512, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(const 
   using TL = Tile<T, D, BQ>;
   using F = typename At<T>::F;
   constexpr int NW = 8, BN = 64 * NK, NS = D / 32, NC = D / 16, RS = 32, NE = RS / 16;   // RS: query rows of a step
+  constexpr bool F16 = std::is_same<T, f16>::value;
   __shared__ __align__(16) T lds[4 * BQ * D];    // [2][q, d_out][BQ][D]
   __shared__ __align__(16) f32x4 px[2][4][NK * NE * 64];  // P of a step, by its parity and the pair, as accumulators
   __shared__ __align__(16) float ls[2][BQ], de[2][BQ];   // lse * log2(e) and delta per row
@@ -153,7 +193,7 @@ __global__ __launch_bounds__(512, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(const 
     if (threadIdx.x < BQ) {
       const int row = j * BQ + threadIdx.x, c = min(row, rows.last), tok = over_g(f, c);
       const int64_t at = ((int64_t)b * f.T + tok) * Hq + h * f.G + (c - tok * f.G);
-      m_ls = f.lse[at] * kLog2e;
+      m_ls = f.lse[at] * kLog2e - (F16 ? kProb16 : 0.f);
       m_de = p.delta[at];
       m_tk = row <= rows.last ? tok : -1;   // a row past the last one sees no key
       m_lw = low(tok);
@@ -161,6 +201,9 @@ __global__ __launch_bounds__(512, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(const 
     m_hi = low(over_g(f, min(j * BQ + BQ - 1, rows.last)));
   };
   bool odd = false;
+  float power[NK];   // of the keys' score gradients (F16)
+#pragma unroll
+  for (int i = 0; i < NK; ++i) power[i] = kFirst16;
   // The parts of a step of RS query rows.  Both waves multiply rows x by their own
   // operand (forward) and rows y, transposed, by the result (back).
   using Acc = f32x4[NK][NE];
@@ -225,6 +268,7 @@ __global__ __launch_bounds__(512, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(const 
           s[i][e][z] = MASKED && pr[i][e][z] == 0.f ? 0.f : d;   // (hidden rows of d_out may hold anything)
         }
     }
+    if constexpr (F16) fit16(s, acc, power);
   };
   auto back = [&](auto mask, const Acc& s, const T* y) {
     constexpr bool MASKED = decltype(mask)::value;
@@ -290,8 +334,10 @@ __global__ __launch_bounds__(512, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(const 
     const int t = key + 16 * i;
     if (t >= f.T) continue;
     const int64_t at = (((int64_t)b * f.T + t) * f.Hkv + h) * D;
+    const float back16 = first ? 0x1p-14f : 0x1p-14f / power[i];   // 2^-kProb16
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
+      if constexpr (F16) acc[i][c] *= back16;
       float x[4] = {acc[i][c][0], acc[i][c][1], acc[i][c][2], acc[i][c][3]};
       if (first && odd) {   // what the queries that see this key had left out of dV (dK of such a query is NaN by its scores)
 #pragma unroll 1
@@ -341,6 +387,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(con
   using TL = Tile<T, D, BN>;
   using F = typename At<T>::F;
   constexpr int BM = 16 * NQ * NW, NS = D / 32, NC = D / 16;
+  constexpr bool F16 = std::is_same<T, f16>::value;
   __shared__ __align__(16) T lds[4 * BN * D];   // [2][K, V][BN][D]
   const AF& f = p.f;
 
@@ -399,10 +446,13 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(con
   kr.last = vr.last = p1;
 
   f32x4 dq[NQ][NC];
+  float power[NQ];   // of the rows' score gradients (F16)
 #pragma unroll
-  for (int i = 0; i < NQ; ++i)
+  for (int i = 0; i < NQ; ++i) {
+    power[i] = kFirst16;
 #pragma unroll
     for (int c = 0; c < NC; ++c) dq[i][c] = zero4();
+  }
 
   auto fetch = [&](int j) {
     T* t = lds + (j & 1) * 2 * BN * D;
@@ -450,9 +500,8 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(con
           }
         }
     }
-    F df[NQ];
 #pragma unroll
-    for (int i = 0; i < NQ; ++i) {
+    for (int i = 0; i < NQ; ++i)
 #pragma unroll
       for (int e = 0; e < 2; ++e)
 #pragma unroll
@@ -464,8 +513,10 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(con
             dp[i][e][x] = key <= pos[i] && key >= low[i] ? dp[i][e][x] : 0.f;
           }
         }
-      df[i] = frag8<T>(dp[i][0], dp[i][1]);
-    }
+    if constexpr (F16) fit16(dp, dq, power);
+    F df[NQ];
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) df[i] = frag8<T>(dp[i][0], dp[i][1]);
     const bool bad = MASKED && TL::odd32(kt);   // (a query that sees such a key is NaN by its scores)
     F kc[2][4];
     batches<NC / 4, D == 256>([&](int b) {
@@ -504,8 +555,10 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(con
     if (row >= nrow) continue;
     const int t = over_g(f, row), g = row - t * f.G;
     T* op = (T*)p.dq + (((int64_t)b * f.T + t) * Hq + h * f.G + g) * D;
+    const float back16 = 1.f / power[i];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
+      if constexpr (F16) dq[i][c] *= back16;
       const float x[4] = {dq[i][c][0] * p.scale, dq[i][c][1] * p.scale, dq[i][c][2] * p.scale, dq[i][c][3] * p.scale};
       st4<T>(op + 16 * c + 4 * q, x);
     }
