@@ -466,7 +466,7 @@ class _AttentionFn(torch.autograd.Function):
         scale, window = ctx.meta
         if d_out is None:
             return (None,) * 6
-        d_out = d_out.contiguous()
+        d_out = _rows16(d_out.contiguous())   # (a concatenation hands out slices that start anywhere)
         dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
         if q.numel():
             block = _attention_block(q, k, v, out, low, lse, starts, scale, window)
