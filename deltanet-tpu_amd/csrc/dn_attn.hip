@@ -44,6 +44,11 @@ bool wide(const void* p, const int64_t* s, int dtype, int n) {
   return ((uintptr_t)p & 15) == 0;
 }
 
+// Rows and tokens are counted in 32 bits, in steps of up to 1024 past the last one.
+constexpr int64_t kMostIndex = ((int64_t)1 << 31) - 1024;
+// a window that no row is longer than is none
+int window_of(int window, int64_t most) { return window >= most ? 0 : window; }
+
 // checks that the entries share; NULL if all is well
 const char* shape_error(int64_t tokens, int Hq, int Hkv, int D, int dtype, float scale, int window) {
   if (D != 64 && D != 128 && D != 256) return "head dimension must be 64, 128 or 256";
@@ -52,7 +57,7 @@ const char* shape_error(int64_t tokens, int Hq, int Hkv, int D, int dtype, float
   const float e = scale * kLog2e;
   if (!(e - e == 0.f)) return "scale must be finite";
   if (window < 0) return "window must not be negative";
-  if (tokens * Hq >= ((int64_t)1 << 31)) return "too many query rows";
+  if (tokens * Hq >= kMostIndex) return "too many query rows";
   return nullptr;
 }
 
@@ -63,7 +68,8 @@ int paged_params(const dn_paged_attention_args* a, AF& p) {
   if (const char* m = shape_error(a->N, a->Hq, a->Hkv, a->D, a->dtype, a->scale, a->window)) return bad(m);
   if (a->pages <= 0 || a->max_pages <= 0 || a->page_size <= 0 || (a->page_size & (a->page_size - 1)))
     return bad("the cache needs pages of a power of two tokens");
-  if ((int64_t)a->max_pages * a->page_size >= ((int64_t)1 << 31)) return bad("a sequence must have fewer than 2^31 tokens");
+  const int64_t most = (int64_t)a->max_pages * a->page_size;
+  if (most >= kMostIndex) return bad("a sequence must have fewer than 2^31 - 1024 tokens");
   if (a->N && !a->B) return bad("tokens without a sequence");
   if (a->cu_seqlens == nullptr && a->B && a->N % a->B) return bad("without cu_seqlens every sequence has N / B new tokens");
   if (a->N && (!a->q || !a->k_cache || !a->v_cache || !a->out || !a->page_table || !a->seq_lens)) return bad("missing tensor pointer");
@@ -72,7 +78,7 @@ int paged_params(const dn_paged_attention_args* a, AF& p) {
     return bad("attention rows must start on 16 bytes");
   p.B = a->B; p.N = a->N; p.T = a->cu_seqlens ? 0 : a->B ? a->N / a->B : 0;
   set_heads(p, a->Hq, a->Hkv);
-  p.window = a->window;
+  p.window = window_of(a->window, most);
   p.pages = a->pages; p.max_pages = a->max_pages;
   while ((1 << p.shift) < a->page_size) ++p.shift;
   p.sc = a->scale * kLog2e;
@@ -109,7 +115,7 @@ extern "C" int dn_paged_attention(const dn_paged_attention_args* a, void* worksp
 }
 
 extern "C" int dn_document_starts(const void* seg, int32_t seg_dtype, int32_t batched, int32_t B, int32_t L, int32_t* starts, void* stream) {
-  if (B < 0 || L < 0 || (seg_dtype != DN_I32 && seg_dtype != DN_I64)) return bad("bad segment ids");
+  if (B < 0 || L < 0 || L >= kMostIndex || (seg_dtype != DN_I32 && seg_dtype != DN_I64)) return bad("bad segment ids");
   if (B == 0 || L == 0) return DN_OK;
   if (!seg || !starts) return bad("missing tensor pointer");
   hipLaunchKernelGGL(k_doc_starts, dim3(B), dim3(kScan), 0, (hipStream_t)stream, seg, seg_dtype == DN_I64, batched, L, starts);
@@ -129,7 +135,7 @@ int attention_params(const dn_attention_args* a, AF& p) {
     return bad("attention rows must start on 16 bytes");
   p.B = a->B; p.T = a->L; p.N = a->B * a->L;
   set_heads(p, a->Hq, a->Hkv);
-  p.window = a->window;
+  p.window = window_of(a->window, a->L);
   p.sc = a->scale * kLog2e;
   p.q = a->q; p.k = a->k; p.v = a->v; p.out = a->out; p.low = a->out_low; p.lse = a->lse; p.start = a->starts;
   for (int i = 0; i < 3; ++i) { p.qs[i] = a->q_strides[i]; p.ks[i] = a->k_strides[i]; p.vs[i] = a->v_strides[i]; }

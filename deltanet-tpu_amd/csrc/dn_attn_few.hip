@@ -62,7 +62,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_few(const AF p) {
     const int skip = u - t.first, take = min(t.units - skip, uend - u);
     const int j0 = k0 + skip, j1 = j0 + take;   // units of this piece
     const int last = max(p1, 0);
-    const int lo1 = p.window ? p1 - p.window + 1 : 0;
+    const int lo1 = first_key(p, p1);
 
     F qf[NQ][NS];
     int pos[NQ], low[NQ];
@@ -77,7 +77,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_few(const AF p) {
 #pragma unroll
         for (int c = 0; c < NS; ++c) qf[i][c] = minus8<T>(qf[i][c]);
       pos[i] = off + tk;
-      low[i] = p.window ? pos[i] - p.window + 1 : 0;
+      low[i] = first_key(p, pos[i]);
     }
 
 #pragma unroll
@@ -212,7 +212,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_few(const AF p) {
             const int key0 = j * kUnit + 32 * w;
             if (!(key0 + 31 > p0 || key0 < lo1)) continue;
 #pragma unroll 1
-            for (int key = max(key0, max(low[i], 0)); key <= min(key0 + 31, pos[i]); ++key)
+            for (int key = max(key0, low[i]); key <= min(key0 + 31, pos[i]); ++key)
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const float y = (float)rv(key)[16 * c + 4 * q + e];

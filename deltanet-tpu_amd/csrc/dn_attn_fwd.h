@@ -11,7 +11,7 @@ struct AF {
   int B, N, T;               // sequences; new tokens in all; per sequence (0: cu)
   int Hkv, G;                // query heads = Hkv * G, query head h reads key head h / G
   uint32_t gm; int gs;       // division by G (set_heads)
-  int window;                // keys that a query sees, itself the last; 0: all
+  int window;                // keys that a query sees, itself the last; 0: all (as for any that no row is longer than)
   int shift, pages, max_pages;
   float sc;                  // scale * log2(e), any sign
   const void *q, *k, *v;
@@ -121,10 +121,14 @@ __device__ __forceinline__ Span span_of(const AF& p, int b) {
   return s;
 }
 
+// The first key that a query at position pos sees by the window; positions below 0,
+// which see none, count as 0, so that no difference leaves 32 bits.
+__device__ __forceinline__ int first_key(const AF& p, int pos) { return p.window ? max(max(pos, 0) - p.window + 1, 0) : 0; }
+
 // Keys [lo, hi) that rows [row0, row1) of a sequence see between them, in units.
 __device__ __forceinline__ void units_of(const AF& p, const Span& s, int row0, int row1, int unit, int& u0, int& u1) {
   const int off = s.len - s.n, p0 = off + over_g(p, row0), p1 = off + over_g(p, row1 - 1);
-  u0 = p.window ? max(p0 - p.window + 1, 0) / unit : 0;
+  u0 = first_key(p, p0) / unit;
   u1 = p1 < 0 ? u0 : p1 / unit + 1;
   u1 = max(u1, u0 + 1);   // a tile without keys is work too: it writes zeros
 }

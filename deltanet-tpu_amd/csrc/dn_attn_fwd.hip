@@ -62,10 +62,10 @@ __global__ __launch_bounds__(64 * NW * KG, sizeof(T) == 2 ? 2 : 1) void k_attn(c
 #pragma unroll
       for (int c = 0; c < NS; ++c) qf[i][c] = minus8<T>(qf[i][c]);
     pos[i] = off + t;
-    low[i] = p.window ? pos[i] - p.window + 1 : 0;
+    low[i] = first_key(p, pos[i]);
     if (!PAGED && p.start) low[i] = max(low[i], p.start[s.b * p.T + t]);
   }
-  int lo0 = p.window ? max(p0 - p.window + 1, 0) : 0, lo1 = p.window ? p1 - p.window + 1 : 0;   // first keys of the first and last row
+  int lo0 = first_key(p, p0), lo1 = first_key(p, p1);   // first keys of the first and last row
   if (!PAGED && p.start) {
     lo0 = max(lo0, p.start[s.b * p.T + p0]);
     lo1 = max(lo1, p.start[s.b * p.T + p1]);
@@ -334,7 +334,7 @@ __global__ __launch_bounds__(64 * NW * KG, sizeof(T) == 2 ? 2 : 1) void k_attn(c
       if (odd) {
 #pragma unroll 1
         for (int key = j0 * BN; key < j1 * BN; ++key) {
-          if (key >= max(low[i], 0) && key <= pos[i] && (key / BN * BN + BN - 1 > p0 || key / BN * BN < lo1)) {
+          if (key >= low[i] && key <= pos[i] && (key / BN * BN + BN - 1 > p0 || key / BN * BN < lo1)) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const float y = (float)vr(key)[16 * c + 4 * q + e];

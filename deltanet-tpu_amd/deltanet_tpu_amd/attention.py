@@ -333,6 +333,10 @@ def _attention_common(D, Hq, Hkv, dtype, scale, window):
     return scale
 
 
+def _window(window):
+    return min(window or 0, 0x7fffffff)   # (rows are shorter)
+
+
 def paged_attention(q, k_cache, v_cache, page_table, seq_lens, *, cu_seqlens=None, scale=None, window=None,
                     return_lse: bool = False):
     """Causal attention of new tokens over a paged cache that holds their keys and
@@ -368,7 +372,7 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, *, cu_seqlens=Non
     out = q.new_empty(q.shape)
     lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device) if return_lse else None
     block = _lib.PAGED_ATTENTION_PACK(
-        _lib.DN_ABI_VERSION, N, B, Hq, Hkv, D, _DT[q.dtype], window or 0, pages, page, page_table.shape[1], scale,
+        _lib.DN_ABI_VERSION, N, B, Hq, Hkv, D, _DT[q.dtype], _window(window), pages, page, page_table.shape[1], scale,
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
         page_table.data_ptr(), seq_lens.data_ptr(), 0 if cu_seqlens is None else cu_seqlens.data_ptr(),
         qsb, qst, q.stride(-2), kcs[0], kcs[1], kcs[2], vcs[0], vcs[1], vcs[2], page_table.stride(0))
@@ -420,7 +424,7 @@ def _attention_block(q, k, v, out, low, lse, starts, scale, window):
     B, L, Hq, D = q.shape
     qs, ks, vs = q.stride(), k.stride(), v.stride()
     return _lib.ATTENTION_PACK(
-        _lib.DN_ABI_VERSION, B, L, Hq, k.shape[2], D, _DT[q.dtype], window or 0, scale, q.data_ptr(), k.data_ptr(),
+        _lib.DN_ABI_VERSION, B, L, Hq, k.shape[2], D, _DT[q.dtype], _window(window), scale, q.data_ptr(), k.data_ptr(),
         v.data_ptr(), out.data_ptr(), 0 if low is None else low.data_ptr(), 0 if lse is None else lse.data_ptr(), 0 if starts is None else starts.data_ptr(),
         qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2])
 

@@ -312,7 +312,8 @@ int dn_kv_append(const dn_kv_append_args* a, void* stream);
  * and lse -inf.  Page numbers outside the cache are read as its nearest page and
  * seq_lens past the page table as its end.  Nothing that a query must not see
  * reaches it, infinities and NaNs included.  scale: any finite number, 0 and
- * negative ones too. */
+ * negative ones too.  A window that reaches past the page table is none; page
+ * tables of 2^31 - 1024 tokens or more are refused. */
 typedef struct dn_paged_attention_args {
   int32_t abi_version;
   int32_t N, B, Hq, Hkv, D;     /* D: 64, 128 or 256                             */

@@ -26,3 +26,36 @@ def test_cotangent_off_16_bytes(dev, dt):
     got = torch.autograd.grad(whole, x, torch.cat([torch.ones(3, dtype=q.dtype, device=dev), do.flatten()]))
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 5, 2 ** 31, 2 ** 40])
+@pytest.mark.parametrize("wide", [False, True])
+def test_windows_past_every_key(dev, wide, window):
+    """A window that reaches past the first token is no window, for tokens of
+    positions below 0 next to others too."""
+    new, lens = [30, 1, 6, 1], [12, 700, 3, 0]
+    kc, vc, pt, sl, cu, ks, vs = _paged(9, new, lens, 2, 128, 16, "bf16", dev)
+    if wide:
+        pt = _wide(pt, 16)
+    q = _rows(10, sum(new), 8, 128)
+    out = paged_attention(q.to(dev), kc, vc, pt, sl, cu_seqlens=cu, window=window)
+    _check_paged(out, None, q, ks, vs, new, lens, "bf16")
+    assert torch.equal(out, paged_attention(q.to(dev), kc, vc, pt, sl, cu_seqlens=cu))
+    q, k, v, do = (t.to(dev) for t in _inputs(1, 150, 2, 1, 64, "bf16"))
+    assert torch.equal(causal_attention(q, k, v, window=window), causal_attention(q, k, v))
+    for a, b in zip(_grads(dev, q, k, v, do, window=window), _grads(dev, q, k, v, do)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("wide", [False, True])
+def test_window_of_the_capacity(dev, wide):
+    """The longest windows that hide something, at the cache's end and one token off."""
+    new, lens = [1, 2, 40], [320, 319, 320]
+    kc, vc, pt, sl, cu, ks, vs = _paged(9, new, lens, 1, 64, 16, "bf16", dev)
+    pt = _wide(pt, 16) if wide else pt[:, :20].contiguous()
+    q = _rows(10, sum(new), 4, 64)
+    for window in (318, 319, 320, 321):
+        _check_paged(paged_attention(q.to(dev), kc, vc, pt, sl, cu_seqlens=cu, window=window), None, q, ks, vs, new, lens, "bf16", window)
+    q, k, v = (_rows(s, 1, 150, 2, 64) for s in (1, 2, 3))
+    for window in (148, 149, 150, 151):
+        _check_rows(causal_attention(q.to(dev), k.to(dev), v.to(dev), window=window), None, q, k, v, "bf16", None, window)
