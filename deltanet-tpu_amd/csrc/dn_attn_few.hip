@@ -46,7 +46,9 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_few(const AF p) {
   T* vt = reinterpret_cast<T*>(smem + w * kV);
 
   const float scale = exponent_scale(p);
+  const Rest rest(p);
   const Plan plan(p, BM, kUnit);
+  rest.clear<T, D>(p);
   const int W = min((int)gridDim.x, plan.C);   // each has a unit at least
   if ((int)blockIdx.x >= W) return;
   int u = first_unit(blockIdx.x, W, plan.C);

@@ -107,6 +107,28 @@ __device__ __forceinline__ bool find_tile(const AF& p, int tile, int BM, Seq& s)
   return false;
 }
 
+// New tokens that cu gives to no sequence, in front of the first and after the last
+// (a batch of fixed size that is not full): [0, c0) and [c1, N).  Their results are
+// zeros (lse -inf), which all threads of a launch write together.
+struct Rest {
+  int c0, c1;
+  __device__ __forceinline__ Rest(const AF& p) : c0(0), c1(p.N) {
+    if (p.cu == nullptr) return;
+    c0 = min(max(p.cu[0], 0), p.N);
+    c1 = min(max(p.cu[p.B], c0), p.N);
+  }
+  template <class T, int D> __device__ __forceinline__ void clear(const AF& p) const {
+    if (c0 == 0 && c1 == p.N) return;
+    constexpr int per = D * sizeof(T) / 16;   // pieces of 16 bytes
+    const int64_t Hq = p.Hkv * p.G, n = (c0 + p.N - c1) * Hq * per;
+    for (int64_t x = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; x < n; x += (int64_t)gridDim.x * blockDim.x) {
+      const int64_t i = x / per, row = i < c0 * Hq ? i : i + (c1 - c0) * Hq;
+      *reinterpret_cast<f32x4*>((char*)p.out + (row * per + x % per) * 16) = zero4();
+      if (p.lse && x % per == 0) p.lse[row] = -INFINITY;
+    }
+  }
+};
+
 // A sequence of a paged call: its first new token among all, new tokens, tokens in all.
 struct Span { int c0, n, len; };
 __device__ __forceinline__ Span span_of(const AF& p, int b) {

@@ -35,7 +35,10 @@ __global__ __launch_bounds__(64 * NW * KG, sizeof(T) == 2 ? 2 : 1) void k_attn(c
   const int nt = gridDim.x / p.Hkv;
   const int h = blockIdx.x % p.Hkv;
   Seq s;
-  if (!find_tile(p, nt - 1 - (int)(blockIdx.x / p.Hkv), BM, s)) return;
+  const Rest rest(p);
+  const bool found = find_tile(p, nt - 1 - (int)(blockIdx.x / p.Hkv), BM, s);
+  if constexpr (PAGED) rest.clear<T, D>(p);
+  if (!found) return;
   s.b = __builtin_amdgcn_readfirstlane(s.b);
   s.c0 = __builtin_amdgcn_readfirstlane(s.c0);
   s.n = __builtin_amdgcn_readfirstlane(s.n);

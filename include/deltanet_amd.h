@@ -309,7 +309,8 @@ int dn_kv_append(const dn_kv_append_args* a, void* stream);
  * last `window` of them.  Positions, pages and sequences as in dn_kv_append_args
  * (the new tokens' keys and values are in the cache already); query head h reads
  * key head h / (Hq / Hkv).  A query without a key (a position below 0) gets zeros
- * and lse -inf.  Page numbers outside the cache are read as its nearest page and
+ * and lse -inf, and so does a token that cu_seqlens, which must not fall, gives to
+ * no sequence (before its first entry, from its last on).  Page numbers outside the cache are read as its nearest page and
  * seq_lens past the page table as its end.  Nothing that a query must not see
  * reaches it, infinities and NaNs included.  scale: any finite number, 0 and
  * negative ones too.  A window that reaches past the page table is none; page

@@ -59,3 +59,24 @@ def test_window_of_the_capacity(dev, wide):
     q, k, v = (_rows(s, 1, 150, 2, 64) for s in (1, 2, 3))
     for window in (148, 149, 150, 151):
         _check_rows(causal_attention(q.to(dev), k.to(dev), v.to(dev), window=window), None, q, k, v, "bf16", None, window)
+
+
+@pytest.mark.parametrize("before,after", [(0, 9), (3, 0), (40, 700), (1, 1)])
+@pytest.mark.parametrize("new,lens", [([1, 2, 1], [900, 30, 2]), ([70, 0, 130], [70, 9, 500]), ([0, 0], [4, 0])])
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("dt,D", [("bf16", 128), ("f32", 64), ("f16", 256)])
+def test_tokens_of_no_sequence(dev, dt, D, wide, new, lens, before, after):
+    """Tokens in front of cu_seqlens[0] and from cu_seqlens[-1] on get zeros (lse
+    -inf) whatever the memory of the result held; the others are what they are."""
+    kc, vc, pt, sl, cu, ks, vs = _paged(3, new, lens, 2, D, 16, dt, dev)
+    if wide:
+        pt = _wide(pt, 16)
+    n = sum(new)
+    q = _rows(4, before + n + after, 4, D, dt=dt)
+    full = lambda: (torch.full(q.shape, math.nan, dtype=q.dtype, device=dev), torch.full(q.shape[:2], math.nan, device=dev))
+    del [full()][:]   # (what the allocator hands out next)
+    out, lse = paged_attention(q.to(dev), kc, vc, pt, sl, cu_seqlens=cu + before, return_lse=True)
+    mid = slice(before, before + n)
+    _check_paged(out[mid], lse[mid], q[mid], ks, vs, new, lens, dt)
+    for s in (slice(0, before), slice(before + n, None)):
+        assert not out[s].any() and (lse[s] == -math.inf).all()
