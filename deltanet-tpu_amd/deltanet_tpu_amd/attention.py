@@ -16,6 +16,7 @@ import math
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _lib
 from .gdn2 import _DT, _is_integer_dtype, _raw_stream, _require_gpu
@@ -54,6 +55,18 @@ def _on_gpu(*ts):
     except AttributeError:
         pass
     return _require_gpu(*ts).index
+
+
+def _differentiated(*ts):
+    """Whether a derivative goes through one of them (None aside): backwards, or as a
+    forward-mode tangent, which no ``requires_grad`` shows."""
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    if _forward_ad._current_level >= 0:
+        return any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in ts)
+    return False
 
 
 def _dense_channels(t):
@@ -167,7 +180,7 @@ class _RotaryFn(torch.autograd.Function):
         if not given:
             return (None,) * 7
         a, b = given[0], given[1] if len(given) > 1 else None
-        if torch.is_grad_enabled():   # create_graph: the rotation of the gradients is differentiable in turn
+        if torch.is_grad_enabled() or _differentiated(a, b):   # create_graph: the rotation of the gradients is differentiable in turn
             turned = _RotaryFn.apply(a, b, pos, ps, table, interleaved, not inverse)
             turned = turned if b is not None else (turned, None)
         else:
@@ -187,8 +200,8 @@ def apply_rotary(q, k, positions, table, *, interleaved: bool = False):
     or (L,) for every row alike, (N,) for rank 3.  table: from ``rotary_table``.
     Pairs are (i, i + R/2), or (2i, 2i + 1) with ``interleaved``.  A position
     outside the table gives NaN in the rotated channels.  Products in float32,
-    one rounding.  Differentiable in q and k, any number of times.  Returns (q', k') with k' None if k
-    is None; the results are contiguous.
+    one rounding.  Differentiable in q and k, any number of times (backwards; tangents
+    are refused).  Returns (q', k') with k' None if k is None; the results are contiguous.
     """
     if q.ndim not in (3, 4):
         raise ValueError(f"q must have rank 3 (N, Hq, D) or rank 4 (B, L, Hq, D), got shape {tuple(q.shape)}.")
@@ -211,7 +224,7 @@ def apply_rotary(q, k, positions, table, *, interleaved: bool = False):
     if flat:
         q, k, ps = q[None], None if k is None else k[None], (0, ps[-1])
     q, k = _dense_channels(q), None if k is None else _dense_channels(k)
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    if _differentiated(q, k):
         r = _RotaryFn.apply(q, k, positions, ps, table, bool(interleaved), False)
         q_out, k_out = r if k is not None else (r, None)
     else:
@@ -288,7 +301,7 @@ def paged_kv_append(k, v, k_cache, v_cache, page_table, seq_lens, *, cu_seqlens=
     B, N, ksb, kst = _check_pages(page_table, seq_lens, cu_seqlens, k, "k")
     R = _check_table(table, D) if table is not None else 0
     vs, kcs, vcs = v.stride(), k_cache.stride(), v_cache.stride()
-    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
+    if _differentiated(k, v):
         raise ValueError("paged_kv_append is not differentiable; call it under torch.no_grad().")
     if N and pages:
         block = _lib.KV_APPEND_PACK(
@@ -360,7 +373,7 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, *, cu_seqlens=Non
     if q.dtype is not k_cache.dtype or q.shape[-1] != D:
         raise ValueError(f"q {tuple(q.shape)} {q.dtype} must have the cache's channels and type ({D}, {k_cache.dtype}).")
     dev = _on_gpu(q, k_cache, v_cache, page_table, seq_lens, cu_seqlens)
-    if torch.is_grad_enabled() and q.requires_grad:
+    if _differentiated(q):
         raise ValueError("paged_attention is not differentiable; use causal_attention for training.")
     q = _rows16(q)
     B, N, qsb, qst = _check_pages(page_table, seq_lens, cu_seqlens, q, "q")
@@ -480,7 +493,7 @@ class _AttentionFn(torch.autograd.Function):
             ws = q.new_empty(-(-need // q.element_size()))
             _call("dn_attention_bwd", q.get_device(), block, d_out.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                   ws.data_ptr(), need)
-        if torch.is_grad_enabled():   # create_graph
+        if torch.is_grad_enabled() or _differentiated(d_out):   # create_graph
             dq, dk, dv = _NoSecond.apply(dq, dk, dv, d_out, q, k, v)
         return dq, dk, dv, None, None, None
 
@@ -494,8 +507,8 @@ def causal_attention(q, k, v, *, segment_ids=None, cu_seqlens=None, scale=None, 
     to itself, or the last ``window`` of them.  scale: any finite number,
     1 / sqrt(D) unless given.  Sums and softmax statistics in float32.  Returns the
     output in q's shape and type, and with ``return_lse`` also the log of the sum of
-    exponentials (B, L, Hq) in float32.  Differentiable in q, k and v (not through the
-    lse); gradients come in the inputs' type, those of k and v summed over the heads
+    exponentials (B, L, Hq) in float32.  Differentiable in q, k and v (backwards and
+    once, not through the lse); gradients come in the inputs' type, those of k and v summed over the heads
     that share them, and are the same bits every time.
     """
     if q.ndim != 4:
@@ -513,7 +526,7 @@ def causal_attention(q, k, v, *, segment_ids=None, cu_seqlens=None, scale=None, 
     if segment_ids is not None or cu_seqlens is not None:
         starts = _document_starts(segment_ids, cu_seqlens, B, L, q.device)
     q, k, v = _rows16(q), _rows16(k), _rows16(v)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if _differentiated(q, k, v):
         out, lse = _AttentionFn.apply(q, k, v, starts, scale, window)
     else:
         out, _, lse = _attention_forward(q, k, v, starts, scale, window, return_lse)

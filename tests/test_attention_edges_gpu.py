@@ -80,3 +80,42 @@ def test_tokens_of_no_sequence(dev, dt, D, wide, new, lens, before, after):
     _check_paged(out[mid], lse[mid], q[mid], ks, vs, new, lens, dt)
     for s in (slice(0, before), slice(before + n, None)):
         assert not out[s].any() and (lse[s] == -math.inf).all()
+
+
+def test_forward_mode_tangents_are_refused(dev):
+    """A tangent that would be dropped raises; inputs without one work beside it."""
+    import torch.autograd.forward_ad as fwd
+    q, k, v, t = (torch.randn(1, 9, 2, 64, device=dev) for _ in range(4))
+    table, pos = rotary_table(16, 32, device=dev), torch.arange(9, device=dev)
+    kc, vc = (torch.randn(2, 16, 2, 64, device=dev) for _ in range(2))
+    pt, sl = torch.zeros(1, 1, dtype=torch.int32, device=dev), torch.full((1,), 9, dtype=torch.int32, device=dev)
+    want = causal_attention(q, k, v), apply_rotary(q, k, pos, table), paged_attention(q, kc, vc, pt, sl)
+    with fwd.dual_level():
+        dual = lambda x: fwd.make_dual(x, t)
+        for x in ((dual(q), k, v), (q, dual(k), v), (q, k, dual(v))):
+            with pytest.raises((RuntimeError, NotImplementedError), match="forward"):
+                causal_attention(*x)
+        for x in ((dual(q), k), (q, dual(k)), (dual(q), None)):
+            with pytest.raises((RuntimeError, NotImplementedError), match="forward"):
+                apply_rotary(*x, pos, table)
+        with pytest.raises(ValueError, match="not differentiable"):
+            paged_attention(dual(q), kc, vc, pt, sl)
+        with pytest.raises(ValueError, match="not differentiable"):
+            paged_kv_append(dual(k), v, kc, vc, pt, sl)
+        assert torch.equal(causal_attention(q, k, v), want[0])
+        assert torch.equal(apply_rotary(q, k, pos, table)[1], want[1][1])
+        assert torch.equal(paged_attention(q, kc, vc, pt, sl), want[2])
+
+
+def test_tangents_of_cotangents_are_refused(dev):
+    """Forward over reverse: the gradient of a dual cotangent."""
+    import torch.autograd.forward_ad as fwd
+    q = torch.randn(1, 9, 2, 64, device=dev, requires_grad=True)
+    w, t = torch.randn(1, 9, 2, 64, device=dev), torch.randn(1, 9, 2, 64, device=dev)
+    table, pos = rotary_table(16, 32, device=dev), torch.arange(9, device=dev)
+    for f in (lambda: causal_attention(q, q, q), lambda: apply_rotary(q, None, pos, table)[0]):
+        want, = torch.autograd.grad(f(), q, w)
+        with fwd.dual_level():
+            with pytest.raises((RuntimeError, NotImplementedError), match="forward"):
+                torch.autograd.grad(f(), q, fwd.make_dual(w, t))
+            assert torch.equal(torch.autograd.grad(f(), q, w)[0], want)
