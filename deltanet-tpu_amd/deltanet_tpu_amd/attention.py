@@ -301,7 +301,7 @@ def paged_kv_append(k, v, k_cache, v_cache, page_table, seq_lens, *, cu_seqlens=
     B, N, ksb, kst = _check_pages(page_table, seq_lens, cu_seqlens, k, "k")
     R = _check_table(table, D) if table is not None else 0
     vs, kcs, vcs = v.stride(), k_cache.stride(), v_cache.stride()
-    if _differentiated(k, v):
+    if _differentiated(k, v, k_cache, v_cache):
         raise ValueError("paged_kv_append is not differentiable; call it under torch.no_grad().")
     if N and pages:
         block = _lib.KV_APPEND_PACK(
@@ -373,7 +373,7 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, *, cu_seqlens=Non
     if q.dtype is not k_cache.dtype or q.shape[-1] != D:
         raise ValueError(f"q {tuple(q.shape)} {q.dtype} must have the cache's channels and type ({D}, {k_cache.dtype}).")
     dev = _on_gpu(q, k_cache, v_cache, page_table, seq_lens, cu_seqlens)
-    if _differentiated(q):
+    if _differentiated(q, k_cache, v_cache):
         raise ValueError("paged_attention is not differentiable; use causal_attention for training.")
     q = _rows16(q)
     B, N, qsb, qst = _check_pages(page_table, seq_lens, cu_seqlens, q, "q")

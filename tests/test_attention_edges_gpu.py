@@ -119,3 +119,32 @@ def test_tangents_of_cotangents_are_refused(dev):
             with pytest.raises((RuntimeError, NotImplementedError), match="forward"):
                 torch.autograd.grad(f(), q, fwd.make_dual(w, t))
             assert torch.equal(torch.autograd.grad(f(), q, w)[0], want)
+
+
+def test_caches_that_require_grad_are_refused(dev):
+    """Attention over a cache that requires grad, or a store in it, would lose it."""
+    q, k = torch.randn(1, 4, 64, device=dev), torch.randn(1, 2, 64, device=dev)
+    kc, vc = (torch.randn(2, 16, 2, 64, device=dev) for _ in range(2))
+    pt, sl = torch.zeros(1, 1, dtype=torch.int32, device=dev), torch.ones(1, dtype=torch.int32, device=dev)
+    g = lambda c: c.clone().requires_grad_(True)
+    for caches in ((g(kc), vc), (kc, g(vc))):
+        with pytest.raises(ValueError, match="not differentiable"):
+            paged_attention(q, *caches, pt, sl)
+        with pytest.raises(ValueError, match="not differentiable"):
+            paged_kv_append(k, k, *caches, pt, sl)
+        with torch.no_grad():
+            paged_attention(q, *caches, pt, sl)
+            paged_kv_append(k, k, *caches, pt, sl)
+
+
+def test_caches_with_tangents_are_refused(dev):
+    import torch.autograd.forward_ad as fwd
+    q, k = torch.randn(1, 4, 64, device=dev), torch.randn(1, 2, 64, device=dev)
+    kc, vc = (torch.randn(2, 16, 2, 64, device=dev) for _ in range(2))
+    pt, sl = torch.zeros(1, 1, dtype=torch.int32, device=dev), torch.ones(1, dtype=torch.int32, device=dev)
+    with fwd.dual_level():
+        dual = fwd.make_dual(kc, torch.ones_like(kc))
+        with pytest.raises(ValueError, match="not differentiable"):
+            paged_attention(q, dual, vc, pt, sl)
+        with pytest.raises(ValueError, match="not differentiable"):
+            paged_kv_append(k, k, dual, vc, pt, sl)
