@@ -28,6 +28,7 @@ _INT = {torch.int32: _lib.DN_I32, torch.int64: _lib.DN_I64}
 
 _current = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _calls = _lib._packed_calls
+_bump = torch.autograd.graph.increment_version
 
 
 def _call(name, dev, block, *args):
@@ -311,6 +312,9 @@ def paged_kv_append(k, v, k_cache, v_cache, page_table, seq_lens, *, cu_seqlens=
             table.data_ptr() if R else 0, ksb, kst, k.stride(-2), vs[0], vs[0] if v.ndim == 3 else vs[1], vs[-2],
             kcs[0], kcs[1], kcs[2], vcs[0], vcs[1], vcs[2], page_table.stride(0))
         _call("dn_kv_append", dev, block)
+        for c in (k_cache, v_cache):   # autograd sees the store (inference tensors have no version)
+            if not c.is_inference():
+                _bump(c)
     return k_cache, v_cache
 
 

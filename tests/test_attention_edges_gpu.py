@@ -148,3 +148,22 @@ def test_caches_with_tangents_are_refused(dev):
             paged_attention(q, dual, vc, pt, sl)
         with pytest.raises(ValueError, match="not differentiable"):
             paged_kv_append(k, k, dual, vc, pt, sl)
+
+
+def test_append_is_seen_as_a_write(dev):
+    """What autograd has kept of a cache is out of date after a store in it; caches
+    made in inference mode are stored in too."""
+    k = torch.randn(1, 2, 64, device=dev)
+    kc, vc = (torch.randn(2, 16, 2, 64, device=dev) for _ in range(2))
+    pt, sl = torch.zeros(1, 1, dtype=torch.int32, device=dev), torch.ones(1, dtype=torch.int32, device=dev)
+    w = torch.ones((), device=dev, requires_grad=True)
+    for c in (kc, vc):
+        y = (c * w).sum()
+        paged_kv_append(k, k, kc, vc, pt, sl)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    with torch.inference_mode():
+        kc, vc = (torch.zeros(2, 16, 2, 64, device=dev) for _ in range(2))
+        paged_kv_append(k, k, kc, vc, pt, sl)
+    paged_kv_append(k, 2 * k, kc, vc, pt, sl)
+    assert torch.equal(kc[0, 0], k[0]) and torch.equal(vc[0, 0], 2 * k[0])
