@@ -286,14 +286,12 @@ bool wide(const void* p, const int64_t* s, int n) {
   return aligned(p);
 }
 
-// Threads that fill the card a few times over: with fewer (token, item) pairs
-// than this each thread takes one head, with more it takes four and reads its
-// angles once for them.
-constexpr int64_t kManyThreads = 1 << 18;
-// A result larger than the L2s (8 x 4 MB) is not in them when it is read next:
-// stored past them, two heads per thread, 84 MB of queries and keys take 32.5 us
-// (5.2 TB/s) instead of 44.
-constexpr int64_t kCached = 32 << 20;
+// Threads of one head each that fill the card a few times over.  From there on (2^24
+// elements) a thread takes several heads and reads its angles once for them: four in
+// the append; two in the rotation, which stores past the caches, for its result does
+// not fit the L2s (8 x 4 MB) and is not in them when it is read next: 84 MB of queries
+// and keys take 32.5 us (5.2 TB/s) in place of 44.
+constexpr int64_t kManyThreads = 1 << 20;
 
 template <class F> void by_type(int dt, F f) {
   if (dt == DN_BF16) f((bf16)0.f);
@@ -334,8 +332,7 @@ extern "C" int dn_rotary(const dn_rotary_args* a, void* stream) {
   by_type(a->dtype, [&](auto z) {
     using T = decltype(z);
     if (!fast) hipLaunchKernelGGL((k_rotary_any<T>), dim3((unsigned)blocks, H), dim3(256), 0, st, p);
-    else if (n * H < 4 * kManyThreads) hipLaunchKernelGGL((k_rotary<T, 1, false>), dim3((unsigned)blocks, H), dim3(256), 0, st, p);
-    else if (N * H * a->D * (int64_t)sizeof(T) <= kCached) hipLaunchKernelGGL((k_rotary<T, 4, false>), dim3((unsigned)blocks, (H + 3) / 4), dim3(256), 0, st, p);
+    else if (n * H < kManyThreads) hipLaunchKernelGGL((k_rotary<T, 1, false>), dim3((unsigned)blocks, H), dim3(256), 0, st, p);
     else hipLaunchKernelGGL((k_rotary<T, 2, true>), dim3((unsigned)blocks, (H + 1) / 2), dim3(256), 0, st, p);
   });
   const hipError_t e = hipGetLastError();
@@ -375,7 +372,7 @@ extern "C" int dn_kv_append(const dn_kv_append_args* a, void* stream) {
       using T = decltype(z);
       using TC = decltype(zc);
       if (!fast) hipLaunchKernelGGL((k_append_any<T, TC>), dim3((unsigned)blocks, H2), dim3(256), 0, st, p);
-      else if (n * H2 < 4 * kManyThreads || a->H % 4) hipLaunchKernelGGL((k_append<T, TC, 1>), dim3((unsigned)blocks, H2), dim3(256), 0, st, p);
+      else if (n * H2 < kManyThreads || a->H % 4) hipLaunchKernelGGL((k_append<T, TC, 1>), dim3((unsigned)blocks, H2), dim3(256), 0, st, p);
       else hipLaunchKernelGGL((k_append<T, TC, 4>), dim3((unsigned)blocks, H2 / 4), dim3(256), 0, st, p);
     });
   });
