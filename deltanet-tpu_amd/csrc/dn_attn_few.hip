@@ -258,7 +258,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_few(const AF p) {
       if (whole) {
         const int tk = over_g(p, row0 + row), g = row0 + row - tk * p.G;
         const int64_t at = (int64_t)(t.s.c0 + tk) * p.Hkv * p.G + t.h * p.G + g;
-        const float f = z == 0.f ? 0.f : 1.f / z;
+        const float f = off + tk < 0 ? 0.f : 1.f / z;   // (a sum of 0 over keys that are seen is no number)
         const float y[4] = {a[0] * f, a[1] * f, a[2] * f, a[3] * f};
         st4<T>((T*)p.out + at * D + 4 * ch, y);
         if (p.lse && ch == 0) p.lse[at] = z == 0.f ? -INFINITY : kLn2 * (m + __log2f(z));
@@ -324,7 +324,7 @@ __global__ __launch_bounds__(256) void k_attn_join(const AF p, int groups) {
     z = z * f + g * ps[k][D + 1];
     m = n;
   }
-  const float f = z == 0.f ? 0.f : 1.f / z;
+  const float f = t.s.len - t.s.n + i - t.s.c0 < 0 ? 0.f : 1.f / z;   // (as above)
   const float y[4] = {a[0] * f, a[1] * f, a[2] * f, a[3] * f};
   st4<T>((T*)p.out + (int64_t)blockIdx.x * D + 4 * ch, y);
   if (p.lse && ch == 0) p.lse[blockIdx.x] = z == 0.f ? -INFINITY : kLn2 * (m + __log2f(z));

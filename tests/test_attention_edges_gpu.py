@@ -167,3 +167,29 @@ def test_append_is_seen_as_a_write(dev):
         paged_kv_append(k, k, kc, vc, pt, sl)
     paged_kv_append(k, 2 * k, kc, vc, pt, sl)
     assert torch.equal(kc[0, 0], k[0]) and torch.equal(vc[0, 0], 2 * k[0])
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("n", [1, 5])
+def test_keys_that_cannot_be_chosen(dev, dt, n):
+    """Scores of -inf have no weight; a query that sees no other key has no result,
+    the same in the kernels of few and of many rows, in one workgroup or several."""
+    new, lens = [n, n, 1], [40, 1500, 0]
+    kc, vc, pt, sl, cu, ks, vs = _paged(3, new, lens, 1, 64, 16, dt, dev)
+    q = _rows(4, sum(new), 2, 64, dt=dt)
+    q[..., 0] = 1.0
+    kc[pt[0, :3].long(), :, :, 0] = -math.inf                     # all of sequence 0
+    for at in (3, 700, 1499):                                     # some of sequence 1
+        kc[int(pt[1, at // 16]), at % 16, :, 0] = -math.inf
+    for table in (pt, _wide(pt, 16)):
+        out, lse = paged_attention(q.to(dev), kc, vc, table, sl, cu_seqlens=cu, return_lse=True)
+        assert torch.isnan(out[:n]).all() and not torch.isfinite(lse[:n]).any()
+        assert not out[2 * n:].any()
+        vis = A.visible(n, 1500, 1500 - n)
+        vis[:, [3, 700, 1499]] = False
+        for h in range(2):
+            ref, _, tol = A.attend(q[n:2 * n, h].double(), ks[1][:, 0].double(), vs[1][:, 0].double(), vis, 0.125, dt)
+            _near(out[n:2 * n, h], ref, tol, f"head {h}")
+    big = torch.full((1, 200, 1, 64), -math.inf, dtype=A.DT[dt], device=dev)   # (every row, whole rows)
+    one = torch.ones(1, 200, 2, 64, dtype=A.DT[dt], device=dev)
+    assert torch.isnan(causal_attention(one, big, one[:, :, :1])).all()
