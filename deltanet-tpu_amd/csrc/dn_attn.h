@@ -57,6 +57,14 @@ template <class T> __device__ __forceinline__ typename At<T>::F frag8(const f32x
   return __builtin_convertvector((f8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}), typename At<T>::F);
 }
 
+// What that rounding cut off, itself rounded.
+template <class T> __device__ __forceinline__ typename At<T>::F rest8(const f32x4& a, const f32x4& b, const typename At<T>::F& f) {
+  f32x4 x, y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = a[e] - (float)f[e], y[e] = b[e] - (float)f[4 + e];
+  return frag8<T>(x, y);
+}
+
 // A value and the one of the lane N (32, 16) lanes away, in either order.
 template <int N> __device__ __forceinline__ void both(float x, float& a, float& b) {
   const unsigned u = __builtin_bit_cast(unsigned, x);
