@@ -156,10 +156,12 @@ __global__ __launch_bounds__(64 * NW * KG, sizeof(T) == 2 ? 2 : 1) void k_attn(c
   };
   bool odd = false;   // infinities or NaNs in a masked tile were left out
   // 32 keys of a tile; MASKED: some query must not see some of them.  16-bit types
-  // multiply the values by such tiles' probabilities in two parts, SPLIT: short rows
-  // and documents lie in them, where the rounding of few probabilities is an error of
-  // the output (2.1e-3 of it in bf16, 1.65e-3 with both parts) and, by the row sums
-  // that read it, of the gradient (dq 2.5e-3, 2.4e-3).  At D = 256
+  // multiply the values by such tiles' probabilities in two parts, SPLIT, where a
+  // gradient may follow: short rows and documents lie in them, where the rounding of
+  // few probabilities is an error of the output (2.0e-3 to 2.1e-3 of it in bf16, 1.5e-3
+  // with both parts) and, by the row sums that read it, of the gradient (dq 2.6e-3,
+  // 2.35e-3).  (Over pages: 86.6 to 89.3 us under a window of 1024, 12 x
+  // 400 tokens over 3000.)  At D = 256
   // the first values are read under the exponentials and the others VB operands
   // ahead, in this order (1006 against 1066 us for 2 x 4096 tokens over 4096 cached); at 128 the
   // compiler's own order is better (601 against 668 us for 2 x 8192).
@@ -168,7 +170,7 @@ __global__ __launch_bounds__(64 * NW * KG, sizeof(T) == 2 ? 2 : 1) void k_attn(c
     if constexpr (D == 256) __builtin_amdgcn_sched_barrier(0);
   };
   auto step = [&](auto masked, auto between, const T* kt, const T* vt, int key0) {
-    constexpr bool MASKED = decltype(masked)::value, SPLIT = MASKED && sizeof(T) == 2;
+    constexpr bool MASKED = decltype(masked)::value, SPLIT = MASKED && !PAGED && sizeof(T) == 2;
     f32x4 sc[NQ][2];
 #pragma unroll
     for (int i = 0; i < NQ; ++i) sc[i][0] = sc[i][1] = zero4();
