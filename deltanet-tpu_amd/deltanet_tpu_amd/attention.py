@@ -28,7 +28,8 @@ _INT = {torch.int32: _lib.DN_I32, torch.int64: _lib.DN_I64}
 
 _current = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _calls = _lib._packed_calls
-_bump = torch.autograd.graph.increment_version
+_grad_enabled = torch.is_grad_enabled
+_bump = getattr(torch._C, "_increment_version", torch.autograd.graph.increment_version)
 
 
 def _call(name, dev, block, *args):
@@ -61,13 +62,11 @@ def _on_gpu(*ts):
 def _differentiated(*ts):
     """Whether a derivative goes through one of them (None aside): backwards, or as a
     forward-mode tangent, which no ``requires_grad`` shows."""
-    if torch.is_grad_enabled():
+    if _grad_enabled():
         for t in ts:
             if t is not None and t.requires_grad:
                 return True
-    if _forward_ad._current_level >= 0:
-        return any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in ts)
-    return False
+    return _forward_ad._current_level >= 0 and any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in ts)
 
 
 def _dense_channels(t):
@@ -312,9 +311,8 @@ def paged_kv_append(k, v, k_cache, v_cache, page_table, seq_lens, *, cu_seqlens=
             table.data_ptr() if R else 0, ksb, kst, k.stride(-2), vs[0], vs[0] if v.ndim == 3 else vs[1], vs[-2],
             kcs[0], kcs[1], kcs[2], vcs[0], vcs[1], vcs[2], page_table.stride(0))
         _call("dn_kv_append", dev, block)
-        for c in (k_cache, v_cache):   # autograd sees the store (inference tensors have no version)
-            if not c.is_inference():
-                _bump(c)
+        # autograd sees the store (inference tensors have no version)
+        _bump([c for c in (k_cache, v_cache) if not c.is_inference()])
     return k_cache, v_cache
 
 
