@@ -11,7 +11,7 @@
 //
 // 64 sequences of up to 16384 tokens (2.2 GB of keys and values, D = 128): 409 + 9 us,
 // 5.4 TB/s, where a copy reaches 5.2; 32 drafts of up to 5 tokens (283 MB, D = 256):
-// 63 to 68 + 6 us; one token over 1000: 10 + 5 us, the chain of lengths, page table,
+// 62 to 70 + 6 us; one token over 1000: 10 + 5 us, the chain of lengths, page table,
 // keys, products and the join.
 #include <type_traits>
 

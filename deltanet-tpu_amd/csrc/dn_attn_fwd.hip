@@ -2,13 +2,14 @@
 //
 // One pass over the keys per tile of query rows (rows of a key head's whole group,
 // token first, so that a tile of keys is read once for all of them): S^T = K Q^T,
-// exponentials against a reference that is known before the loop, O^T += V^T P^T,
-// everything in registers but the tiles of keys and values, which direct loads
-// bring into LDS a tile ahead.  Bound by the matrix units and what keeps them
-// waiting, LDS reads and the exponentials of two waves per SIMD: 46 % of the
-// matrix units' time at 2 x 8192 tokens, D = 128 (550 to 580 us, 970 TFLOP/s), 41 %
-// at D = 256 (prompts of 4096 over 4096 cached: 900 us, 915 TFLOP/s), where each LDS
-// operand serves 16 rows, not 32.  A library product reaches 1414 TFLOP/s here.
+// exponentials against a reference that is known before the loop (and raised within
+// it in float16 alone), O^T += V^T P^T, everything in registers but the tiles of keys
+// and values, which direct loads bring into LDS a tile ahead.  Bound by the matrix
+// units and what keeps them waiting, LDS reads and the exponentials of two waves per
+// SIMD: 46 % of the matrix units' time at 2 x 8192 tokens, D = 128 (525 to 580 us,
+// 950 to 1050 TFLOP/s), 43 % at D = 256 (prompts of 4096 over 4096 cached: 860 to 900
+// us, 915 to 957 TFLOP/s), where each LDS operand serves 16 rows, not 32.  A library
+// product reaches 1414 TFLOP/s here.
 #include <type_traits>
 
 #include "dn_attn_fwd.h"
