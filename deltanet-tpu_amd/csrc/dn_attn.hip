@@ -114,6 +114,37 @@ extern "C" int dn_paged_attention(const dn_paged_attention_args* a, void* worksp
   return e == hipSuccess ? DN_OK : set_error(DN_E_LAUNCH, hipGetErrorString(e));
 }
 
+namespace {
+// (units of a call are counted in 32 bits: 32 keys of a tile of 16 rows at the least)
+int tree_params(const dn_paged_attention_args* a, const uint64_t* visible, int words, AF& p) {
+  if (const int rc = paged_params(a, p)) return rc;
+  if (words < 1 || words > 16) return bad("trees have 1 to 16 words of visible tokens");
+  if (a->window && a->window < 64 * words) return bad("the window of a tree must take in its words");
+  if (p.N && !visible) return bad("missing tensor pointer");
+  if (p.N && ((int64_t)p.N * p.G / 16 + p.B) * p.Hkv * ((((int64_t)p.max_pages << p.shift) + 31) / 32) >= (int64_t)1 << 31)
+    return bad("too many rows over too many tokens");
+  p.vis = visible; p.words = words;
+  return DN_OK;
+}
+}  // namespace
+
+extern "C" size_t dn_paged_tree_attention_workspace_size(const dn_paged_attention_args* a, int32_t words) {
+  AF p{};
+  if (tree_params(a, reinterpret_cast<const uint64_t*>(8), words, p) != DN_OK || p.N == 0) return 0;
+  return attn_tree_bytes(p, a->D, a->dtype) + 256;
+}
+
+extern "C" int dn_paged_tree_attention(const dn_paged_attention_args* a, const uint64_t* visible, int32_t words, void* workspace,
+                                       size_t workspace_bytes, void* stream) {
+  AF p{};
+  if (const int rc = tree_params(a, visible, words, p)) return rc;
+  if (p.N == 0) return DN_OK;
+  if (!workspace || workspace_bytes < attn_tree_bytes(p, a->D, a->dtype) + 256) return set_error(DN_E_WORKSPACE, "workspace missing or too small");
+  p.part = (float*)(((uintptr_t)workspace + 255) & ~(uintptr_t)255);
+  const hipError_t e = attn_tree(p, a->D, a->dtype, (hipStream_t)stream);
+  return e == hipSuccess ? DN_OK : set_error(DN_E_LAUNCH, hipGetErrorString(e));
+}
+
 extern "C" int dn_document_starts(const void* seg, int32_t seg_dtype, int32_t batched, int32_t B, int32_t L, int32_t* starts, void* stream) {
   if (B < 0 || L < 0 || L >= kMostIndex || (seg_dtype != DN_I32 && seg_dtype != DN_I64)) return bad("bad segment ids");
   if (B == 0 || L == 0) return DN_OK;

@@ -15,7 +15,7 @@
 // keys, products and the join.
 #include <type_traits>
 
-#include "dn_attn_fwd.h"
+#include "dn_attn_split.h"
 
 namespace dn {
 namespace {
@@ -23,12 +23,9 @@ namespace {
 constexpr int kWaves = 4, kUnit = 32 * kWaves;
 constexpr int kGroups = 512;   // workgroups of a launch: two per CU
 
-__device__ __forceinline__ int first_unit(int w, int W, int C) { return (int)((int64_t)w * C / W); }
-
-// A partial result: BM rows of D sums, then BM maxima, then BM sums of exponentials.
-template <int D, int BM> constexpr int64_t slot_floats() { return (int64_t)BM * (D + 2); }
-
-template <class T, int D, int NQ>
+// TREE: which of its sequence's new tokens a row sees stands in its words (tree_bits);
+// the keys in front of them are those of every row.
+template <class T, int D, int NQ, bool TREE>
 __global__ __launch_bounds__(64 * kWaves) void k_attn_few(const AF p) {
   using TL = Tile<T, D, 32>;
   using F = typename At<T>::F;
@@ -47,7 +44,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_few(const AF p) {
 
   const float scale = exponent_scale(p);
   const Rest rest(p);
-  const Plan plan(p, BM, kUnit);
+  const PlanOf<TREE> plan(p, BM, kUnit);
   rest.clear<T, D>(p);
   const int W = min((int)gridDim.x, plan.C);   // each has a unit at least
   if ((int)blockIdx.x >= W) return;
@@ -58,13 +55,14 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_few(const AF p) {
     Task t;
     if (!plan.of_unit(u, t)) break;
     const int rows = t.s.n * p.G, row0 = t.m * BM, row1 = min(row0 + BM, rows);
-    const int off = t.s.len - t.s.n, p0 = off + over_g(p, row0), p1 = off + over_g(p, row1 - 1);
+    // the keys that all rows see end with p0, those that any sees with p1
+    const int off = t.s.len - t.s.n, p0 = TREE ? off - 1 : off + over_g(p, row0), p1 = TREE ? t.s.len - 1 : off + over_g(p, row1 - 1);
     int k0, k1;
-    units_of(p, t.s, row0, row1, kUnit, k0, k1);
+    units_of<TREE>(p, t.s, row0, row1, kUnit, k0, k1);
     const int skip = u - t.first, take = min(t.units - skip, uend - u);
     const int j0 = k0 + skip, j1 = j0 + take;   // units of this piece
     const int last = max(p1, 0);
-    const int lo1 = first_key(p, p1);
+    const int lo1 = first_key(p, p1);   // (none later, of any row)
 
     F qf[NQ][NS];
     int pos[NQ], low[NQ];
@@ -78,9 +76,10 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_few(const AF p) {
       if (p.sc < 0.f)
 #pragma unroll
         for (int c = 0; c < NS; ++c) qf[i][c] = minus8<T>(qf[i][c]);
-      pos[i] = off + tk;
-      low[i] = first_key(p, pos[i]);
+      pos[i] = TREE ? t.s.c0 + tk : off + tk;   // trees: the token, whose words say what it sees
+      low[i] = TREE ? tree_low(p, tree_words(p, pos[i]), off, t.s.n) : first_key(p, pos[i]);
     }
+    auto bits_of = [&](int i, int key0) { return tree_bits(p, tree_words(p, pos[i]), off, t.s.len, low[i], key0); };
 
 #pragma unroll
     for (int i = 0; i < NQ; ++i)
@@ -156,12 +155,14 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_few(const AF p) {
 #pragma unroll
       for (int i = 0; i < NQ; ++i) {
         if (masked) {
+          const uint32_t bits = TREE ? bits_of(i, key0) >> (4 * q) : 0;
 #pragma unroll
           for (int e = 0; e < 2; ++e)
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
               const int key = key0 + 16 * e + 4 * q + x;
-              sc[i][e][x] = key <= pos[i] && key >= low[i] ? sc[i][e][x] : -INFINITY;
+              const bool sees = TREE ? bits >> (16 * e + x) & 1 : key <= pos[i] && key >= low[i];
+              sc[i][e][x] = sees ? sc[i][e][x] : -INFINITY;
             }
         }
         const float m = fmaxf(fmaxf(fmaxf(sc[i][0][0], sc[i][0][1]), fmaxf(sc[i][0][2], sc[i][0][3])),
@@ -214,9 +215,10 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_few(const AF p) {
             const int key0 = j * kUnit + 32 * w;
             if (!(key0 + 31 > p0 || key0 < lo1)) continue;
 #pragma unroll 1
-            for (int key = max(key0, low[i]); key <= min(key0 + 31, pos[i]); ++key)
+            for (int key = max(key0, low[i]); key <= min(key0 + 31, TREE ? p1 : pos[i]); ++key)
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
+                if (TREE && !(bits_of(i, key0) >> (key - key0) & 1)) continue;
                 const float y = (float)rv(key)[16 * c + 4 * q + e];
                 if (!__builtin_isfinite(y)) o[i][c][e] += y;
               }
@@ -258,7 +260,8 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_few(const AF p) {
       if (whole) {
         const int tk = over_g(p, row0 + row), g = row0 + row - tk * p.G;
         const int64_t at = (int64_t)(t.s.c0 + tk) * p.Hkv * p.G + t.h * p.G + g;
-        const float f = off + tk < 0 ? 0.f : 1.f / z;   // (a sum of 0 over keys that are seen is no number)
+        const bool none = TREE ? tree_empty(p, t.s.c0 + tk, t.s) : off + tk < 0;
+        const float f = none ? 0.f : 1.f / z;   // (a sum of 0 over keys that are seen is no number)
         const float y[4] = {a[0] * f, a[1] * f, a[2] * f, a[3] * f};
         st4<T>((T*)p.out + at * D + 4 * ch, y);
         if (p.lse && ch == 0) p.lse[at] = z == 0.f ? -INFINITY : kLn2 * (m + __log2f(z));
@@ -275,61 +278,6 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_few(const AF p) {
   }
 }
 
-// Joins the parts of a query row if more than one workgroup had some: D/4 threads
-// per part, 1024/D parts at a time.
-template <class T, int D, int BM>
-__global__ __launch_bounds__(256) void k_attn_join(const AF p, int groups) {
-  constexpr int NP = 1024 / D;
-  __shared__ float ps[NP][D + 4];
-  Task t;
-  int row;
-  const int Hq = p.Hkv * p.G, i = blockIdx.x / Hq, hq = blockIdx.x - i * Hq;
-  const Plan plan(p, BM, kUnit);
-  const int W = min(groups, plan.C);
-  if (!plan.of_row(i, hq, t, row)) return;
-  // the workgroup that has unit u: the last w with w C / W <= u
-  auto owner = [&](int u) { return (int)((((int64_t)u + 1) * W + plan.C - 1) / plan.C) - 1; };
-  const int w0 = owner(t.first), w1 = owner(t.first + t.units - 1);
-  if (w0 == w1) return;
-  row -= t.m * BM;
-  const int ch = threadIdx.x % (D / 4), part = threadIdx.x / (D / 4);
-  f32x4 a = zero4();
-  float m = -INFINITY, z = 0.f;
-#pragma unroll 4
-  for (int w = w0 + part; w <= w1; w += NP) {
-    const float* s = p.part + (2 * (int64_t)w + (w == w0 ? 1 : 0)) * slot_floats<D, BM>();
-    const f32x4 y = *reinterpret_cast<const f32x4*>(s + row * D + 4 * ch);
-    const float mw = s[BM * D + row], zw = s[BM * D + BM + row];
-    const float n = fmaxf(m, mw);
-    const float f = m == -INFINITY ? 0.f : fast_exp2(m - n), g = mw == -INFINITY ? 0.f : fast_exp2(mw - n);
-    if (f != 1.f) a *= f;
-    if (g != 0.f) a += g * y;
-    z = z * f + g * zw;
-    m = n;
-  }
-  *reinterpret_cast<f32x4*>(&ps[part][4 * ch]) = a;
-  if (ch == 0) {
-    ps[part][D] = m;
-    ps[part][D + 1] = z;
-  }
-  __syncthreads();
-  if (part) return;
-#pragma unroll
-  for (int k = 1; k < NP; ++k) {
-    const float mw = ps[k][D], n = fmaxf(m, mw);
-    const float f = m == -INFINITY ? 0.f : fast_exp2(m - n), g = mw == -INFINITY ? 0.f : fast_exp2(mw - n);
-    const f32x4 y = *reinterpret_cast<const f32x4*>(&ps[k][4 * ch]);
-    if (f != 1.f) a *= f;
-    if (g != 0.f) a += g * y;
-    z = z * f + g * ps[k][D + 1];
-    m = n;
-  }
-  const float f = t.s.len - t.s.n + i - t.s.c0 < 0 ? 0.f : 1.f / z;   // (as above)
-  const float y[4] = {a[0] * f, a[1] * f, a[2] * f, a[3] * f};
-  st4<T>((T*)p.out + (int64_t)blockIdx.x * D + 4 * ch, y);
-  if (p.lse && ch == 0) p.lse[blockIdx.x] = z == 0.f ? -INFINITY : kLn2 * (m + __log2f(z));
-}
-
 int row_tile(const AF& p) { return (int64_t)p.N * p.G <= (int64_t)16 * p.B ? 16 : 32; }
 int64_t most_tasks(const AF& p) {
   const int BM = row_tile(p);
@@ -339,14 +287,14 @@ int64_t most_tasks(const AF& p) {
 int64_t most_units(const AF& p) { return most_tasks(p) * ((((int64_t)p.max_pages << p.shift) + kUnit - 1) / kUnit); }
 int64_t groups_of(const AF& p) { return std::min<int64_t>(kGroups, most_units(p)); }
 
-template <class T, int D> hipError_t run(const AF& p, hipStream_t st) {
+template <class T, int D, bool TREE> hipError_t run(const AF& p, hipStream_t st) {
   const unsigned W = (unsigned)groups_of(p), rows = (unsigned)p.N * p.Hkv * p.G;
   if (row_tile(p) == 16) {
-    hipLaunchKernelGGL((k_attn_few<T, D, 1>), dim3(W), dim3(64 * kWaves), 0, st, p);
-    if (W > 1) hipLaunchKernelGGL((k_attn_join<T, D, 16>), dim3(rows), dim3(256), 0, st, p, (int)W);
+    hipLaunchKernelGGL((k_attn_few<T, D, 1, TREE>), dim3(W), dim3(64 * kWaves), 0, st, p);
+    if (W > 1) hipLaunchKernelGGL((k_attn_join<T, D, 16, kUnit, TREE>), dim3(rows), dim3(256), 0, st, p, (int)W);
   } else {
-    hipLaunchKernelGGL((k_attn_few<T, D, 2>), dim3(W), dim3(64 * kWaves), 0, st, p);
-    if (W > 1) hipLaunchKernelGGL((k_attn_join<T, D, 32>), dim3(rows), dim3(256), 0, st, p, (int)W);
+    hipLaunchKernelGGL((k_attn_few<T, D, 2, TREE>), dim3(W), dim3(64 * kWaves), 0, st, p);
+    if (W > 1) hipLaunchKernelGGL((k_attn_join<T, D, 32, kUnit, TREE>), dim3(rows), dim3(256), 0, st, p, (int)W);
   }
   return hipGetLastError();
 }
@@ -387,7 +335,8 @@ size_t attn_few_bytes(const AF& p, int D) { return (size_t)groups_of(p) * 2 * ro
 hipError_t attn_few(const AF& p, int D, int dtype, hipStream_t st) {
   auto go = [&](auto z) {
     using T = decltype(z);
-    return D == 64 ? run<T, 64>(p, st) : D == 128 ? run<T, 128>(p, st) : run<T, 256>(p, st);
+    if (p.vis) return D == 64 ? run<T, 64, true>(p, st) : D == 128 ? run<T, 128, true>(p, st) : run<T, 256, true>(p, st);
+    return D == 64 ? run<T, 64, false>(p, st) : D == 128 ? run<T, 128, false>(p, st) : run<T, 256, false>(p, st);
   };
   return dtype == DN_BF16 ? go((bf16)0.f) : dtype == DN_F16 ? go((f16)0.f) : go(0.f);
 }

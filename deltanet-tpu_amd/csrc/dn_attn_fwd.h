@@ -23,6 +23,8 @@ struct AF {
   const int32_t* start;      // contiguous: NULL or the first token of each token's document (B, T)
   int64_t qs[3], ks[3], vs[3];   // batch or page, token, head
   int64_t pts;
+  const uint64_t* vis;       // trees: (tokens, words) bits of the new tokens that a new token sees
+  int words;
 };
 
 // Rows of K or V in memory: contiguous, or through a page table.
@@ -147,9 +149,53 @@ __device__ __forceinline__ Span span_of(const AF& p, int b) {
 // which see none, count as 0, so that no difference leaves 32 bits.
 __device__ __forceinline__ int first_key(const AF& p, int pos) { return p.window ? max(max(pos, 0) - p.window + 1, 0) : 0; }
 
+// Drafted trees.  A new token sees the keys in front of its sequence's new tokens, the
+// window aside, and of those the ones whose bit is set in its words: key `off` is new
+// token 0.  low: the first key that a window of all that it sees leaves (at least 64
+// words of it, so that no new token falls out).
+__device__ __forceinline__ const uint64_t* tree_words(const AF& p, int token) { return p.vis + (int64_t)token * p.words; }
+__device__ __forceinline__ int tree_count(const AF& p, const uint64_t* w, int off, int n) {
+  int c = 0;
+  for (int i = 0; i < p.words && 64 * i < n; ++i) {
+    uint64_t x = w[i];
+    if (n - 64 * i < 64) x &= (1ull << (n - 64 * i)) - 1;
+    const int d = -off - 64 * i;   // new tokens at positions below 0 are none
+    if (d > 0) x = d < 64 ? x >> d << d : 0;
+    c += __popcll(x);
+  }
+  return c;
+}
+__device__ __forceinline__ int tree_low(const AF& p, const uint64_t* w, int off, int n) {
+  return p.window ? max(off + tree_count(p, w, off, n) - p.window, 0) : 0;
+}
+__device__ __forceinline__ bool tree_empty(const AF& p, int token, const Span& s) {
+  const int off = s.len - s.n;
+  return off <= 0 && tree_count(p, tree_words(p, token), off, s.n) == 0;
+}
+// Which of the 32 keys from key0 on it sees.
+__device__ __forceinline__ uint32_t tree_bits(const AF& p, const uint64_t* w, int off, int len, int low, int key0) {
+  const int rel = key0 - off;
+  uint32_t m = ~0u;
+  if (rel > -32) {
+    uint64_t x = 0;
+    if (rel < 0) {
+      x = w[0] << -rel | ((1ull << -rel) - 1);
+    } else {
+      const int i = rel >> 6, s = rel & 63;
+      if (i < p.words) x = w[i] >> s;
+      if (s > 32 && i + 1 < p.words) x |= w[i + 1] << (64 - s);
+    }
+    m = (uint32_t)x;
+  }
+  if (low > key0) m &= low - key0 < 32 ? ~0u << (low - key0) : 0;
+  if (len - key0 < 32) m &= len > key0 ? (1u << (len - key0)) - 1 : 0;
+  return m;
+}
+
 // Keys [lo, hi) that rows [row0, row1) of a sequence see between them, in units.
+template <bool TREE = false>
 __device__ __forceinline__ void units_of(const AF& p, const Span& s, int row0, int row1, int unit, int& u0, int& u1) {
-  const int off = s.len - s.n, p0 = off + over_g(p, row0), p1 = off + over_g(p, row1 - 1);
+  const int off = s.len - s.n, p0 = TREE ? off - 1 : off + over_g(p, row0), p1 = TREE ? s.len - 1 : off + over_g(p, row1 - 1);
   u0 = first_key(p, p0) / unit;
   u1 = p1 < 0 ? u0 : p1 / unit + 1;
   u1 = max(u1, u0 + 1);   // a tile without keys is work too: it writes zeros
@@ -176,13 +222,13 @@ __device__ __forceinline__ int scan(int x) {   // inclusive, over a wave
   }
   return x;
 }
-struct Plan {
+template <bool TREE> struct PlanOf {
   const AF& p;
   int BM, unit;
   Span s0;       // of sequence `lane`
   int mine0, sum0;   // its units over all heads, and with those before it
   int C;         // units of the call
-  __device__ __forceinline__ Plan(const AF& p_, int BM_, int unit_) : p(p_), BM(BM_), unit(unit_) {
+  __device__ __forceinline__ PlanOf(const AF& p_, int BM_, int unit_) : p(p_), BM(BM_), unit(unit_) {
     load(0, s0, mine0);
     sum0 = scan(mine0);
     C = __builtin_amdgcn_readfirstlane(__shfl(sum0, 63));
@@ -200,9 +246,15 @@ struct Plan {
     if (b >= p.B) return;
     s = span_of(p, b);
     const int rows = s.n * p.G;
+    if constexpr (TREE) {   // (all its tiles see the same)
+      int u0, u1;
+      units_of<TREE>(p, s, 0, 1, unit, u0, u1);
+      mine = (u1 - u0) * ((rows + BM - 1) / BM) * p.Hkv;
+      return;
+    }
     for (int r = 0; r < rows; r += BM) {
       int u0, u1;
-      units_of(p, s, r, min(r + BM, rows), unit, u0, u1);
+      units_of<TREE>(p, s, r, min(r + BM, rows), unit, u0, u1);
       mine += u1 - u0;
     }
     mine *= p.Hkv;
@@ -235,7 +287,7 @@ struct Plan {
   __device__ __forceinline__ int tile_units(const Task& t, int m) const {
     int u0, u1;
     const int rows = t.s.n * p.G;
-    units_of(p, t.s, m * BM, min((m + 1) * BM, rows), unit, u0, u1);
+    units_of<TREE>(p, t.s, m * BM, min((m + 1) * BM, rows), unit, u0, u1);
     return u1 - u0;
   }
   // the task that holds unit u < C
@@ -244,6 +296,12 @@ struct Plan {
     if (!find([&](const Span&, int sum) { return sum > u; }, t, per)) return false;
     t.h = (u - t.first) / per;
     t.first += t.h * per;
+    if constexpr (TREE) {
+      t.units = tile_units(t, 0);
+      t.m = (u - t.first) / t.units;
+      t.first += t.m * t.units;
+      return true;
+    }
     for (t.m = 0;; ++t.m) {   // (one tile in all but ragged calls)
       t.units = tile_units(t, t.m);
       if (u < t.first + t.units) return true;
@@ -258,11 +316,18 @@ struct Plan {
     row = (i - t.s.c0) * p.G + hq - t.h * p.G;
     t.m = row / BM;
     t.first += t.h * per;
+    if constexpr (TREE) {
+      t.units = tile_units(t, 0);
+      t.first += t.m * t.units;
+      return true;
+    }
     for (int m = 0; m < t.m; ++m) t.first += tile_units(t, m);
     t.units = tile_units(t, t.m);
     return true;
   }
 };
+
+using Plan = PlanOf<false>;
 
 // Attention over many rows per sequence (training, prompts): head dimension and
 // type checked by the caller.
@@ -273,6 +338,10 @@ hipError_t attn_many(const AF& p, int D, int dtype, bool paged, hipStream_t st);
 bool attn_few_takes(const AF& p, int D, int dtype);
 size_t attn_few_bytes(const AF& p, int D);
 hipError_t attn_few(const AF& p, int D, int dtype, hipStream_t st);
+
+// The same for drafted trees (p.vis set), of any number of rows and any pages.
+size_t attn_tree_bytes(const AF& p, int D, int dtype);
+hipError_t attn_tree(const AF& p, int D, int dtype, hipStream_t st);
 
 // The gradient (contiguous rows): p with out, lse and start of the forward, d_out
 // dense, the three gradients dense, delta (tokens, Hkv G) floats of scratch.

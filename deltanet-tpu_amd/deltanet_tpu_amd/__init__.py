@@ -1,10 +1,12 @@
 """deltanet_tpu_amd: MI355X-native (gfx950 HIP) drop-in for the forward
 delta-rule recurrence core of maelie-labs/deltanet-tpu (chunk_gdn2,
 gdn2_decode_step and their variants).  See ``gdn2.py`` for the API, and
-``attention.py`` for the softmax-attention layers of a hybrid model."""
+``attention.py`` and ``serving.py`` for the softmax-attention layers of a hybrid
+model."""
 
-from .attention import apply_rotary, causal_attention, paged_attention, paged_kv_append, rotary_table
+from .attention import apply_rotary, causal_attention, norm_rotary, paged_attention, paged_kv_append, rotary_table
 from .gdn2 import chunk_gdn2, gdn2_decode_step, gdn2_decode_steps
+from .serving import page_pool, paged_kv_keep, paged_qkv_append, paged_reserve, paged_slots, paged_tree_attention
 from .variants import (
     chunk_delta_rule,
     chunk_gdn,
@@ -32,8 +34,15 @@ __all__ = [
     "delta_rule_decode_step",
     "rotary_table",
     "apply_rotary",
+    "norm_rotary",
     "paged_kv_append",
     "paged_attention",
     "causal_attention",
+    "page_pool",
+    "paged_reserve",
+    "paged_slots",
+    "paged_qkv_append",
+    "paged_tree_attention",
+    "paged_kv_keep",
     "__version__",
 ]

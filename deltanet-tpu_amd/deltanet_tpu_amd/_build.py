@@ -13,7 +13,7 @@ CSRC = os.path.join(PKG_ROOT, "csrc")
 INCLUDE = os.path.join(REPO_ROOT, "include")
 SOURCES = ("dn_prefill.hip", "dn_prefill_long.hip", "dn_backward.hip", "dn_decode.hip",
            "dn_rotary.hip", "dn_attn.hip", "dn_attn_fwd.hip", "dn_attn_few.hip",
-           "dn_attn_bwd.hip")
+           "dn_attn_bwd.hip", "dn_attn_tree.hip", "dn_norm.hip", "dn_pages.hip")
 OUT = os.path.join(HERE, "libdeltanet_amd.so")
 
 

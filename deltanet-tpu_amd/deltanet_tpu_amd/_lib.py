@@ -145,11 +145,80 @@ class AttentionArgs(ctypes.Structure):
     ]
 
 
+class NormRotaryArgs(ctypes.Structure):
+    """Mirror of ``dn_norm_rotary_args``."""
+
+    _fields_ = [
+        ("abi_version", _c_i32),
+        ("B", _c_i32), ("L", _c_i32), ("Hq", _c_i32), ("Hk", _c_i32), ("D", _c_i32), ("R", _c_i32),
+        ("dtype", _c_i32), ("weight_dtype", _c_i32), ("pos_dtype", _c_i32), ("interleaved", _c_i32), ("rows", _c_i32),
+        ("eps", ctypes.c_float), ("weight_offset", ctypes.c_float),
+        ("q", _c_ptr), ("k", _c_ptr), ("q_weight", _c_ptr), ("k_weight", _c_ptr), ("q_out", _c_ptr), ("k_out", _c_ptr),
+        ("pos", _c_ptr), ("table", _c_ptr),
+        ("q_strides", _c_i64 * 3), ("k_strides", _c_i64 * 3), ("pos_strides", _c_i64 * 2),
+    ]
+
+
+class NormRotaryGrads(ctypes.Structure):
+    """Mirror of ``dn_norm_rotary_grads``."""
+
+    _fields_ = [
+        ("d_q", _c_ptr), ("d_k", _c_ptr), ("dq", _c_ptr), ("dk", _c_ptr), ("dq_weight", _c_ptr), ("dk_weight", _c_ptr),
+        ("d_q_strides", _c_i64 * 3), ("d_k_strides", _c_i64 * 3),
+    ]
+
+
+class QkvAppendArgs(ctypes.Structure):
+    """Mirror of ``dn_qkv_append_args``."""
+
+    _fields_ = [
+        ("abi_version", _c_i32),
+        ("B", _c_i32), ("L", _c_i32), ("Hq", _c_i32), ("Hkv", _c_i32), ("D", _c_i32), ("R", _c_i32),
+        ("dtype", _c_i32), ("cache_dtype", _c_i32), ("weight_dtype", _c_i32), ("pos_dtype", _c_i32),
+        ("interleaved", _c_i32), ("rows", _c_i32), ("pages", _c_i32), ("page_size", _c_i32),
+        ("eps", ctypes.c_float), ("weight_offset", ctypes.c_float),
+        ("q", _c_ptr), ("k", _c_ptr), ("v", _c_ptr), ("q_weight", _c_ptr), ("k_weight", _c_ptr), ("q_out", _c_ptr),
+        ("k_cache", _c_ptr), ("v_cache", _c_ptr), ("slots", _c_ptr), ("pos", _c_ptr), ("table", _c_ptr),
+        ("q_strides", _c_i64 * 3), ("k_strides", _c_i64 * 3), ("v_strides", _c_i64 * 3), ("kc_strides", _c_i64 * 3),
+        ("vc_strides", _c_i64 * 3),
+    ]
+
+
+class PagedSlotsArgs(ctypes.Structure):
+    """Mirror of ``dn_paged_slots_args``."""
+
+    _fields_ = [
+        ("abi_version", _c_i32),
+        ("N", _c_i32), ("B", _c_i32), ("page_size", _c_i32), ("max_pages", _c_i32), ("words", _c_i32),
+        ("page_table", _c_ptr), ("seq_lens", _c_ptr), ("cu_seqlens", _c_ptr), ("held", _c_ptr), ("parents", _c_ptr),
+        ("positions", _c_ptr), ("slots", _c_ptr), ("visible", _c_ptr),
+        ("page_table_stride", _c_i64),
+    ]
+
+
+class KvKeepArgs(ctypes.Structure):
+    """Mirror of ``dn_kv_keep_args``."""
+
+    _fields_ = [
+        ("abi_version", _c_i32),
+        ("layers", _c_i32), ("B", _c_i32), ("H", _c_i32), ("D", _c_i32), ("most", _c_i32), ("dtype", _c_i32),
+        ("pages", _c_i32), ("page_size", _c_i32), ("max_pages", _c_i32),
+        ("k_cache", _c_ptr), ("v_cache", _c_ptr), ("page_table", _c_ptr), ("starts", _c_ptr), ("kept", _c_ptr), ("lens", _c_ptr),
+        ("kc_strides", _c_i64 * 4), ("vc_strides", _c_i64 * 4), ("page_table_stride", _c_i64),
+    ]
+
+
 # The same blocks in one call (the order and alignment of the fields above).
 ROTARY_PACK = struct.Struct("@12i6P8q").pack
 KV_APPEND_PACK = struct.Struct("@13i8P13q").pack
 PAGED_ATTENTION_PACK = struct.Struct("@11if8P10q").pack
 ATTENTION_PACK = struct.Struct("@8if7P9q").pack
+NORM_ROTARY_PACK = struct.Struct("@12i2f8P8q").pack
+NORM_ROTARY_GRADS_PACK = struct.Struct("@6P6q").pack
+QKV_APPEND_PACK = struct.Struct("@15i2f11P15q").pack
+PAGED_SLOTS_PACK = struct.Struct("@6i8Pq").pack
+KV_KEEP_PACK = struct.Struct("@10i6P9q").pack
+MAX_SEQUENCES = 4096   # DN_MAX_SEQUENCES
 
 
 EXPORTED_SYMBOLS = (
@@ -171,6 +240,15 @@ EXPORTED_SYMBOLS = (
     "dn_attention_fwd",
     "dn_attention_bwd_workspace_size",
     "dn_attention_bwd",
+    "dn_norm_rotary",
+    "dn_norm_rotary_bwd_workspace_size",
+    "dn_norm_rotary_bwd",
+    "dn_qkv_append",
+    "dn_paged_reserve",
+    "dn_paged_slots",
+    "dn_paged_tree_attention_workspace_size",
+    "dn_paged_tree_attention",
+    "dn_kv_keep",
     "dn_last_error",
     "dn_abi_version",
     "dn_profile_begin",
@@ -206,18 +284,32 @@ _PACKED = {   # argument types behind the packed argument block, and the result'
     "dn_attention_fwd": ([_c_ptr], ctypes.c_int),
     "dn_attention_bwd_workspace_size": ([], ctypes.c_size_t),
     "dn_attention_bwd": ([_c_ptr] * 5 + [ctypes.c_size_t, _c_ptr], ctypes.c_int),
+    "dn_norm_rotary": ([_c_ptr], ctypes.c_int),
+    "dn_norm_rotary_bwd_workspace_size": ([], ctypes.c_size_t),
+    "dn_norm_rotary_bwd": ([ctypes.c_char_p, _c_ptr, ctypes.c_size_t, _c_ptr], ctypes.c_int),
+    "dn_qkv_append": ([_c_ptr], ctypes.c_int),
+    "dn_paged_slots": ([_c_ptr], ctypes.c_int),
+    "dn_paged_tree_attention_workspace_size": ([_c_i32], ctypes.c_size_t),
+    "dn_paged_tree_attention": ([_c_ptr, _c_i32, _c_ptr, ctypes.c_size_t, _c_ptr], ctypes.c_int),
+    "dn_kv_keep": ([_c_ptr], ctypes.c_int),
+}
+_PLAIN = {   # entries without an argument block
+    "dn_paged_reserve": [_c_ptr, _c_i32, _c_ptr, _c_i64, _c_i32, _c_i32, _c_i32, _c_ptr, _c_ptr, _c_ptr, _c_ptr],
 }
 
 
 def packed_call(name):
     """An entry point of the loaded library that takes its argument block as
-    packed bytes."""
+    packed bytes (or, of ``_PLAIN``, its arguments one by one)."""
     f = _packed_calls.get(name)
     if f is None:
         lib = load_library()
         f = getattr(ctypes.CDLL(lib._name, handle=lib._handle), name)
-        args, f.restype = _PACKED[name]
-        f.argtypes = [ctypes.c_char_p, *args]
+        if name in _PLAIN:
+            f.argtypes, f.restype = _PLAIN[name], ctypes.c_int
+        else:
+            args, f.restype = _PACKED[name]
+            f.argtypes = [ctypes.c_char_p, *args]
         _packed_calls[name] = f
     return f
 

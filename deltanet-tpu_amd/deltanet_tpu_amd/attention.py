@@ -21,7 +21,7 @@ from torch.autograd import forward_ad as _forward_ad
 from . import _lib
 from .gdn2 import _DT, _is_integer_dtype, _raw_stream, _require_gpu
 
-__all__ = ["rotary_table", "apply_rotary", "paged_kv_append", "paged_attention", "causal_attention"]
+__all__ = ["rotary_table", "apply_rotary", "norm_rotary", "paged_kv_append", "paged_attention", "causal_attention"]
 
 _INT = {torch.int32: _lib.DN_I32, torch.int64: _lib.DN_I64}
 
@@ -229,6 +229,158 @@ def apply_rotary(q, k, positions, table, *, interleaved: bool = False):
         q_out, k_out = r if k is not None else (r, None)
     else:
         q_out, k_out = _rotary_launch(q, k, positions, ps, table, interleaved, False)
+    if flat:
+        q_out, k_out = q_out[0], None if k_out is None else k_out[0]
+    return q_out, k_out
+
+
+# ---------------------------------------------------------------------------
+# norms of heads
+# ---------------------------------------------------------------------------
+
+def _finite(name, x):
+    try:
+        x = float(x)
+    except (TypeError, ValueError) as e:
+        raise ValueError(f"{name} must be convertible to a concrete float, got {type(x)}: {e}")
+    if not abs(x) <= 3e38:
+        raise ValueError(f"{name} must be finite in float32, got {x}.")
+    return x
+
+
+def _check_norm(eps, offset):
+    eps, offset = _finite("eps", eps), _finite("weight_offset", offset)
+    if eps < 0.0:
+        raise ValueError(f"eps must not be negative, got {eps}.")
+    return eps, offset
+
+
+def _check_weights(D, *ws):
+    for w in ws:
+        if w.dtype not in _DT or w.dtype is not ws[0].dtype or w.shape != (D,) or (D > 1 and w.stride(0) != 1):
+            raise ValueError(f"norm weights must be contiguous ({D},) tensors of one type, float32, bfloat16 or float16, got {w.dtype} {tuple(w.shape)}.")
+
+
+def _norm_block(q, k, qw, kw, q_out, k_out, pos, ps, table, eps, offset, interleaved):
+    one = k if q is None else q
+    B, L, _, D = one.shape
+    none = (0, 0, 0)
+    sq, sk = none if q is None else q.stride(), none if k is None else k.stride()
+    at = lambda t: 0 if t is None else t.data_ptr()
+    return _lib.NORM_ROTARY_PACK(
+        _lib.DN_ABI_VERSION, B, L, 0 if q is None else q.shape[2], 0 if k is None else k.shape[2], D, 0 if table is None else table.shape[1],
+        _DT[one.dtype], _DT[(kw if q is None else qw).dtype], _lib.DN_I32 if pos is None else _INT[pos.dtype], 1 if interleaved else 0,
+        0 if table is None else table.shape[0], eps, offset, at(q), at(k), at(qw), at(kw), at(q_out), at(k_out), at(pos), at(table),
+        sq[0], sq[1], sq[2], sk[0], sk[1], sk[2], ps[0], ps[1])
+
+
+def _norm_launch(q, k, qw, kw, pos, ps, table, eps, offset, interleaved):
+    q_out, k_out = q.new_empty(q.shape), None if k is None else k.new_empty(k.shape)
+    _call("dn_norm_rotary", q.get_device(), _norm_block(q, k, qw, kw, q_out, k_out, pos, ps, table, eps, offset, interleaved))
+    return q_out, k_out
+
+
+class _NormRotaryFn(torch.autograd.Function):
+    """Keeps the inputs; the backward computes the heads' norms again."""
+
+    @staticmethod
+    def forward(ctx, q, k, qw, kw, pos, ps, table, eps, offset, interleaved):
+        ctx.save_for_backward(q, k, qw, kw, pos, table)
+        ctx.meta = ps, eps, offset, interleaved
+        ctx.set_materialize_grads(False)
+        q_out, k_out = _norm_launch(q, k, qw, kw, pos, ps, table, eps, offset, interleaved)
+        return (q_out, k_out) if k is not None else q_out
+
+    @staticmethod
+    def backward(ctx, dq, dk=None):
+        q, k, qw, kw, pos, table = ctx.saved_tensors
+        ps, eps, offset, interleaved = ctx.meta
+        if dq is None and dk is None:
+            return (None,) * 10
+        d_q, d_k = (None if g is None else _dense_channels(g) for g in (dq, dk))
+        # a side whose result nobody used has no gradient
+        q, qw = (None, None) if d_q is None else (q, qw)
+        k, kw = (None, None) if d_k is None else (k, kw)
+        new = lambda t: None if t is None else t.new_empty(t.shape)
+        gq, gk = new(q), new(k)
+        gqw, gkw = (torch.zeros_like(w) if w is not None and not one.numel() else new(w) for w, one in ((qw, q), (kw, k)))
+        one = k if q is None else q
+        if one.shape[0] * one.shape[1]:
+            block = _norm_block(q, k, qw, kw, None, None, pos, ps, table, eps, offset, interleaved)
+            at = lambda t: 0 if t is None else t.data_ptr()
+            none = (0, 0, 0)
+            sq, sk = none if d_q is None else d_q.stride(), none if d_k is None else d_k.stride()
+            grads = _lib.NORM_ROTARY_GRADS_PACK(at(d_q), at(d_k), at(gq), at(gk), at(gqw), at(gkw), *sq[:3], *sk[:3])
+            need = _lib.packed_call("dn_norm_rotary_bwd_workspace_size")(block)
+            ws = torch.empty(-(-need // 4), dtype=torch.float32, device=one.device)
+            _call("dn_norm_rotary_bwd", one.get_device(), block, grads, ws.data_ptr(), need)
+        if torch.is_grad_enabled() or _differentiated(d_q, d_k):   # create_graph
+            gq, gk, gqw, gkw = _NoSecondNorm.apply(gq, gk, gqw, gkw, d_q, d_k, q, k, qw, kw)
+        return gq, gk, gqw, gkw, None, None, None, None, None, None
+
+
+class _NoSecondNorm(torch.autograd.Function):
+    """Gradients that depend on the cotangents and the inputs, whose own gradient is refused."""
+
+    @staticmethod
+    def forward(ctx, gq, gk, gqw, gkw, *_):
+        return gq, gk, gqw, gkw
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("norm_rotary is once_differentiable: the gradient of its gradient is not implemented.")
+
+
+def norm_rotary(q, k, q_weight, k_weight, positions=None, table=None, *, eps: float = 1e-6, weight_offset: float = 0.0,
+                interleaved: bool = False):
+    """Queries and keys normed head by head, y = x / sqrt(mean(x^2) + eps) *
+    (weight_offset + weight), and then rotated as by ``apply_rotary``, in one pass.
+
+    q: (B, L, Hq, D) or (N, Hq, D); k: the same with Hk heads, or None (with k_weight
+    None); both float32, bfloat16 or float16, channels contiguous, any other strides.
+    q_weight, k_weight: (D,), both of one of these types.  weight_offset: 1 for
+    weights kept as differences from 1.  positions, table, interleaved: as in
+    ``apply_rotary``; neither positions nor table: no rotation.  Statistics and
+    products in float32, one rounding at the end.  Differentiable in q, k and the
+    weights (backwards and once; tangents are refused); the weights' gradients are
+    summed in float32 and are the same bits every time.  Returns (q', k') with k' None
+    if k is None; the results are contiguous.
+    """
+    if q.ndim not in (3, 4):
+        raise ValueError(f"q must have rank 3 (N, Hq, D) or rank 4 (B, L, Hq, D), got shape {tuple(q.shape)}.")
+    if q.dtype not in _DT:
+        raise ValueError(f"q must be float32, bfloat16 or float16, got {q.dtype}.")
+    if k is not None and (k.ndim != q.ndim or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1] or k.dtype != q.dtype):
+        raise ValueError(f"k {tuple(k.shape)} {k.dtype} must match q {tuple(q.shape)} {q.dtype} in all but the heads.")
+    if (k is None) != (k_weight is None) or (positions is None) != (table is None):
+        raise ValueError("k goes with k_weight, and positions with table.")
+    D = q.shape[-1]
+    if D < 1:
+        raise ValueError("q must have a channel.")
+    _check_weights(D, *([q_weight] if k is None else [q_weight, k_weight]))
+    eps, weight_offset = _check_norm(eps, weight_offset)
+    if table is not None:
+        _check_table(table, D)
+        if positions.dtype not in _INT:
+            raise ValueError(f"positions must be int32 or int64, got {positions.dtype}.")
+    _on_gpu(q, k, q_weight, k_weight, positions, table)
+    lead, ps = q.shape[:-2], (0, 0)
+    if positions is not None:
+        if positions.shape == lead:
+            ps = positions.stride()
+        elif positions.ndim == 1 and positions.shape[0] == lead[-1]:
+            ps = (0, positions.stride(0))
+        else:
+            raise ValueError(f"positions {tuple(positions.shape)} must have the token dimensions of q {tuple(lead)}, or the last of them.")
+    flat = q.ndim == 3
+    if flat:
+        q, k, ps = q[None], None if k is None else k[None], (0, ps[-1])
+    q, k = _dense_channels(q), None if k is None else _dense_channels(k)
+    if _differentiated(q, k, q_weight, k_weight):
+        r = _NormRotaryFn.apply(q, k, q_weight, k_weight, positions, ps, table, eps, weight_offset, bool(interleaved))
+        q_out, k_out = r if k is not None else (r, None)
+    else:
+        q_out, k_out = _norm_launch(q, k, q_weight, k_weight, positions, ps, table, eps, weight_offset, interleaved)
     if flat:
         q_out, k_out = q_out[0], None if k_out is None else k_out[0]
     return q_out, k_out

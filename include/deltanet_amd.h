@@ -382,6 +382,159 @@ size_t dn_attention_bwd_workspace_size(const dn_attention_args* a);
 int dn_attention_bwd(const dn_attention_args* a, const void* d_out, void* dq, void* dk, void* dv,
                      void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Around those layers: norms of queries and keys for each head, and the
+ * bookkeeping of a server that verifies drafted trees (page tables, slots,
+ * attention of trees, the accepted tokens).  Conventions as above.
+ * ------------------------------------------------------------------------- */
+
+/* Norm of every head of q and k and the rotation of its first R channels in one
+ * pass: y = x / sqrt(mean(x^2) + eps) * (weight_offset + weight), rotated as in
+ * dn_rotary_args (R = 0: not).  Statistics and products in float32, one rounding. */
+typedef struct dn_norm_rotary_args {
+  int32_t abi_version;
+  int32_t B, L, Hq, Hk, D, R;   /* Hk = 0: no k                                  */
+  int32_t dtype;                /* DN_F32 / DN_BF16 / DN_F16: q, k and results   */
+  int32_t weight_dtype;         /* DN_F32 / DN_BF16 / DN_F16                     */
+  int32_t pos_dtype;            /* DN_I32 / DN_I64                               */
+  int32_t interleaved;
+  int32_t rows;                 /* positions that the table covers               */
+  float eps, weight_offset;
+  const void* q;                /* (B,L,Hq,D), strides q_strides                 */
+  const void* k;                /* (B,L,Hk,D), strides k_strides                 */
+  const void* q_weight;         /* (D,)                                          */
+  const void* k_weight;
+  void* q_out;                  /* (B,L,Hq,D) dense; not read by the gradient    */
+  void* k_out;
+  const void* pos;              /* (B,L), strides pos_strides (0: shared)        */
+  const float* table;           /* (rows, R)                                     */
+  int64_t q_strides[3];         /* batch, token, head                            */
+  int64_t k_strides[3];
+  int64_t pos_strides[2];       /* batch, token                                  */
+} dn_norm_rotary_args;
+
+int dn_norm_rotary(const dn_norm_rotary_args* a, void* stream);
+
+/* Gradients of sum(q_out * d_q) + sum(k_out * d_k): dq and dk dense in `dtype`,
+ * the weights' (NULL if not wanted) in weight_dtype, summed in float32 in an order
+ * that depends on the sizes alone. */
+typedef struct dn_norm_rotary_grads {
+  const void* d_q;              /* (B,L,Hq,D), strides d_q_strides               */
+  const void* d_k;
+  void* dq;
+  void* dk;
+  void* dq_weight;              /* (D,)                                          */
+  void* dk_weight;
+  int64_t d_q_strides[3];
+  int64_t d_k_strides[3];
+} dn_norm_rotary_grads;
+
+size_t dn_norm_rotary_bwd_workspace_size(const dn_norm_rotary_args* a);
+int dn_norm_rotary_bwd(const dn_norm_rotary_args* a, const dn_norm_rotary_grads* d, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The serving form: new tokens' queries normed (unless the weights are NULL) and
+ * rotated into q_out, their keys the same into k_cache, their values into v_cache.
+ * slots (B,L) int64: page * page_size + token of the page; a token whose slot is
+ * outside the cache is not stored.  pos (B,L): the position that it is rotated by;
+ * a token at a negative one is none: its queries are zeros and it is not stored. */
+typedef struct dn_qkv_append_args {
+  int32_t abi_version;
+  int32_t B, L, Hq, Hkv, D, R;
+  int32_t dtype, cache_dtype, weight_dtype, pos_dtype;
+  int32_t interleaved, rows;
+  int32_t pages, page_size;     /* page_size a power of two                      */
+  float eps, weight_offset;
+  const void* q;                /* (B,L,Hq,D), strides q_strides                 */
+  const void* k;                /* (B,L,Hkv,D)                                   */
+  const void* v;
+  const void* q_weight;         /* (D,), or both NULL                            */
+  const void* k_weight;
+  void* q_out;                  /* (B,L,Hq,D) dense                              */
+  void* k_cache;                /* (pages,page_size,Hkv,D), strides kc_strides   */
+  void* v_cache;
+  const int64_t* slots;         /* (B,L) dense                                   */
+  const void* pos;              /* (B,L) dense                                   */
+  const float* table;           /* (rows, R); NULL if R = 0                      */
+  int64_t q_strides[3];         /* batch, token, head                            */
+  int64_t k_strides[3];
+  int64_t v_strides[3];
+  int64_t kc_strides[3];        /* page, token, head                             */
+  int64_t vc_strides[3];
+} dn_qkv_append_args;
+
+int dn_qkv_append(const dn_qkv_append_args* a, void* stream);
+
+/* Pages taken from a pool and given back, so that sequence b has as many as its
+ * lens[b] tokens need.  pool (2 + capacity) int32: the number of free pages, a word
+ * that is 0 between calls, the free pages (a stack).  held (B) int32: the pages that
+ * each sequence has, the first of its row of page_table; both are updated.  Pages
+ * that sequences no longer need go onto the stack first, the last page of the last
+ * sequence first of all; then sequences take from its top, in their order.  From the
+ * first for which it does not hold enough on, sequences that need more get none, and
+ * neither does one that needs more than max_pages; short_of[b] is the number of pages
+ * that it lacks.  B at most DN_MAX_SEQUENCES. */
+#define DN_MAX_SEQUENCES 4096
+int dn_paged_reserve(int32_t* pool, int32_t capacity, int32_t* page_table, int64_t page_table_stride, int32_t max_pages,
+                     int32_t B, int32_t page_size, int32_t* held, const int32_t* lens, int32_t* short_of, void* stream);
+
+/* Slots and positions of the N new tokens of a call.  New token i of sequence b, n_b
+ * of them, has slot page_table[b][x / page_size] * page_size + x % page_size with
+ * x = seq_lens[b] - n_b + i, or -1 if x is negative, past the page table or past the
+ * held[b] pages (held NULL: not checked), or its page negative.  Its position is x; with
+ * parents (N) int32, the place of each token's parent among its sequence's new ones
+ * (one that is not in front of it: none), seq_lens[b] - n_b plus the number of its
+ * ancestors.  visible (N, words) uint64: bit j says that the token descends from new
+ * token j or is it.  Of a sequence with more than 64 words new tokens, those past them
+ * are no tokens.  No token, as those that cu_seqlens gives to no sequence: position
+ * and slot -1, visible 0. */
+typedef struct dn_paged_slots_args {
+  int32_t abi_version;
+  int32_t N, B, page_size, max_pages, words;   /* words: at most 16; 0 without parents */
+  const int32_t* page_table;    /* (B,max_pages), row stride page_table_stride   */
+  const int32_t* seq_lens;
+  const int32_t* cu_seqlens;    /* (B + 1), or NULL: N / B each                  */
+  const int32_t* held;
+  const int32_t* parents;
+  int32_t* positions;           /* (N)                                           */
+  int64_t* slots;               /* (N)                                           */
+  uint64_t* visible;            /* (N, words) dense                              */
+  int64_t page_table_stride;
+} dn_paged_slots_args;
+
+int dn_paged_slots(const dn_paged_slots_args* a, void* stream);
+
+/* Attention of drafted trees: as dn_paged_attention, but a new token sees all tokens
+ * of its sequence in front of the new ones, and of the new ones those whose bit is set
+ * in its row of visible (N, words) (dn_paged_slots, or any others; none past 64 words).
+ * With `window`, at least 64 words, the last `window` of those.  A token that sees
+ * nothing gets zeros and lse -inf. */
+size_t dn_paged_tree_attention_workspace_size(const dn_paged_attention_args* a, int32_t words);
+int dn_paged_tree_attention(const dn_paged_attention_args* a, const uint64_t* visible, int32_t words, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
+/* Keys and values of accepted tokens moved to the front: token starts[b] + kept[b][i]
+ * of sequence b to starts[b] + i, in every layer, for the entries of kept in front of
+ * the first that is negative, not above the one before it or past the page table;
+ * lens[b] = starts[b] + their number.  A token is not moved from or to a page outside
+ * the cache. */
+typedef struct dn_kv_keep_args {
+  int32_t abi_version;
+  int32_t layers, B, H, D, most;   /* most: entries of kept per sequence         */
+  int32_t dtype;
+  int32_t pages, page_size, max_pages;
+  void* k_cache;                /* (layers,pages,page_size,H,D), strides kc_strides */
+  void* v_cache;
+  const int32_t* page_table;
+  const int32_t* starts;        /* (B)                                           */
+  const int32_t* kept;          /* (B, most) dense                               */
+  int32_t* lens;                /* (B)                                           */
+  int64_t kc_strides[4];        /* layer, page, token, head                      */
+  int64_t vc_strides[4];
+  int64_t page_table_stride;
+} dn_kv_keep_args;
+
+int dn_kv_keep(const dn_kv_keep_args* a, void* stream);
+
 /* Kernel timing instrumentation (no counterpart in the reference; for
  * benchmarks and profilers).  Between dn_profile_begin() and dn_profile_end()
  * every dn_prefill_fwd call (from any thread of the process) records HIP events on its
