@@ -278,6 +278,61 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_few(const AF p) {
   }
 }
 
+// Joins the parts of a query row if more than one workgroup had some: D/4 threads
+// per part, 1024/D parts at a time.
+template <class T, int D, int BM>
+__global__ __launch_bounds__(256) void k_attn_join(const AF p, int groups) {
+  constexpr int NP = 1024 / D;
+  __shared__ float ps[NP][D + 4];
+  Task t;
+  int row;
+  const int Hq = p.Hkv * p.G, i = blockIdx.x / Hq, hq = blockIdx.x - i * Hq;
+  const Plan plan(p, BM, kUnit);
+  const int W = min(groups, plan.C);
+  if (!plan.of_row(i, hq, t, row)) return;
+  // the workgroup that has unit u: the last w with w C / W <= u
+  auto owner = [&](int u) { return (int)((((int64_t)u + 1) * W + plan.C - 1) / plan.C) - 1; };
+  const int w0 = owner(t.first), w1 = owner(t.first + t.units - 1);
+  if (w0 == w1) return;
+  row -= t.m * BM;
+  const int ch = threadIdx.x % (D / 4), part = threadIdx.x / (D / 4);
+  f32x4 a = zero4();
+  float m = -INFINITY, z = 0.f;
+#pragma unroll 4
+  for (int w = w0 + part; w <= w1; w += NP) {
+    const float* s = p.part + (2 * (int64_t)w + (w == w0 ? 1 : 0)) * slot_floats<D, BM>();
+    const f32x4 y = *reinterpret_cast<const f32x4*>(s + row * D + 4 * ch);
+    const float mw = s[BM * D + row], zw = s[BM * D + BM + row];
+    const float n = fmaxf(m, mw);
+    const float f = m == -INFINITY ? 0.f : fast_exp2(m - n), g = mw == -INFINITY ? 0.f : fast_exp2(mw - n);
+    if (f != 1.f) a *= f;
+    if (g != 0.f) a += g * y;
+    z = z * f + g * zw;
+    m = n;
+  }
+  *reinterpret_cast<f32x4*>(&ps[part][4 * ch]) = a;
+  if (ch == 0) {
+    ps[part][D] = m;
+    ps[part][D + 1] = z;
+  }
+  __syncthreads();
+  if (part) return;
+#pragma unroll
+  for (int k = 1; k < NP; ++k) {
+    const float mw = ps[k][D], n = fmaxf(m, mw);
+    const float f = m == -INFINITY ? 0.f : fast_exp2(m - n), g = mw == -INFINITY ? 0.f : fast_exp2(mw - n);
+    const f32x4 y = *reinterpret_cast<const f32x4*>(&ps[k][4 * ch]);
+    if (f != 1.f) a *= f;
+    if (g != 0.f) a += g * y;
+    z = z * f + g * ps[k][D + 1];
+    m = n;
+  }
+  const float f = t.s.len - t.s.n + i - t.s.c0 < 0 ? 0.f : 1.f / z;   // (as above)
+  const float y[4] = {a[0] * f, a[1] * f, a[2] * f, a[3] * f};
+  st4<T>((T*)p.out + (int64_t)blockIdx.x * D + 4 * ch, y);
+  if (p.lse && ch == 0) p.lse[blockIdx.x] = z == 0.f ? -INFINITY : kLn2 * (m + __log2f(z));
+}
+
 int row_tile(const AF& p) { return (int64_t)p.N * p.G <= (int64_t)16 * p.B ? 16 : 32; }
 int64_t most_tasks(const AF& p) {
   const int BM = row_tile(p);
@@ -287,15 +342,23 @@ int64_t most_tasks(const AF& p) {
 int64_t most_units(const AF& p) { return most_tasks(p) * ((((int64_t)p.max_pages << p.shift) + kUnit - 1) / kUnit); }
 int64_t groups_of(const AF& p) { return std::min<int64_t>(kGroups, most_units(p)); }
 
-template <class T, int D, bool TREE> hipError_t run(const AF& p, hipStream_t st) {
+template <class T, int D> hipError_t run(const AF& p, hipStream_t st) {
   const unsigned W = (unsigned)groups_of(p), rows = (unsigned)p.N * p.Hkv * p.G;
   if (row_tile(p) == 16) {
-    hipLaunchKernelGGL((k_attn_few<T, D, 1, TREE>), dim3(W), dim3(64 * kWaves), 0, st, p);
-    if (W > 1) hipLaunchKernelGGL((k_attn_join<T, D, 16, kUnit, TREE>), dim3(rows), dim3(256), 0, st, p, (int)W);
+    hipLaunchKernelGGL((k_attn_few<T, D, 1, false>), dim3(W), dim3(64 * kWaves), 0, st, p);
+    if (W > 1) hipLaunchKernelGGL((k_attn_join<T, D, 16>), dim3(rows), dim3(256), 0, st, p, (int)W);
   } else {
-    hipLaunchKernelGGL((k_attn_few<T, D, 2, TREE>), dim3(W), dim3(64 * kWaves), 0, st, p);
-    if (W > 1) hipLaunchKernelGGL((k_attn_join<T, D, 32, kUnit, TREE>), dim3(rows), dim3(256), 0, st, p, (int)W);
+    hipLaunchKernelGGL((k_attn_few<T, D, 2, false>), dim3(W), dim3(64 * kWaves), 0, st, p);
+    if (W > 1) hipLaunchKernelGGL((k_attn_join<T, D, 32>), dim3(rows), dim3(256), 0, st, p, (int)W);
   }
+  return hipGetLastError();
+}
+
+// trees in float32 (tree_few)
+template <int D, int NQ> hipError_t run_tree(const AF& p, hipStream_t st) {
+  const unsigned W = (unsigned)groups_of(p);
+  hipLaunchKernelGGL((k_attn_few<float, D, NQ, true>), dim3(W), dim3(64 * kWaves), 0, st, p);
+  launch_tree_join<float, D, 16 * NQ, kUnit, 1>(p, W, most_tasks(p), st);
   return hipGetLastError();
 }
 
@@ -330,15 +393,27 @@ bool attn_few_takes(const AF& p, int D, int dtype) {
   return tiles <= (D == 256 ? 64 : 128) && walk >= std::max<int64_t>(1024, 64 * tiles);
 }
 
+// Drafted trees in float32 whose rows fill 16 or 32 of a tile: the products take the
+// time there, and the kernel of trees makes 64 rows of them.  MEASURE.  At D = 256 there
+// are no registers for 32.
+bool tree_few(const AF& p, int D, int dtype) {
+  return dtype == DN_F32 && p.shift >= 4 && (int64_t)p.N * p.G <= (int64_t)(D == 256 ? 16 : 32) * p.B;
+}
+
 size_t attn_few_bytes(const AF& p, int D) { return (size_t)groups_of(p) * 2 * row_tile(p) * (D + 2) * sizeof(float); }
 
 hipError_t attn_few(const AF& p, int D, int dtype, hipStream_t st) {
   auto go = [&](auto z) {
     using T = decltype(z);
-    if (p.vis) return D == 64 ? run<T, 64, true>(p, st) : D == 128 ? run<T, 128, true>(p, st) : run<T, 256, true>(p, st);
-    return D == 64 ? run<T, 64, false>(p, st) : D == 128 ? run<T, 128, false>(p, st) : run<T, 256, false>(p, st);
+    return D == 64 ? run<T, 64>(p, st) : D == 128 ? run<T, 128>(p, st) : run<T, 256>(p, st);
   };
   return dtype == DN_BF16 ? go((bf16)0.f) : dtype == DN_F16 ? go((f16)0.f) : go(0.f);
+}
+
+hipError_t attn_tree_few(const AF& p, int D, hipStream_t st) {
+  if (D == 256) return run_tree<256, 1>(p, st);
+  if (row_tile(p) == 16) return D == 64 ? run_tree<64, 1>(p, st) : run_tree<128, 1>(p, st);
+  return D == 64 ? run_tree<64, 2>(p, st) : run_tree<128, 2>(p, st);
 }
 
 }  // namespace dn

@@ -308,6 +308,34 @@ template <bool TREE> struct PlanOf {
       t.first += t.units;
     }
   }
+  // task number x of all
+  __device__ __forceinline__ bool of_task(int x, Task& t) const {
+    static_assert(TREE, "all tiles of a sequence have as many units");
+    Span s = s0;
+    int mine = mine0, before = 0;
+    t.first = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+      if (b0) load(b0, s, mine);
+      const int tasks = (s.n * p.G + BM - 1) / BM * p.Hkv, ts = scan(tasks), us = scan(mine);
+      const unsigned long long in = __ballot(before + ts > x);
+      if (in) {
+        const int w = __builtin_ctzll(in);
+        auto of = [&](int y) { return __builtin_amdgcn_readfirstlane(__shfl(y, w)); };
+        t.b = b0 + w;
+        t.s = {of(s.c0), of(s.n), of(s.len)};
+        const int n = of(tasks), tiles = n / p.Hkv;
+        x -= before + of(ts) - n;
+        t.units = of(mine) / n;
+        t.h = x / tiles;
+        t.m = x - t.h * tiles;
+        t.first += of(us) - of(mine) + x * t.units;
+        return true;
+      }
+      before += __builtin_amdgcn_readfirstlane(__shfl(ts, 63));
+      t.first += __builtin_amdgcn_readfirstlane(__shfl(us, 63));
+    }
+    return false;
+  }
   // the task of new token i's row for query head hq, and the row
   __device__ __forceinline__ bool of_row(int i, int hq, Task& t, int& row) const {
     int per;
@@ -339,7 +367,10 @@ bool attn_few_takes(const AF& p, int D, int dtype);
 size_t attn_few_bytes(const AF& p, int D);
 hipError_t attn_few(const AF& p, int D, int dtype, hipStream_t st);
 
-// The same for drafted trees (p.vis set), of any number of rows and any pages.
+bool tree_few(const AF& p, int D, int dtype);
+hipError_t attn_tree_few(const AF& p, int D, hipStream_t st);
+
+// Drafted trees (p.vis set), of any number of rows and any pages.
 size_t attn_tree_bytes(const AF& p, int D, int dtype);
 hipError_t attn_tree(const AF& p, int D, int dtype, hipStream_t st);
 

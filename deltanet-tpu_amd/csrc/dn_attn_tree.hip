@@ -12,14 +12,26 @@
 namespace dn {
 namespace {
 
-// NW waves of 16 NQ rows, tiles of BN keys.
-template <class T, int D, int NQ, int NW, int BN>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_tree(const AF p) {
+// Waits until at most N of this wave's direct loads into LDS are in flight, then for
+// everyone's: the tile that was asked for first is there, and nobody reads any more
+// the one before it.
+template <int N> __device__ __forceinline__ void loads_but() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+// NW waves of 16 NQ rows, tiles of BN keys, ST of them in LDS: one that is read, the
+// others on their way.  PG: pages of 16 tokens or more, so that the rows of one load
+// lie in one page, whose number is read through the scalar cache (a vector load's wait
+// would be one for all loads in flight).
+template <class T, int D, int NQ, int NW, int BN, int ST, bool PG, int UNITS>
+__global__ __launch_bounds__(64 * NW, 2 * ST * BN * D * (int)sizeof(T) <= 80 * 1024 ? 2 : 1) void k_attn_tree(const AF p) {
   using TL = Tile<T, D, BN>;
   using F = typename At<T>::F;
-  constexpr float kLift = std::is_same<T, f16>::value ? 7.f : 0.f;   // (as in the kernel of few rows)
+  constexpr bool F16 = std::is_same<T, f16>::value;
+  constexpr float kLift = F16 ? 7.f : 0.f, kRange = 60.f;   // (kLift: as in the kernel of few rows)
   constexpr int BM = 16 * NQ * NW, NS = D / 32, NC = D / 16;
-  __shared__ __align__(16) T lds[4 * BN * D];   // [2][K, V][BN][D]
+  constexpr int kLoads = 2 * (BN / TL::kLoad) * NS / NW;   // of a wave and tile
+  __shared__ __align__(16) T lds[ST * 2 * BN * D];   // [ST][K, V][BN][D]
   const int l = lane_id(), r = l & 15, q = l >> 4;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
@@ -27,10 +39,12 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_tree(c
   const Rest rest(p);
   const PlanOf<true> plan(p, BM, BN);
   rest.clear<T, D>(p);
-  const int W = min((int)gridDim.x, plan.C);
-  if ((int)blockIdx.x >= W) return;
-  int u = first_unit(blockIdx.x, W, plan.C);
-  const int uend = first_unit(blockIdx.x + 1, W, plan.C);
+  const int W = shares<UNITS>(gridDim.x, plan.C);
+  // neighbours in work on one die: the tiles of rows over the same keys meet in its cache
+  const int me = W == (int)gridDim.x && W % 8 == 0 ? (int)blockIdx.x % 8 * (W / 8) + (int)blockIdx.x / 8 : (int)blockIdx.x;
+  if (me >= W) return;
+  int u = first_unit(me, W, plan.C);
+  const int uend = first_unit(me + 1, W, plan.C);
 #pragma unroll 1
   while (u < uend) {
     Task t;
@@ -57,32 +71,70 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_tree(c
       token[i] = t.s.c0 + tk;
       low[i] = tree_low(p, tree_words(p, token[i]), off, t.s.n);
     }
-    Rows<T, true> kr, vr;
-    kr.base = (const T*)p.k + t.h * p.ks[2];
+    Rows<T, true> vr;   // (for the values that are not finite)
     vr.base = (const T*)p.v + t.h * p.vs[2];
-    kr.token = p.ks[1]; vr.token = p.vs[1];
-    kr.page = p.ks[0]; vr.page = p.vs[0];
-    kr.pt = vr.pt = p.pt + t.b * p.pts;
-    kr.shift = vr.shift = p.shift;
-    kr.pages = vr.pages = p.pages;
-    kr.last = vr.last = last;
-    auto fetch = [&](int j) {
-      T* to = lds + (j - j0 & 1) * 2 * BN * D;
-      TL::template load<NW>(to, w, [&](int x) { return kr(j * BN + x); });
-      TL::template load<NW>(to + BN * D, w, [&](int x) { return vr(j * BN + x); });
+    vr.token = p.vs[1]; vr.page = p.vs[0]; vr.pt = p.pt + t.b * p.pts; vr.shift = p.shift; vr.pages = p.pages; vr.last = last;
+    const T* kb = (const T*)p.k + t.h * p.ks[2];
+    const auto pt = (const __attribute__((address_space(4))) int32_t*)(uintptr_t)vr.pt;
+    // where this lane reads of tile j
+    constexpr int groups = BN / TL::kLoad;
+    const T *ks = nullptr, *vs = nullptr;
+    T* to = nullptr;
+    auto aim = [&](int j) {
+      const int row = j * BN + w % groups * TL::kLoad + l / TL::kPieces;
+      int at = min(row, last), pg;
+      if constexpr (PG) {
+        const int first = min(__builtin_amdgcn_readfirstlane(row), last);
+        pg = pt[first >> p.shift];
+        at = min(at, first | ((1 << p.shift) - 1));
+      } else {
+        pg = vr.pt[at >> p.shift];
+      }
+      pg = min(max(pg, 0), p.pages - 1);
+      const int in = at & ((1 << p.shift) - 1), x = TL::piece(w % groups * TL::kLoad + l / TL::kPieces, l % TL::kPieces) * TL::kPer;
+      ks = kb + pg * p.ks[0] + in * p.ks[1] + x;
+      vs = vr.base + pg * p.vs[0] + in * p.vs[1] + x;
+      to = lds + (j - j0) % ST * 2 * BN * D;
+    };
+    // Tiles of 64 keys at D = 256 are asked for in four parts between the products of the
+    // one before, as in the kernel of whole rows; others at once.
+    constexpr bool SPREAD = D == 256 && BN == 64;
+    auto fetch = [&](auto part) {
+      constexpr int P = decltype(part)::value;
+      if constexpr (P < 2) TL::template load_part<NW, P, 2>(to, w, ks);
+      else TL::template load_part<NW, P - 2, 2>(to + BN * D, w, vs);
+    };
+    auto fetch_all = [&] {
+      TL::template load_part<NW, 0, 1>(to, w, ks);
+      TL::template load_part<NW, 0, 1>(to + BN * D, w, vs);
     };
     f32x4 o[NQ][NC];
-    float mx[NQ], sum[NQ];
+    float mx[NQ], top[NQ], sum[NQ];
 #pragma unroll
-    for (int i = 0; i < NQ; ++i) {
-      mx[i] = -INFINITY;
-      sum[i] = 0.f;
-#pragma unroll
-      for (int c = 0; c < NC; ++c) o[i][c] = zero4();
-    }
+    for (int i = 0; i < NQ; ++i) mx[i] = -INFINITY;
     bool odd = false;
-    auto step = [&](auto masked, const T* kt, const T* vt, int key0) {
-      constexpr bool MASKED = decltype(masked)::value;
+    auto rescale = [&](int i, float m) {
+      const float f = m == -INFINITY ? 1.f : fast_exp2(mx[i] - m);
+      mx[i] = m;
+      sum[i] *= f;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) o[i][c] *= f;
+    };
+    // 32 keys.  Probabilities are relative to mx, the maximum of a piece's first tile
+    // and of its masked ones (LEARN, kept up to 2^kLazy); the tiles between only note what
+    // their largest scores were.  A row that went more than 2^kRange beyond is found at the
+    // piece's end, and the piece done again from what is known then: sums are as exact with
+    // any reference up to there.  float16 has no such range, its rows are raised on the way.
+    auto hides = [&](int key0) { return key0 + 32 > off || key0 < lo1; };   // some row must not see some of 32 keys
+    auto learns = [&](int j) { return j == j0 || (j + 1) * BN > off || j * BN < lo1; };
+    constexpr bool AHEAD = D == 256 && sizeof(T) == 2;
+    constexpr int VB = AHEAD ? 4 : 1, NB = NC / VB;
+    auto in_order = [] {
+      if constexpr (AHEAD) __builtin_amdgcn_sched_barrier(0);
+    };
+    auto step = [&](auto learn, auto between, const T* kt, const T* vt, int key0) {
+      constexpr bool LEARN = decltype(learn)::value;
+      const bool masked = LEARN && hides(key0);
       f32x4 sc[NQ][2];
 #pragma unroll
       for (int i = 0; i < NQ; ++i) sc[i][0] = sc[i][1] = zero4();
@@ -94,11 +146,21 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_tree(c
 #pragma unroll
           for (int i = 0; i < NQ; ++i) At<T>::mma(sc[i][e], kf, qf[i][c]);
         }
-      float mt[NQ];
+      F vf[2][VB];
+      auto values = [&](int n) {
+#pragma unroll
+        for (int c = 0; c < VB; ++c) vf[n & 1][c] = TL::col8(vt, n * VB + c, r, q);
+      };
+      if constexpr (AHEAD) {
+        in_order();
+        values(0);
+        in_order();
+      }
       bool grow = false;
+      float mt[NQ];
 #pragma unroll
       for (int i = 0; i < NQ; ++i) {
-        if (MASKED) {
+        if (LEARN && masked) {
           const uint32_t bits = tree_bits(p, tree_words(p, token[i]), off, t.s.len, low[i], key0) >> (4 * q);
 #pragma unroll
           for (int e = 0; e < 2; ++e)
@@ -107,18 +169,18 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_tree(c
         }
         const float m = fmaxf(fmaxf(fmaxf(sc[i][0][0], sc[i][0][1]), fmaxf(sc[i][0][2], sc[i][0][3])),
                               fmaxf(fmaxf(sc[i][1][0], sc[i][1][1]), fmaxf(sc[i][1][2], sc[i][1][3])));
-        mt[i] = max_q(m) * scale - kLift;
-        grow |= mt[i] > mx[i] + kLazy;
+        if constexpr (LEARN) {
+          mt[i] = max_q(m) * scale - kLift;
+          grow |= mt[i] > mx[i] + kLazy;
+        } else {
+          top[i] = fmaxf(top[i], m);
+          if (F16) grow |= __builtin_fmaf(m, scale, -mx[i]) > kLift + kLazy;
+        }
       }
-      if (__any(grow)) {
+      if constexpr (LEARN || F16) {
+        if (__any(grow)) {
 #pragma unroll
-        for (int i = 0; i < NQ; ++i) {
-          const float m = fmaxf(mx[i], mt[i]);
-          const float f = m == -INFINITY ? 1.f : fast_exp2(mx[i] - m);
-          mx[i] = m;
-          sum[i] *= f;
-#pragma unroll
-          for (int c = 0; c < NC; ++c) o[i][c] *= f;
+          for (int i = 0; i < NQ; ++i) rescale(i, fmaxf(mx[i], LEARN ? mt[i] : max_q(top[i]) * scale - kLift));
         }
       }
       F pf[NQ];
@@ -134,31 +196,76 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_tree(c
           }
         pf[i] = frag8<T>(sc[i][0], sc[i][1]);
       }
-      const bool bad = MASKED && TL::odd32(vt);
-      if (MASKED) odd |= bad;
+      between();
+      const bool bad = LEARN && masked && TL::odd32(vt);
+      if (LEARN) odd |= bad;
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        F vf = TL::col8(vt, c, r, q);
-        if (MASKED && bad) vf = finite8<T>(vf);
+      for (int n = 0; n < NB; ++n) {
+        if (!AHEAD || n + 1 < NB) values(AHEAD ? n + 1 : n);
+        in_order();
+        if (LEARN && bad) {
 #pragma unroll
-        for (int i = 0; i < NQ; ++i) At<T>::mma(o[i][c], vf, pf[i]);
+          for (int c = 0; c < VB; ++c) vf[n & 1][c] = finite8<T>(vf[n & 1][c]);
+        }
+#pragma unroll
+        for (int c = 0; c < VB; ++c)
+#pragma unroll
+          for (int i = 0; i < NQ; ++i) At<T>::mma(o[i][n * VB + c], vf[n & 1][c], pf[i]);
       }
     };
-    auto masked_step = [&](int key0) { return key0 + 31 >= off || key0 < lo1; };
-    fetch(j0);
-#pragma unroll 1
-    for (int j = j0; j < j1; ++j) {
-      loads_barrier();   // the tiles are there, those before them no longer read
-      if (j + 1 < j1) fetch(j + 1);
-      const T* kt = lds + (j - j0 & 1) * 2 * BN * D;
-      const T* vt = kt + BN * D;
-      if (masked_step(j * BN) || masked_step(j * BN + BN - 32)) {
-#pragma unroll 1
-        for (int x = 0; x < BN; x += 32) step(std::true_type{}, kt + x * 32, vt + x * 32, j * BN + x);
-      } else {
+    // the waits for the queries land here and not, for all loads in flight, in the loop
 #pragma unroll
-        for (int x = 0; x < BN; x += 32) step(std::false_type{}, kt + x * 32, vt + x * 32, j * BN + x);
+    for (int i = 0; i < NQ; ++i)
+#pragma unroll
+      for (int c = 0; c < NS; ++c) settle(qf[i][c]);
+#pragma unroll 1
+    for (int pass = 0;; ++pass) {
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) {
+        top[i] = -INFINITY;
+        sum[i] = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) o[i][c] = zero4();
       }
+#pragma unroll
+      for (int i = 0; i + 1 < ST; ++i)
+        if (j0 + i < j1) {
+          aim(j0 + i);
+          fetch_all();
+        }
+#pragma unroll 1
+      for (int j = j0; j < j1; ++j) {
+        if (ST > 2 && j + ST - 2 < j1) loads_but<(ST - 2) * kLoads>();
+        else loads_but<0>();
+        const bool more = j + ST - 1 < j1;
+        if (more) aim(j + ST - 1);
+        const T* kt = lds + (j - j0) % ST * 2 * BN * D;
+        const T* vt = kt + BN * D;
+        if (learns(j)) {
+          if (more) fetch_all();
+#pragma unroll 1
+          for (int x = 0; x < BN; x += 32) step(std::true_type{}, [] {}, kt + x * 32, vt + x * 32, j * BN + x);
+        } else if constexpr (SPREAD) {
+          if (more) fetch(std::integral_constant<int, 0>{});
+          step(std::false_type{}, [&] { if (more) fetch(std::integral_constant<int, 1>{}); }, kt, vt, j * BN);
+          if (more) fetch(std::integral_constant<int, 2>{});
+          step(std::false_type{}, [&] { if (more) fetch(std::integral_constant<int, 3>{}); }, kt + 32 * 32, vt + 32 * 32, j * BN + 32);
+        } else {
+          if (more) fetch_all();
+#pragma unroll
+          for (int x = 0; x < BN; x += 32) step(std::false_type{}, [] {}, kt + x * 32, vt + x * 32, j * BN + x);
+        }
+      }
+      if (F16 || pass == 1) break;
+      bool over = false;
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) {
+        top[i] = max_q(top[i]) * scale;
+        over |= top[i] > mx[i] + kRange;
+      }
+      if (!__syncthreads_or(over)) break;
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) mx[i] = top[i] > mx[i] + kRange ? top[i] : mx[i];   // (the other rows keep their bits)
     }
     if (odd) {   // infinities and NaNs that some row must not see: to those that do
 #pragma unroll
@@ -166,22 +273,18 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_tree(c
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
 #pragma unroll 1
-          for (int j = j0; j < j1; ++j) {
-            if (!(masked_step(j * BN) || masked_step(j * BN + BN - 32))) continue;
-#pragma unroll 1
-            for (int key = j * BN; key < min((j + 1) * BN, t.s.len); ++key) {
-              if (!(tree_bits(p, tree_words(p, token[i]), off, t.s.len, low[i], key & ~31) >> (key & 31) & 1)) continue;
+          for (int key = j0 * BN; key < min(j1 * BN, t.s.len); ++key) {
+            if (!hides(key & ~31) || !(tree_bits(p, tree_words(p, token[i]), off, t.s.len, low[i], key & ~31) >> (key & 31) & 1)) continue;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float y = (float)vr(key)[16 * c + 4 * q + e];
-                if (!__builtin_isfinite(y)) o[i][c][e] += y;
-              }
+            for (int e = 0; e < 4; ++e) {
+              const float y = (float)vr(key)[16 * c + 4 * q + e];
+              if (!__builtin_isfinite(y)) o[i][c][e] += y;
             }
           }
         }
     }
     const bool whole = take == t.units;
-    float* slot = p.part + (2 * (int64_t)blockIdx.x + (skip == 0 ? 1 : 0)) * slot_floats<D, BM>();
+    float* slot = p.part + (2 * (int64_t)me + (skip == 0 ? 1 : 0)) * slot_floats<D, BM>();
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
       const float z = sum_q(sum[i]);
@@ -215,43 +318,54 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_tree(c
 int64_t most_tasks(const AF& p, int BM) {
   return (p.cu ? (int64_t)p.N * p.G / BM + p.B : (int64_t)p.B * (((int64_t)p.T * p.G + BM - 1) / BM)) * p.Hkv;
 }
-template <class T, int D> struct Form {
-  static constexpr int NQ = sizeof(T) == 4 || D < 256 ? 2 : 1, NW = sizeof(T) == 4 || D < 256 ? 4 : 8, BN = sizeof(T) == 4 ? 32 : 64;
-  static constexpr int BM = 16 * NQ * NW;
-  static constexpr int per_cu = 4 * BN * D * (int)sizeof(T) <= 80 * 1024 && sizeof(T) == 2 ? 2 : 1;
+template <class T, int D, int NQ, int NW, int BN, int ST> struct FormOf {
+  static constexpr int BM = 16 * NQ * NW, kUnits = 64 / BN;
+  static constexpr int kPerCU = NW == 4 && 2 * ST * BN * D * (int)sizeof(T) <= 80 * 1024 ? 2 : 1;
   static int64_t groups(const AF& p) {
-    return std::min<int64_t>(256 * per_cu, most_tasks(p, BM) * ((((int64_t)p.max_pages << p.shift) + BN - 1) / BN));
+    return std::min<int64_t>(256 * kPerCU, most_tasks(p, BM) * ((((int64_t)p.max_pages << p.shift) + BN - 1) / BN));
   }
   static size_t bytes(const AF& p) { return (size_t)groups(p) * 2 * BM * (D + 2) * sizeof(float); }
   static hipError_t run(const AF& p, hipStream_t st) {
-    const unsigned W = (unsigned)groups(p), rows = (unsigned)p.N * p.Hkv * p.G;
-    hipLaunchKernelGGL((k_attn_tree<T, D, NQ, NW, BN>), dim3(W), dim3(64 * NW), 0, st, p);
-    if (W > 1) hipLaunchKernelGGL((k_attn_join<T, D, BM, BN, true>), dim3(rows), dim3(256), 0, st, p, (int)W);
+    const unsigned W = (unsigned)groups(p);
+    if (p.shift >= 4) hipLaunchKernelGGL((k_attn_tree<T, D, NQ, NW, BN, ST, true, kUnits>), dim3(W), dim3(64 * NW), 0, st, p);
+    else hipLaunchKernelGGL((k_attn_tree<T, D, NQ, NW, BN, ST, false, kUnits>), dim3(W), dim3(64 * NW), 0, st, p);
+    launch_tree_join<T, D, BM, BN, kUnits>(p, W, most_tasks(p, BM), st);
     return hipGetLastError();
   }
 };
-
-template <class G> auto by_form(int D, int dtype, G g) {
+// The form for the mean number of rows of a sequence and key head: MEASURE.
+template <class T, int D, class G> auto by_rows(const AF& p, G g) {
+  const int64_t rows = (int64_t)p.N * p.G, B = p.B;
+  if constexpr (sizeof(T) == 4) {
+    if (rows <= 128 * B) return g(FormOf<T, D, 1, 4, 32, 2>{});
+    return g(FormOf<T, D, 1, 8, 32, 2>{});
+  } else if constexpr (D == 256) {
+    if (rows <= 96 * B) return g(FormOf<T, D, 1, 4, 32, 2>{});
+    return g(FormOf<T, D, 1, 8, 64, 2>{});
+  } else {
+    if (rows <= 64 * B) return g(FormOf<T, D, 1, 4, 32, D == 64 ? 3 : 2>{});
+    if (rows < 192 * B) return g(FormOf<T, D, 2, 4, D == 64 ? 64 : 32, 2>{});
+    return g(FormOf<T, D, 2, 8, 64, 2>{});
+  }
+}
+template <class G> auto by_form(const AF& p, int D, int dtype, G g) {
   auto go = [&](auto z) {
     using T = decltype(z);
-    return D == 64 ? g(Form<T, 64>{}) : D == 128 ? g(Form<T, 128>{}) : g(Form<T, 256>{});
+    return D == 64 ? by_rows<T, 64>(p, g) : D == 128 ? by_rows<T, 128>(p, g) : by_rows<T, 256>(p, g);
   };
   return dtype == DN_BF16 ? go((bf16)0.f) : dtype == DN_F16 ? go((f16)0.f) : go(0.f);
 }
 
-// Rows that fill a tile of the kernel of few rows; pages of 16 tokens at least there.
-bool few(const AF& p) { return p.shift >= 4 && (int64_t)p.N * p.G <= (int64_t)32 * p.B; }
-
 }  // namespace
 
 size_t attn_tree_bytes(const AF& p, int D, int dtype) {
-  if (few(p)) return attn_few_bytes(p, D);
-  return by_form(D, dtype, [&](auto f) { return decltype(f)::bytes(p); });
+  if (tree_few(p, D, dtype)) return attn_few_bytes(p, D);
+  return by_form(p, D, dtype, [&](auto f) { return decltype(f)::bytes(p); });
 }
 
 hipError_t attn_tree(const AF& p, int D, int dtype, hipStream_t st) {
-  if (few(p)) return attn_few(p, D, dtype, st);
-  return by_form(D, dtype, [&](auto f) { return decltype(f)::run(p, st); });
+  if (tree_few(p, D, dtype)) return attn_tree_few(p, D, st);
+  return by_form(p, D, dtype, [&](auto f) { return decltype(f)::run(p, st); });
 }
 
 }  // namespace dn

@@ -275,7 +275,8 @@ __global__ __launch_bounds__(kThreads) void k_slots_tree(const SP p) {
 // accepted tokens
 // ---------------------------------------------------------------------------
 struct KP {
-  int layers, B, H, pieces, most, pages, shift, max_pages;   // pieces: of a head
+  int layers, B, most, pages, shift, max_pages;
+  uint32_t H, pieces;   // pieces: of a head
   char *k, *v;
   const int32_t *pt, *starts, *kept;
   int32_t* lens;
@@ -286,13 +287,14 @@ struct KP {
 // piece of every kept token, kBatch of them read before the first is written: what is
 // kept rises, so no later token lies where an earlier one goes.
 constexpr int kBatch = 8, kPath = 64;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 template <class V> __global__ __launch_bounds__(kThreads) void k_keep(const KP p) {
   __shared__ int from_page[kPath], from_in[kPath], to_page[kPath], to_in[kPath];
   __shared__ int s_count;
   const int b = blockIdx.y;
   const int start = p.starts[b];
   const int64_t end = (int64_t)p.max_pages << p.shift;
-  const int64_t n = (int64_t)p.layers * 2 * p.H * p.pieces;
+  const uint32_t n = (uint32_t)p.layers * 2 * p.H * p.pieces;
   int before = -1, total = 0;
 #pragma unroll 1
   for (int i0 = 0; i0 < p.most; i0 += kPath) {
@@ -319,23 +321,23 @@ template <class V> __global__ __launch_bounds__(kThreads) void k_keep(const KP p
     __syncthreads();
     const int c = s_count;
     total += c;
-    for (int64_t x = (int64_t)blockIdx.x * kThreads + threadIdx.x; x < n; x += (int64_t)gridDim.x * kThreads) {
-      const int piece = (int)(x % p.pieces);
-      int64_t y = x / p.pieces;
-      const int h = (int)(y % p.H);
-      y /= p.H;
+    for (uint32_t x = blockIdx.x * kThreads + threadIdx.x; x < n; x += gridDim.x * kThreads) {
+      const uint32_t piece = x % p.pieces, head = x / p.pieces, h = head % p.H, y = head / p.H;
       const bool val = y & 1;
-      const int64_t* st = val ? p.vs : p.ks;
-      char* base = (val ? p.v : p.k) + (y >> 1) * st[0] + h * st[3] + piece * (int64_t)sizeof(V);
+      const int64_t s0 = val ? p.vs[0] : p.ks[0], s1 = val ? p.vs[1] : p.ks[1], s2 = val ? p.vs[2] : p.ks[2], s3 = val ? p.vs[3] : p.ks[3];
+      char* base = (val ? p.v : p.k) + (int64_t)(y >> 1) * s0 + h * s3 + piece * (int64_t)sizeof(V);
 #pragma unroll 1
       for (int i = 0; i < c; i += kBatch) {
         V r[kBatch];
+        bool move[kBatch];
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e) {
+          move[e] = i + e < c && from_page[i + e] >= 0;
+          if (move[e]) r[e] = *reinterpret_cast<const V*>(base + from_page[i + e] * s1 + from_in[i + e] * s2);
+        }
 #pragma unroll
         for (int e = 0; e < kBatch; ++e)
-          if (i + e < c && from_page[i + e] >= 0) r[e] = *reinterpret_cast<const V*>(base + from_page[i + e] * st[1] + from_in[i + e] * st[2]);
-#pragma unroll
-        for (int e = 0; e < kBatch; ++e)
-          if (i + e < c && from_page[i + e] >= 0) *reinterpret_cast<V*>(base + to_page[i + e] * st[1] + to_in[i + e] * st[2]) = r[e];
+          if (move[e]) *reinterpret_cast<V*>(base + to_page[i + e] * s1 + to_in[i + e] * s2) = r[e];
       }
     }
     if (c < 64) break;
@@ -425,9 +427,10 @@ extern "C" int dn_kv_keep(const dn_kv_keep_args* a, void* stream) {
   const int piece = all % 16 == 0 ? 16 : e;
   p.pieces = a->D * e / piece;
   const int64_t n = (int64_t)p.layers * 2 * p.H * p.pieces;
+  if (n > 0x7fffffff) return bad("too many layers and heads");
   const dim3 grid((unsigned)std::min<int64_t>(std::max<int64_t>((n + kThreads - 1) / kThreads, 1), 1024), p.B);
   hipStream_t st = (hipStream_t)stream;
-  if (piece == 16) hipLaunchKernelGGL(k_keep<uint4>, grid, dim3(kThreads), 0, st, p);
+  if (piece == 16) hipLaunchKernelGGL(k_keep<u32x4>, grid, dim3(kThreads), 0, st, p);
   else if (e == 4) hipLaunchKernelGGL(k_keep<uint32_t>, grid, dim3(kThreads), 0, st, p);
   else hipLaunchKernelGGL(k_keep<uint16_t>, grid, dim3(kThreads), 0, st, p);
   return launched();

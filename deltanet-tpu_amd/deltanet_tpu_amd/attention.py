@@ -261,22 +261,31 @@ def _check_weights(D, *ws):
             raise ValueError(f"norm weights must be contiguous ({D},) tensors of one type, float32, bfloat16 or float16, got {w.dtype} {tuple(w.shape)}.")
 
 
-def _norm_block(q, k, qw, kw, q_out, k_out, pos, ps, table, eps, offset, interleaved):
-    one = k if q is None else q
-    B, L, _, D = one.shape
-    none = (0, 0, 0)
-    sq, sk = none if q is None else q.stride(), none if k is None else k.stride()
-    at = lambda t: 0 if t is None else t.data_ptr()
+def _norm_block(q, k, qw, kw, q_out, k_out, pos, table, meta):
+    """The argument block; one of q and k may be None, with its weights."""
+    ps0, ps1, eps, offset, inter = meta
+    one, w = (k, kw) if q is None else (q, qw)
+    B, L, Hq, D = one.shape
+    q0, q1, q2, _ = k0, k1, k2, _ = one.stride()
+    if q is None:
+        Hq, Hk = 0, Hq
+    elif k is None:
+        Hk = 0
+    else:
+        Hk = k.shape[2]
+        k0, k1, k2, _ = k.stride()
+    rows, R = (0, 0) if table is None else table.shape
     return _lib.NORM_ROTARY_PACK(
-        _lib.DN_ABI_VERSION, B, L, 0 if q is None else q.shape[2], 0 if k is None else k.shape[2], D, 0 if table is None else table.shape[1],
-        _DT[one.dtype], _DT[(kw if q is None else qw).dtype], _lib.DN_I32 if pos is None else _INT[pos.dtype], 1 if interleaved else 0,
-        0 if table is None else table.shape[0], eps, offset, at(q), at(k), at(qw), at(kw), at(q_out), at(k_out), at(pos), at(table),
-        sq[0], sq[1], sq[2], sk[0], sk[1], sk[2], ps[0], ps[1])
+        _lib.DN_ABI_VERSION, B, L, Hq, Hk, D, R, _DT[one.dtype], _DT[w.dtype], _lib.DN_I32 if pos is None else _INT[pos.dtype], inter, rows,
+        eps, offset, 0 if q is None else q.data_ptr(), 0 if k is None else k.data_ptr(), 0 if qw is None else qw.data_ptr(),
+        0 if kw is None else kw.data_ptr(), 0 if q_out is None else q_out.data_ptr(), 0 if k_out is None else k_out.data_ptr(),
+        0 if pos is None else pos.data_ptr(), 0 if table is None else table.data_ptr(), q0, q1, q2, k0, k1, k2, ps0, ps1)
 
 
-def _norm_launch(q, k, qw, kw, pos, ps, table, eps, offset, interleaved):
-    q_out, k_out = q.new_empty(q.shape), None if k is None else k.new_empty(k.shape)
-    _call("dn_norm_rotary", q.get_device(), _norm_block(q, k, qw, kw, q_out, k_out, pos, ps, table, eps, offset, interleaved))
+def _norm_launch(q, k, qw, kw, pos, table, meta):
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    k_out = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
+    _call("dn_norm_rotary", q.get_device(), _norm_block(q, k, qw, kw, q_out, k_out, pos, table, meta))
     return q_out, k_out
 
 
@@ -284,39 +293,48 @@ class _NormRotaryFn(torch.autograd.Function):
     """Keeps the inputs; the backward computes the heads' norms again."""
 
     @staticmethod
-    def forward(ctx, q, k, qw, kw, pos, ps, table, eps, offset, interleaved):
+    def forward(ctx, q, k, qw, kw, pos, table, meta):
         ctx.save_for_backward(q, k, qw, kw, pos, table)
-        ctx.meta = ps, eps, offset, interleaved
+        ctx.meta = meta
         ctx.set_materialize_grads(False)
-        q_out, k_out = _norm_launch(q, k, qw, kw, pos, ps, table, eps, offset, interleaved)
+        q_out, k_out = _norm_launch(q, k, qw, kw, pos, table, meta)
         return (q_out, k_out) if k is not None else q_out
 
     @staticmethod
-    def backward(ctx, dq, dk=None):
+    def backward(ctx, d_q, d_k=None):
         q, k, qw, kw, pos, table = ctx.saved_tensors
-        ps, eps, offset, interleaved = ctx.meta
-        if dq is None and dk is None:
-            return (None,) * 10
-        d_q, d_k = (None if g is None else _dense_channels(g) for g in (dq, dk))
+        gq = gk = gqw = gkw = None
+        q0 = q1 = q2 = k0 = k1 = k2 = 0
         # a side whose result nobody used has no gradient
-        q, qw = (None, None) if d_q is None else (q, qw)
-        k, kw = (None, None) if d_k is None else (k, kw)
-        new = lambda t: None if t is None else t.new_empty(t.shape)
-        gq, gk = new(q), new(k)
-        gqw, gkw = (torch.zeros_like(w) if w is not None and not one.numel() else new(w) for w, one in ((qw, q), (kw, k)))
-        one = k if q is None else q
-        if one.shape[0] * one.shape[1]:
-            block = _norm_block(q, k, qw, kw, None, None, pos, ps, table, eps, offset, interleaved)
-            at = lambda t: 0 if t is None else t.data_ptr()
-            none = (0, 0, 0)
-            sq, sk = none if d_q is None else d_q.stride(), none if d_k is None else d_k.stride()
-            grads = _lib.NORM_ROTARY_GRADS_PACK(at(d_q), at(d_k), at(gq), at(gk), at(gqw), at(gkw), *sq[:3], *sk[:3])
-            need = _lib.packed_call("dn_norm_rotary_bwd_workspace_size")(block)
-            ws = torch.empty(-(-need // 4), dtype=torch.float32, device=one.device)
-            _call("dn_norm_rotary_bwd", one.get_device(), block, grads, ws.data_ptr(), need)
-        if torch.is_grad_enabled() or _differentiated(d_q, d_k):   # create_graph
+        if d_q is None:
+            if d_k is None:
+                return None, None, None, None, None, None, None
+            q = qw = None
+        else:
+            d_q = _dense_channels(d_q)
+            gq, gqw = torch.empty_like(q, memory_format=torch.contiguous_format), torch.empty_like(qw)
+            q0, q1, q2, _ = d_q.stride()
+        if d_k is None:
+            k = kw = None
+        else:
+            d_k = _dense_channels(d_k)
+            gk, gkw = torch.empty_like(k, memory_format=torch.contiguous_format), torch.empty_like(kw)
+            k0, k1, k2, _ = d_k.stride()
+        block = _norm_block(q, k, qw, kw, None, None, pos, table, ctx.meta)
+        need = (_calls.get("dn_norm_rotary_bwd_workspace_size") or _lib.packed_call("dn_norm_rotary_bwd_workspace_size"))(block)
+        if need:
+            ws = (k if q is None else q).new_empty(need, dtype=torch.uint8)
+            grads = _lib.NORM_ROTARY_GRADS_PACK(
+                0 if d_q is None else d_q.data_ptr(), 0 if d_k is None else d_k.data_ptr(), 0 if gq is None else gq.data_ptr(),
+                0 if gk is None else gk.data_ptr(), 0 if gqw is None else gqw.data_ptr(), 0 if gkw is None else gkw.data_ptr(), q0, q1, q2, k0, k1, k2)
+            _call("dn_norm_rotary_bwd", ws.get_device(), block, grads, ws.data_ptr(), need)
+        else:   # no token, or no head
+            for g in (gqw, gkw):
+                if g is not None:
+                    g.zero_()
+        if _grad_enabled() or _differentiated(d_q, d_k):   # create_graph
             gq, gk, gqw, gkw = _NoSecondNorm.apply(gq, gk, gqw, gkw, d_q, d_k, q, k, qw, kw)
-        return gq, gk, gqw, gkw, None, None, None, None, None, None
+        return gq, gk, gqw, gkw, None, None, None
 
 
 class _NoSecondNorm(torch.autograd.Function):
@@ -346,6 +364,45 @@ def norm_rotary(q, k, q_weight, k_weight, positions=None, table=None, *, eps: fl
     summed in float32 and are the same bits every time.  Returns (q', k') with k' None
     if k is None; the results are contiguous.
     """
+    qs = q.shape
+    if not (3 <= len(qs) <= 4 and q.dtype in _DT and qs[-1] > 0 and type(eps) is float and 0.0 <= eps <= 3e38 and type(weight_offset) is float
+            and -3e38 <= weight_offset <= 3e38 and q_weight.dtype in _DT and q_weight.shape == qs[-1:] and q_weight.is_contiguous()
+            and (k_weight is None if k is None else k_weight is not None and k.dtype is q.dtype and k.ndim == len(qs) and k.shape[:-2] == qs[:-2]
+                 and k.shape[-1] == qs[-1] and k_weight.dtype is q_weight.dtype and k_weight.shape == q_weight.shape and k_weight.is_contiguous())
+            and (table is None if positions is None else table is not None)):
+        eps, weight_offset = _check_norm_rotary(q, k, q_weight, k_weight, positions, table, eps, weight_offset)
+    ps0 = ps1 = 0
+    if table is not None:
+        _check_table(table, qs[-1])
+        if positions.dtype not in _INT:
+            raise ValueError(f"positions must be int32 or int64, got {positions.dtype}.")
+    _on_gpu(q, k, q_weight, k_weight, positions, table)
+    if table is not None:
+        at = positions.shape
+        if at == qs[:-2]:
+            ps1 = positions.stride(-1)
+            if len(at) == 2:
+                ps0 = positions.stride(0)
+        elif len(at) == 1 and at[0] == qs[-3]:
+            ps1 = positions.stride(0)
+        else:
+            raise ValueError(f"positions {tuple(at)} must have the token dimensions of q {tuple(qs[:-2])}, or the last of them.")
+    flat = len(qs) == 3
+    if flat:
+        q, k = q[None], None if k is None else k[None]
+    q, k = _dense_channels(q), None if k is None else _dense_channels(k)
+    meta = ps0, ps1, eps, weight_offset, 1 if interleaved else 0
+    if _differentiated(q, k, q_weight, k_weight):
+        r = _NormRotaryFn.apply(q, k, q_weight, k_weight, positions, table, meta)
+        q_out, k_out = r if k is not None else (r, None)
+    else:
+        q_out, k_out = _norm_launch(q, k, q_weight, k_weight, positions, table, meta)
+    if flat:
+        q_out, k_out = q_out[0], None if k_out is None else k_out[0]
+    return q_out, k_out
+
+
+def _check_norm_rotary(q, k, q_weight, k_weight, positions, table, eps, weight_offset):
     if q.ndim not in (3, 4):
         raise ValueError(f"q must have rank 3 (N, Hq, D) or rank 4 (B, L, Hq, D), got shape {tuple(q.shape)}.")
     if q.dtype not in _DT:
@@ -358,32 +415,7 @@ def norm_rotary(q, k, q_weight, k_weight, positions=None, table=None, *, eps: fl
     if D < 1:
         raise ValueError("q must have a channel.")
     _check_weights(D, *([q_weight] if k is None else [q_weight, k_weight]))
-    eps, weight_offset = _check_norm(eps, weight_offset)
-    if table is not None:
-        _check_table(table, D)
-        if positions.dtype not in _INT:
-            raise ValueError(f"positions must be int32 or int64, got {positions.dtype}.")
-    _on_gpu(q, k, q_weight, k_weight, positions, table)
-    lead, ps = q.shape[:-2], (0, 0)
-    if positions is not None:
-        if positions.shape == lead:
-            ps = positions.stride()
-        elif positions.ndim == 1 and positions.shape[0] == lead[-1]:
-            ps = (0, positions.stride(0))
-        else:
-            raise ValueError(f"positions {tuple(positions.shape)} must have the token dimensions of q {tuple(lead)}, or the last of them.")
-    flat = q.ndim == 3
-    if flat:
-        q, k, ps = q[None], None if k is None else k[None], (0, ps[-1])
-    q, k = _dense_channels(q), None if k is None else _dense_channels(k)
-    if _differentiated(q, k, q_weight, k_weight):
-        r = _NormRotaryFn.apply(q, k, q_weight, k_weight, positions, ps, table, eps, weight_offset, bool(interleaved))
-        q_out, k_out = r if k is not None else (r, None)
-    else:
-        q_out, k_out = _norm_launch(q, k, q_weight, k_weight, positions, ps, table, eps, weight_offset, interleaved)
-    if flat:
-        q_out, k_out = q_out[0], None if k_out is None else k_out[0]
-    return q_out, k_out
+    return _check_norm(eps, weight_offset)
 
 
 # ---------------------------------------------------------------------------

@@ -17,6 +17,8 @@ Nothing here reads a device tensor on the host; all of it can be captured in a g
 
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import _lib
@@ -28,6 +30,13 @@ from .gdn2 import _DT
 __all__ = ["page_pool", "paged_reserve", "paged_slots", "paged_qkv_append", "paged_tree_attention", "paged_kv_keep"]
 
 _NODES = 1024   # new tokens of a tree
+_SCALE = {D: 1.0 / math.sqrt(D) for D in (64, 128, 256)}
+_CONTIGUOUS, _I32, _I64 = torch.contiguous_format, torch.int32, torch.int64
+
+# A step calls these once or once per layer, a token or two per sequence at a time, and
+# what it costs on the host is most of such a call.  So each asks in one expression
+# whether everything is as it mostly is, and goes through the checks with their messages
+# (the functions _check_..., which decide) only if it is not.
 
 
 def _check_page_size(page_size):
@@ -48,9 +57,13 @@ def _check_int32(name, t, shape):
         raise ValueError(f"{name} must be a contiguous int32 tensor {shape}, got {t.dtype} {tuple(t.shape)}.")
 
 
-def _written(*ts):
+def _written(ts):
     # autograd sees the store (inference tensors have no version)
-    _bump([t for t in ts if not t.is_inference()])
+    for t in ts:
+        if t.is_inference():
+            ts = [t for t in ts if not t.is_inference()]
+            break
+    _bump(ts)
 
 
 def page_pool(pages, *, device=None):
@@ -81,6 +94,22 @@ def paged_reserve(pool, page_table, held, lens, *, page_size: int):
     order in which it was taken, so that growing and trimming leave the pool as it was.
     B is at most 4096.
     """
+    B, most = page_table.shape if page_table.ndim == 2 else (-1, 0)
+    if not (type(page_size) is int and 0 < page_size <= 1 << 30 and not page_size & (page_size - 1) and 0 <= B <= _lib.MAX_SEQUENCES and most > 0
+            and page_table.dtype is _I32 and pool.dtype is _I32 and held.dtype is _I32 and lens.dtype is _I32
+            and page_table.stride(1) == 1 and pool.ndim == 1 and pool.is_contiguous() and held.shape == lens.shape == (B,) and held.is_contiguous()
+            and lens.is_contiguous() and 2 <= pool.shape[0] <= 0x7fffffff - B * most):
+        _check_reserve(pool, page_table, held, lens, page_size)
+    dev = _on_gpu(pool, page_table, held, lens)
+    short = torch.empty_like(lens)
+    if B:
+        _call("dn_paged_reserve", dev, pool.data_ptr(), pool.shape[0] - 2, page_table.data_ptr(), page_table.stride(0), most, B,
+              page_size, held.data_ptr(), lens.data_ptr(), short.data_ptr())
+        _written((pool, page_table, held))
+    return short
+
+
+def _check_reserve(pool, page_table, held, lens, page_size):
     _check_page_size(page_size)
     B = _check_table_rows(page_table)
     if pool.dtype is not torch.int32 or pool.ndim != 1 or pool.shape[0] < 2 or not pool.is_contiguous():
@@ -91,13 +120,6 @@ def paged_reserve(pool, page_table, held, lens, *, page_size: int):
         raise ValueError(f"paged_reserve takes at most {_lib.MAX_SEQUENCES} sequences, got {B}.")
     if B * page_table.shape[1] + pool.shape[0] > 0x7fffffff:
         raise ValueError("page_table and pool have too many pages.")
-    dev = _on_gpu(pool, page_table, held, lens)
-    short = torch.empty_like(lens)
-    if B:
-        _call("dn_paged_reserve", dev, pool.data_ptr(), pool.shape[0] - 2, page_table.data_ptr(), page_table.stride(0), page_table.shape[1], B,
-              page_size, held.data_ptr(), lens.data_ptr(), short.data_ptr())
-        _written(pool, page_table, held)
-    return short
 
 
 def paged_slots(page_table, seq_lens, tokens: int, *, page_size: int, cu_seqlens=None, held=None, parents=None, nodes=None):
@@ -122,6 +144,28 @@ def paged_slots(page_table, seq_lens, tokens: int, *, page_size: int, cu_seqlens
     token sees new token j of its sequence: itself and its ancestors.  Tokens that
     cu_seqlens gives to no sequence have position and slot -1 and see nothing.
     """
+    B, most = page_table.shape if page_table.ndim == 2 else (-1, 0)
+    if not (type(page_size) is int and 0 < page_size <= 1 << 30 and not page_size & (page_size - 1) and B > 0 and most > 0
+            and type(tokens) is int and 0 <= tokens <= 0x7fffffff and page_table.dtype is _I32 and page_table.stride(1) == 1
+            and seq_lens.dtype is _I32 and seq_lens.shape == (B,) and seq_lens.is_contiguous()
+            and (tokens % B == 0 if cu_seqlens is None else cu_seqlens.dtype is _I32 and cu_seqlens.shape == (B + 1,) and cu_seqlens.is_contiguous())
+            and (held is None or held.dtype is _I32 and held.shape == (B,) and held.is_contiguous())
+            and (nodes is None if parents is None else type(nodes) is int and 1 <= nodes <= _NODES and parents.dtype is _I32
+                 and parents.shape == (tokens,) and parents.is_contiguous())):
+        _check_slots(page_table, seq_lens, tokens, page_size, cu_seqlens, held, parents, nodes)
+    dev = _on_gpu(page_table, seq_lens, cu_seqlens, held, parents)
+    words = 0 if parents is None else (nodes + 63) >> 6
+    positions, slots = seq_lens.new_empty(tokens), seq_lens.new_empty(tokens, dtype=_I64)
+    visible = slots.new_empty((tokens, words)) if words else None
+    if tokens:
+        _call("dn_paged_slots", dev, _lib.PAGED_SLOTS_PACK(
+            _lib.DN_ABI_VERSION, tokens, B, page_size, most, words, page_table.data_ptr(), seq_lens.data_ptr(),
+            0 if cu_seqlens is None else cu_seqlens.data_ptr(), 0 if held is None else held.data_ptr(), 0 if parents is None else parents.data_ptr(),
+            positions.data_ptr(), slots.data_ptr(), 0 if visible is None else visible.data_ptr(), page_table.stride(0)))
+    return (positions, slots, visible) if words else (positions, slots)
+
+
+def _check_slots(page_table, seq_lens, tokens, page_size, cu_seqlens, held, parents, nodes):
     _check_page_size(page_size)
     B = _check_table_rows(page_table)
     if isinstance(tokens, bool) or not isinstance(tokens, int) or not 0 <= tokens <= 0x7fffffff:
@@ -135,22 +179,10 @@ def paged_slots(page_table, seq_lens, tokens: int, *, page_size: int, cu_seqlens
         raise ValueError(f"without cu_seqlens every sequence has tokens / B of them, got {tokens} for {B}.")
     if (parents is None) != (nodes is None):
         raise ValueError("parents goes with nodes.")
-    words = 0
     if parents is not None:
         _check_int32("parents", parents, (tokens,))
         if isinstance(nodes, bool) or not isinstance(nodes, int) or not 1 <= nodes <= _NODES:
             raise ValueError(f"nodes must be an integer from 1 to {_NODES}, got {nodes!r}.")
-        words = -(-nodes // 64)
-    dev = _on_gpu(page_table, seq_lens, cu_seqlens, held, parents)
-    positions = torch.empty(tokens, dtype=torch.int32, device=page_table.device)
-    slots = torch.empty(tokens, dtype=torch.int64, device=page_table.device)
-    visible = torch.empty((tokens, words), dtype=torch.int64, device=page_table.device) if words else None
-    if tokens:
-        at = lambda t: 0 if t is None else t.data_ptr()
-        _call("dn_paged_slots", dev, _lib.PAGED_SLOTS_PACK(
-            _lib.DN_ABI_VERSION, tokens, B, page_size, page_table.shape[1], words, page_table.data_ptr(), seq_lens.data_ptr(), at(cu_seqlens),
-            at(held), at(parents), positions.data_ptr(), slots.data_ptr(), at(visible), page_table.stride(0)))
-    return (positions, slots, visible) if words else (positions, slots)
 
 
 def paged_qkv_append(q, k, v, k_cache, v_cache, slots, positions, *, q_weight=None, k_weight=None, eps: float = 1e-6,
@@ -169,6 +201,44 @@ def paged_qkv_append(q, k, v, k_cache, v_cache, slots, positions, *, q_weight=No
     position past the table gives NaN in the rotated channels.  Slots must differ.
     Products in float32, one rounding.  Returns the queries, contiguous in q's shape and type.
     """
+    cs, qs, ks = k_cache.shape, q.shape, k.shape
+    dt, ct, lead = q.dtype, k_cache.dtype, slots.shape
+    kcs, vcs = k_cache.stride(), v_cache.stride()
+    wt = dt if q_weight is None else q_weight.dtype
+    if not (len(cs) == 4 and v_cache.shape == cs and v_cache.dtype is ct and ct in _DT and dt in _DT and k.dtype is dt and v.dtype is dt
+            and kcs[3] == vcs[3] == 1 and cs[1] > 0 and not cs[1] & (cs[1] - 1) and len(qs) in (3, 4) and qs[:-2] == lead and v.shape == ks
+            and ks[:-2] == lead and ks[-2:] == cs[2:] and qs[-1] == cs[3] and slots.dtype is _I64 and slots.is_contiguous()
+            and positions.dtype in _INT and positions.shape == lead and positions.is_contiguous()
+            and type(eps) is float and 0.0 <= eps <= 3e38 and type(weight_offset) is float and -3e38 <= weight_offset <= 3e38
+            and (k_weight is None if q_weight is None else k_weight is not None and k_weight.dtype is wt and wt in _DT
+                 and q_weight.shape == k_weight.shape == cs[3:] and q_weight.is_contiguous() and k_weight.is_contiguous())):
+        eps, weight_offset = _check_qkv_append(q, k, v, k_cache, v_cache, slots, positions, q_weight, k_weight, eps, weight_offset)
+    pages, page, Hkv, D = cs
+    R = 0 if table is None else _check_table(table, D)
+    dev = _on_gpu(q, k, v, k_cache, v_cache, slots, positions, q_weight, k_weight, table)
+    if _differentiated(q, k, v, k_cache, v_cache, q_weight, k_weight):
+        raise ValueError("paged_qkv_append is not differentiable; call it under torch.no_grad() (norm_rotary is its form for training).")
+    qt, kt, vt = q.stride(), k.stride(), v.stride()
+    if not qt[-1] == kt[-1] == vt[-1] == 1:
+        q, k, v = _dense_channels(q), _dense_channels(k), _dense_channels(v)
+        qt, kt, vt = q.stride(), k.stride(), v.stride()
+    out = torch.empty_like(q, memory_format=_CONTIGUOUS)
+    if len(qs) == 3:   # (strides of the batch: there is one)
+        B, T, qb, kb, vb = 1, qs[0], 0, 0, 0
+    else:
+        B, T, qb, kb, vb = qs[0], qs[1], qt[0], kt[0], vt[0]
+    if B and T:
+        _call("dn_qkv_append", dev, _lib.QKV_APPEND_PACK(
+            _lib.DN_ABI_VERSION, B, T, qs[-2], Hkv, D, R, _DT[dt], _DT[ct], _DT[wt],
+            _INT[positions.dtype], 1 if interleaved else 0, table.shape[0] if R else 0, pages, page, eps, weight_offset,
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), 0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(),
+            out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr(), positions.data_ptr(), table.data_ptr() if R else 0,
+            qb, qt[-3], qt[-2], kb, kt[-3], kt[-2], vb, vt[-3], vt[-2], kcs[0], kcs[1], kcs[2], vcs[0], vcs[1], vcs[2]))
+        _written((k_cache, v_cache))
+    return out
+
+
+def _check_qkv_append(q, k, v, k_cache, v_cache, slots, positions, q_weight, k_weight, eps, weight_offset):
     pages, page, Hkv, D = _check_caches(k_cache, v_cache)
     if page < 1 or page & (page - 1):
         raise ValueError(f"page_size must be a power of two, got {page}.")
@@ -186,25 +256,7 @@ def paged_qkv_append(q, k, v, k_cache, v_cache, slots, positions, *, q_weight=No
         raise ValueError("q_weight goes with k_weight.")
     if q_weight is not None:
         _check_weights(D, q_weight, k_weight)
-    eps, weight_offset = _check_norm(eps, weight_offset)
-    R = _check_table(table, D) if table is not None else 0
-    dev = _on_gpu(q, k, v, k_cache, v_cache, slots, positions, q_weight, k_weight, table)
-    if _differentiated(q, k, v, k_cache, v_cache, q_weight, k_weight):
-        raise ValueError("paged_qkv_append is not differentiable; call it under torch.no_grad() (norm_rotary is its form for training).")
-    q, k, v = _dense_channels(q), _dense_channels(k), _dense_channels(v)
-    out = q.new_empty(q.shape)
-    B, T = (1, lead[0]) if len(lead) == 1 else lead
-    if B * T:
-        qs, ks, vs = ((0, *t.stride()) if t.ndim == 3 else t.stride() for t in (q, k, v))
-        kcs, vcs = k_cache.stride(), v_cache.stride()
-        _call("dn_qkv_append", dev, _lib.QKV_APPEND_PACK(
-            _lib.DN_ABI_VERSION, B, T, q.shape[-2], Hkv, D, R, _DT[q.dtype], _DT[k_cache.dtype], _DT[q.dtype if q_weight is None else q_weight.dtype],
-            _INT[positions.dtype], 1 if interleaved else 0, table.shape[0] if R else 0, pages, page, eps, weight_offset,
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), 0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(),
-            out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr(), positions.data_ptr(), table.data_ptr() if R else 0,
-            qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], kcs[0], kcs[1], kcs[2], vcs[0], vcs[1], vcs[2]))
-        _written(k_cache, v_cache)
-    return out
+    return _check_norm(eps, weight_offset)
 
 
 def paged_tree_attention(q, k_cache, v_cache, page_table, seq_lens, visible, *, cu_seqlens=None, scale=None, window=None,
@@ -221,13 +273,53 @@ def paged_tree_attention(q, k_cache, v_cache, page_table, seq_lens, visible, *, 
     tokens that a token sees.  A token that sees nothing gets zeros (lse -inf).
     Returns as ``paged_attention`` does.
     """
+    cs, qs, ct = k_cache.shape, q.shape, k_cache.dtype
+    kcs, vcs, qt = k_cache.stride(), v_cache.stride(), q.stride()
+    N, words = visible.shape if visible.ndim == 2 else (-1, 0)
+    B, most = page_table.shape if page_table.ndim == 2 else (-1, 0)
+    nd, e = len(qs), 4 if ct is torch.float32 else 2
+    if not (len(cs) == 4 and v_cache.shape == cs and v_cache.dtype is ct and q.dtype is ct and ct in _DT and kcs[3] == vcs[3] == 1
+            and cs[0] > 0 and cs[1] > 0 and not cs[1] & (cs[1] - 1) and 3 <= nd <= 4 and qs[-1] == cs[3] and cs[3] in _SCALE
+            and cs[2] > 0 and qs[-2] > 0 and qs[-2] % cs[2] == 0 and B >= 0 and most > 0 and page_table.dtype is _I32 and page_table.stride(1) == 1
+            and seq_lens.dtype is _I32 and seq_lens.shape == (B,) and seq_lens.is_contiguous()
+            and (qs[0] == B and N == (B if nd == 3 else B * qs[1]) if cu_seqlens is None else nd == 3 and qs[0] == N and cu_seqlens.dtype is _I32
+                 and cu_seqlens.shape == (B + 1,) and cu_seqlens.is_contiguous())
+            and visible.dtype is _I64 and visible.is_contiguous() and 1 <= words <= _NODES >> 6 and scale is None and window is None
+            and not ((kcs[0] | kcs[1] | kcs[2] | vcs[0] | vcs[1] | vcs[2]) * e | k_cache.data_ptr() | v_cache.data_ptr()) & 15):
+        scale = _check_tree_attention(q, k_cache, v_cache, page_table, seq_lens, visible, cu_seqlens, scale, window)
+    else:
+        scale = _SCALE[cs[3]]
+    pages, page, Hkv, D = cs
+    dev = _on_gpu(q, k_cache, v_cache, page_table, seq_lens, visible, cu_seqlens)
+    if _differentiated(q, k_cache, v_cache):
+        raise ValueError("paged_tree_attention is not differentiable; call it under torch.no_grad().")
+    if qt[-1] != 1 or (q.data_ptr() | (qt[0] | qt[-3] | qt[-2]) * e) & 15:
+        q = _rows16(q)
+        qt = q.stride()
+    out = torch.empty_like(q, memory_format=_CONTIGUOUS)
+    lse = torch.empty(qs[:-1], dtype=torch.float32, device=q.device) if return_lse else None
+    if N:
+        block = _lib.PAGED_ATTENTION_PACK(
+            _lib.DN_ABI_VERSION, N, B, qs[-2], Hkv, D, _DT[ct], _window(window), pages, page, most, scale,
+            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+            page_table.data_ptr(), seq_lens.data_ptr(), 0 if cu_seqlens is None else cu_seqlens.data_ptr(),
+            qt[0], qt[0] if nd == 3 else qt[1], qt[-2], kcs[0], kcs[1], kcs[2], vcs[0], vcs[1], vcs[2], page_table.stride(0))
+        size = _calls.get("dn_paged_tree_attention_workspace_size") or _lib.packed_call("dn_paged_tree_attention_workspace_size")
+        need = size(block, words)
+        ws = q.new_empty(-(-need // e))
+        _call("dn_paged_tree_attention", dev, block, visible.data_ptr(), words, ws.data_ptr(), need)
+    return (out, lse) if return_lse else out
+
+
+def _check_tree_attention(q, k_cache, v_cache, page_table, seq_lens, visible, cu_seqlens, scale, window):
+    """The checks; the scale as a number."""
     pages, page, Hkv, D = _check_caches(k_cache, v_cache)
     if page < 1 or page & (page - 1) or pages < 1:
         raise ValueError(f"page_size must be a power of two and the cache have a page, got {tuple(k_cache.shape)}.")
     if q.dtype is not k_cache.dtype or q.shape[-1] != D:
         raise ValueError(f"q {tuple(q.shape)} {q.dtype} must have the cache's channels and type ({D}, {k_cache.dtype}).")
     _check_table_rows(page_table)
-    B, N, _, _ = _check_pages(page_table, seq_lens, cu_seqlens, q, "q")
+    _, N, _, _ = _check_pages(page_table, seq_lens, cu_seqlens, q, "q")
     scale = _attention_common(D, q.shape[-2], Hkv, q.dtype, scale, window)
     if visible.dtype is not torch.int64 or visible.ndim != 2 or visible.shape[0] != N or not 1 <= visible.shape[1] <= _NODES // 64 \
             or not visible.is_contiguous():
@@ -235,27 +327,11 @@ def paged_tree_attention(q, k_cache, v_cache, page_table, seq_lens, visible, *, 
     words = visible.shape[1]
     if window is not None and window < 64 * words:
         raise ValueError(f"the window of a tree must take in the {64 * words} new tokens that visible has bits for, got {window}.")
-    dev = _on_gpu(q, k_cache, v_cache, page_table, seq_lens, visible, cu_seqlens)
-    if _differentiated(q, k_cache, v_cache):
-        raise ValueError("paged_tree_attention is not differentiable; call it under torch.no_grad().")
+    _on_gpu(q, k_cache, v_cache, page_table, seq_lens, visible, cu_seqlens)
     kcs, vcs = k_cache.stride(), v_cache.stride()
     if (k_cache.data_ptr() | v_cache.data_ptr() | (kcs[0] | kcs[1] | kcs[2] | vcs[0] | vcs[1] | vcs[2]) * q.element_size()) & 15:
         raise ValueError(f"cache rows must start on 16 bytes, got strides {kcs} and {vcs}.")
-    q = _rows16(q)
-    qsb, qst = q.stride(0), q.stride(q.ndim - 3)
-    out = q.new_empty(q.shape)
-    lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device) if return_lse else None
-    if N:
-        block = _lib.PAGED_ATTENTION_PACK(
-            _lib.DN_ABI_VERSION, N, B, q.shape[-2], Hkv, D, _DT[q.dtype], _window(window), pages, page, page_table.shape[1], scale,
-            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
-            page_table.data_ptr(), seq_lens.data_ptr(), 0 if cu_seqlens is None else cu_seqlens.data_ptr(),
-            qsb, qst, q.stride(-2), kcs[0], kcs[1], kcs[2], vcs[0], vcs[1], vcs[2], page_table.stride(0))
-        size = _calls.get("dn_paged_tree_attention_workspace_size") or _lib.packed_call("dn_paged_tree_attention_workspace_size")
-        need = size(block, words)
-        ws = q.new_empty(-(-need // q.element_size()))
-        _call("dn_paged_tree_attention", dev, block, visible.data_ptr(), words, ws.data_ptr(), need)
-    return (out, lse) if return_lse else out
+    return scale
 
 
 def paged_kv_keep(k_cache, v_cache, page_table, starts, kept):
@@ -271,11 +347,34 @@ def paged_kv_keep(k_cache, v_cache, page_table, starts, kept):
     that are written must not be shared.  Returns int32 (B,): the sequences' lengths
     then, starts plus the number of tokens kept, for ``paged_reserve``.
     """
+    cs, ct = k_cache.shape, k_cache.dtype
+    ks, vs = k_cache.stride(), v_cache.stride()
+    B, most = kept.shape if kept.ndim == 2 else (-1, 0)
+    if not (4 <= len(cs) <= 5 and v_cache.shape == cs and v_cache.dtype is ct and ct in _DT and ks[-1] == vs[-1] == 1 and cs[-3] > 0
+            and not cs[-3] & (cs[-3] - 1) and page_table.ndim == 2 and page_table.dtype is _I32 and page_table.shape[0] == B <= 65535
+            and page_table.shape[1] > 0 and page_table.stride(1) == 1 and starts.dtype is _I32 and starts.shape == (B,) and starts.is_contiguous()
+            and kept.dtype is _I32 and kept.is_contiguous()):
+        _check_keep(k_cache, v_cache, page_table, starts, kept)
+    dev = _on_gpu(k_cache, v_cache, page_table, starts, kept)
+    if _differentiated(k_cache, v_cache):
+        raise ValueError("paged_kv_keep is not differentiable; call it under torch.no_grad().")
+    lens = torch.empty_like(starts)
+    if B:
+        many = len(cs) == 5
+        _call("dn_kv_keep", dev, _lib.KV_KEEP_PACK(
+            _lib.DN_ABI_VERSION, cs[0] if many else 1, B, cs[-2], cs[-1], most, _DT[ct], cs[-4], cs[-3], page_table.shape[1],
+            k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(), starts.data_ptr(), kept.data_ptr(), lens.data_ptr(),
+            ks[0] if many else 0, ks[-4], ks[-3], ks[-2], vs[0] if many else 0, vs[-4], vs[-3], vs[-2], page_table.stride(0)))
+        _written((k_cache, v_cache))
+    return lens
+
+
+def _check_keep(k_cache, v_cache, page_table, starts, kept):
     many = k_cache.ndim == 5 and v_cache.ndim == 5
     if many and k_cache.shape[0] != v_cache.shape[0]:
         raise ValueError(f"v_cache {tuple(v_cache.shape)} must have the layers of k_cache {tuple(k_cache.shape)}.")
     one = (lambda c: c[0] if c.shape[0] else c.new_empty(c.shape[1:])) if many else (lambda c: c)
-    pages, page, H, D = _check_caches(one(k_cache), one(v_cache))
+    _, page, _, _ = _check_caches(one(k_cache), one(v_cache))
     if page < 1 or page & (page - 1):
         raise ValueError(f"page_size must be a power of two, got {page}.")
     B = _check_table_rows(page_table)
@@ -285,15 +384,3 @@ def paged_kv_keep(k_cache, v_cache, page_table, starts, kept):
     _check_int32("kept", kept, (B, kept.shape[1]))
     if B > 65535:
         raise ValueError(f"paged_kv_keep takes at most 65535 sequences, got {B}.")
-    dev = _on_gpu(k_cache, v_cache, page_table, starts, kept)
-    if _differentiated(k_cache, v_cache):
-        raise ValueError("paged_kv_keep is not differentiable; call it under torch.no_grad().")
-    lens = torch.empty_like(starts)
-    if B:
-        ks, vs = ((0, *c.stride())[-5:] for c in (k_cache, v_cache))
-        _call("dn_kv_keep", dev, _lib.KV_KEEP_PACK(
-            _lib.DN_ABI_VERSION, k_cache.shape[0] if many else 1, B, H, D, kept.shape[1], _DT[k_cache.dtype], pages, page, page_table.shape[1],
-            k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(), starts.data_ptr(), kept.data_ptr(), lens.data_ptr(),
-            ks[0], ks[1], ks[2], ks[3], vs[0], vs[1], vs[2], vs[3], page_table.stride(0)))
-        _written(k_cache, v_cache)
-    return lens
