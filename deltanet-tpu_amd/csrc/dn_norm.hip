@@ -5,12 +5,14 @@
 // z = rotation(y).  For dz: g = rotation^T(dz), h = g (offset + w),
 // dx = r (h - x r^2 mean(h x)), dw = sum of g x r over tokens and heads.
 //
-// Streams: every head is read once and written once.  A thread owns 16 channels of a
-// token (dn_rotary.h) and D / 16 neighbouring lanes a head, whose sums they exchange
-// in registers; the angles and the weights are read once for the heads of a thread.
+// Streams: every head is read once and written once.  A thread owns two groups of 16
+// bytes of a head that are each other's partners in the rotation of halves (and hold
+// whole pairs of the interleaved one), and its neighbours the groups beside them, so
+// that every load and store of a wave is of whole lines; D / 16 (float32: D / 8) lanes
+// exchange a head's sums in registers.  The angles and the weights are read once for
+// the heads of a thread.
 #include "dn_attn.h"
 #include "dn_host.h"
-#include "dn_rotary.h"
 
 namespace dn {
 
@@ -70,19 +72,92 @@ __device__ __forceinline__ int64_t pos_of(const HP& p, int b, int l) {
   return p.pos64 ? ((const int64_t*)p.pos)[i] : (int64_t)((const int32_t*)p.pos)[i];
 }
 
-// 8 weights of any type, plus the offset
-__device__ __forceinline__ void weights8(const void* w, int dt, int at, float offset, float* o) {
-  if (dt == DT_F32) ld8<float>((const float*)w + at, o);
-  else if (dt == DT_BF16) ld8<bf16>((const bf16*)w + at, o);
-  else ld8<f16>((const f16*)w + at, o);
+template <class T> constexpr int kWidth = 16 / (int)sizeof(T);   // channels of a group
+// W values of a type, in floats
+template <int W, class T> __device__ __forceinline__ void load(const T* p, float* o) {
+  typedef T V __attribute__((ext_vector_type(W)));
+  const V a = *reinterpret_cast<const V*>(p);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) o[i] += offset;
+  for (int i = 0; i < W; ++i) o[i] = (float)a[i];
+}
+template <int W, bool PAST, class T> __device__ __forceinline__ void store(T* p, const float* v) {
+  typedef T V __attribute__((ext_vector_type(W)));
+  V a;
+#pragma unroll
+  for (int i = 0; i < W; ++i) a[i] = (T)v[i];
+  if constexpr (PAST) __builtin_nontemporal_store(a, reinterpret_cast<V*>(p));
+  else *reinterpret_cast<V*>(p) = a;
 }
 
-template <bool PAST> __device__ __forceinline__ void put8(void* p, int dt, int64_t at, const float* v) {
-  if (dt == DT_F32) st8<float, PAST>((float*)p + at, v);
-  else if (dt == DT_BF16) st8<bf16, PAST>((bf16*)p + at, v);
-  else st8<f16, PAST>((f16*)p + at, v);
+// The two groups of lane `it` of a head; those of the first R channels are rotated.
+struct Item { int a, b; bool turn; };
+template <int W> __device__ __forceinline__ Item item_of(int it, int D, int R) {
+  const int nr = R / (2 * W);
+  if (it < nr) return {it * W, (R >> 1) + it * W, true};
+  return {R + (it - nr) * W, R + ((D - R) >> 1) + (it - nr) * W, false};
+}
+// Cosines and sines of its pairs: one set for the halves, W / 2 for each group of
+// interleaved ones.  A position outside the table: NaN.
+template <int W> __device__ __forceinline__ void angles(const float* table, int64_t pos, int rows, int R, const Item& it, bool inter, float sign, float* c, float* s) {
+  if (pos < 0 || pos >= rows) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) c[i] = s[i] = __builtin_nanf("");
+    return;
+  }
+  const float* r = table + pos * R;
+  if (inter) {
+    load<W / 2>(r + it.a / 2, c);
+    load<W / 2>(r + it.b / 2, c + W / 2);
+    load<W / 2>(r + (R + it.a) / 2, s);
+    load<W / 2>(r + (R + it.b) / 2, s + W / 2);
+  } else {
+    load<W>(r + it.a, c);
+    load<W>(r + (R >> 1) + it.a, s);
+  }
+#pragma unroll
+  for (int i = 0; i < W; ++i) s[i] *= sign;
+}
+// (x, y) -> (x c - y s, y c + x s) for its pairs
+template <int W> __device__ __forceinline__ void turn(float* x, float* y, const float* c, const float* s, bool inter) {
+  if (inter) {
+#pragma unroll
+    for (int i = 0; i < W / 2; ++i) {
+      const float a = x[2 * i], b = x[2 * i + 1], d = y[2 * i], e = y[2 * i + 1];
+      x[2 * i] = a * c[i] - b * s[i];
+      x[2 * i + 1] = b * c[i] + a * s[i];
+      y[2 * i] = d * c[W / 2 + i] - e * s[W / 2 + i];
+      y[2 * i + 1] = e * c[W / 2 + i] + d * s[W / 2 + i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const float a = x[i], b = y[i];
+      x[i] = a * c[i] - b * s[i];
+      y[i] = b * c[i] + a * s[i];
+    }
+  }
+}
+// One pair, or one channel that is not rotated: any sizes.
+__device__ __forceinline__ void pair_of(int i, int R, bool inter, int& a, int& b) {
+  const int half = R >> 1;
+  if (i >= half) { a = R + (i - half); b = -1; }
+  else if (inter) { a = 2 * i; b = a + 1; }
+  else { a = i; b = i + half; }
+}
+
+// weights of any type, plus the offset
+template <int W> __device__ __forceinline__ void weights(const void* w, int dt, int at, float offset, float* o) {
+  if (dt == DT_F32) load<W>((const float*)w + at, o);
+  else if (dt == DT_BF16) load<W>((const bf16*)w + at, o);
+  else load<W>((const f16*)w + at, o);
+#pragma unroll
+  for (int i = 0; i < W; ++i) o[i] += offset;
+}
+
+template <int W, bool PAST> __device__ __forceinline__ void put(void* p, int dt, int64_t at, const float* v) {
+  if (dt == DT_F32) store<W, PAST>((float*)p + at, v);
+  else if (dt == DT_BF16) store<W, PAST>((bf16*)p + at, v);
+  else store<W, PAST>((f16*)p + at, v);
 }
 __device__ __forceinline__ void put1(void* p, int dt, int64_t at, float v) {
   if (dt == DT_F32) ((float*)p)[at] = v;
@@ -122,9 +197,10 @@ template <class T, bool PAGED> __device__ __forceinline__ Dst dst_of(const HP& p
 // x: (token, item) in groups of P threads, y: NH heads of q, k or v.
 template <class T, int P, int NH, bool PAGED, bool PAST>
 __global__ __launch_bounds__(256) void k_heads(const HP p) {
+  constexpr int W = kWidth<T>;
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int i = threadIdx.x % P;
-  const bool live = id / P < p.N && i < p.D >> 4;
+  const bool live = id / P < p.N && i < p.D / (2 * W);
   const int64_t t = min(id / P, (int64_t)p.N - 1);
   int y = blockIdx.y, side = 0;
   for (; side < 2; ++side) {
@@ -133,26 +209,26 @@ __global__ __launch_bounds__(256) void k_heads(const HP p) {
     y -= n;
   }
   const int h0 = y * NH, H = p.H[side], b = (int)(t / p.L), l = (int)(t % p.L);
-  const Item it = item_of(i, p.R, p.inter);
+  const Item it = item_of<W>(i, p.D, p.R);
   const T* s = (const T*)p.x[side] + b * p.xs[side][0] + l * p.xs[side][1] + h0 * p.xs[side][2];
-  float u[NH][8], v[NH][8];
+  float u[NH][W], v[NH][W];
 #pragma unroll
   for (int h = 0; h < NH; ++h) {
     if (live && h0 + h < H) {
-      ld8<T>(s + h * p.xs[side][2] + it.a, u[h]);
-      ld8<T>(s + h * p.xs[side][2] + it.b, v[h]);
+      load<W>(s + h * p.xs[side][2] + it.a, u[h]);
+      load<W>(s + h * p.xs[side][2] + it.b, v[h]);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) u[h][e] = v[h][e] = 0.f;
+      for (int e = 0; e < W; ++e) u[h][e] = v[h][e] = 0.f;
     }
   }
   const int64_t pos = PAGED || p.R ? pos_of(p, b, l) : 0;
-  float c[8], sn[8], wa[8], wb[8];
-  const bool turn = side < 2 && live && it.row >= 0, norm = side < 2 && p.w[0];
-  if (turn) angles8(p.table, pos, p.rows, p.R, it.row, 1.f, c, sn);
+  float c[W], sn[W], wa[W], wb[W];
+  const bool turns = side < 2 && live && it.turn, norm = side < 2 && p.w[0];
+  if (turns) angles<W>(p.table, pos, p.rows, p.R, it, p.inter, 1.f, c, sn);
   if (norm && live) {
-    weights8(p.w[side], p.wdt, it.a, p.offset, wa);
-    weights8(p.w[side], p.wdt, it.b, p.offset, wb);
+    weights<W>(p.w[side], p.wdt, it.a, p.offset, wa);
+    weights<W>(p.w[side], p.wdt, it.b, p.offset, wb);
   }
   const Dst d = dst_of<T, PAGED>(p, side, t, pos);
   const float over = 1.f / p.D;
@@ -161,24 +237,24 @@ __global__ __launch_bounds__(256) void k_heads(const HP p) {
     if (norm) {
       float z = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) z += u[h][e] * u[h][e] + v[h][e] * v[h][e];
+      for (int e = 0; e < W; ++e) z += u[h][e] * u[h][e] + v[h][e] * v[h][e];
       const float r = rsqrt32(sum_lanes<P>(z) * over + p.eps);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
+      for (int e = 0; e < W; ++e) {
         u[h][e] = u[h][e] * r * wa[e];
         v[h][e] = v[h][e] * r * wb[e];
       }
     }
     if (!live || h0 + h >= H) continue;
-    if (turn) turn8(u[h], v[h], c, sn, p.inter);
+    if (turns) turn<W>(u[h], v[h], c, sn, p.inter);
     if (PAGED && side == 0 && d.none) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) u[h][e] = v[h][e] = 0.f;
+      for (int e = 0; e < W; ++e) u[h][e] = v[h][e] = 0.f;
     }
     if (!d.store) continue;
     const int64_t at = d.at + (h0 + h) * d.head;
-    put8<PAST>(p.out[side], d.dt, at + it.a, u[h]);
-    put8<PAST>(p.out[side], d.dt, at + it.b, v[h]);
+    put<W, PAST>(p.out[side], d.dt, at + it.a, u[h]);
+    put<W, PAST>(p.out[side], d.dt, at + it.b, v[h]);
   }
 }
 
@@ -228,9 +304,10 @@ __global__ __launch_bounds__(256) void k_heads_any(const HP p) {
 // The gradient.  Groups of P threads walk over tokens; y: NH heads of q or k.
 template <class T, int P, int NH>
 __global__ __launch_bounds__(256) void k_heads_grad(const HP p, const GP g) {
-  __shared__ float sums[256 / P][P * 16];
+  constexpr int W = kWidth<T>;
+  __shared__ float sums[256 / P][P * 2 * W];
   const int i = threadIdx.x % P;
-  const bool own = i < p.D >> 4;
+  const bool own = i < p.D / (2 * W);
   int y = blockIdx.y, side = 0;
   const int nq = (p.H[0] + NH - 1) / NH;
   if (y >= nq) {
@@ -238,13 +315,13 @@ __global__ __launch_bounds__(256) void k_heads_grad(const HP p, const GP g) {
     y -= nq;
   }
   const int h0 = y * NH, H = p.H[side];
-  const Item it = item_of(i, p.R, p.inter);
-  float wa[8], wb[8], da[8], db[8];
+  const Item it = item_of<W>(i, p.D, p.R);
+  float wa[W], wb[W], da[W], db[W];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) wa[e] = wb[e] = da[e] = db[e] = 0.f;
+  for (int e = 0; e < W; ++e) wa[e] = wb[e] = da[e] = db[e] = 0.f;
   if (own) {
-    weights8(p.w[side], p.wdt, it.a, p.offset, wa);
-    weights8(p.w[side], p.wdt, it.b, p.offset, wb);
+    weights<W>(p.w[side], p.wdt, it.a, p.offset, wa);
+    weights<W>(p.w[side], p.wdt, it.b, p.offset, wb);
   }
   const float over = 1.f / p.D;
 #pragma unroll 1
@@ -252,48 +329,48 @@ __global__ __launch_bounds__(256) void k_heads_grad(const HP p, const GP g) {
     const int b = (int)(t / p.L), l = (int)(t % p.L);
     const T* s = (const T*)p.x[side] + b * p.xs[side][0] + l * p.xs[side][1] + h0 * p.xs[side][2];
     const T* z = (const T*)g.dz[side] + b * g.zs[side][0] + l * g.zs[side][1] + h0 * g.zs[side][2];
-    float u[NH][8], v[NH][8], gu[NH][8], gv[NH][8];
+    float u[NH][W], v[NH][W], gu[NH][W], gv[NH][W];
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
       if (own && h0 + h < H) {
-        ld8<T>(s + h * p.xs[side][2] + it.a, u[h]);
-        ld8<T>(s + h * p.xs[side][2] + it.b, v[h]);
-        ld8<T>(z + h * g.zs[side][2] + it.a, gu[h]);
-        ld8<T>(z + h * g.zs[side][2] + it.b, gv[h]);
+        load<W>(s + h * p.xs[side][2] + it.a, u[h]);
+        load<W>(s + h * p.xs[side][2] + it.b, v[h]);
+        load<W>(z + h * g.zs[side][2] + it.a, gu[h]);
+        load<W>(z + h * g.zs[side][2] + it.b, gv[h]);
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) u[h][e] = v[h][e] = gu[h][e] = gv[h][e] = 0.f;
+        for (int e = 0; e < W; ++e) u[h][e] = v[h][e] = gu[h][e] = gv[h][e] = 0.f;
       }
     }
-    float c[8], sn[8];
-    const bool turn = own && it.row >= 0;
-    if (turn) angles8(p.table, pos_of(p, b, l), p.rows, p.R, it.row, -1.f, c, sn);
+    float c[W], sn[W];
+    const bool turns = own && it.turn;
+    if (turns) angles<W>(p.table, pos_of(p, b, l), p.rows, p.R, it, p.inter, -1.f, c, sn);
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
-      if (turn) turn8(gu[h], gv[h], c, sn, p.inter);
+      if (turns) turn<W>(gu[h], gv[h], c, sn, p.inter);
       float xx = 0.f, hx = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
+      for (int e = 0; e < W; ++e) {
         xx += u[h][e] * u[h][e] + v[h][e] * v[h][e];
         hx += gu[h][e] * wa[e] * u[h][e] + gv[h][e] * wb[e] * v[h][e];
       }
       const float r = rsqrt32(sum_lanes<P>(xx) * over + p.eps), k = sum_lanes<P>(hx) * over * r * r;
       if (!own || h0 + h >= H) continue;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
+      for (int e = 0; e < W; ++e) {
         da[e] += gu[h][e] * u[h][e] * r;
         db[e] += gv[h][e] * v[h][e] * r;
         gu[h][e] = r * (gu[h][e] * wa[e] - u[h][e] * k);
         gv[h][e] = r * (gv[h][e] * wb[e] - v[h][e] * k);
       }
       T* d = (T*)g.dx[side] + (t * H + h0 + h) * p.D;
-      st8<T, true>(d + it.a, gu[h]);
-      st8<T, true>(d + it.b, gv[h]);
+      store<W, true>(d + it.a, gu[h]);
+      store<W, true>(d + it.b, gv[h]);
     }
   }
   if (own) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < W; ++e) {
       sums[threadIdx.x / P][it.a + e] = da[e];
       sums[threadIdx.x / P][it.b + e] = db[e];
     }
@@ -399,14 +476,15 @@ template <class F> void by_type(int dt, F f) {
   else f(0.f);
 }
 template <int N> struct Num { static constexpr int value = N; };
-// lanes of a head: the power of two from D / 16 on
-template <class F> void by_lanes(int D, F f) {
-  if (D <= 64) f(Num<4>{});
-  else if (D <= 128) f(Num<8>{});
-  else if (D <= 256) f(Num<16>{});
-  else f(Num<32>{});
+// lanes of a head: a power of two, two groups each
+template <class T, class F> void by_lanes(int D, F f) {
+  constexpr int W = kWidth<T>;
+  if (D <= 64) f(Num<32 / W>{});
+  else if (D <= 128) f(Num<64 / W>{});
+  else if (D <= 256) f(Num<128 / W>{});
+  else f(Num<256 / W>{});
 }
-constexpr int kMostD = 512;   // of the kernels with a thread per 16 channels
+constexpr int kMostD = 512;   // of these kernels
 constexpr int kMostBlocks = 0x7fffffff;
 
 // Threads of one head each that fill the card a few times over; from there on a
@@ -422,8 +500,9 @@ const char* heads_error(const HP& p, int dtype, int pos_dtype) {
   if (!(p.eps >= 0.f) || !(p.eps - p.eps == 0.f) || !(p.offset - p.offset == 0.f)) return "eps and offset must be finite, eps not negative";
   return nullptr;
 }
-bool fast_heads(const HP& p) {
-  if (p.D % 16 || p.R % 16 || p.D > kMostD || !aligned(p.table) || !aligned(p.w[0]) || !aligned(p.w[1])) return false;
+bool fast_heads(const HP& p, int dtype) {
+  const int two = dtype == DN_F32 ? 8 : 16;   // channels of a lane
+  if (p.D % two || p.R % two || p.D > kMostD || !aligned(p.table) || !aligned(p.w[0]) || !aligned(p.w[1])) return false;
   for (int i = 0; i < 3; ++i)
     if (p.H[i] && !(wide(p.x[i], p.xs[i], 3) && aligned(p.out[i]))) return false;
   return true;
@@ -441,7 +520,7 @@ template <bool PAGED> int launch_heads(const HP& p, int dtype, bool fast, hipStr
       hipLaunchKernelGGL((k_heads_any<T, PAGED>), dim3((unsigned)blocks), dim3(256), 0, st, p);
       return;
     }
-    by_lanes(p.D, [&](auto lanes) {
+    by_lanes<T>(p.D, [&](auto lanes) {
       constexpr int P = decltype(lanes)::value;
       const int64_t blocks = ((int64_t)p.N * P + 255) / 256;
       if (!(ok = blocks <= kMostBlocks)) return;
@@ -480,23 +559,23 @@ int norm_params(const dn_norm_rotary_args* a, HP& p) {
 constexpr int kGradHeads = 2;
 constexpr int64_t kGradBlocks = 2048;
 struct GradPlan { int x, rows_q, rows_k; };
-GradPlan grad_plan(const HP& p, bool fast) {
+GradPlan grad_plan(const HP& p, int dtype, bool fast) {
   if (!fast) {
     const int x = (int)std::min<int64_t>((int64_t)p.N * std::max(p.H[0], p.H[1]), kGradBlocks);
     return {x, x, x};
   }
-  int P = 4;
-  while (P * 16 < p.D) P *= 2;
+  int P = dtype == DN_F32 ? 8 : 4;
+  while (P * (dtype == DN_F32 ? 8 : 16) < p.D) P *= 2;
   const int64_t most = ((int64_t)p.N * P + 255) / 256;
   const int x = (int)std::max<int64_t>(1, std::min(most, kGradBlocks / chunks(p, kGradHeads)));
   return {x, x * ((p.H[0] + kGradHeads - 1) / kGradHeads), x * ((p.H[1] + kGradHeads - 1) / kGradHeads)};
 }
 // (the two forms' plans may differ: the larger)
-size_t grad_bytes(const HP& p) {
+size_t grad_bytes(const HP& p, int dtype) {
   size_t n = 0;
   for (const bool fast : {false, true}) {
     if (fast && p.D > kMostD) continue;
-    const GradPlan g = grad_plan(p, fast);
+    const GradPlan g = grad_plan(p, dtype, fast);
     n = std::max(n, ((size_t)g.rows_q + g.rows_k) * p.D * sizeof(float));
   }
   return n + 256;
@@ -512,13 +591,13 @@ extern "C" int dn_norm_rotary(const dn_norm_rotary_args* a, void* stream) {
   if (const int rc = norm_params(a, p)) return rc;
   if (p.N == 0 || p.H[0] + p.H[1] == 0) return DN_OK;
   if ((p.H[0] && !p.out[0]) || (p.H[1] && !p.out[1])) return bad("missing tensor pointer");
-  return launch_heads<false>(p, a->dtype, fast_heads(p), (hipStream_t)stream);
+  return launch_heads<false>(p, a->dtype, fast_heads(p, a->dtype), (hipStream_t)stream);
 }
 
 extern "C" size_t dn_norm_rotary_bwd_workspace_size(const dn_norm_rotary_args* a) {
   HP p{};
   if (norm_params(a, p) != DN_OK || p.N == 0 || p.H[0] + p.H[1] == 0) return 0;
-  return grad_bytes(p);
+  return grad_bytes(p, a->dtype);
 }
 
 extern "C" int dn_norm_rotary_bwd(const dn_norm_rotary_args* a, const dn_norm_rotary_grads* d, void* workspace, size_t workspace_bytes, void* stream) {
@@ -527,15 +606,15 @@ extern "C" int dn_norm_rotary_bwd(const dn_norm_rotary_args* a, const dn_norm_ro
   if (const int rc = norm_params(a, p)) return rc;
   if (p.N == 0 || p.H[0] + p.H[1] == 0) return DN_OK;
   if ((p.H[0] && (!d->d_q || !d->dq)) || (p.H[1] && (!d->d_k || !d->dk))) return bad("missing tensor pointer");
-  if (!workspace || workspace_bytes < grad_bytes(p)) return set_error(DN_E_WORKSPACE, "workspace missing or too small");
+  if (!workspace || workspace_bytes < grad_bytes(p, a->dtype)) return set_error(DN_E_WORKSPACE, "workspace missing or too small");
   GP g{};
   g.dz[0] = d->d_q; g.dz[1] = d->d_k; g.dx[0] = d->dq; g.dx[1] = d->dk;
   for (int i = 0; i < 3; ++i) { g.zs[0][i] = d->d_q_strides[i]; g.zs[1][i] = d->d_k_strides[i]; }
   g.part = (float*)(((uintptr_t)workspace + 255) & ~(uintptr_t)255);
   p.out[0] = d->dq; p.out[1] = d->dk;
-  bool fast = fast_heads(p);
+  bool fast = fast_heads(p, a->dtype);
   for (int i = 0; i < 2; ++i) fast = fast && (!p.H[i] || wide(g.dz[i], g.zs[i], 3));
-  const GradPlan plan = grad_plan(p, fast);
+  const GradPlan plan = grad_plan(p, a->dtype, fast);
   hipStream_t st = (hipStream_t)stream;
   by_type(a->dtype, [&](auto z) {
     using T = decltype(z);
@@ -543,7 +622,7 @@ extern "C" int dn_norm_rotary_bwd(const dn_norm_rotary_args* a, const dn_norm_ro
       hipLaunchKernelGGL((k_heads_grad_any<T>), dim3(plan.x, 2), dim3(64), 0, st, p, g);
       return;
     }
-    by_lanes(p.D, [&](auto lanes) {
+    by_lanes<T>(p.D, [&](auto lanes) {
       constexpr int P = decltype(lanes)::value;
       hipLaunchKernelGGL((k_heads_grad<T, P, kGradHeads>), dim3(plan.x, chunks(p, kGradHeads)), dim3(256), 0, st, p, g);
     });
@@ -579,6 +658,6 @@ extern "C" int dn_qkv_append(const dn_qkv_append_args* a, void* stream) {
       (p.R && (!p.table || p.rows <= 0)))
     return bad("missing tensor pointer");
   if (!p.w[0] != !p.w[1]) return bad("both of the norms' weights, or none");
-  const bool fast = fast_heads(p) && (!p.H[1] || (wide(p.out[1], p.cs[0], 3) && wide(p.out[2], p.cs[1], 3)));
+  const bool fast = fast_heads(p, a->dtype) && (!p.H[1] || (wide(p.out[1], p.cs[0], 3) && wide(p.out[2], p.cs[1], 3)));
   return launch_heads<true>(p, a->dtype, fast, (hipStream_t)stream);
 }

@@ -64,24 +64,32 @@ struct RP {
 // pages: a page that is taken is read off the stack, or, if it lies among those given
 // back in this call, from the row of the sequence that gives it, which nothing
 // overwrites.  Lengths and counts are written by the block that comes to its end last,
-// when all others have read them.
+// when all others have read them; it reads nothing that they wrote, so that the count
+// of those that ended needs no fence.
 __global__ __launch_bounds__(kThreads) void k_reserve(const RP p) {
   extern __shared__ int lds[];   // [2][B]: pages taken, given back by the sequences in front
   int *taken = lds, *given = lds + p.B;
   __shared__ int waves[kThreads / 64], s_last;
-  const int per = (p.B + kThreads - 1) / kThreads, b0 = min((int)threadIdx.x * per, p.B), b1 = min(b0 + per, p.B);
   const int count = min(max(p.pool[0], 0), p.capacity);
   auto needs = [&](int b, int& h, int& need) {
     h = min(max(p.held[b], 0), p.max_pages);
     const int n = max(p.lens[b], 0);
     need = (n >> p.shift) + ((n & ((1 << p.shift) - 1)) != 0);
   };
-  int grow = 0, back = 0;
-  for (int b = b0; b < b1; ++b) {
+#pragma unroll 4
+  for (int b = threadIdx.x; b < p.B; b += kThreads) {
     int h, need;
     needs(b, h, need);
-    if (need <= p.max_pages) grow += max(need - h, 0);
-    back += max(h - need, 0);
+    taken[b] = need <= p.max_pages ? max(need - h, 0) : 0;
+    given[b] = max(h - need, 0);
+  }
+  __syncthreads();
+  // a run of sequences per thread
+  const int per = (p.B + kThreads - 1) / kThreads, b0 = min((int)threadIdx.x * per, p.B), b1 = min(b0 + per, p.B);
+  int grow = 0, back = 0;
+  for (int b = b0; b < b1; ++b) {
+    grow += taken[b];
+    back += given[b];
   }
   int F, all;
   int f = block_scan(back, waves, F), a = block_scan(grow, waves, all);
@@ -89,16 +97,12 @@ __global__ __launch_bounds__(kThreads) void k_reserve(const RP p) {
   // sequences take while what all up to them need is there
   int got = 0;
   for (int b = b0; b < b1; ++b) {
-    int h, need;
-    needs(b, h, need);
-    const int g = need <= p.max_pages ? max(need - h, 0) : 0;
+    const int g = taken[b], x = given[b];
     taken[b] = a;
     given[b] = f;
-    const bool fits = a + g <= full;
     a += g;
-    f += max(h - need, 0);
-    if (fits) got = a;   // (what those that fit take is what all up to the last of them need)
-    if (blockIdx.x == 0) p.short_of[b] = need > h && (!fits || need > p.max_pages) ? need - h : 0;
+    f += x;
+    if (a <= full) got = a;   // (what those that fit take is what all up to the last of them need)
   }
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) got = max(got, __shfl_xor(got, o));
@@ -117,29 +121,27 @@ __global__ __launch_bounds__(kThreads) void k_reserve(const RP p) {
     return p.table[b * p.stride + need + (x - given[b])];
   };
   const int me = blockIdx.x * kThreads + threadIdx.x, step = gridDim.x * kThreads;
+#pragma unroll 2
   for (int k = me; k < A; k += step) {
     const int b = last_at_most(taken, p.B, k), at = full - 1 - k;
-    const int page = at < count ? p.pool[2 + at] : given_page(F - 1 - (at - count));
     const int col = min(max(p.held[b], 0), p.max_pages) + (k - taken[b]);
-    p.table[b * p.stride + col] = page;
+    p.table[b * p.stride + col] = at < count ? p.pool[2 + at] : given_page(F - 1 - (at - count));
   }
+#pragma unroll 2
   for (int k = me; k < min(left, p.capacity) - count; k += step) p.pool[2 + count + k] = given_page(F - 1 - k);
   __syncthreads();
   if (gridDim.x > 1) {
-    if (threadIdx.x == 0) {
-      __threadfence();
-      s_last = atomicAdd(&p.pool[1], 1) == (int)gridDim.x - 1;
-      __threadfence();
-    }
+    if (threadIdx.x == 0) s_last = __hip_atomic_fetch_add(&p.pool[1], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
     __syncthreads();
     if (!s_last) return;
   }
-  for (int b = b0; b < b1; ++b) {
+#pragma unroll 4
+  for (int b = threadIdx.x; b < p.B; b += kThreads) {
     int h, need;
     needs(b, h, need);
-    if (need < h) p.held[b] = need;
-    else if (need <= p.max_pages && taken[b] + (need - h) <= full) p.held[b] = need;
-    else p.held[b] = h;
+    const bool fits = need <= p.max_pages && (need <= h || taken[b] + (need - h) <= full);
+    p.short_of[b] = fits ? 0 : need - h;
+    p.held[b] = fits ? need : h;
   }
   if (threadIdx.x == 0) {
     p.pool[0] = min(left, p.capacity);
@@ -398,7 +400,7 @@ extern "C" int dn_paged_slots(const dn_paged_slots_args* a, void* stream) {
     hipLaunchKernelGGL(k_slots_tree, dim3(p.B), dim3(kThreads), 0, (hipStream_t)stream, p);
   } else {
     // parts of 1024 tokens, as many as the longest sequence may have, but no more blocks than fill the card
-    const int64_t parts = std::min<int64_t>((p.cu ? p.N : p.T) / 1024 + 1, std::max<int64_t>(1, 2048 / p.B));
+    const int64_t parts = std::min<int64_t>((p.cu ? p.N : p.T) / 1024 + 1, std::max<int64_t>(1, 8192 / p.B));
     hipLaunchKernelGGL(k_slots, dim3(p.B, (unsigned)parts), dim3(kThreads), 0, (hipStream_t)stream, p);
   }
   return launched();
