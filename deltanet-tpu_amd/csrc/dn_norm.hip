@@ -74,9 +74,11 @@ __device__ __forceinline__ int64_t pos_of(const HP& p, int b, int l) {
 
 template <class T> constexpr int kWidth = 16 / (int)sizeof(T);   // channels of a group
 // W values of a type, in floats
-template <int W, class T> __device__ __forceinline__ void load(const T* p, float* o) {
+template <int W, bool PAST = false, class T> __device__ __forceinline__ void load(const T* p, float* o) {
   typedef T V __attribute__((ext_vector_type(W)));
-  const V a = *reinterpret_cast<const V*>(p);
+  V a;
+  if constexpr (PAST) a = __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+  else a = *reinterpret_cast<const V*>(p);
 #pragma unroll
   for (int i = 0; i < W; ++i) o[i] = (float)a[i];
 }
@@ -194,15 +196,21 @@ template <class T, bool PAGED> __device__ __forceinline__ Dst dst_of(const HP& p
   return d;
 }
 
-// x: (token, item) in groups of P threads, y: NH heads of q, k or v.
+template <int NH> __host__ __device__ __forceinline__ int chunks_of(const HP& p) {
+  return (p.H[0] + NH - 1) / NH + (p.H[1] + NH - 1) / NH + (p.H[2] + NH - 1) / NH;
+}
+
+// Blocks: chunks of NH heads of q, k or v innermost, so that a token's heads are read
+// and written at about the same time, then (token, item) in groups of P threads.
 template <class T, int P, int NH, bool PAGED, bool PAST>
 __global__ __launch_bounds__(256) void k_heads(const HP p) {
   constexpr int W = kWidth<T>;
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const uint32_t nc = chunks_of<NH>(p);
+  const int64_t id = (int64_t)(blockIdx.x / nc) * 256 + threadIdx.x;
   const int i = threadIdx.x % P;
   const bool live = id / P < p.N && i < p.D / (2 * W);
   const int64_t t = min(id / P, (int64_t)p.N - 1);
-  int y = blockIdx.y, side = 0;
+  int y = blockIdx.x % nc, side = 0;
   for (; side < 2; ++side) {
     const int n = (p.H[side] + NH - 1) / NH;
     if (y < n) break;
@@ -215,8 +223,8 @@ __global__ __launch_bounds__(256) void k_heads(const HP p) {
 #pragma unroll
   for (int h = 0; h < NH; ++h) {
     if (live && h0 + h < H) {
-      load<W>(s + h * p.xs[side][2] + it.a, u[h]);
-      load<W>(s + h * p.xs[side][2] + it.b, v[h]);
+      load<W, PAGED && PAST>(s + h * p.xs[side][2] + it.a, u[h]);
+      load<W, PAGED && PAST>(s + h * p.xs[side][2] + it.b, v[h]);
     } else {
 #pragma unroll
       for (int e = 0; e < W; ++e) u[h][e] = v[h][e] = 0.f;
@@ -487,8 +495,11 @@ template <class T, class F> void by_lanes(int D, F f) {
 constexpr int kMostD = 512;   // of these kernels
 constexpr int kMostBlocks = 0x7fffffff;
 
-// Threads of one head each that fill the card a few times over; from there on a
-// thread takes two heads and stores past the caches.
+// Threads of one head each that fill the card a few times over; from there on a thread
+// takes two heads and stores past the caches, and in serving, where no gradient reads
+// them again, loads past them too (16384 tokens of prompts, 227 MB, that no cache holds:
+// 49 us, stores alone past them 51, neither 52; blocks of one chunk of heads for all
+// tokens before the next 56).
 constexpr int64_t kManyThreads = 1 << 20;
 
 // the checks that the entries share; NULL if all is well
@@ -507,8 +518,6 @@ bool fast_heads(const HP& p, int dtype) {
     if (p.H[i] && !(wide(p.x[i], p.xs[i], 3) && aligned(p.out[i]))) return false;
   return true;
 }
-int chunks(const HP& p, int NH) { return (p.H[0] + NH - 1) / NH + (p.H[1] + NH - 1) / NH + (p.H[2] + NH - 1) / NH; }
-
 template <bool PAGED> int launch_heads(const HP& p, int dtype, bool fast, hipStream_t st) {
   const int H = p.H[0] + p.H[1] + p.H[2];
   bool ok = true;
@@ -523,9 +532,9 @@ template <bool PAGED> int launch_heads(const HP& p, int dtype, bool fast, hipStr
     by_lanes<T>(p.D, [&](auto lanes) {
       constexpr int P = decltype(lanes)::value;
       const int64_t blocks = ((int64_t)p.N * P + 255) / 256;
-      if (!(ok = blocks <= kMostBlocks)) return;
-      if ((int64_t)p.N * P * H < kManyThreads) hipLaunchKernelGGL((k_heads<T, P, 1, PAGED, false>), dim3((unsigned)blocks, chunks(p, 1)), dim3(256), 0, st, p);
-      else hipLaunchKernelGGL((k_heads<T, P, 2, PAGED, !PAGED>), dim3((unsigned)blocks, chunks(p, 2)), dim3(256), 0, st, p);
+      if (!(ok = blocks * chunks_of<1>(p) <= kMostBlocks)) return;
+      if ((int64_t)p.N * P * H < kManyThreads) hipLaunchKernelGGL((k_heads<T, P, 1, PAGED, false>), dim3((unsigned)(blocks * chunks_of<1>(p))), dim3(256), 0, st, p);
+      else hipLaunchKernelGGL((k_heads<T, P, 2, PAGED, true>), dim3((unsigned)(blocks * chunks_of<2>(p))), dim3(256), 0, st, p);
     });
   });
   if (!ok) return bad("too many tokens");
@@ -567,7 +576,7 @@ GradPlan grad_plan(const HP& p, int dtype, bool fast) {
   int P = dtype == DN_F32 ? 8 : 4;
   while (P * (dtype == DN_F32 ? 8 : 16) < p.D) P *= 2;
   const int64_t most = ((int64_t)p.N * P + 255) / 256;
-  const int x = (int)std::max<int64_t>(1, std::min(most, kGradBlocks / chunks(p, kGradHeads)));
+  const int x = (int)std::max<int64_t>(1, std::min(most, kGradBlocks / chunks_of<kGradHeads>(p)));
   return {x, x * ((p.H[0] + kGradHeads - 1) / kGradHeads), x * ((p.H[1] + kGradHeads - 1) / kGradHeads)};
 }
 // (the two forms' plans may differ: the larger)
@@ -624,7 +633,7 @@ extern "C" int dn_norm_rotary_bwd(const dn_norm_rotary_args* a, const dn_norm_ro
     }
     by_lanes<T>(p.D, [&](auto lanes) {
       constexpr int P = decltype(lanes)::value;
-      hipLaunchKernelGGL((k_heads_grad<T, P, kGradHeads>), dim3(plan.x, chunks(p, kGradHeads)), dim3(256), 0, st, p, g);
+      hipLaunchKernelGGL((k_heads_grad<T, P, kGradHeads>), dim3(plan.x, chunks_of<kGradHeads>(p)), dim3(256), 0, st, p, g);
     });
   });
   if (d->dq_weight || d->dk_weight)

@@ -367,18 +367,19 @@ int shift_of(int page_size) {
 
 using namespace dn;
 
-extern "C" int dn_paged_reserve(int32_t* pool, int32_t capacity, int32_t* page_table, int64_t page_table_stride, int32_t max_pages,
-                                int32_t B, int32_t page_size, int32_t* held, const int32_t* lens, int32_t* short_of, void* stream) {
-  if (capacity < 0 || B < 0) return bad("bad sizes");
-  if (B > DN_MAX_SEQUENCES) return bad("at most 4096 sequences");
-  if (const char* m = page_error(page_size, max_pages)) return bad(m);
+extern "C" int dn_paged_reserve(const dn_paged_reserve_args* a, void* stream) {
+  if (a == nullptr) return bad("null args");
+  if (a->abi_version != DN_ABI_VERSION) return set_error(DN_E_ABI, "dn_paged_reserve_args built for another ABI version");
+  if (a->capacity < 0 || a->B < 0) return bad("bad sizes");
+  if (a->B > DN_MAX_SEQUENCES) return bad("at most 4096 sequences");
+  if (const char* m = page_error(a->page_size, a->max_pages)) return bad(m);
   // (every count of pages stays within 32 bits)
-  if ((int64_t)B * max_pages + capacity > 0x7fffffff) return bad("too many pages");
-  if (B == 0) return DN_OK;
-  if (!pool || !page_table || !held || !lens || !short_of) return bad("missing tensor pointer");
-  RP p{pool, page_table, held, short_of, lens, page_table_stride, capacity, max_pages, B, shift_of(page_size)};
-  const int blocks = (int)std::min<int64_t>(256, ((int64_t)B * max_pages + 2047) / 2048);
-  hipLaunchKernelGGL(k_reserve, dim3(blocks), dim3(kThreads), 2 * B * sizeof(int), (hipStream_t)stream, p);
+  if ((int64_t)a->B * a->max_pages + a->capacity > 0x7fffffff) return bad("too many pages");
+  if (a->B == 0) return DN_OK;
+  if (!a->pool || !a->page_table || !a->held || !a->lens || !a->short_of) return bad("missing tensor pointer");
+  const RP p{a->pool, a->page_table, a->held, a->short_of, a->lens, a->page_table_stride, a->capacity, a->max_pages, a->B, shift_of(a->page_size)};
+  const int blocks = (int)std::min<int64_t>(256, ((int64_t)a->B * a->max_pages + 2047) / 2048);
+  hipLaunchKernelGGL(k_reserve, dim3(blocks), dim3(kThreads), 2 * a->B * sizeof(int), (hipStream_t)stream, p);
   return launched();
 }
 

@@ -184,6 +184,17 @@ class QkvAppendArgs(ctypes.Structure):
     ]
 
 
+class PagedReserveArgs(ctypes.Structure):
+    """Mirror of ``dn_paged_reserve_args``."""
+
+    _fields_ = [
+        ("abi_version", _c_i32),
+        ("capacity", _c_i32), ("B", _c_i32), ("page_size", _c_i32), ("max_pages", _c_i32),
+        ("pool", _c_ptr), ("page_table", _c_ptr), ("held", _c_ptr), ("lens", _c_ptr), ("short_of", _c_ptr),
+        ("page_table_stride", _c_i64),
+    ]
+
+
 class PagedSlotsArgs(ctypes.Structure):
     """Mirror of ``dn_paged_slots_args``."""
 
@@ -216,6 +227,7 @@ ATTENTION_PACK = struct.Struct("@8if7P9q").pack
 NORM_ROTARY_PACK = struct.Struct("@12i2f8P8q").pack
 NORM_ROTARY_GRADS_PACK = struct.Struct("@6P6q").pack
 QKV_APPEND_PACK = struct.Struct("@15i2f11P15q").pack
+PAGED_RESERVE_PACK = struct.Struct("@5i5Pq").pack
 PAGED_SLOTS_PACK = struct.Struct("@6i8Pq").pack
 KV_KEEP_PACK = struct.Struct("@10i6P9q").pack
 MAX_SEQUENCES = 4096   # DN_MAX_SEQUENCES
@@ -288,28 +300,24 @@ _PACKED = {   # argument types behind the packed argument block, and the result'
     "dn_norm_rotary_bwd_workspace_size": ([], ctypes.c_size_t),
     "dn_norm_rotary_bwd": ([ctypes.c_char_p, _c_ptr, ctypes.c_size_t, _c_ptr], ctypes.c_int),
     "dn_qkv_append": ([_c_ptr], ctypes.c_int),
+    "dn_paged_reserve": ([_c_ptr], ctypes.c_int),
     "dn_paged_slots": ([_c_ptr], ctypes.c_int),
     "dn_paged_tree_attention_workspace_size": ([_c_i32], ctypes.c_size_t),
     "dn_paged_tree_attention": ([_c_ptr, _c_i32, _c_ptr, ctypes.c_size_t, _c_ptr], ctypes.c_int),
     "dn_kv_keep": ([_c_ptr], ctypes.c_int),
 }
-_PLAIN = {   # entries without an argument block
-    "dn_paged_reserve": [_c_ptr, _c_i32, _c_ptr, _c_i64, _c_i32, _c_i32, _c_i32, _c_ptr, _c_ptr, _c_ptr, _c_ptr],
-}
+
 
 
 def packed_call(name):
     """An entry point of the loaded library that takes its argument block as
-    packed bytes (or, of ``_PLAIN``, its arguments one by one)."""
+    packed bytes."""
     f = _packed_calls.get(name)
     if f is None:
         lib = load_library()
         f = getattr(ctypes.CDLL(lib._name, handle=lib._handle), name)
-        if name in _PLAIN:
-            f.argtypes, f.restype = _PLAIN[name], ctypes.c_int
-        else:
-            args, f.restype = _PACKED[name]
-            f.argtypes = [ctypes.c_char_p, *args]
+        args, f.restype = _PACKED[name]
+        f.argtypes = [ctypes.c_char_p, *args]
         _packed_calls[name] = f
     return f
 

@@ -311,13 +311,15 @@ class _NormRotaryFn(torch.autograd.Function):
                 return None, None, None, None, None, None, None
             q = qw = None
         else:
-            d_q = _dense_channels(d_q)
+            if d_q.stride(-1) != 1:
+                d_q = _dense_channels(d_q)
             gq, gqw = torch.empty_like(q, memory_format=torch.contiguous_format), torch.empty_like(qw)
             q0, q1, q2, _ = d_q.stride()
         if d_k is None:
             k = kw = None
         else:
-            d_k = _dense_channels(d_k)
+            if d_k.stride(-1) != 1:
+                d_k = _dense_channels(d_k)
             gk, gkw = torch.empty_like(k, memory_format=torch.contiguous_format), torch.empty_like(kw)
             k0, k1, k2, _ = d_k.stride()
         block = _norm_block(q, k, qw, kw, None, None, pos, table, ctx.meta)
@@ -332,7 +334,7 @@ class _NormRotaryFn(torch.autograd.Function):
             for g in (gqw, gkw):
                 if g is not None:
                     g.zero_()
-        if _grad_enabled() or _differentiated(d_q, d_k):   # create_graph
+        if _grad_enabled() or _forward_ad._current_level >= 0 and _differentiated(d_q, d_k):   # create_graph
             gq, gk, gqw, gkw = _NoSecondNorm.apply(gq, gk, gqw, gkw, d_q, d_k, q, k, qw, kw)
         return gq, gk, gqw, gkw, None, None, None
 
@@ -372,27 +374,31 @@ def norm_rotary(q, k, q_weight, k_weight, positions=None, table=None, *, eps: fl
             and (table is None if positions is None else table is not None)):
         eps, weight_offset = _check_norm_rotary(q, k, q_weight, k_weight, positions, table, eps, weight_offset)
     ps0 = ps1 = 0
+    dev = q.get_device()
     if table is not None:
-        _check_table(table, qs[-1])
+        rows, R = table.shape if table.ndim == 2 else (0, 0)
+        if not (table.dtype is torch.float32 and rows > 0 and 2 <= R <= qs[-1] and not R & 1 and table.is_contiguous()):
+            _check_table(table, qs[-1])
         if positions.dtype not in _INT:
             raise ValueError(f"positions must be int32 or int64, got {positions.dtype}.")
-    _on_gpu(q, k, q_weight, k_weight, positions, table)
-    if table is not None:
-        at = positions.shape
+        at, st = positions.shape, positions.stride()
         if at == qs[:-2]:
-            ps1 = positions.stride(-1)
-            if len(at) == 2:
-                ps0 = positions.stride(0)
+            ps0, ps1 = st if len(at) == 2 else (0, st[0])
         elif len(at) == 1 and at[0] == qs[-3]:
-            ps1 = positions.stride(0)
+            ps1 = st[0]
         else:
             raise ValueError(f"positions {tuple(at)} must have the token dimensions of q {tuple(qs[:-2])}, or the last of them.")
+    if not (q_weight.get_device() == dev >= 0 and (k is None or k.get_device() == k_weight.get_device() == dev)
+            and (table is None or positions.get_device() == table.get_device() == dev)):
+        _on_gpu(q, k, q_weight, k_weight, positions, table)
     flat = len(qs) == 3
     if flat:
         q, k = q[None], None if k is None else k[None]
-    q, k = _dense_channels(q), None if k is None else _dense_channels(k)
+    if q.stride(-1) != 1 or k is not None and k.stride(-1) != 1:
+        q, k = _dense_channels(q), None if k is None else _dense_channels(k)
     meta = ps0, ps1, eps, weight_offset, 1 if interleaved else 0
-    if _differentiated(q, k, q_weight, k_weight):
+    if _grad_enabled() and (q.requires_grad or q_weight.requires_grad or k is not None and (k.requires_grad or k_weight.requires_grad)) \
+            or _forward_ad._current_level >= 0 and _differentiated(q, k, q_weight, k_weight):
         r = _NormRotaryFn.apply(q, k, q_weight, k_weight, positions, table, meta)
         q_out, k_out = r if k is not None else (r, None)
     else:

@@ -23,7 +23,7 @@ import torch
 
 from . import _lib
 from .attention import (
-    _INT, _attention_common, _bump, _call, _calls, _check_caches, _check_norm, _check_pages, _check_table, _check_weights,
+    _INT, _attention_common, _forward_ad, _grad_enabled, _bump, _call, _calls, _check_caches, _check_norm, _check_pages, _check_table, _check_weights,
     _dense_channels, _differentiated, _on_gpu, _rows16, _window)
 from .gdn2 import _DT
 
@@ -57,13 +57,12 @@ def _check_int32(name, t, shape):
         raise ValueError(f"{name} must be a contiguous int32 tensor {shape}, got {t.dtype} {tuple(t.shape)}.")
 
 
-def _written(ts):
-    # autograd sees the store (inference tensors have no version)
-    for t in ts:
-        if t.is_inference():
-            ts = [t for t in ts if not t.is_inference()]
-            break
-    _bump(ts)
+def _written(*ts):
+    """autograd sees the store (inference tensors have no version)"""
+    try:
+        _bump(ts)
+    except RuntimeError:
+        _bump([t for t in ts if not t.is_inference()])
 
 
 def page_pool(pages, *, device=None):
@@ -100,12 +99,15 @@ def paged_reserve(pool, page_table, held, lens, *, page_size: int):
             and page_table.stride(1) == 1 and pool.ndim == 1 and pool.is_contiguous() and held.shape == lens.shape == (B,) and held.is_contiguous()
             and lens.is_contiguous() and 2 <= pool.shape[0] <= 0x7fffffff - B * most):
         _check_reserve(pool, page_table, held, lens, page_size)
-    dev = _on_gpu(pool, page_table, held, lens)
+    dev = pool.get_device()
+    if not page_table.get_device() == held.get_device() == lens.get_device() == dev >= 0:
+        _on_gpu(pool, page_table, held, lens)
     short = torch.empty_like(lens)
     if B:
-        _call("dn_paged_reserve", dev, pool.data_ptr(), pool.shape[0] - 2, page_table.data_ptr(), page_table.stride(0), most, B,
-              page_size, held.data_ptr(), lens.data_ptr(), short.data_ptr())
-        _written((pool, page_table, held))
+        _call("dn_paged_reserve", dev, _lib.PAGED_RESERVE_PACK(
+            _lib.DN_ABI_VERSION, pool.shape[0] - 2, B, page_size, most, pool.data_ptr(), page_table.data_ptr(), held.data_ptr(),
+            lens.data_ptr(), short.data_ptr(), page_table.stride(0)))
+        _written(pool, page_table, held)
     return short
 
 
@@ -153,7 +155,10 @@ def paged_slots(page_table, seq_lens, tokens: int, *, page_size: int, cu_seqlens
             and (nodes is None if parents is None else type(nodes) is int and 1 <= nodes <= _NODES and parents.dtype is _I32
                  and parents.shape == (tokens,) and parents.is_contiguous())):
         _check_slots(page_table, seq_lens, tokens, page_size, cu_seqlens, held, parents, nodes)
-    dev = _on_gpu(page_table, seq_lens, cu_seqlens, held, parents)
+    dev = page_table.get_device()
+    if not (seq_lens.get_device() == dev >= 0 and (cu_seqlens is None or cu_seqlens.get_device() == dev) and (held is None or held.get_device() == dev)
+            and (parents is None or parents.get_device() == dev)):
+        _on_gpu(page_table, seq_lens, cu_seqlens, held, parents)
     words = 0 if parents is None else (nodes + 63) >> 6
     positions, slots = seq_lens.new_empty(tokens), seq_lens.new_empty(tokens, dtype=_I64)
     visible = slots.new_empty((tokens, words)) if words else None
@@ -214,9 +219,17 @@ def paged_qkv_append(q, k, v, k_cache, v_cache, slots, positions, *, q_weight=No
                  and q_weight.shape == k_weight.shape == cs[3:] and q_weight.is_contiguous() and k_weight.is_contiguous())):
         eps, weight_offset = _check_qkv_append(q, k, v, k_cache, v_cache, slots, positions, q_weight, k_weight, eps, weight_offset)
     pages, page, Hkv, D = cs
-    R = 0 if table is None else _check_table(table, D)
-    dev = _on_gpu(q, k, v, k_cache, v_cache, slots, positions, q_weight, k_weight, table)
-    if _differentiated(q, k, v, k_cache, v_cache, q_weight, k_weight):
+    rows = R = 0
+    if table is not None:
+        _check_table(table, D)
+        rows, R = table.shape
+    dev = q.get_device()
+    if not (k.get_device() == v.get_device() == k_cache.get_device() == v_cache.get_device() == slots.get_device() == positions.get_device() == dev >= 0
+            and (q_weight is None or q_weight.get_device() == k_weight.get_device() == dev) and (table is None or table.get_device() == dev)):
+        _on_gpu(q, k, v, k_cache, v_cache, slots, positions, q_weight, k_weight, table)
+    if (_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or k_cache.requires_grad or v_cache.requires_grad
+                             or q_weight is not None and (q_weight.requires_grad or k_weight.requires_grad))) \
+            or _forward_ad._current_level >= 0 and _differentiated(q, k, v, k_cache, v_cache, q_weight, k_weight):
         raise ValueError("paged_qkv_append is not differentiable; call it under torch.no_grad() (norm_rotary is its form for training).")
     qt, kt, vt = q.stride(), k.stride(), v.stride()
     if not qt[-1] == kt[-1] == vt[-1] == 1:
@@ -230,11 +243,11 @@ def paged_qkv_append(q, k, v, k_cache, v_cache, slots, positions, *, q_weight=No
     if B and T:
         _call("dn_qkv_append", dev, _lib.QKV_APPEND_PACK(
             _lib.DN_ABI_VERSION, B, T, qs[-2], Hkv, D, R, _DT[dt], _DT[ct], _DT[wt],
-            _INT[positions.dtype], 1 if interleaved else 0, table.shape[0] if R else 0, pages, page, eps, weight_offset,
+            _INT[positions.dtype], 1 if interleaved else 0, rows, pages, page, eps, weight_offset,
             q.data_ptr(), k.data_ptr(), v.data_ptr(), 0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(),
             out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr(), positions.data_ptr(), table.data_ptr() if R else 0,
             qb, qt[-3], qt[-2], kb, kt[-3], kt[-2], vb, vt[-3], vt[-2], kcs[0], kcs[1], kcs[2], vcs[0], vcs[1], vcs[2]))
-        _written((k_cache, v_cache))
+        _written(k_cache, v_cache)
     return out
 
 
@@ -290,8 +303,12 @@ def paged_tree_attention(q, k_cache, v_cache, page_table, seq_lens, visible, *, 
     else:
         scale = _SCALE[cs[3]]
     pages, page, Hkv, D = cs
-    dev = _on_gpu(q, k_cache, v_cache, page_table, seq_lens, visible, cu_seqlens)
-    if _differentiated(q, k_cache, v_cache):
+    dev = q.get_device()
+    if not (k_cache.get_device() == v_cache.get_device() == page_table.get_device() == seq_lens.get_device() == visible.get_device() == dev >= 0
+            and (cu_seqlens is None or cu_seqlens.get_device() == dev)):
+        _on_gpu(q, k_cache, v_cache, page_table, seq_lens, visible, cu_seqlens)
+    if _grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad) \
+            or _forward_ad._current_level >= 0 and _differentiated(q, k_cache, v_cache):
         raise ValueError("paged_tree_attention is not differentiable; call it under torch.no_grad().")
     if qt[-1] != 1 or (q.data_ptr() | (qt[0] | qt[-3] | qt[-2]) * e) & 15:
         q = _rows16(q)
@@ -355,8 +372,10 @@ def paged_kv_keep(k_cache, v_cache, page_table, starts, kept):
             and page_table.shape[1] > 0 and page_table.stride(1) == 1 and starts.dtype is _I32 and starts.shape == (B,) and starts.is_contiguous()
             and kept.dtype is _I32 and kept.is_contiguous()):
         _check_keep(k_cache, v_cache, page_table, starts, kept)
-    dev = _on_gpu(k_cache, v_cache, page_table, starts, kept)
-    if _differentiated(k_cache, v_cache):
+    dev = k_cache.get_device()
+    if not v_cache.get_device() == page_table.get_device() == starts.get_device() == kept.get_device() == dev >= 0:
+        _on_gpu(k_cache, v_cache, page_table, starts, kept)
+    if _grad_enabled() and (k_cache.requires_grad or v_cache.requires_grad) or _forward_ad._current_level >= 0 and _differentiated(k_cache, v_cache):
         raise ValueError("paged_kv_keep is not differentiable; call it under torch.no_grad().")
     lens = torch.empty_like(starts)
     if B:
@@ -365,7 +384,7 @@ def paged_kv_keep(k_cache, v_cache, page_table, starts, kept):
             _lib.DN_ABI_VERSION, cs[0] if many else 1, B, cs[-2], cs[-1], most, _DT[ct], cs[-4], cs[-3], page_table.shape[1],
             k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(), starts.data_ptr(), kept.data_ptr(), lens.data_ptr(),
             ks[0] if many else 0, ks[-4], ks[-3], ks[-2], vs[0] if many else 0, vs[-4], vs[-3], vs[-2], page_table.stride(0)))
-        _written((k_cache, v_cache))
+        _written(k_cache, v_cache)
     return lens
 
 

@@ -474,8 +474,18 @@ int dn_qkv_append(const dn_qkv_append_args* a, void* stream);
  * neither does one that needs more than max_pages; short_of[b] is the number of pages
  * that it lacks.  B at most DN_MAX_SEQUENCES. */
 #define DN_MAX_SEQUENCES 4096
-int dn_paged_reserve(int32_t* pool, int32_t capacity, int32_t* page_table, int64_t page_table_stride, int32_t max_pages,
-                     int32_t B, int32_t page_size, int32_t* held, const int32_t* lens, int32_t* short_of, void* stream);
+typedef struct dn_paged_reserve_args {
+  int32_t abi_version;
+  int32_t capacity, B, page_size, max_pages;   /* page_size a power of two       */
+  int32_t* pool;                /* (2 + capacity)                                */
+  int32_t* page_table;          /* (B,max_pages), row stride page_table_stride   */
+  int32_t* held;                /* (B)                                           */
+  const int32_t* lens;          /* (B)                                           */
+  int32_t* short_of;            /* (B)                                           */
+  int64_t page_table_stride;
+} dn_paged_reserve_args;
+
+int dn_paged_reserve(const dn_paged_reserve_args* a, void* stream);
 
 /* Slots and positions of the N new tokens of a call.  New token i of sequence b, n_b
  * of them, has slot page_table[b][x / page_size] * page_size + x % page_size with

@@ -9,7 +9,7 @@ from deltanet_tpu_amd import _lib
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 BLOCKS = {"dn_norm_rotary_args": (_lib.NormRotaryArgs, _lib.NORM_ROTARY_PACK), "dn_norm_rotary_grads": (_lib.NormRotaryGrads, _lib.NORM_ROTARY_GRADS_PACK),
-          "dn_qkv_append_args": (_lib.QkvAppendArgs, _lib.QKV_APPEND_PACK), "dn_paged_slots_args": (_lib.PagedSlotsArgs, _lib.PAGED_SLOTS_PACK),
+          "dn_qkv_append_args": (_lib.QkvAppendArgs, _lib.QKV_APPEND_PACK), "dn_paged_reserve_args": (_lib.PagedReserveArgs, _lib.PAGED_RESERVE_PACK), "dn_paged_slots_args": (_lib.PagedSlotsArgs, _lib.PAGED_SLOTS_PACK),
           "dn_kv_keep_args": (_lib.KvKeepArgs, _lib.KV_KEEP_PACK)}
 
 
@@ -85,14 +85,13 @@ def test_c_entries_refuse_before_any_launch():
     a.B = 0
     assert P("dn_qkv_append")(bytes(a), None) == 0
 
-    r = lambda *x: P("dn_paged_reserve")(*x, None)
-    ok = [0x1000, 5, 0x1000, 4, 4, 2, 16, 0x1000, 0x1000, 0x1000]
-    sub = lambda i, x: ok[:i] + [x] + ok[i + 1:]
-    assert r(*sub(5, 5000)) == -1 and b"4096" in err()
-    assert r(*sub(6, 12)) == -1 and b"power of two" in err()
-    assert r(*sub(4, 1 << 30)) == -1 and b"too many pages" in err()
-    assert r(*sub(0, None)) == -1 and b"missing" in err()
-    assert r(*sub(5, 0)) == 0
+    ok = dict(abi_version=V, capacity=5, B=2, page_size=16, max_pages=4, pool=0x1000, page_table=0x1000, held=0x1000, lens=0x1000, short_of=0x1000)
+    r = lambda **k: P("dn_paged_reserve")(bytes(_set(_lib.PagedReserveArgs(), **{**ok, **k})), None)
+    assert r(B=5000) == -1 and b"4096" in err()
+    assert r(page_size=12) == -1 and b"power of two" in err()
+    assert r(max_pages=1 << 30) == -1 and b"too many pages" in err()
+    assert r(pool=None) == -1 and b"missing" in err()
+    assert r(B=0) == 0 and r(abi_version=9) == -4
 
     s = _set(_lib.PagedSlotsArgs(), abi_version=V, N=3, B=2, page_size=16, max_pages=4)
     assert P("dn_paged_slots")(bytes(s), None) == -1 and b"N / B" in err()
