@@ -394,8 +394,10 @@ bool attn_few_takes(const AF& p, int D, int dtype) {
 }
 
 // Drafted trees in float32 whose rows fill 16 or 32 of a tile: the products take the
-// time there, and the kernel of trees makes 64 rows of them.  MEASURE.  At D = 256 there
-// are no registers for 32.
+// time there, and the kernel of trees makes 64 rows of them (us, this kernel / that one,
+// D = 128: 64 x 4 tokens over 4096 372 / 627, 32 x 8 261 / 326; D = 64 206 / 333, 153 / 176;
+// D = 256 423 / 746).  At D = 256 there are no registers for 32 rows (815 / 390).  In 16 bits
+// that kernel is the faster one (D = 128 64 x 4 207 / 193, 32 x 8 129 / 108).
 bool tree_few(const AF& p, int D, int dtype) {
   return dtype == DN_F32 && p.shift >= 4 && (int64_t)p.N * p.G <= (int64_t)(D == 256 ? 16 : 32) * p.B;
 }

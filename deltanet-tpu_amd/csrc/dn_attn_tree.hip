@@ -5,6 +5,13 @@
 // LDS a tile ahead by direct loads, and a workgroup takes an even share of all
 // sequences' keys, wherever tiles of rows begin and end in it; what several hold parts
 // of is joined by a second launch.  Only the last keys, the trees' own, are masked.
+//
+// Up to 64 rows it is bound by reading the keys once: 64 x 4 tokens over 4096 (1.08 GB, D =
+// 128) 193 us, 5.6 TB/s, where a copy of 4 GB reaches 4.8.  Trees of up to 64 over up to
+// 16384 (0.58 GB, some of it read for two tiles of 128 rows) 150 + 16 us, of up to 25 over
+// up to 4096 (D = 256, float16, 0.29 GB) 72 + 12.  With more rows the LDS reads bound it, as
+// in the kernel of whole rows: 64 x 64 over 2000 203 us, 680 TFLOP/s.  16 tokens over 1000:
+// 13 + 5 us, the chain of lengths, page table, keys, products and the join.
 #include <type_traits>
 
 #include "dn_attn_split.h"
@@ -333,7 +340,17 @@ template <class T, int D, int NQ, int NW, int BN, int ST> struct FormOf {
     return hipGetLastError();
   }
 };
-// The form for the mean number of rows of a sequence and key head: MEASURE.
+// The form, by the mean number of rows of a sequence and key head; us with the join,
+// bf16, of 64 / 128 / 256 rows a tile (at D = 256: 64 / 128), sequences x new tokens over
+// cached tokens, 4 query heads a key head:
+// - D = 128: 64 x 4 / 4096 193, 208, 370; 32 x 8 / 4096 108, 127, 187; 8 x 16 / 8192 65, 70,
+//   104; 16 x 21 / 8192 (64 and 16384 at most) 173, 166, 243; 8 x 64 / 8192 143, 105, 112;
+//   64 x 64 / 2000 408, 270, 203;
+// - D = 64: 64 x 4 / 4096 112, 125, 212; 8 x 32 / 8192 58, 48, 66; 64 x 64 / 2000 211, 158, 132;
+// - D = 256: 64 x 4 / 4096 196, 222; 16 x 21 / 8192 170, 182; 8 x 64 / 8192 131, 116; 64 x 64
+//   / 2000 280, 262;
+// - float32: D = 128 8 x 16 / 8192 180, 310; 8 x 64 / 8192 619, 621; D = 256 213, 314 and 741,
+//   598.
 template <class T, int D, class G> auto by_rows(const AF& p, G g) {
   const int64_t rows = (int64_t)p.N * p.G, B = p.B;
   if constexpr (sizeof(T) == 4) {
@@ -344,7 +361,7 @@ template <class T, int D, class G> auto by_rows(const AF& p, G g) {
     return g(FormOf<T, D, 1, 8, 64, 2>{});
   } else {
     if (rows <= 64 * B) return g(FormOf<T, D, 1, 4, 32, D == 64 ? 3 : 2>{});
-    if (rows < 192 * B) return g(FormOf<T, D, 2, 4, D == 64 ? 64 : 32, 2>{});
+    if (rows < 192 * B) return g(FormOf<T, D, 2, 4, 64, 2>{});
     return g(FormOf<T, D, 2, 8, 64, 2>{});
   }
 }

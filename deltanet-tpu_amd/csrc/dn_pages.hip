@@ -2,10 +2,12 @@
 // accepted tokens of drafted trees moved to the front.
 //
 // Nothing here computes: bound by the launch and a chain of two or three dependent
-// loads (lengths, page table, store) at a token or two per sequence, by the stores of
-// tables and slots in long queues of prompts.
-#include "dn_host.h"
+// loads (lengths, page table, store) at a token or two per sequence, 2.7 us a launch, by
+// the stores in long queues of prompts: 5.6 million tokens' positions and slots (67 MB)
+// 15.4 us.  Accepted tokens of 64 sequences in 12 layers (13 MB) move in 6.7 us, one
+// user's in 4.9.
 #include "dn_common.h"
+#include "dn_host.h"
 
 namespace dn {
 
@@ -24,7 +26,7 @@ __device__ __forceinline__ int scan64(int x) {   // inclusive, over a wave
 }
 
 // x summed over the block's threads in front, and over all of them
-__device__ __forceinline__ int block_scan(int x, int* waves, int& all) {
+template <int NT> __device__ __forceinline__ int block_scan(int x, int* waves, int& all) {
   const int w = threadIdx.x >> 6, s = scan64(x);
   __syncthreads();   // (its last use)
   if (lane_id() == 63) waves[w] = s;
@@ -32,7 +34,7 @@ __device__ __forceinline__ int block_scan(int x, int* waves, int& all) {
   int before = 0;
   all = 0;
 #pragma unroll
-  for (int i = 0; i < kThreads / 64; ++i) {
+  for (int i = 0; i < NT / 64; ++i) {
     if (i < w) before += waves[i];
     all += waves[i];
   }
@@ -66,10 +68,10 @@ struct RP {
 // overwrites.  Lengths and counts are written by the block that comes to its end last,
 // when all others have read them; it reads nothing that they wrote, so that the count
 // of those that ended needs no fence.
-__global__ __launch_bounds__(kThreads) void k_reserve(const RP p) {
+template <int NT> __global__ __launch_bounds__(NT) void k_reserve(const RP p) {
   extern __shared__ int lds[];   // [2][B]: pages taken, given back by the sequences in front
   int *taken = lds, *given = lds + p.B;
-  __shared__ int waves[kThreads / 64], s_last;
+  __shared__ int waves[NT / 64], s_last;
   const int count = min(max(p.pool[0], 0), p.capacity);
   auto needs = [&](int b, int& h, int& need) {
     h = min(max(p.held[b], 0), p.max_pages);
@@ -77,7 +79,7 @@ __global__ __launch_bounds__(kThreads) void k_reserve(const RP p) {
     need = (n >> p.shift) + ((n & ((1 << p.shift) - 1)) != 0);
   };
 #pragma unroll 4
-  for (int b = threadIdx.x; b < p.B; b += kThreads) {
+  for (int b = threadIdx.x; b < p.B; b += NT) {
     int h, need;
     needs(b, h, need);
     taken[b] = need <= p.max_pages ? max(need - h, 0) : 0;
@@ -85,14 +87,14 @@ __global__ __launch_bounds__(kThreads) void k_reserve(const RP p) {
   }
   __syncthreads();
   // a run of sequences per thread
-  const int per = (p.B + kThreads - 1) / kThreads, b0 = min((int)threadIdx.x * per, p.B), b1 = min(b0 + per, p.B);
+  const int per = (p.B + NT - 1) / NT, b0 = min((int)threadIdx.x * per, p.B), b1 = min(b0 + per, p.B);
   int grow = 0, back = 0;
   for (int b = b0; b < b1; ++b) {
     grow += taken[b];
     back += given[b];
   }
   int F, all;
-  int f = block_scan(back, waves, F), a = block_scan(grow, waves, all);
+  int f = block_scan<NT>(back, waves, F), a = block_scan<NT>(grow, waves, all);
   const int full = count + F;
   // sequences take while what all up to them need is there
   int got = 0;
@@ -111,7 +113,7 @@ __global__ __launch_bounds__(kThreads) void k_reserve(const RP p) {
   __syncthreads();
   int A = 0;
 #pragma unroll
-  for (int i = 0; i < kThreads / 64; ++i) A = max(A, waves[i]);
+  for (int i = 0; i < NT / 64; ++i) A = max(A, waves[i]);
   const int left = full - A;
   // page number x of those given back, in the order of the sequences and their pages
   auto given_page = [&](int x) {
@@ -120,7 +122,7 @@ __global__ __launch_bounds__(kThreads) void k_reserve(const RP p) {
     needs(b, h, need);
     return p.table[b * p.stride + need + (x - given[b])];
   };
-  const int me = blockIdx.x * kThreads + threadIdx.x, step = gridDim.x * kThreads;
+  const int me = blockIdx.x * NT + threadIdx.x, step = gridDim.x * NT;
 #pragma unroll 2
   for (int k = me; k < A; k += step) {
     const int b = last_at_most(taken, p.B, k), at = full - 1 - k;
@@ -136,7 +138,7 @@ __global__ __launch_bounds__(kThreads) void k_reserve(const RP p) {
     if (!s_last) return;
   }
 #pragma unroll 4
-  for (int b = threadIdx.x; b < p.B; b += kThreads) {
+  for (int b = threadIdx.x; b < p.B; b += NT) {
     int h, need;
     needs(b, h, need);
     const bool fits = need <= p.max_pages && (need <= h || taken[b] + (need - h) <= full);
@@ -378,8 +380,13 @@ extern "C" int dn_paged_reserve(const dn_paged_reserve_args* a, void* stream) {
   if (a->B == 0) return DN_OK;
   if (!a->pool || !a->page_table || !a->held || !a->lens || !a->short_of) return bad("missing tensor pointer");
   const RP p{a->pool, a->page_table, a->held, a->short_of, a->lens, a->page_table_stride, a->capacity, a->max_pages, a->B, shift_of(a->page_size)};
-  const int blocks = (int)std::min<int64_t>(256, ((int64_t)a->B * a->max_pages + 2047) / 2048);
-  hipLaunchKernelGGL(k_reserve, dim3(blocks), dim3(kThreads), 2 * a->B * sizeof(int), (hipStream_t)stream, p);
+  // blocks of 16 waves hide the searches of many pages (350000 of 2048 sequences: 10.6 us,
+  // blocks of 4 waves 15.3), those of 4 start sooner where there are few (a token or a tree
+  // of 64 sequences: 2.8 and 4.5 us, 5.0 for the latter by 16 waves)
+  const int64_t entries = (int64_t)a->B * a->max_pages;
+  const size_t lds = 2 * a->B * sizeof(int);
+  if (entries <= 65536) hipLaunchKernelGGL(k_reserve<256>, dim3((unsigned)((entries + 2047) / 2048)), dim3(256), lds, (hipStream_t)stream, p);
+  else hipLaunchKernelGGL(k_reserve<1024>, dim3((unsigned)std::min<int64_t>(256, (entries + 4095) / 4096)), dim3(1024), lds, (hipStream_t)stream, p);
   return launched();
 }
 
