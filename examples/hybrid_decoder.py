@@ -10,6 +10,10 @@ The same weights run three ways through this package:
   state per sequence;
 - then one token per sequence and step (``gdn_decode_step``, the same two calls).
 
+With ``normed`` the attention layers norm their queries and keys head by head: in the
+rotation's pass (``norm_rotary``), and in serving on their way into the cache
+(``paged_qkv_append`` at the slots that ``paged_slots`` gives for all layers).
+
 ``python examples/hybrid_decoder.py`` runs a few training steps, serves two prompts
 and compares each served token's logits with those of the whole row.
 """
@@ -27,7 +31,8 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 sys.path.insert(0, os.path.join(ROOT, "deltanet-tpu_amd"))
 
 from deltanet_tpu_amd import (  # noqa: E402
-    apply_rotary, causal_attention, chunk_gdn, gdn_decode_step, paged_attention, paged_kv_append, rotary_table)
+    apply_rotary, causal_attention, chunk_gdn, gdn_decode_step, norm_rotary, paged_attention, paged_kv_append, paged_qkv_append,
+    paged_slots, rotary_table)
 
 
 class DeltaLayer(torch.nn.Module):
@@ -64,10 +69,12 @@ class DeltaLayer(torch.nn.Module):
 
 
 class AttentionLayer(torch.nn.Module):
-    """Grouped-query attention, a part of each head rotated by its position."""
+    """Grouped-query attention, a part of each head rotated by its position, and
+    queries and keys normed before it if ``normed`` (weights kept as differences from 1)."""
 
-    def __init__(self, width, Hq, Hkv, D):
+    def __init__(self, width, Hq, Hkv, D, normed=False):
         super().__init__()
+        self.norms = torch.nn.ParameterList(torch.nn.Parameter(torch.zeros(D)) for _ in range(2 if normed else 0))
         self.Hq, self.Hkv, self.D = Hq, Hkv, D
         self.inp = torch.nn.Linear(width, (Hq + 2 * Hkv) * D, bias=False)
         self.out = torch.nn.Linear(Hq * D, width, bias=False)
@@ -77,28 +84,34 @@ class AttentionLayer(torch.nn.Module):
 
     def forward(self, x, seg, positions, table):
         q, k, v = self.project(x)
-        q, k = apply_rotary(q, k, positions, table)
+        if len(self.norms):
+            q, k = norm_rotary(q, k, *self.norms, positions, table, weight_offset=1.0)
+        else:
+            q, k = apply_rotary(q, k, positions, table)
         return self.out(causal_attention(q, k, v, segment_ids=seg).flatten(2))
 
-    def cached(self, x, positions, table, cache, pages, lens, cu):
+    def cached(self, x, positions, slots, table, cache, pages, lens, cu):
         """New tokens (N, width) of all sequences: stored, then attended with what is there."""
         q, k, v = self.project(x)
-        paged_kv_append(k, v, *cache, pages, lens, cu_seqlens=cu, table=table)
-        q, _ = apply_rotary(q, None, positions, table)
+        if len(self.norms):
+            q = paged_qkv_append(q, k, v, *cache, slots, positions, q_weight=self.norms[0], k_weight=self.norms[1], weight_offset=1.0, table=table)
+        else:
+            paged_kv_append(k, v, *cache, pages, lens, cu_seqlens=cu, table=table)
+            q, _ = apply_rotary(q, None, positions, table)
         return self.out(paged_attention(q, *cache, pages, lens, cu_seqlens=cu).flatten(1))
 
 
 class HybridDecoder(torch.nn.Module):
-    def __init__(self, vocab=512, width=512, blocks=2, deltas=3, Hk=2, Hv=4, Hq=8, Hkv=2, D=128, rotary=64, most=4096, page=64):
+    def __init__(self, vocab=512, width=512, blocks=2, deltas=3, Hk=2, Hv=4, Hq=8, Hkv=2, D=128, rotary=64, most=4096, page=64, normed=False):
         super().__init__()
         self.embed = torch.nn.Embedding(vocab, width)
         self.layers = torch.nn.ModuleList()
         for _ in range(blocks):
             self.layers.extend(DeltaLayer(width, Hk, Hv) for _ in range(deltas))
-            self.layers.append(AttentionLayer(width, Hq, Hkv, D))
+            self.layers.append(AttentionLayer(width, Hq, Hkv, D, normed))
         self.norms = torch.nn.ModuleList(torch.nn.RMSNorm(width) for _ in self.layers)
         self.head = torch.nn.Linear(width, vocab, bias=False)
-        self.rotary, self.most, self.page = rotary, most, page
+        self.rotary, self.most, self.page, self.normed = rotary, most, page, normed
 
     def table(self):
         return rotary_table(self.most, self.rotary, device=self.head.weight.device)
@@ -138,12 +151,13 @@ class HybridDecoder(torch.nn.Module):
                 state.append(tuple(torch.empty(shape, dtype=dt, device=dev) for _ in range(2)))
 
         def run(x, positions, cu, prompt):
+            slots = paged_slots(pages, lens, len(x), page_size=self.page, cu_seqlens=cu)[1] if self.normed else None
             for layer, norm, s in zip(self.layers, self.norms, state):
                 y = norm(x)
                 if isinstance(layer, DeltaLayer):
                     x = x + (layer.prompt(y, spans, s) if prompt else layer.token(y, s))
                 else:
-                    x = x + layer.cached(y, positions, table, s, pages, lens, cu)
+                    x = x + layer.cached(y, positions, slots, table, s, pages, lens, cu)
             return self.head(x)
 
         positions = torch.cat([torch.arange(x, device=dev) for x in n])
@@ -188,9 +202,10 @@ def main():
     ap = argparse.ArgumentParser(description="A small hybrid decoder: training and paged serving")
     ap.add_argument("--dtype", choices=("bf16", "f32"), default="bf16")
     ap.add_argument("--steps", type=int, default=3)
+    ap.add_argument("--normed", action="store_true", help="norm queries and keys head by head")
     args = ap.parse_args()
     torch.manual_seed(0)
-    model = HybridDecoder().to("cuda", torch.bfloat16 if args.dtype == "bf16" else torch.float32)
+    model = HybridDecoder(normed=args.normed).to("cuda", torch.bfloat16 if args.dtype == "bf16" else torch.float32)
     print("losses", " ".join(f"{x:.4f}" for x in train_steps(model, args.steps)))
     print(f"served against whole rows: {serving_error(model):.2e}")
 
