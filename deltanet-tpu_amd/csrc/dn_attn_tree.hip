@@ -26,6 +26,9 @@ template <int N> __device__ __forceinline__ void loads_but() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
+// (Two sets of waves on every other tile of keys, joined in LDS, for half the parts: 214 us
+// in place of 179 for trees of up to 64, 112 of 84 at D = 256.)
+//
 // NW waves of 16 NQ rows, tiles of BN keys, ST of them in LDS: one that is read, the
 // others on their way.  PG: pages of 16 tokens or more, so that the rows of one load
 // lie in one page, whose number is read through the scalar cache (a vector load's wait
@@ -348,7 +351,7 @@ template <class T, int D, int NQ, int NW, int BN, int ST> struct FormOf {
 //   64 x 64 / 2000 408, 270, 203;
 // - D = 64: 64 x 4 / 4096 112, 125, 212; 8 x 32 / 8192 58, 48, 66; 64 x 64 / 2000 211, 158, 132;
 // - D = 256: 64 x 4 / 4096 196, 222; 16 x 21 / 8192 170, 182; 8 x 64 / 8192 131, 116; 64 x 64
-//   / 2000 280, 262;
+//   / 2000 280, 262; 1 x 16 / 1000, where the card has less to do than it holds, 18, 16.5;
 // - float32: D = 128 8 x 16 / 8192 180, 310; 8 x 64 / 8192 619, 621; D = 256 213, 314 and 741,
 //   598.
 template <class T, int D, class G> auto by_rows(const AF& p, G g) {
@@ -357,7 +360,8 @@ template <class T, int D, class G> auto by_rows(const AF& p, G g) {
     if (rows <= 128 * B) return g(FormOf<T, D, 1, 4, 32, 2>{});
     return g(FormOf<T, D, 1, 8, 32, 2>{});
   } else if constexpr (D == 256) {
-    if (rows <= 96 * B) return g(FormOf<T, D, 1, 4, 32, 2>{});
+    const int64_t units = most_tasks(p, 64) * ((((int64_t)p.max_pages << p.shift) + 63) / 64);
+    if (rows <= 96 * B && units > 512) return g(FormOf<T, D, 1, 4, 32, 2>{});
     return g(FormOf<T, D, 1, 8, 64, 2>{});
   } else {
     if (rows <= 64 * B) return g(FormOf<T, D, 1, 4, 32, D == 64 ? 3 : 2>{});
