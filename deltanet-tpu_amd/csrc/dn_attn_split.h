@@ -52,16 +52,29 @@ __global__ __launch_bounds__(256) void k_tree_join(const AF p, int groups) {
     f32x4 a = zero4();
     float m = -INFINITY, z = 0.f;
     if (live) {
-#pragma unroll 4
-      for (int w = w0 + k; w <= w1; w += per) {
-        const float* s = p.part + (2 * (int64_t)w + (w == w0 ? 1 : 0)) * slot_floats<D, BM>();
-        const f32x4 y = *reinterpret_cast<const f32x4*>(s + row * D + 4 * ch);
-        const float mw = s[BM * D + row], zw = s[BM * D + BM + row], x = fmaxf(m, mw);
-        const float f = m == -INFINITY ? 0.f : fast_exp2(m - x), g = mw == -INFINITY ? 0.f : fast_exp2(mw - x);
-        if (f != 1.f) a *= f;
-        if (g != 0.f) a += g * y;
-        z = z * f + g * zw;
-        m = x;
+#pragma unroll 1
+      for (int w = w0 + k; w <= w1; w += 4 * per) {   // four parts at a time, all on their way at once
+        f32x4 y[4];
+        float mw[4], zw[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int v = min(w + e * per, w1);
+          const float* s = p.part + (2 * (int64_t)v + (v == w0 ? 1 : 0)) * slot_floats<D, BM>();
+          y[e] = *reinterpret_cast<const f32x4*>(s + row * D + 4 * ch);
+          mw[e] = s[BM * D + row];
+          zw[e] = s[BM * D + BM + row];
+        }
+        __builtin_amdgcn_sched_barrier(0);   // (the compiler would load each where it is used)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (w + e * per > w1) mw[e] = -INFINITY, zw[e] = 0.f;
+          const float x = fmaxf(m, mw[e]);
+          const float f = m == -INFINITY ? 0.f : fast_exp2(m - x), g = mw[e] == -INFINITY ? 0.f : fast_exp2(mw[e] - x);
+          if (f != 1.f) a *= f;
+          if (g != 0.f) a += g * y[e];
+          z = z * f + g * zw[e];
+          m = x;
+        }
       }
     }
     if (per > 1) {
