@@ -57,14 +57,6 @@ def _check_int32(name, t, shape):
         raise ValueError(f"{name} must be a contiguous int32 tensor {shape}, got {t.dtype} {tuple(t.shape)}.")
 
 
-def _written(*ts):
-    """autograd sees the store (inference tensors have no version)"""
-    try:
-        _bump(ts)
-    except RuntimeError:
-        _bump([t for t in ts if not t.is_inference()])
-
-
 def page_pool(pages, *, device=None):
     """A pool of the cache's pages 0 .. pages - 1, all of them free: an int32 tensor
     (2 + pages) with the number of free pages, a word that the kernels use and that is
@@ -107,7 +99,7 @@ def paged_reserve(pool, page_table, held, lens, *, page_size: int):
         _call("dn_paged_reserve", dev, _lib.PAGED_RESERVE_PACK(
             _lib.DN_ABI_VERSION, pool.shape[0] - 2, B, page_size, most, pool.data_ptr(), page_table.data_ptr(), held.data_ptr(),
             lens.data_ptr(), short.data_ptr(), page_table.stride(0)))
-        _written(pool, page_table, held)
+        _bump((pool, page_table, held))   # autograd sees the stores
     return short
 
 
@@ -247,7 +239,7 @@ def paged_qkv_append(q, k, v, k_cache, v_cache, slots, positions, *, q_weight=No
             q.data_ptr(), k.data_ptr(), v.data_ptr(), 0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(),
             out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr(), positions.data_ptr(), table.data_ptr() if R else 0,
             qb, qt[-3], qt[-2], kb, kt[-3], kt[-2], vb, vt[-3], vt[-2], kcs[0], kcs[1], kcs[2], vcs[0], vcs[1], vcs[2]))
-        _written(k_cache, v_cache)
+        _bump((k_cache, v_cache))   # autograd sees the stores
     return out
 
 
@@ -384,7 +376,7 @@ def paged_kv_keep(k_cache, v_cache, page_table, starts, kept):
             _lib.DN_ABI_VERSION, cs[0] if many else 1, B, cs[-2], cs[-1], most, _DT[ct], cs[-4], cs[-3], page_table.shape[1],
             k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(), starts.data_ptr(), kept.data_ptr(), lens.data_ptr(),
             ks[0] if many else 0, ks[-4], ks[-3], ks[-2], vs[0] if many else 0, vs[-4], vs[-3], vs[-2], page_table.stride(0)))
-        _written(k_cache, v_cache)
+        _bump((k_cache, v_cache))   # autograd sees the stores
     return lens
 
 
