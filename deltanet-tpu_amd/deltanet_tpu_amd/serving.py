@@ -77,7 +77,8 @@ def paged_reserve(pool, page_table, held, lens, *, page_size: int):
 
     pool: from ``page_pool``.  page_table: int32 (B, max_pages), the first ``held[b]``
     entries of row b are its pages.  held, lens: int32 (B,).  pool, page_table and held
-    are updated in place.  Pages that are no longer needed go back first; then
+    are updated in place; a page belongs to one sequence, and calls on one pool follow
+    one another on a stream.  Pages that are no longer needed go back first; then
     sequences take theirs in the order of the batch.  From the first for which the pool
     does not hold enough on, those that need more get nothing, and neither does one
     that needs more than max_pages.  Returns int32 (B,): the pages that a sequence is

@@ -111,3 +111,39 @@ def test_a_graph_of_two_calls(dev):
         got = [x.clone() for x in out]
         assert all(torch.equal(a, b) for a, b in zip(got, both())), t
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("new,G", [([4, 2, 7], 2), ([3, 8, 1], 4), ([20, 11], 4), ([40, 64], 6)])
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("D", [64, 256])
+def test_windows_of_every_tile(dev, dt, D, new, G):
+    """The window's first key in the middle of a tile, in the first tile, in front of all;
+    what lies before it may hold anything."""
+    lens = [n + x for n, x in zip(new, (333, 64, 20))]
+    kc, vc, pt, sl, cu, ks, vs = _paged(60, new, lens, 1, D, 16, dt, dev)
+    for c in (kc, vc):   # (the window of the first sequence leaves its first pages)
+        c[int(pt[0, 2])] = math.nan
+    q = _rows(61, sum(new), G, D, dt=dt)
+    _, seen = S.trees(new, 62)
+    for window in (64, 111, 250):
+        out, lse = paged_tree_attention(q.to(dev), kc, vc, pt, sl, S.words(seen, 1).to(dev), cu_seqlens=cu, window=window, return_lse=True)
+        _check(out, lse, q, ks, vs, new, lens, seen, dt, window, count=1)
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16"])
+@pytest.mark.parametrize("T,G", [(4, 2), (7, 4), (30, 4), (64, 8)])
+@pytest.mark.parametrize("odd", [math.nan, math.inf])
+def test_hidden_values_of_every_tile(dev, dt, T, G, odd):
+    """A draft whose value is not finite reaches those alone that see it, in every form."""
+    D, n = 128, 150 + T
+    kc, vc, pt, sl, cu, _, _ = _paged(63, [T], [n], 1, D, 16, dt, dev, junk=odd)
+    q = _rows(64, T, G, D, dt=dt).to(dev)
+    _, seen = S.trees([T], 65)
+    words = S.words(seen, 1).to(dev)
+    base = paged_tree_attention(q, kc, vc, pt, sl, words, cu_seqlens=cu)
+    at = 150 + T // 2
+    vc[int(pt[0, at // 16]), at % 16, :, 9] = odd
+    out = paged_tree_attention(q, kc, vc, pt, sl, words, cu_seqlens=cu)
+    hit = seen[0][:, T // 2].to(dev)
+    assert torch.isfinite(base).all() and torch.equal(out[~hit], base[~hit])
+    assert not torch.isfinite(out[hit][..., 9]).any() and torch.isfinite(out[hit][..., 10:]).all()
