@@ -388,10 +388,10 @@ __global__ __launch_bounds__(256) void k_heads_grad(const HP p, const GP g) {
   }
   __syncthreads();
   for (int ch = threadIdx.x; ch < p.D; ch += 256) {
-    float a = 0.f;
+    double a = 0.0;   // (the sums of sums lose nothing more)
 #pragma unroll 8
     for (int x = 0; x < 256 / P; ++x) a += sums[x][ch];
-    g.part[((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * p.D + ch] = a;
+    g.part[((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * p.D + ch] = (float)a;
   }
 }
 
@@ -452,24 +452,26 @@ __global__ __launch_bounds__(64) void k_heads_grad_any(const HP p, const GP g) {
   }
 }
 
-// dw of 4 channels of one side: the rows of partial sums, in an order of their own.
+// dw of 4 channels of one side: the rows of partial sums, in 64 bits and an order of
+// their own.
 __global__ __launch_bounds__(256) void k_weight_grad(const float* part, int D, int rows_q, int rows_k, int wdt, void* dwq, void* dwk) {
   const int side = blockIdx.y, n = side ? rows_k : rows_q;
   void* out = side ? dwk : dwq;
   if (out == nullptr) return;
   part += side ? (int64_t)rows_q * D : 0;
   const int ch = blockIdx.x * 4 + (threadIdx.x & 3);
-  float a = 0.f;
+  double a = 0.0;
   if (ch < D)
 #pragma unroll 4
     for (int x = threadIdx.x >> 2; x < n; x += 64) a += part[(int64_t)x * D + ch];
   // over the lanes with the same channel, then over the waves
 #pragma unroll
   for (int o = 4; o < 64; o <<= 1) a += __shfl_xor(a, o);
-  __shared__ float s[4][4];
+  __shared__ double s[4][4];
   if (lane_id() < 4) s[threadIdx.x >> 6][lane_id()] = a;
   __syncthreads();
-  if (threadIdx.x < 4 && ch < D) put1(out, wdt, ch, (s[0][threadIdx.x] + s[1][threadIdx.x]) + (s[2][threadIdx.x] + s[3][threadIdx.x]));
+  if (threadIdx.x < 4 && ch < D)
+    put1(out, wdt, ch, (float)((s[0][threadIdx.x] + s[1][threadIdx.x]) + (s[2][threadIdx.x] + s[3][threadIdx.x])));
 }
 
 bool float_type(int dt) { return dt == DN_F32 || dt == DN_BF16 || dt == DN_F16; }

@@ -363,7 +363,7 @@ def norm_rotary(q, k, q_weight, k_weight, positions=None, table=None, *, eps: fl
     ``apply_rotary``; neither positions nor table: no rotation.  Statistics and
     products in float32, one rounding at the end.  Differentiable in q, k and the
     weights (backwards and once; tangents are refused); the weights' gradients are
-    summed in float32 and are the same bits every time.  Returns (q', k') with k' None
+    summed in 32 bits or more and are the same bits every time.  Returns (q', k') with k' None
     if k is None; the results are contiguous.
     """
     qs = q.shape

@@ -290,7 +290,8 @@ def paged_tree_attention(q, k_cache, v_cache, page_table, seq_lens, visible, *, 
             and seq_lens.dtype is _I32 and seq_lens.shape == (B,) and seq_lens.is_contiguous()
             and (qs[0] == B and N == (B if nd == 3 else B * qs[1]) if cu_seqlens is None else nd == 3 and qs[0] == N and cu_seqlens.dtype is _I32
                  and cu_seqlens.shape == (B + 1,) and cu_seqlens.is_contiguous())
-            and visible.dtype is _I64 and visible.is_contiguous() and 1 <= words <= _NODES >> 6 and scale is None and window is None
+            and visible.dtype is _I64 and visible.is_contiguous() and 1 <= words <= _NODES >> 6 and scale is None
+            and (window is None or type(window) is int and window >= 64 * words)
             and not ((kcs[0] | kcs[1] | kcs[2] | vcs[0] | vcs[1] | vcs[2]) * e | k_cache.data_ptr() | v_cache.data_ptr()) & 15):
         scale = _check_tree_attention(q, k_cache, v_cache, page_table, seq_lens, visible, cu_seqlens, scale, window)
     else:
