@@ -191,12 +191,13 @@ __device__ __forceinline__ int64_t slot_of(const SP& p, int b, const Seq& s, int
 __device__ __forceinline__ void clear_rest(const SP& p) {
   if (p.cu == nullptr) return;
   const int c0 = min(max(p.cu[0], 0), p.N), c1 = min(max(p.cu[p.B], c0), p.N);
-  const int me = (blockIdx.y * gridDim.x + blockIdx.x) * blockDim.x + threadIdx.x, step = gridDim.x * gridDim.y * blockDim.x;
+  const int64_t me = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * kThreads + threadIdx.x, step = (int64_t)gridDim.x * gridDim.y * kThreads;
   for (int64_t i = me; i < c0; i += step) no_token(p, (int)i);
-  for (int64_t i = (int64_t)c1 + me; i < p.N; i += step) no_token(p, (int)i);
+  for (int64_t i = c1 + me; i < p.N; i += step) no_token(p, (int)i);
 }
 
 // x: sequences, y: parts of their tokens
+constexpr int kMostSequences = 0xffffff;   // a launch has fewer than 2^32 threads
 __global__ __launch_bounds__(kThreads) void k_slots(const SP p) {
   clear_rest(p);
   const int b = blockIdx.x;
@@ -379,6 +380,7 @@ extern "C" int dn_paged_reserve(const dn_paged_reserve_args* a, void* stream) {
   if ((int64_t)a->B * a->max_pages + a->capacity > 0x7fffffff) return bad("too many pages");
   if (a->B == 0) return DN_OK;
   if (!a->pool || !a->page_table || !a->held || !a->lens || !a->short_of) return bad("missing tensor pointer");
+  if (a->B > 1 && a->page_table_stride < a->max_pages) return bad("the rows of the page table overlap");
   const RP p{a->pool, a->page_table, a->held, a->short_of, a->lens, a->page_table_stride, a->capacity, a->max_pages, a->B, shift_of(a->page_size)};
   // blocks of 16 waves hide the searches of many pages (350000 of 2048 sequences: 10.6 us,
   // blocks of 4 waves 15.3), those of 4 start sooner where there are few (a token or a tree
@@ -396,6 +398,7 @@ extern "C" int dn_paged_slots(const dn_paged_slots_args* a, void* stream) {
   if (a->N < 0 || a->B < 0) return bad("bad sizes");
   if (const char* m = page_error(a->page_size, a->max_pages)) return bad(m);
   if (a->N && !a->B) return bad("tokens without a sequence");
+  if (a->B > kMostSequences) return bad("too many sequences");
   if (a->cu_seqlens == nullptr && a->B && a->N % a->B) return bad("without cu_seqlens every sequence has N / B new tokens");
   if (a->parents ? a->words < 1 || a->words * 64 > kNodes : a->words != 0) return bad("trees have 1 to 16 words of visible tokens");
   if (a->N == 0) return DN_OK;

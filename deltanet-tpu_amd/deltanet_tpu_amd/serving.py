@@ -89,7 +89,7 @@ def paged_reserve(pool, page_table, held, lens, *, page_size: int):
     B, most = page_table.shape if page_table.ndim == 2 else (-1, 0)
     if not (type(page_size) is int and 0 < page_size <= 1 << 30 and not page_size & (page_size - 1) and 0 <= B <= _lib.MAX_SEQUENCES and most > 0
             and page_table.dtype is _I32 and pool.dtype is _I32 and held.dtype is _I32 and lens.dtype is _I32
-            and page_table.stride(1) == 1 and pool.ndim == 1 and pool.is_contiguous() and held.shape == lens.shape == (B,) and held.is_contiguous()
+            and page_table.stride(1) == 1 and page_table.stride(0) >= most and pool.ndim == 1 and pool.is_contiguous() and held.shape == lens.shape == (B,) and held.is_contiguous()
             and lens.is_contiguous() and 2 <= pool.shape[0] <= 0x7fffffff - B * most):
         _check_reserve(pool, page_table, held, lens, page_size)
     dev = pool.get_device()
@@ -113,6 +113,8 @@ def _check_reserve(pool, page_table, held, lens, page_size):
     _check_int32("lens", lens, (B,))
     if B > _lib.MAX_SEQUENCES:
         raise ValueError(f"paged_reserve takes at most {_lib.MAX_SEQUENCES} sequences, got {B}.")
+    if B > 1 and page_table.stride(0) < page_table.shape[1]:
+        raise ValueError(f"the rows of page_table overlap, got strides {page_table.stride()} of {tuple(page_table.shape)}.")
     if B * page_table.shape[1] + pool.shape[0] > 0x7fffffff:
         raise ValueError("page_table and pool have too many pages.")
 

@@ -121,3 +121,13 @@ def test_c_entries_refuse_before_any_launch():
     assert P("dn_kv_keep")(bytes(k), None) == -1 and b"sizes" in err()
     k.B = 0
     assert P("dn_kv_keep")(bytes(k), None) == 0
+
+
+def test_c_entries_refuse_overlapping_rows_and_too_many_sequences():
+    lib = _lib.load_library()
+    err, P, V = lib.dn_last_error, _lib.packed_call, _lib.DN_ABI_VERSION
+    r = _set(_lib.PagedReserveArgs(), abi_version=V, B=2, page_size=4, max_pages=3, page_table_stride=2, pool=0x1000,
+             page_table=0x1000, held=0x1000, lens=0x1000, short_of=0x1000)
+    assert P("dn_paged_reserve")(bytes(r), None) == -1 and b"overlap" in err()
+    s = _set(_lib.PagedSlotsArgs(), abi_version=V, N=1, B=1 << 24, page_size=4, max_pages=3, cu_seqlens=0x1000)
+    assert P("dn_paged_slots")(bytes(s), None) == -1 and b"too many sequences" in err()

@@ -198,3 +198,15 @@ def test_empty_calls(dev):
     assert paged_kv_keep(kc, kc, t, _i32([3, 4], dev), _i32([[0], [-1]], dev)).tolist() == [4, 4]
     kc = torch.ones(4, 16, 2, 64, device=dev)
     assert paged_kv_keep(kc, kc.clone(), t, _i32([3, 4], dev), torch.zeros(2, 0, dtype=torch.int32, device=dev)).tolist() == [3, 4]
+
+
+@pytest.mark.parametrize("tree", [False, True])
+def test_slots_of_more_sequences_than_31_bits_of_threads(dev, tree):
+    """8.4 million sequences without a new token: all tokens are nobody's."""
+    B, N = (1 << 23) + 5, 1000
+    extra = {"parents": _i32([-1] * N, dev), "nodes": 3} if tree else {}
+    table, lens = torch.zeros(B, 1, dtype=torch.int32, device=dev), torch.zeros(B, dtype=torch.int32, device=dev)
+    for at in (0, 400, N):
+        cu = torch.full((B + 1,), at, dtype=torch.int32, device=dev)
+        got = paged_slots(table, lens, N, page_size=4, cu_seqlens=cu, **extra)
+        assert got[0].eq(-1).all() and got[1].eq(-1).all() and not (tree and got[2].any())

@@ -132,3 +132,9 @@ def test_keep_refusals():
     refuses("only on a ROCm GPU", f, *ok, error=RuntimeError)
 
 
+
+
+def test_rows_of_a_table_that_overlap_are_refused():
+    """Pages are written into the rows: a table with one row for all has no place for them."""
+    refuses("overlap", paged_reserve, page_pool(5, device="cpu"), i32(1, 4).expand(3, 4), i32(3), i32(3), page_size=16)
+    refuses("overlap", paged_reserve, page_pool(5, device="cpu"), i32(9).as_strided((3, 4), (2, 1)), i32(3), i32(3), page_size=16)
