@@ -63,11 +63,15 @@ template <int P> __device__ __forceinline__ float sum_lanes(float x) {
   return x;
 }
 
-// 1 / sqrt(a): the instruction's result (one step off at most) and a Newton step
+// 1 / sqrt(a): the instruction's result (one step off at most) and a Newton step.  The
+// instruction takes numbers below the normal ones for 0 (eps of 0, heads near 2^-64).
 __device__ __forceinline__ float rsqrt32(float a) {
+  const bool tiny = a < 0x1p-96f;
+  if (tiny) a *= 0x1p64f;
   const float y = __builtin_amdgcn_rsqf(a);
-  const float z = __builtin_fmaf(y * 0.5f, __builtin_fmaf(-a * y, y, 1.f), y);
-  return __builtin_isfinite(z) ? z : y;   // (0 and infinity)
+  float z = __builtin_fmaf(y * 0.5f, __builtin_fmaf(-a * y, y, 1.f), y);
+  if (!__builtin_isfinite(z)) z = y;   // (0 and infinity)
+  return tiny ? z * 0x1p32f : z;
 }
 
 __device__ __forceinline__ int64_t pos_of(const HP& p, int b, int l) {
@@ -269,46 +273,47 @@ __global__ __launch_bounds__(256) void k_heads(const HP p) {
   }
 }
 
-// A wave per head: any sizes, strides and alignment.
+// A wave per head at a time: any sizes, strides and alignment.
 template <class T, bool PAGED>
 __global__ __launch_bounds__(256) void k_heads_any(const HP p) {
   const int H = p.H[0] + p.H[1] + p.H[2];
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= (int64_t)p.N * H) return;
-  const int64_t t = row / H;
-  int h = (int)(row % H), side = 0;
-  for (; side < 2 && h >= p.H[side]; ++side) h -= p.H[side];
-  const int b = (int)(t / p.L), l = (int)(t % p.L);
-  const T* s = (const T*)p.x[side] + b * p.xs[side][0] + l * p.xs[side][1] + h * p.xs[side][2];
-  const int64_t pos = PAGED || p.R ? pos_of(p, b, l) : 0;
-  const Dst d = dst_of<T, PAGED>(p, side, t, pos);
-  const int64_t at = d.at + h * d.head;
-  const bool norm = side < 2 && p.w[0];
-  float r = 1.f;
-  if (norm) {
-    float z = 0.f;
-    for (int c = lane_id(); c < p.D; c += 64) z += (float)s[c] * (float)s[c];
-    r = rsqrt32(sum_lanes<64>(z) * (1.f / p.D) + p.eps);
-  }
-  if (!d.store) return;
-  const bool zero = PAGED && side == 0 && d.none;
-  auto value = [&](int c) {
-    const float x = (float)s[c];
-    return norm ? x * r * (p.offset + ld_f(p.w[side], c, p.wdt)) : x;
-  };
-  for (int i = lane_id(); i < p.D - (p.R >> 1); i += 64) {
-    int ca, cb;
-    pair_of(i, p.R, p.inter, ca, cb);
-    float x = value(ca), y = cb >= 0 ? value(cb) : 0.f;
-    if (cb >= 0 && side < 2) {
-      const bool in = pos >= 0 && pos < p.rows;
-      const float c = in ? p.table[pos * p.R + i] : __builtin_nanf(""), sn = in ? p.table[pos * p.R + (p.R >> 1) + i] : __builtin_nanf("");
-      const float a = x, e = y;
-      x = a * c - e * sn;
-      y = e * c + a * sn;
+#pragma unroll 1
+  for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); row < (int64_t)p.N * H; row += (int64_t)gridDim.x * 4) {
+    const int64_t t = row / H;
+    int h = (int)(row % H), side = 0;
+    for (; side < 2 && h >= p.H[side]; ++side) h -= p.H[side];
+    const int b = (int)(t / p.L), l = (int)(t % p.L);
+    const T* s = (const T*)p.x[side] + b * p.xs[side][0] + l * p.xs[side][1] + h * p.xs[side][2];
+    const int64_t pos = PAGED || p.R ? pos_of(p, b, l) : 0;
+    const Dst d = dst_of<T, PAGED>(p, side, t, pos);
+    const int64_t at = d.at + h * d.head;
+    const bool norm = side < 2 && p.w[0];
+    float r = 1.f;
+    if (norm) {
+      float z = 0.f;
+      for (int c = lane_id(); c < p.D; c += 64) z += (float)s[c] * (float)s[c];
+      r = rsqrt32(sum_lanes<64>(z) * (1.f / p.D) + p.eps);
     }
-    put1(p.out[side], d.dt, at + ca, zero ? 0.f : x);
-    if (cb >= 0) put1(p.out[side], d.dt, at + cb, zero ? 0.f : y);
+    if (!d.store) continue;
+    const bool zero = PAGED && side == 0 && d.none;
+    auto value = [&](int c) {
+      const float x = (float)s[c];
+      return norm ? x * r * (p.offset + ld_f(p.w[side], c, p.wdt)) : x;
+    };
+    for (int i = lane_id(); i < p.D - (p.R >> 1); i += 64) {
+      int ca, cb;
+      pair_of(i, p.R, p.inter, ca, cb);
+      float x = value(ca), y = cb >= 0 ? value(cb) : 0.f;
+      if (cb >= 0 && side < 2) {
+        const bool in = pos >= 0 && pos < p.rows;
+        const float c = in ? p.table[pos * p.R + i] : __builtin_nanf(""), sn = in ? p.table[pos * p.R + (p.R >> 1) + i] : __builtin_nanf("");
+        const float a = x, e = y;
+        x = a * c - e * sn;
+        y = e * c + a * sn;
+      }
+      put1(p.out[side], d.dt, at + ca, zero ? 0.f : x);
+      if (cb >= 0) put1(p.out[side], d.dt, at + cb, zero ? 0.f : y);
+    }
   }
 }
 
@@ -498,7 +503,7 @@ template <class T, class F> void by_lanes(int D, F f) {
   else f(Num<256 / W>{});
 }
 constexpr int kMostD = 512;   // of these kernels
-constexpr int kMostBlocks = 0x7fffffff;
+constexpr int kMostTokens = 0x7fffffff, kMostBlocks = 0xffffff;   // a launch has fewer than 2^32 threads
 
 // Threads of one head each that fill the card a few times over; from there on a thread
 // takes two heads and stores past the caches, and in serving, where no gradient reads
@@ -529,17 +534,17 @@ template <bool PAGED> int launch_heads(const HP& p, int dtype, bool fast, hipStr
   by_type(dtype, [&](auto z) {
     using T = decltype(z);
     if (!fast) {
-      const int64_t blocks = ((int64_t)p.N * H + 3) / 4;
-      if (!(ok = blocks <= kMostBlocks)) return;
+      const int64_t blocks = std::min<int64_t>(((int64_t)p.N * H + 3) / 4, kMostBlocks);
       hipLaunchKernelGGL((k_heads_any<T, PAGED>), dim3((unsigned)blocks), dim3(256), 0, st, p);
       return;
     }
     by_lanes<T>(p.D, [&](auto lanes) {
       constexpr int P = decltype(lanes)::value;
-      const int64_t blocks = ((int64_t)p.N * P + 255) / 256;
-      if (!(ok = blocks * chunks_of<1>(p) <= kMostBlocks)) return;
-      if ((int64_t)p.N * P * H < kManyThreads) hipLaunchKernelGGL((k_heads<T, P, 1, PAGED, false>), dim3((unsigned)(blocks * chunks_of<1>(p))), dim3(256), 0, st, p);
-      else hipLaunchKernelGGL((k_heads<T, P, 2, PAGED, true>), dim3((unsigned)(blocks * chunks_of<2>(p))), dim3(256), 0, st, p);
+      const bool few = (int64_t)p.N * P * H < kManyThreads;
+      const int64_t blocks = ((int64_t)p.N * P + 255) / 256 * (few ? chunks_of<1>(p) : chunks_of<2>(p));
+      if (!(ok = blocks <= kMostBlocks)) return;
+      if (few) hipLaunchKernelGGL((k_heads<T, P, 1, PAGED, false>), dim3((unsigned)blocks), dim3(256), 0, st, p);
+      else hipLaunchKernelGGL((k_heads<T, P, 2, PAGED, true>), dim3((unsigned)blocks), dim3(256), 0, st, p);
     });
   });
   if (!ok) return bad("too many tokens");
@@ -550,7 +555,7 @@ template <bool PAGED> int launch_heads(const HP& p, int dtype, bool fast, hipStr
 int norm_params(const dn_norm_rotary_args* a, HP& p) {
   if (a == nullptr) return bad("null args");
   if (a->abi_version != DN_ABI_VERSION) return set_error(DN_E_ABI, "dn_norm_rotary_args built for another ABI version");
-  if (a->B < 0 || a->L < 0 || (int64_t)a->B * a->L > kMostBlocks) return bad("bad sizes");
+  if (a->B < 0 || a->L < 0 || (int64_t)a->B * a->L > kMostTokens) return bad("bad sizes");
   p.N = a->B * a->L; p.L = a->L; p.H[0] = a->Hq; p.H[1] = a->Hk; p.H[2] = 0; p.D = a->D; p.R = a->R; p.rows = a->rows;
   p.inter = a->interleaved != 0; p.pos64 = a->pos_dtype == DN_I64; p.wdt = a->weight_dtype; p.cdt = a->dtype;
   p.eps = a->eps; p.offset = a->weight_offset;
@@ -650,7 +655,7 @@ extern "C" int dn_norm_rotary_bwd(const dn_norm_rotary_args* a, const dn_norm_ro
 extern "C" int dn_qkv_append(const dn_qkv_append_args* a, void* stream) {
   if (a == nullptr) return bad("null args");
   if (a->abi_version != DN_ABI_VERSION) return set_error(DN_E_ABI, "dn_qkv_append_args built for another ABI version");
-  if (a->B < 0 || a->L < 0 || (int64_t)a->B * a->L > kMostBlocks) return bad("bad sizes");
+  if (a->B < 0 || a->L < 0 || (int64_t)a->B * a->L > kMostTokens) return bad("bad sizes");
   HP p{};
   p.N = a->B * a->L; p.L = a->L; p.H[0] = a->Hq; p.H[1] = p.H[2] = a->Hkv; p.D = a->D; p.R = a->R; p.rows = a->rows;
   p.inter = a->interleaved != 0; p.pos64 = a->pos_dtype == DN_I64; p.wdt = a->weight_dtype; p.cdt = a->cache_dtype;

@@ -192,3 +192,32 @@ def test_second_derivatives_are_refused(dev):
     y, = torch.autograd.grad(norm_rotary(x, None, w, None)[0].sum(), w, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         y.sum().backward()
+
+
+@pytest.mark.parametrize("dt,D", [("f32", 128), ("bf16", 64), ("f32", 6)])
+def test_heads_whose_squares_are_below_the_normal_numbers(dev, dt, D):
+    """Channels of 1 and 1.5 times 2^-66 with eps 0: their squares are whole multiples of
+    2^-134, the sum is exact, the mean is rounded to a multiple of 2^-149, half of that of
+    2^-132 or more: 2^-18 of it, 2^-19 of the root, 3 times that of the terms of dx: less
+    than twice what the tolerance has for the other roundings."""
+    g = torch.Generator().manual_seed(D)
+    x = (torch.randint(2, 4, (5, 3, D), generator=g) * (2 * torch.randint(0, 2, (5, 3, D), generator=g) - 1)).double() * 2.0 ** -67
+    w, dz = _rows(1, D, dt="f32"), _rows(2, 5, 3, D, dt=dt)
+    xs = [x.to(dz.dtype).to(dev).requires_grad_(True), w.to(dev).requires_grad_(True)]
+    y, _ = norm_rotary(xs[0], None, xs[1], None, eps=0.0)
+    ref, tol = S.normed(x, w.double(), 0.0, 0.0, None, None, False, dt)
+    _near(y, ref, 3 * tol)
+    dx, dw, tx, tw = S.normed_grad(x, w.double(), dz.double(), 0.0, 0.0, None, None, False, dt, "f32")
+    gx, gw = torch.autograd.grad(y, xs, dz.to(dev))
+    _near(gx, dx, 3 * tx, "dx")
+    _near(gw, dw, 3 * tw, "dw")
+
+
+def test_more_heads_than_a_launch_has_waves(dev):
+    """67 million heads of 2 channels: the first and the last tokens as by calls of their own."""
+    L, H, D = 1048600, 65, 2
+    x = torch.randn(1, L, H, D, device=dev, dtype=torch.bfloat16)
+    w = torch.tensor([0.5, 2.0], device=dev)
+    y, _ = norm_rotary(x, None, w, None)
+    for part in (slice(0, 1000), slice(L // 2, L // 2 + 1000), slice(L - 1000, L)):
+        assert torch.equal(y[:, part], norm_rotary(x[:, part], None, w, None)[0])
