@@ -120,6 +120,7 @@ __global__ __launch_bounds__(64 * NW, 2 * ST * BN * D * (int)sizeof(T) <= 80 * 1
     };
     f32x4 o[NQ][NC];
     float mx[NQ], top[NQ], sum[NQ];
+    bool late[NQ];   // scores of the tiles between were beyond the reference of their time
 #pragma unroll
     for (int i = 0; i < NQ; ++i) mx[i] = -INFINITY;
     bool odd = false;
@@ -132,11 +133,14 @@ __global__ __launch_bounds__(64 * NW, 2 * ST * BN * D * (int)sizeof(T) <= 80 * 1
     };
     // 32 keys.  Probabilities are relative to mx, the maximum of a piece's first tile
     // and of its masked ones (LEARN, kept up to 2^kLazy); the tiles between only note what
-    // their largest scores were.  A row that went more than 2^kRange beyond is found at the
-    // piece's end, and the piece done again from what is known then: sums are as exact with
-    // any reference up to there.  float16 has no such range, its rows are raised on the way.
+    // their largest scores were.  A row that went more than 2^kRange beyond the mx that it
+    // was summed by is found before a masked tile raises that, or at the piece's end, and the
+    // piece done again from the largest score that is known then, which nothing raises any
+    // more: sums are as exact with any reference up to 2^kRange below.  float16 has no such
+    // range, its rows are raised on the way.  (The tile that begins with the last of the
+    // windows' first keys is the first of which that row sees any: it is LEARN too.)
     auto hides = [&](int key0) { return key0 + 32 > off || key0 < lo1; };   // some row must not see some of 32 keys
-    auto learns = [&](int j) { return j == j0 || (j + 1) * BN > off || j * BN < lo1; };
+    auto learns = [&](int j) { return j == j0 || (j + 1) * BN > off || j * BN <= lo1; };
     constexpr bool AHEAD = D == 256 && sizeof(T) == 2;
     constexpr int VB = AHEAD ? 4 : 1, NB = NC / VB;
     auto in_order = [] {
@@ -190,7 +194,10 @@ __global__ __launch_bounds__(64 * NW, 2 * ST * BN * D * (int)sizeof(T) <= 80 * 1
       if constexpr (LEARN || F16) {
         if (__any(grow)) {
 #pragma unroll
-          for (int i = 0; i < NQ; ++i) rescale(i, fmaxf(mx[i], LEARN ? mt[i] : max_q(top[i]) * scale - kLift));
+          for (int i = 0; i < NQ; ++i) {
+            if (!F16) late[i] |= max_q(top[i]) * scale > mx[i] + kRange;
+            rescale(i, fmaxf(mx[i], LEARN ? mt[i] : max_q(top[i]) * scale - kLift));
+          }
         }
       }
       F pf[NQ];
@@ -234,6 +241,7 @@ __global__ __launch_bounds__(64 * NW, 2 * ST * BN * D * (int)sizeof(T) <= 80 * 1
       for (int i = 0; i < NQ; ++i) {
         top[i] = -INFINITY;
         sum[i] = 0.f;
+        late[i] = false;
 #pragma unroll
         for (int c = 0; c < NC; ++c) o[i][c] = zero4();
       }
@@ -271,11 +279,12 @@ __global__ __launch_bounds__(64 * NW, 2 * ST * BN * D * (int)sizeof(T) <= 80 * 1
 #pragma unroll
       for (int i = 0; i < NQ; ++i) {
         top[i] = max_q(top[i]) * scale;
-        over |= top[i] > mx[i] + kRange;
+        late[i] |= top[i] > mx[i] + kRange;
+        over |= late[i];
       }
       if (!__syncthreads_or(over)) break;
 #pragma unroll
-      for (int i = 0; i < NQ; ++i) mx[i] = top[i] > mx[i] + kRange ? top[i] : mx[i];   // (the other rows keep their bits)
+      for (int i = 0; i < NQ; ++i) mx[i] = late[i] ? fmaxf(top[i], mx[i]) : mx[i];
     }
     if (odd) {   // infinities and NaNs that some row must not see: to those that do
 #pragma unroll
