@@ -149,6 +149,32 @@ __device__ __forceinline__ Span span_of(const AF& p, int b) {
 // which see none, count as 0, so that no difference leaves 32 bits.
 __device__ __forceinline__ int first_key(const AF& p, int pos) { return p.window ? max(max(pos, 0) - p.window + 1, 0) : 0; }
 
+// Whether a row's sums left float32's range, by all four lanes that share it.
+template <int NC> __device__ __forceinline__ bool left_range(const f32x4 (&o)[NC]) {
+  float x = 0.f;   // (0 times an infinity or a NaN is a NaN)
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x = __builtin_fmaf(o[c][e], 0.f, x);
+  return !(sum_q(x) == 0.f);
+}
+
+// Whether keys [key0, key1) have finite values that may have done it, by all threads of
+// a workgroup: 2^32 times 2^60 (what an exponential may be) times as many keys as there
+// can be stays within it.  (Values that are not finite call for no other reference, and
+// the results that they are not part of keep their bits.)
+template <int D, class T, bool PAGED> __device__ __forceinline__ bool has_large(const Rows<T, PAGED>& v, int key0, int key1) {
+  bool large = false;
+  int i = threadIdx.x;
+  settle(i);   // (addresses are computed here, not in front of the callers' loops)
+#pragma unroll 1
+  for (int key = key0 + i / D; key < key1; key += blockDim.x / D) {
+    const float y = fabsf((float)v(key)[i % D]);
+    large |= y >= 0x1p32f && y < INFINITY;
+  }
+  return __syncthreads_or(large);
+}
+
 // Drafted trees.  A new token sees the keys in front of its sequence's new tokens, the
 // window aside, and of those the ones whose bit is set in its words: key `off` is new
 // token 0.  low: the first key that a window of all that it sees leaves (at least 64

@@ -89,7 +89,8 @@ __global__ __launch_bounds__(64 * NW * KG, sizeof(T) == 2 ? 2 : 1) void k_attn(c
   // The exponents' reference is a query's score with itself, which it always sees:
   // no maximum has to be known while the sums run.  Sums of exponentials up to
   // 2^kRange above it are as exact as any in a type with float32's range; the
-  // rare row that goes beyond is found at the end, and the tile done again with
+  // rare row that goes beyond, or whose products with the values leave the range all
+  // the same (values from 2^68 on), is found at the end, and the tile done again with
   // the maxima that are known then.
   // float16 has no such range, and loses bits below 2^-14: there the own key starts
   // at 2^6, and a row whose largest gets to 2^15 has its reference raised on the way
@@ -277,20 +278,24 @@ __global__ __launch_bounds__(64 * NW * KG, sizeof(T) == 2 ? 2 : 1) void k_attn(c
         for (int u = 0; u < BN; u += 32) step(std::false_type{}, [] {}, kt + u * 32, vt + u * 32, j * BN + u);
       }
     }
-    bool over = false;
+    if (F16 || pass == 1) break;
+    bool over = false, out = false;
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
       top[i] = max_q(top[i]) * scale;
       over |= top[i] > mx[i] + kRange;
-      if (!F16 && KG > 1 && q == 0) s_top[kg][(w * NQ + i) * 16 + r] = top[i];
+      out |= top[i] > mx[i] && left_range(o[i]);
+      if (KG > 1 && q == 0) s_top[kg][(w * NQ + i) * 16 + r] = top[i];
     }
-    if (F16 || pass == 1 || !__syncthreads_or(over)) break;
+    if (__builtin_expect(!__syncthreads_or(over || out), 1)) break;
+    // (values that are not finite: once more by the same references, to the same bits)
+    const float range = __syncthreads_or(out) && has_large<D>(vr, j0 * BN, min(j1 * BN, p1 + 1)) ? 0.f : kRange;
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
 #pragma unroll
       for (int g = 0; g < KG; ++g)
         if (KG > 1) top[i] = fmaxf(top[i], s_top[g][(w * NQ + i) * 16 + r]);
-      mx[i] = top[i] > mx[i] + kRange ? top[i] : mx[i];   // (the other rows keep their bits)
+      mx[i] = top[i] > mx[i] + range ? top[i] : mx[i];   // (the other rows keep their bits)
     }
     __syncthreads();
   }

@@ -120,7 +120,7 @@ __global__ __launch_bounds__(64 * NW, 2 * ST * BN * D * (int)sizeof(T) <= 80 * 1
     };
     f32x4 o[NQ][NC];
     float mx[NQ], top[NQ], sum[NQ];
-    bool late[NQ];   // scores of the tiles between were beyond the reference of their time
+    bool late = false;   // scores of the tiles between were beyond the reference of their time
 #pragma unroll
     for (int i = 0; i < NQ; ++i) mx[i] = -INFINITY;
     bool odd = false;
@@ -136,8 +136,9 @@ __global__ __launch_bounds__(64 * NW, 2 * ST * BN * D * (int)sizeof(T) <= 80 * 1
     // their largest scores were.  A row that went more than 2^kRange beyond the mx that it
     // was summed by is found before a masked tile raises that, or at the piece's end, and the
     // piece done again from the largest score that is known then, which nothing raises any
-    // more: sums are as exact with any reference up to 2^kRange below.  float16 has no such
-    // range, its rows are raised on the way.  (The tile that begins with the last of the
+    // more: sums are as exact with any reference up to 2^kRange below.  A row whose products
+    // with the values left the range all the same (values from 2^68 on) goes that way too.
+    // float16 has no such range, its rows are raised on the way.  (The tile that begins with the last of the
     // windows' first keys is the first of which that row sees any: it is LEARN too.)
     auto hides = [&](int key0) { return key0 + 32 > off || key0 < lo1; };   // some row must not see some of 32 keys
     auto learns = [&](int j) { return j == j0 || (j + 1) * BN > off || j * BN <= lo1; };
@@ -195,7 +196,7 @@ __global__ __launch_bounds__(64 * NW, 2 * ST * BN * D * (int)sizeof(T) <= 80 * 1
         if (__any(grow)) {
 #pragma unroll
           for (int i = 0; i < NQ; ++i) {
-            if (!F16) late[i] |= max_q(top[i]) * scale > mx[i] + kRange;
+            if (!F16) late |= __any(max_q(top[i]) * scale > mx[i] + kRange);
             rescale(i, fmaxf(mx[i], LEARN ? mt[i] : max_q(top[i]) * scale - kLift));
           }
         }
@@ -241,7 +242,6 @@ __global__ __launch_bounds__(64 * NW, 2 * ST * BN * D * (int)sizeof(T) <= 80 * 1
       for (int i = 0; i < NQ; ++i) {
         top[i] = -INFINITY;
         sum[i] = 0.f;
-        late[i] = false;
 #pragma unroll
         for (int c = 0; c < NC; ++c) o[i][c] = zero4();
       }
@@ -275,16 +275,18 @@ __global__ __launch_bounds__(64 * NW, 2 * ST * BN * D * (int)sizeof(T) <= 80 * 1
         }
       }
       if (F16 || pass == 1) break;
-      bool over = false;
+      bool over = late, out = false;
 #pragma unroll
       for (int i = 0; i < NQ; ++i) {
         top[i] = max_q(top[i]) * scale;
-        late[i] |= top[i] > mx[i] + kRange;
-        over |= late[i];
+        over |= top[i] > mx[i] + kRange;
+        out |= left_range(o[i]);
       }
-      if (!__syncthreads_or(over)) break;
+      if (__builtin_expect(!__syncthreads_or(over || out), 1)) break;
+      // (values that are not finite: once more as it was, to the same bits)
+      const bool raise = __syncthreads_or(over) || has_large<D>(vr, j0 * BN, min(j1 * BN, t.s.len));
 #pragma unroll
-      for (int i = 0; i < NQ; ++i) mx[i] = late[i] ? fmaxf(top[i], mx[i]) : mx[i];
+      for (int i = 0; i < NQ; ++i) mx[i] = raise ? fmaxf(top[i], mx[i]) : -INFINITY;
     }
     if (odd) {   // infinities and NaNs that some row must not see: to those that do
 #pragma unroll

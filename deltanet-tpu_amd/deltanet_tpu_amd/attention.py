@@ -553,7 +553,8 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, *, cu_seqlens=Non
     page_table and seq_lens as in ``paged_kv_append``; query head h reads key head
     h // (Hq // Hkv).  A query at position p sees positions 0 .. p, or the last
     ``window`` of them.  scale: any finite number, 1 / sqrt(D) unless given.  Sums and
-    softmax statistics in float32.  A query without a key gets zeros (lse -inf), and
+    softmax statistics in float32 (which the sums stay within as long as the largest value
+    times the tokens that a query sees is below 2^120).  A query without a key gets zeros (lse -inf), and
     so do tokens in front of cu_seqlens[0] and from cu_seqlens[-1] on (a batch of fixed
     size that is not full); in between cu_seqlens must not fall.  Returns the output in
     q's shape and type, and with ``return_lse`` also the log of the sum of exponentials

@@ -312,7 +312,8 @@ int dn_kv_append(const dn_kv_append_args* a, void* stream);
  * and lse -inf, and so does a token that cu_seqlens, which must not fall, gives to
  * no sequence (before its first entry, from its last on).  Page numbers outside the cache are read as its nearest page and
  * seq_lens past the page table as its end.  Nothing that a query must not see
- * reaches it, infinities and NaNs included.  scale: any finite number, 0 and
+ * reaches it, infinities and NaNs included.  The largest finite value times the keys
+ * that a query sees must stay below 2^120.  scale: any finite number, 0 and
  * negative ones too.  A window that reaches past the page table is none; page
  * tables of 2^31 - 1024 tokens or more are refused. */
 typedef struct dn_paged_attention_args {
