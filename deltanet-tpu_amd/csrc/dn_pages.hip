@@ -283,7 +283,7 @@ struct KP {
   int layers, B, most, pages, shift, max_pages;
   uint32_t H, pieces;   // pieces: of a head
   char *k, *v;
-  const int32_t *pt, *starts, *kept;
+  const int32_t *pt, *starts, *kept, *held;
   int32_t* lens;
   int64_t ks[4], vs[4], pts;   // in bytes
 };
@@ -298,7 +298,7 @@ template <class V> __global__ __launch_bounds__(kThreads) void k_keep(const KP p
   __shared__ int s_count;
   const int b = blockIdx.y;
   const int start = p.starts[b];
-  const int64_t end = (int64_t)p.max_pages << p.shift;
+  const int64_t end = (int64_t)(p.held ? min(p.held[b], p.max_pages) : p.max_pages) * (1 << p.shift);   // (held may be anything)
   const uint32_t n = (uint32_t)p.layers * 2 * p.H * p.pieces;
   int before = -1, total = 0;
 #pragma unroll 1
@@ -429,7 +429,7 @@ extern "C" int dn_kv_keep(const dn_kv_keep_args* a, void* stream) {
   const int e = a->dtype == DN_F32 ? 4 : 2;
   p.layers = a->layers; p.B = a->B; p.H = a->H; p.most = a->most; p.pages = a->pages; p.max_pages = a->max_pages;
   p.shift = shift_of(a->page_size);
-  p.k = (char*)a->k_cache; p.v = (char*)a->v_cache; p.pt = a->page_table; p.starts = a->starts; p.kept = a->kept; p.lens = a->lens;
+  p.k = (char*)a->k_cache; p.v = (char*)a->v_cache; p.pt = a->page_table; p.starts = a->starts; p.kept = a->kept; p.held = a->held; p.lens = a->lens;
   p.pts = a->page_table_stride;
   int64_t all = (int64_t)(uintptr_t)a->k_cache | (int64_t)(uintptr_t)a->v_cache | (int64_t)a->D * e;
   for (int i = 0; i < 4; ++i) {

@@ -15,7 +15,7 @@ import threading
 LIB_NAME = "libdeltanet_amd.so"
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
 
-DN_ABI_VERSION = 2
+DN_ABI_VERSION = 3
 DN_F32, DN_BF16, DN_F16, DN_I32, DN_I64 = 0, 1, 2, 3, 4
 
 _c_i32 = ctypes.c_int32
@@ -215,7 +215,7 @@ class KvKeepArgs(ctypes.Structure):
         ("layers", _c_i32), ("B", _c_i32), ("H", _c_i32), ("D", _c_i32), ("most", _c_i32), ("dtype", _c_i32),
         ("pages", _c_i32), ("page_size", _c_i32), ("max_pages", _c_i32),
         ("k_cache", _c_ptr), ("v_cache", _c_ptr), ("page_table", _c_ptr), ("starts", _c_ptr), ("kept", _c_ptr), ("lens", _c_ptr),
-        ("kc_strides", _c_i64 * 4), ("vc_strides", _c_i64 * 4), ("page_table_stride", _c_i64),
+        ("kc_strides", _c_i64 * 4), ("vc_strides", _c_i64 * 4), ("page_table_stride", _c_i64), ("held", _c_ptr),
     ]
 
 
@@ -229,7 +229,7 @@ NORM_ROTARY_GRADS_PACK = struct.Struct("@6P6q").pack
 QKV_APPEND_PACK = struct.Struct("@15i2f11P15q").pack
 PAGED_RESERVE_PACK = struct.Struct("@5i5Pq").pack
 PAGED_SLOTS_PACK = struct.Struct("@6i8Pq").pack
-KV_KEEP_PACK = struct.Struct("@10i6P9q").pack
+KV_KEEP_PACK = struct.Struct("@10i6P9qP").pack
 MAX_SEQUENCES = 4096   # DN_MAX_SEQUENCES
 
 

@@ -4,15 +4,20 @@ keys and values normed, rotated and stored in one launch, attention of drafted t
 and the accepted tokens moved to the front.  A step that verifies drafts:
 
     short = paged_reserve(pool, page_table, held, lens, page_size=P)
-    positions, slots, visible = paged_slots(page_table, lens, N, page_size=P, cu_seqlens=cu, parents=parents, nodes=T)
+    positions, slots, visible = paged_slots(page_table, lens, N, page_size=P, cu_seqlens=cu, held=held, parents=parents, nodes=T)
     # in every layer:
     q = paged_qkv_append(q, k, v, k_cache, v_cache, slots, positions, q_weight=wq, k_weight=wk, table=table)
     out = paged_tree_attention(q, k_cache, v_cache, page_table, lens, visible, cu_seqlens=cu)
     # the drafts that the model agrees with, ``kept``:
-    lens = paged_kv_keep(k_caches, v_caches, page_table, starts, kept)
+    lens = paged_kv_keep(k_caches, v_caches, page_table, starts, kept, held=held)
     paged_reserve(pool, page_table, held, lens, page_size=P)
 
-Nothing here reads a device tensor on the host; all of it can be captured in a graph.
+Nothing here reads a device tensor on the host; all of it can be captured in a graph.  A
+step goes on where the pool runs short: with ``held``, tokens behind the pages that their
+sequence has get no slot, are not stored and not kept, whatever ``kept`` says, and what
+attention returns for them means nothing; the others' results are right.  (Behind them
+the page table holds numbers of pages that may be another sequence's by now: leave
+``held`` out only where no sequence is ever short.)
 """
 
 from __future__ import annotations
@@ -347,7 +352,7 @@ def _check_tree_attention(q, k_cache, v_cache, page_table, seq_lens, visible, cu
     return scale
 
 
-def paged_kv_keep(k_cache, v_cache, page_table, starts, kept):
+def paged_kv_keep(k_cache, v_cache, page_table, starts, kept, *, held=None):
     """The keys and values of accepted drafts moved to the front of their sequence's
     new tokens, in all layers: token starts + kept[i] goes to starts + i.
 
@@ -356,7 +361,8 @@ def paged_kv_keep(k_cache, v_cache, page_table, starts, kept):
     (B, max_pages).  starts: int32 (B,), each sequence's tokens in front of the new
     ones.  kept: int32 (B, most), the places of the accepted ones among the new,
     rising, with negative numbers behind the last; what comes after an entry that is
-    negative, not above the one before it or past the page table is not kept.  Pages
+    negative, not above the one before it, past the page table or past the pages that its
+    sequence has is not kept; held: int32 (B,), those pages (``paged_reserve``).  Pages
     that are written must not be shared.  Returns int32 (B,): the sequences' lengths
     then, starts plus the number of tokens kept, for ``paged_reserve``.
     """
@@ -366,11 +372,13 @@ def paged_kv_keep(k_cache, v_cache, page_table, starts, kept):
     if not (4 <= len(cs) <= 5 and v_cache.shape == cs and v_cache.dtype is ct and ct in _DT and ks[-1] == vs[-1] == 1 and cs[-3] > 0
             and not cs[-3] & (cs[-3] - 1) and page_table.ndim == 2 and page_table.dtype is _I32 and page_table.shape[0] == B <= 65535
             and page_table.shape[1] > 0 and page_table.stride(1) == 1 and starts.dtype is _I32 and starts.shape == (B,) and starts.is_contiguous()
-            and kept.dtype is _I32 and kept.is_contiguous()):
-        _check_keep(k_cache, v_cache, page_table, starts, kept)
+            and kept.dtype is _I32 and kept.is_contiguous()
+            and (held is None or held.dtype is _I32 and held.shape == (B,) and held.is_contiguous())):
+        _check_keep(k_cache, v_cache, page_table, starts, kept, held)
     dev = k_cache.get_device()
-    if not v_cache.get_device() == page_table.get_device() == starts.get_device() == kept.get_device() == dev >= 0:
-        _on_gpu(k_cache, v_cache, page_table, starts, kept)
+    if not (v_cache.get_device() == page_table.get_device() == starts.get_device() == kept.get_device() == dev >= 0
+            and (held is None or held.get_device() == dev)):
+        _on_gpu(k_cache, v_cache, page_table, starts, kept, held)
     if _grad_enabled() and (k_cache.requires_grad or v_cache.requires_grad) or _forward_ad._current_level >= 0 and _differentiated(k_cache, v_cache):
         raise ValueError("paged_kv_keep is not differentiable; call it under torch.no_grad().")
     lens = torch.empty_like(starts)
@@ -379,12 +387,13 @@ def paged_kv_keep(k_cache, v_cache, page_table, starts, kept):
         _call("dn_kv_keep", dev, _lib.KV_KEEP_PACK(
             _lib.DN_ABI_VERSION, cs[0] if many else 1, B, cs[-2], cs[-1], most, _DT[ct], cs[-4], cs[-3], page_table.shape[1],
             k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(), starts.data_ptr(), kept.data_ptr(), lens.data_ptr(),
-            ks[0] if many else 0, ks[-4], ks[-3], ks[-2], vs[0] if many else 0, vs[-4], vs[-3], vs[-2], page_table.stride(0)))
+            ks[0] if many else 0, ks[-4], ks[-3], ks[-2], vs[0] if many else 0, vs[-4], vs[-3], vs[-2], page_table.stride(0),
+            0 if held is None else held.data_ptr()))
         _bump((k_cache, v_cache))   # autograd sees the stores
     return lens
 
 
-def _check_keep(k_cache, v_cache, page_table, starts, kept):
+def _check_keep(k_cache, v_cache, page_table, starts, kept, held):
     many = k_cache.ndim == 5 and v_cache.ndim == 5
     if many and k_cache.shape[0] != v_cache.shape[0]:
         raise ValueError(f"v_cache {tuple(v_cache.shape)} must have the layers of k_cache {tuple(k_cache.shape)}.")
@@ -397,5 +406,7 @@ def _check_keep(k_cache, v_cache, page_table, starts, kept):
     if kept.ndim != 2:
         raise ValueError(f"kept must be int32 (B, most), got {kept.dtype} {tuple(kept.shape)}.")
     _check_int32("kept", kept, (B, kept.shape[1]))
+    if held is not None:
+        _check_int32("held", held, (B,))
     if B > 65535:
         raise ValueError(f"paged_kv_keep takes at most 65535 sequences, got {B}.")

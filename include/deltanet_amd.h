@@ -36,7 +36,7 @@
 extern "C" {
 #endif
 
-#define DN_ABI_VERSION 2
+#define DN_ABI_VERSION 3
 
 /* element types */
 enum { DN_F32 = 0, DN_BF16 = 1, DN_F16 = 2, DN_I32 = 3, DN_I64 = 4 };
@@ -525,9 +525,10 @@ int dn_paged_tree_attention(const dn_paged_attention_args* a, const uint64_t* vi
 
 /* Keys and values of accepted tokens moved to the front: token starts[b] + kept[b][i]
  * of sequence b to starts[b] + i, in every layer, for the entries of kept in front of
- * the first that is negative, not above the one before it or past the page table;
- * lens[b] = starts[b] + their number.  A token is not moved from or to a page outside
- * the cache. */
+ * the first that is negative, not above the one before it, past the page table or past
+ * the held[b] pages (held NULL: not checked; what a page table holds behind them may be
+ * another sequence's); lens[b] = starts[b] + their number.  A token is not moved from or
+ * to a page outside the cache. */
 typedef struct dn_kv_keep_args {
   int32_t abi_version;
   int32_t layers, B, H, D, most;   /* most: entries of kept per sequence         */
@@ -542,6 +543,7 @@ typedef struct dn_kv_keep_args {
   int64_t kc_strides[4];        /* layer, page, token, head                      */
   int64_t vc_strides[4];
   int64_t page_table_stride;
+  const int32_t* held;          /* (B), or NULL                                  */
 } dn_kv_keep_args;
 
 int dn_kv_keep(const dn_kv_keep_args* a, void* stream);
