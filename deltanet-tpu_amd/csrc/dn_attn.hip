@@ -44,8 +44,6 @@ bool wide(const void* p, const int64_t* s, int dtype, int n) {
   return ((uintptr_t)p & 15) == 0;
 }
 
-// Rows and tokens are counted in 32 bits, in steps of up to 1024 past the last one.
-constexpr int64_t kMostIndex = ((int64_t)1 << 31) - 1024;
 // a window that no row is longer than is none
 int window_of(int window, int64_t most) { return window >= most ? 0 : window; }
 
@@ -124,6 +122,7 @@ int tree_params(const dn_paged_attention_args* a, const uint64_t* visible, int w
   if (p.N && ((int64_t)p.N * p.G / 16 + p.B) * p.Hkv * ((((int64_t)p.max_pages << p.shift) + 31) / 32) >= (int64_t)1 << 31)
     return bad("too many rows over too many tokens");
   p.vis = visible; p.words = words;
+  p.window = window_of(a->window, kMostIndex);   // (lengths may pass the page table)
   return DN_OK;
 }
 }  // namespace

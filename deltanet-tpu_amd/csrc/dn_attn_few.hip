@@ -56,13 +56,13 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_few(const AF p) {
     if (!plan.of_unit(u, t)) break;
     const int rows = t.s.n * p.G, row0 = t.m * BM, row1 = min(row0 + BM, rows);
     // the keys that all rows see end with p0, those that any sees with p1
-    const int off = t.s.len - t.s.n, p0 = TREE ? off - 1 : off + over_g(p, row0), p1 = TREE ? t.s.len - 1 : off + over_g(p, row1 - 1);
+    const int off = t.s.off, p0 = TREE ? min(off, t.s.len) - 1 : off + over_g(p, row0), p1 = TREE ? t.s.len - 1 : off + over_g(p, row1 - 1);
     int k0, k1;
     units_of<TREE>(p, t.s, row0, row1, kUnit, k0, k1);
     const int skip = u - t.first, take = min(t.units - skip, uend - u);
     const int j0 = k0 + skip, j1 = j0 + take;   // units of this piece
     const int last = max(p1, 0);
-    const int lo1 = first_key(p, p1);   // (none later, of any row)
+    const int lo1 = first_key(p, TREE ? off + t.s.n - 1 : p1);   // (none later, of any row)
 
     F qf[NQ][NS];
     int pos[NQ], low[NQ];

@@ -59,7 +59,8 @@ __global__ __launch_bounds__(64 * NW, 2 * ST * BN * D * (int)sizeof(T) <= 80 * 1
   while (u < uend) {
     Task t;
     if (!plan.of_unit(u, t)) break;
-    const int rows = t.s.n * p.G, row0 = t.m * BM, off = t.s.len - t.s.n, last = max(t.s.len - 1, 0);
+    const int rows = t.s.n * p.G, row0 = t.m * BM, off = t.s.off, last = max(t.s.len - 1, 0);
+    const int front = min(off, t.s.len);   // keys that every row sees, but for the window
     int k0, k1;
     units_of<true>(p, t.s, 0, 1, BN, k0, k1);
     const int skip = u - t.first, take = min(t.units - skip, uend - u);
@@ -140,8 +141,8 @@ __global__ __launch_bounds__(64 * NW, 2 * ST * BN * D * (int)sizeof(T) <= 80 * 1
     // with the values left the range all the same (values from 2^68 on) goes that way too.
     // float16 has no such range, its rows are raised on the way.  (The tile that begins with the last of the
     // windows' first keys is the first of which that row sees any: it is LEARN too.)
-    auto hides = [&](int key0) { return key0 + 32 > off || key0 < lo1; };   // some row must not see some of 32 keys
-    auto learns = [&](int j) { return j == j0 || (j + 1) * BN > off || j * BN <= lo1; };
+    auto hides = [&](int key0) { return key0 + 32 > front || key0 < lo1; };   // some row must not see some of 32 keys
+    auto learns = [&](int j) { return j == j0 || (j + 1) * BN > front || j * BN <= lo1; };
     constexpr bool AHEAD = D == 256 && sizeof(T) == 2;
     constexpr int VB = AHEAD ? 4 : 1, NB = NC / VB;
     auto in_order = [] {

@@ -283,8 +283,9 @@ def paged_tree_attention(q, k_cache, v_cache, page_table, seq_lens, visible, *, 
     or any others: bit j % 64 of word j // 64 says that the token sees new token j of
     its sequence (new tokens that have no bit are seen by none; bits past a sequence's
     new tokens mean nothing).  window: at least 64 words; the last ``window`` of the
-    tokens that a token sees.  A token that sees nothing gets zeros (lse -inf).
-    Returns as ``paged_attention`` does.
+    tokens that a token sees.  A token that sees nothing gets zeros (lse -inf).  Tokens
+    that the page table has no place for (seq_lens past it) are seen by none; the others
+    keep their positions.  Returns as ``paged_attention`` does.
     """
     cs, qs, ct = k_cache.shape, q.shape, k_cache.dtype
     kcs, vcs, qt = k_cache.stride(), v_cache.stride(), q.stride()

@@ -518,7 +518,8 @@ int dn_paged_slots(const dn_paged_slots_args* a, void* stream);
  * of its sequence in front of the new ones, and of the new ones those whose bit is set
  * in its row of visible (N, words) (dn_paged_slots, or any others; none past 64 words).
  * With `window`, at least 64 words, the last `window` of those.  A token that sees
- * nothing gets zeros and lse -inf. */
+ * nothing gets zeros and lse -inf.  Tokens that the page table has no place for (seq_lens
+ * past it) are seen by none; the others keep their positions. */
 size_t dn_paged_tree_attention_workspace_size(const dn_paged_attention_args* a, int32_t words);
 int dn_paged_tree_attention(const dn_paged_attention_args* a, const uint64_t* visible, int32_t words, void* workspace,
                             size_t workspace_bytes, void* stream);

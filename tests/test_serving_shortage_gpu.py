@@ -39,10 +39,11 @@ def _whole_rows(srv, mine, layer):
 
 
 @pytest.mark.parametrize("graph", [False, True])
-def test_a_pool_that_runs_short(dev, graph):
+@pytest.mark.parametrize("pages,most", [(9, 40), (40, 2)])
+def test_a_pool_or_table_that_runs_short(dev, graph, pages, most):
     """Every path is accepted, short or not: a sequence keeps what it has pages for, and
     nobody's tokens change.  Outputs as in whole rows, 2e-5 (two orders of the same sums)."""
-    B, T, steps, most, pages = 4, 12, 14, 40, 9
+    B, T, steps = 4, 12, 14
     srv = _Held(dev, B, pages=pages, most=most)
     H = srv.Hq + 2 * srv.Hkv
     bufs = dict(x=torch.zeros(B * T, srv.layers, H, srv.D, device=dev), cu=torch.zeros(B + 1, dtype=torch.int32, device=dev),

@@ -106,3 +106,31 @@ def test_scores_that_grow_within_a_piece(dev, dt, D, n):
         q[..., 0] = 1.0
         k[:, 0] = torch.linspace(0.0, grow, length).to(A.DT[dt])
         _run(dev, dt, q, k, v, 4, 41, [length, 1000], _masks("tree", n), scale=1.0, tag=f"{grow}")
+
+
+@pytest.mark.parametrize("dt,D,page", [("bf16", 128, 16), ("f16", 64, 4), ("f32", 128, 16), ("f32", 256, 4), ("bf16", 256, 64)])
+@pytest.mark.parametrize("n,G", [(7, 2), (20, 4), (64, 6)])
+def test_lengths_past_the_page_table(dev, dt, D, page, n, G):
+    """Drafts that the page table has no place for are seen by none, and the others keep
+    their places; where the window lies past the table a token sees nothing."""
+    room = 320
+    k, v, q = _rows(10, room, D, dt=dt), _rows(11, room, D, dt=dt), _rows(12, n, G, D, dt=dt)
+    kc, vc, pt = _text(dev, k, v, page)
+    lens = [room + x for x in (-3, 0, 1, n // 2, n - 1, n, n + 1, 500, 2 ** 31 - 1 - room)]
+    seen = _masks("tree", n)
+    words = S.words([seen], 1).repeat(len(lens), 1).to(dev)
+    qd = q[None, :, None].expand(len(lens), n, HEADS, G, D).reshape(len(lens), n, HEADS * G, D).to(dev)
+    for window in (None, 64, 200, 400):
+        out, lse = paged_tree_attention(qd, kc, vc, pt.expand(len(lens), -1), torch.tensor(lens, dtype=torch.int32, device=dev), words,
+                                        window=window, return_lse=True)
+        out, lse = out.view(-1, n, HEADS, G, D).double(), lse.view(-1, n, HEADS, G).double()
+        for b, length in enumerate(lens):
+            far = min(length, room + 600)   # (from there on all is context, or all behind the table)
+            vis = S.tree_visible(seen, far, window)[:, :room]
+            for g in range(G):
+                ref, l, tol = A.attend(q[:, g].double(), k[:vis.shape[1]].double(), v[:vis.shape[1]].double(), vis, 1.0 / math.sqrt(D), dt)
+                at = f"window {window} length {length} head {g}"
+                _same(out[b, :, :, g].transpose(0, 1), ref, tol, at)
+                got = lse[b, :, :, g].transpose(0, 1)
+                assert torch.equal(got.isneginf().cpu(), l.isneginf().expand_as(got)), at
+                _same(torch.where(got.isneginf(), 0.0, got), torch.where(l.isneginf(), 0.0, l), torch.full_like(l, 1e-4), at + " lse")
