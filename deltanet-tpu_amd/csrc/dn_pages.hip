@@ -6,6 +6,8 @@
 // the stores in long queues of prompts: 5.6 million tokens' positions and slots (67 MB)
 // 15.4 us.  Accepted tokens of 64 sequences in 12 layers (13 MB) move in 6.7 us, one
 // user's in 4.9.
+#include <atomic>
+
 #include "dn_common.h"
 #include "dn_host.h"
 
@@ -60,19 +62,28 @@ struct RP {
   const int32_t* lens;
   int64_t stride;
   int capacity, max_pages, B, shift;
+  uint32_t tag;   // of this launch; not 0
 };
+constexpr int kTagShift = 9;   // (256 blocks at most)
 
 // Every block adds up all sequences' needs itself and moves an even share of the
 // pages: a page that is taken is read off the stack, or, if it lies among those given
 // back in this call, from the row of the sequence that gives it, which nothing
 // overwrites.  Lengths and counts are written by the block that comes to its end last,
 // when all others have read them; it reads nothing that they wrote, so that the count
-// of those that ended needs no fence.
+// of those that ended needs no fence.  The count lies in the pool's second word under
+// the launch's tag, so that whatever else that word holds counts as none.
 template <int NT> __global__ __launch_bounds__(NT) void k_reserve(const RP p) {
   extern __shared__ int lds[];   // [2][B]: pages taken, given back by the sequences in front
   int *taken = lds, *given = lds + p.B;
   __shared__ int waves[NT / 64], s_last;
   const int count = min(max(p.pool[0], 0), p.capacity);
+  uint32_t* ended = reinterpret_cast<uint32_t*>(&p.pool[1]);
+  if (gridDim.x > 1 && threadIdx.x == 0) {   // (where it fails, another block has put the tag there)
+    uint32_t was = __hip_atomic_load(ended, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (was >> kTagShift != p.tag)
+      __hip_atomic_compare_exchange_strong(ended, &was, p.tag << kTagShift, __ATOMIC_RELAXED, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
   auto needs = [&](int b, int& h, int& need) {
     h = min(max(p.held[b], 0), p.max_pages);
     const int n = max(p.lens[b], 0);
@@ -116,24 +127,26 @@ template <int NT> __global__ __launch_bounds__(NT) void k_reserve(const RP p) {
   for (int i = 0; i < NT / 64; ++i) A = max(A, waves[i]);
   const int left = full - A;
   // page number x of those given back, in the order of the sequences and their pages
+  // (bounded, as below, for lengths that something changes meanwhile)
   auto given_page = [&](int x) {
     const int b = last_at_most(given, p.B, x);
     int h, need;
     needs(b, h, need);
-    return p.table[b * p.stride + need + (x - given[b])];
+    return p.table[b * p.stride + min(need + (x - given[b]), p.max_pages - 1)];
   };
   const int me = blockIdx.x * NT + threadIdx.x, step = gridDim.x * NT;
 #pragma unroll 2
   for (int k = me; k < A; k += step) {
     const int b = last_at_most(taken, p.B, k), at = full - 1 - k;
     const int col = min(max(p.held[b], 0), p.max_pages) + (k - taken[b]);
-    p.table[b * p.stride + col] = at < count ? p.pool[2 + at] : given_page(F - 1 - (at - count));
+    p.table[b * p.stride + min(col, p.max_pages - 1)] = at < count ? p.pool[2 + at] : given_page(F - 1 - (at - count));
   }
 #pragma unroll 2
   for (int k = me; k < min(left, p.capacity) - count; k += step) p.pool[2 + count + k] = given_page(F - 1 - k);
   __syncthreads();
   if (gridDim.x > 1) {
-    if (threadIdx.x == 0) s_last = __hip_atomic_fetch_add(&p.pool[1], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
+    if (threadIdx.x == 0)
+      s_last = __hip_atomic_fetch_add(ended, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (p.tag << kTagShift) + gridDim.x - 1;
     __syncthreads();
     if (!s_last) return;
   }
@@ -381,10 +394,15 @@ extern "C" int dn_paged_reserve(const dn_paged_reserve_args* a, void* stream) {
   if (a->B == 0) return DN_OK;
   if (!a->pool || !a->page_table || !a->held || !a->lens || !a->short_of) return bad("missing tensor pointer");
   if (a->B > 1 && a->page_table_stride < a->max_pages) return bad("the rows of the page table overlap");
-  const RP p{a->pool, a->page_table, a->held, a->short_of, a->lens, a->page_table_stride, a->capacity, a->max_pages, a->B, shift_of(a->page_size)};
-  // blocks of 16 waves hide the searches of many pages (350000 of 2048 sequences: 10.6 us,
-  // blocks of 4 waves 15.3), those of 4 start sooner where there are few (a token or a tree
-  // of 64 sequences: 2.8 and 4.5 us, 5.0 for the latter by 16 waves)
+  static std::atomic<uint32_t> launches{0};
+  const uint32_t tag = launches.fetch_add(1, std::memory_order_relaxed) % ((1u << (32 - kTagShift)) - 1) + 1;
+  const RP p{a->pool, a->page_table, a->held, a->short_of, a->lens, a->page_table_stride, a->capacity, a->max_pages, a->B, shift_of(a->page_size), tag};
+  // Blocks of 16 waves hide the searches of many pages, those of 4 start sooner where there
+  // are few.  us of a launch among others, 4 waves / 16, sequences x columns: a page or three
+  // for each of 64 x 64 4.2 / 4.5, 64 x 512 4.8 / 5.5, 256 x 64 5.0 / 5.8, 256 x 512 5.1 / 5.7,
+  // 1024 x 64 6.6 / 6.5, 2048 x 64 9.3 / 7.7, 2048 x 256 11.1 / 8.2; every page of 64 x 64
+  // 9.8 / 6.7, 256 x 64 11.3 / 9.2, 64 x 1024 10.9 / 9.0, 256 x 512 12.3 / 9.7, 2048 x 171 16.8 /
+  // 11.6.  Servers take a page or three at a time.
   const int64_t entries = (int64_t)a->B * a->max_pages;
   const size_t lds = 2 * a->B * sizeof(int);
   if (entries <= 65536) hipLaunchKernelGGL(k_reserve<256>, dim3((unsigned)((entries + 2047) / 2048)), dim3(256), lds, (hipStream_t)stream, p);

@@ -467,7 +467,7 @@ int dn_qkv_append(const dn_qkv_append_args* a, void* stream);
 
 /* Pages taken from a pool and given back, so that sequence b has as many as its
  * lens[b] tokens need.  pool (2 + capacity) int32: the number of free pages, a word
- * that is 0 between calls, the free pages (a stack).  held (B) int32: the pages that
+ * that the kernels use (0 between calls), the free pages (a stack).  held (B) int32: the pages that
  * each sequence has, the first of its row of page_table; both are updated.  Pages
  * that sequences no longer need go onto the stack first, the last page of the last
  * sequence first of all; then sequences take from its top, in their order.  From the
