@@ -63,16 +63,20 @@ template <int P> __device__ __forceinline__ float sum_lanes(float x) {
   return x;
 }
 
-// 1 / sqrt(a): the instruction's result (one step off at most) and a Newton step.  The
-// instruction takes numbers below the normal ones for 0 (eps of 0, heads near 2^-64).
+// 1 / sqrt(a): the instruction's result (one step off at most) and a Newton step.
 __device__ __forceinline__ float rsqrt32(float a) {
-  const bool tiny = a < 0x1p-96f;
-  if (tiny) a *= 0x1p64f;
   const float y = __builtin_amdgcn_rsqf(a);
-  float z = __builtin_fmaf(y * 0.5f, __builtin_fmaf(-a * y, y, 1.f), y);
-  if (!__builtin_isfinite(z)) z = y;   // (0 and infinity)
-  return tiny ? z * 0x1p32f : z;
+  const float z = __builtin_fmaf(y * 0.5f, __builtin_fmaf(-a * y, y, 1.f), y);
+  return __builtin_isfinite(z) ? z : y;   // (0 and infinity)
 }
+
+// A head whose mean square (with eps) a is below 2^-96, where squares vanish (channels
+// below 2^-48, eps as good as 0), or past the largest number (channels from 2^59 on) is
+// taken times a power of two by which they are all well inside, and eps times its square:
+// x r is the same.
+constexpr float kUp = 0x1p100f, kDown = 0x1p-70f;
+__device__ __forceinline__ bool far_off(float a) { return a < 0x1p-96f || a == INFINITY; }
+__device__ __forceinline__ float scale_of(float a) { return a < 1.f ? kUp : kDown; }
 
 __device__ __forceinline__ int64_t pos_of(const HP& p, int b, int l) {
   const int64_t i = b * p.ps[0] + l * p.ps[1];
@@ -253,7 +257,20 @@ __global__ __launch_bounds__(256) void k_heads(const HP p) {
       float z = 0.f;
 #pragma unroll
       for (int e = 0; e < W; ++e) z += u[h][e] * u[h][e] + v[h][e] * v[h][e];
-      const float r = rsqrt32(sum_lanes<P>(z) * over + p.eps);
+      const float a = sum_lanes<P>(z) * over + p.eps;
+      float r = rsqrt32(a);
+      if (__builtin_expect(far_off(a), 0)) {
+        const float s = scale_of(a);
+        z = 0.f;
+#pragma unroll
+        for (int e = 0; e < W; ++e) z += (u[h][e] * s) * (u[h][e] * s) + (v[h][e] * s) * (v[h][e] * s);
+        const float rs = rsqrt32(sum_lanes<P>(z) * over + p.eps * s * s);
+        // the factor that keeps small channels' bits first
+        const float first = s > 1.f ? s : rs;
+        r = s > 1.f ? rs : s;
+#pragma unroll
+        for (int e = 0; e < W; ++e) u[h][e] *= first, v[h][e] *= first;
+      }
 #pragma unroll
       for (int e = 0; e < W; ++e) {
         u[h][e] = u[h][e] * r * wa[e];
@@ -288,17 +305,28 @@ __global__ __launch_bounds__(256) void k_heads_any(const HP p) {
     const Dst d = dst_of<T, PAGED>(p, side, t, pos);
     const int64_t at = d.at + h * d.head;
     const bool norm = side < 2 && p.w[0];
-    float r = 1.f;
+    float r = 1.f, first = 1.f;
     if (norm) {
-      float z = 0.f;
-      for (int c = lane_id(); c < p.D; c += 64) z += (float)s[c] * (float)s[c];
-      r = rsqrt32(sum_lanes<64>(z) * (1.f / p.D) + p.eps);
+      float by = 1.f;
+      auto mean = [&] {
+        float z = 0.f;
+        for (int c = lane_id(); c < p.D; c += 64) z += ((float)s[c] * by) * ((float)s[c] * by);
+        return sum_lanes<64>(z) * (1.f / p.D) + p.eps * by * by;
+      };
+      const float a = mean();
+      r = rsqrt32(a);
+      if (far_off(a)) {
+        by = scale_of(a);
+        const float rs = rsqrt32(mean());
+        first = by > 1.f ? by : rs;
+        r = by > 1.f ? rs : by;
+      }
     }
     if (!d.store) continue;
     const bool zero = PAGED && side == 0 && d.none;
     auto value = [&](int c) {
       const float x = (float)s[c];
-      return norm ? x * r * (p.offset + ld_f(p.w[side], c, p.wdt)) : x;
+      return norm ? x * first * r * (p.offset + ld_f(p.w[side], c, p.wdt)) : x;
     };
     for (int i = lane_id(); i < p.D - (p.R >> 1); i += 64) {
       int ca, cb;
@@ -370,14 +398,28 @@ __global__ __launch_bounds__(256) void k_heads_grad(const HP p, const GP g) {
         xx += u[h][e] * u[h][e] + v[h][e] * v[h][e];
         hx += gu[h][e] * wa[e] * u[h][e] + gv[h][e] * wb[e] * v[h][e];
       }
-      const float r = rsqrt32(sum_lanes<P>(xx) * over + p.eps), k = sum_lanes<P>(hx) * over * r * r;
+      const float a = sum_lanes<P>(xx) * over + p.eps;
+      float r = rsqrt32(a), by = 1.f;
+      if (__builtin_expect(far_off(a), 0)) {   // x r, and with it dw, is as it was; dx has r once
+        by = scale_of(a);
+        xx = hx = 0.f;
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+          u[h][e] *= by;
+          v[h][e] *= by;
+          xx += u[h][e] * u[h][e] + v[h][e] * v[h][e];
+          hx += gu[h][e] * wa[e] * u[h][e] + gv[h][e] * wb[e] * v[h][e];
+        }
+        r = rsqrt32(sum_lanes<P>(xx) * over + p.eps * by * by);
+      }
+      const float k = sum_lanes<P>(hx) * over * r * r;
       if (!own || h0 + h >= H) continue;
 #pragma unroll
       for (int e = 0; e < W; ++e) {
         da[e] += gu[h][e] * u[h][e] * r;
         db[e] += gv[h][e] * v[h][e] * r;
-        gu[h][e] = r * (gu[h][e] * wa[e] - u[h][e] * k);
-        gv[h][e] = r * (gv[h][e] * wb[e] - v[h][e] * k);
+        gu[h][e] = r * (gu[h][e] * wa[e] - u[h][e] * k) * by;
+        gv[h][e] = r * (gv[h][e] * wb[e] - v[h][e] * k) * by;
       }
       T* d = (T*)g.dx[side] + (t * H + h0 + h) * p.D;
       store<W, true>(d + it.a, gu[h]);
@@ -422,15 +464,15 @@ __global__ __launch_bounds__(64) void k_heads_grad_any(const HP p, const GP g) {
     T* d = (T*)g.dx[side] + row * p.D;
     const int64_t pos = p.R ? pos_of(p, b, l) : 0;
     const bool in = pos >= 0 && pos < p.rows;
-    float r = 1.f, k = 0.f, xx = 0.f, hx = 0.f;
+    float r = 1.f, k = 0.f, xx = 0.f, hx = 0.f, by = 1.f;
     for (int pass = 0; pass < 2; ++pass) {
       for (int i = lane_id(); i < p.D - (p.R >> 1); i += 64) {
         int ca, cb;
         pair_of(i, p.R, p.inter, ca, cb);
-        const float x = (float)s[ca], wx = p.offset + ld_f(p.w[side], ca, p.wdt);
+        const float x = (float)s[ca] * by, wx = p.offset + ld_f(p.w[side], ca, p.wdt);
         float gx = (float)z[ca], y = 0.f, wy = 0.f, gy = 0.f;
         if (cb >= 0) {
-          y = (float)s[cb];
+          y = (float)s[cb] * by;
           wy = p.offset + ld_f(p.w[side], cb, p.wdt);
           const float c = in ? p.table[pos * p.R + i] : __builtin_nanf(""), sn = in ? p.table[pos * p.R + (p.R >> 1) + i] : __builtin_nanf("");
           const float a = gx, e = (float)z[cb];
@@ -441,16 +483,23 @@ __global__ __launch_bounds__(64) void k_heads_grad_any(const HP p, const GP g) {
           xx += x * x + y * y;
           hx += gx * wx * x + gy * wy * y;
         } else {
-          d[ca] = (T)(r * (gx * wx - x * k));
+          d[ca] = (T)(r * (gx * wx - x * k) * by);
           part[ca] += gx * x * r;
           if (cb >= 0) {
-            d[cb] = (T)(r * (gy * wy - y * k));
+            d[cb] = (T)(r * (gy * wy - y * k) * by);
             part[cb] += gy * y * r;
           }
         }
       }
       if (pass == 0) {
-        r = rsqrt32(sum_lanes<64>(xx) * over + p.eps);
+        const float a = sum_lanes<64>(xx) * over + p.eps * by * by;
+        if (by == 1.f && far_off(a)) {   // once more
+          by = scale_of(a);
+          xx = hx = 0.f;
+          pass = -1;
+          continue;
+        }
+        r = rsqrt32(a);
         k = sum_lanes<64>(hx) * over * r * r;
       }
     }
