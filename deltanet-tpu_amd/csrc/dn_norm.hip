@@ -36,7 +36,7 @@ struct HP {
 // what the gradient has besides: dz in, dx out, partial sums of dw
 struct GP {
   const void* dz[2];
-  void* dx[2];
+  void* dx[2];               // NULL: not wanted
   float* part;               // (blocks, D), those of q in front
   int64_t zs[2][3];
 };
@@ -421,6 +421,7 @@ __global__ __launch_bounds__(256) void k_heads_grad(const HP p, const GP g) {
         gu[h][e] = r * (gu[h][e] * wa[e] - u[h][e] * k) * by;
         gv[h][e] = r * (gv[h][e] * wb[e] - v[h][e] * k) * by;
       }
+      if (g.dx[side] == nullptr) continue;
       T* d = (T*)g.dx[side] + (t * H + h0 + h) * p.D;
       store<W, true>(d + it.a, gu[h]);
       store<W, true>(d + it.b, gv[h]);
@@ -483,10 +484,10 @@ __global__ __launch_bounds__(64) void k_heads_grad_any(const HP p, const GP g) {
           xx += x * x + y * y;
           hx += gx * wx * x + gy * wy * y;
         } else {
-          d[ca] = (T)(r * (gx * wx - x * k) * by);
+          if (g.dx[side]) d[ca] = (T)(r * (gx * wx - x * k) * by);
           part[ca] += gx * x * r;
           if (cb >= 0) {
-            d[cb] = (T)(r * (gy * wy - y * k) * by);
+            if (g.dx[side]) d[cb] = (T)(r * (gy * wy - y * k) * by);
             part[cb] += gy * y * r;
           }
         }
@@ -673,7 +674,7 @@ extern "C" int dn_norm_rotary_bwd(const dn_norm_rotary_args* a, const dn_norm_ro
   if (d == nullptr) return bad("null args");
   if (const int rc = norm_params(a, p)) return rc;
   if (p.N == 0 || p.H[0] + p.H[1] == 0) return DN_OK;
-  if ((p.H[0] && (!d->d_q || !d->dq)) || (p.H[1] && (!d->d_k || !d->dk))) return bad("missing tensor pointer");
+  if ((p.H[0] && !d->d_q) || (p.H[1] && !d->d_k)) return bad("missing tensor pointer");
   if (!workspace || workspace_bytes < grad_bytes(p, a->dtype)) return set_error(DN_E_WORKSPACE, "workspace missing or too small");
   GP g{};
   g.dz[0] = d->d_q; g.dz[1] = d->d_k; g.dx[0] = d->dq; g.dx[1] = d->dk;

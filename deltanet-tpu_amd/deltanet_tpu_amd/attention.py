@@ -303,25 +303,32 @@ class _NormRotaryFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, d_q, d_k=None):
         q, k, qw, kw, pos, table = ctx.saved_tensors
+        want_q, want_k, want_qw, want_kw = ctx.needs_input_grad[:4]
         gq = gk = gqw = gkw = None
         q0 = q1 = q2 = k0 = k1 = k2 = 0
-        # a side whose result nobody used has no gradient
-        if d_q is None:
-            if d_k is None:
-                return None, None, None, None, None, None, None
-            q = qw = None
+        # a side whose result nobody used, or whose gradients nobody wants, has none
+        if d_q is None or not (want_q or want_qw):
+            q = qw = d_q = None
         else:
             if d_q.stride(-1) != 1:
                 d_q = _dense_channels(d_q)
-            gq, gqw = torch.empty_like(q, memory_format=torch.contiguous_format), torch.empty_like(qw)
+            if want_q:
+                gq = torch.empty_like(q, memory_format=torch.contiguous_format)
+            if want_qw:
+                gqw = torch.empty_like(qw)
             q0, q1, q2, _ = d_q.stride()
-        if d_k is None:
-            k = kw = None
+        if d_k is None or not (want_k or want_kw):
+            k = kw = d_k = None
         else:
             if d_k.stride(-1) != 1:
                 d_k = _dense_channels(d_k)
-            gk, gkw = torch.empty_like(k, memory_format=torch.contiguous_format), torch.empty_like(kw)
+            if want_k:
+                gk = torch.empty_like(k, memory_format=torch.contiguous_format)
+            if want_kw:
+                gkw = torch.empty_like(kw)
             k0, k1, k2, _ = d_k.stride()
+        if q is None and k is None:
+            return None, None, None, None, None, None, None
         block = _norm_block(q, k, qw, kw, None, None, pos, table, ctx.meta)
         need = (_calls.get("dn_norm_rotary_bwd_workspace_size") or _lib.packed_call("dn_norm_rotary_bwd_workspace_size"))(block)
         if need:
@@ -362,9 +369,11 @@ def norm_rotary(q, k, q_weight, k_weight, positions=None, table=None, *, eps: fl
     weights kept as differences from 1.  positions, table, interleaved: as in
     ``apply_rotary``; neither positions nor table: no rotation.  Statistics and
     products in float32, one rounding at the end.  Differentiable in q, k and the
-    weights (backwards and once; tangents are refused); the weights' gradients are
-    summed in 32 bits or more and are the same bits every time.  Returns (q', k') with k' None
-    if k is None; the results are contiguous.
+    weights (backwards and once; tangents are refused), of which those that want no
+    gradient cost none; the weights' gradients are summed in float32 over the tokens of a
+    thread and in 64 bits over threads and blocks (rounded to float32 in between), and are
+    the same bits every time.  Returns (q', k') with k' None if k is None; the results are
+    contiguous.
     """
     qs = q.shape
     if not (3 <= len(qs) <= 4 and q.dtype in _DT and qs[-1] > 0 and type(eps) is float and 0.0 <= eps <= 3e38 and type(weight_offset) is float

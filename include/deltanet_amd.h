@@ -416,9 +416,10 @@ typedef struct dn_norm_rotary_args {
 
 int dn_norm_rotary(const dn_norm_rotary_args* a, void* stream);
 
-/* Gradients of sum(q_out * d_q) + sum(k_out * d_k): dq and dk dense in `dtype`,
- * the weights' (NULL if not wanted) in weight_dtype, summed in float32 within a block
- * and in 64 bits over them, in an order that depends on the sizes alone. */
+/* Gradients of sum(q_out * d_q) + sum(k_out * d_k), each NULL if not wanted: dq and dk
+ * dense in `dtype`, the weights' in weight_dtype, in an order of sums that depends on the
+ * sizes alone: float32 over the tokens of a thread, 64 bits over the threads of a block
+ * (rounded to float32) and over the blocks. */
 typedef struct dn_norm_rotary_grads {
   const void* d_q;              /* (B,L,Hq,D), strides d_q_strides               */
   const void* d_k;
