@@ -374,17 +374,13 @@ template <bool TREE> struct PlanOf {
   }
   // the task of new token i's row for query head hq, and the row
   __device__ __forceinline__ bool of_row(int i, int hq, Task& t, int& row) const {
+    static_assert(!TREE, "parts of trees are joined by tasks");
     int per;
     if (!find([&](const Span& s, int) { return s.c0 + s.n > i && s.c0 <= i; }, t, per)) return false;
     t.h = over_g(p, hq);
     row = (i - t.s.c0) * p.G + hq - t.h * p.G;
     t.m = row / BM;
     t.first += t.h * per;
-    if constexpr (TREE) {
-      t.units = tile_units(t, 0);
-      t.first += t.m * t.units;
-      return true;
-    }
     for (int m = 0; m < t.m; ++m) t.first += tile_units(t, m);
     t.units = tile_units(t, t.m);
     return true;

@@ -23,7 +23,7 @@ namespace {
 
 struct HP {
   int N, L, H[3], D, R, rows, inter, pos64, wdt, cdt, pages, shift;   // H: query, key and value heads
-  float eps, offset, sign;
+  float eps, offset;
   const void* x[3];          // q, k, v
   const void* w[2];          // NULL: no norm
   void* out[3];              // q', and k' or the caches
