@@ -56,13 +56,14 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_few(const AF p) {
     if (!plan.of_unit(u, t)) break;
     const int rows = t.s.n * p.G, row0 = t.m * BM, row1 = min(row0 + BM, rows);
     // the keys that all rows see end with p0, those that any sees with p1
-    const int off = t.s.off, p0 = TREE ? min(off, t.s.len) - 1 : off + over_g(p, row0), p1 = TREE ? t.s.len - 1 : off + over_g(p, row1 - 1);
+    const int first = t.s.len - t.s.n, len = TREE ? min(t.s.len, table_end(p)) : t.s.len, off = TREE ? min(first, len) : first;
+    const int p0 = TREE ? off - 1 : off + over_g(p, row0), p1 = TREE ? len - 1 : off + over_g(p, row1 - 1);
     int k0, k1;
     units_of<TREE>(p, t.s, row0, row1, kUnit, k0, k1);
     const int skip = u - t.first, take = min(t.units - skip, uend - u);
     const int j0 = k0 + skip, j1 = j0 + take;   // units of this piece
     const int last = max(p1, 0);
-    const int lo1 = first_key(p, TREE ? off + t.s.n - 1 : p1);   // (none later, of any row)
+    const int lo1 = first_key(p, TREE ? t.s.len - 1 : p1);   // (none later, of any row)
 
     F qf[NQ][NS];
     int pos[NQ], low[NQ];
@@ -77,9 +78,9 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_few(const AF p) {
 #pragma unroll
         for (int c = 0; c < NS; ++c) qf[i][c] = minus8<T>(qf[i][c]);
       pos[i] = TREE ? t.s.c0 + tk : off + tk;   // trees: the token, whose words say what it sees
-      low[i] = TREE ? tree_low(p, tree_words(p, pos[i]), off, t.s.n) : first_key(p, pos[i]);
+      low[i] = TREE ? tree_low(p, tree_words(p, pos[i]), first, t.s.n) : first_key(p, pos[i]);
     }
-    auto bits_of = [&](int i, int key0) { return tree_bits(p, tree_words(p, pos[i]), off, t.s.len, low[i], key0); };
+    auto bits_of = [&](int i, int key0) { return tree_bits(p, tree_words(p, pos[i]), off, len, low[i], key0); };
 
 #pragma unroll
     for (int i = 0; i < NQ; ++i)

@@ -135,9 +135,9 @@ struct Rest {
 };
 
 // A sequence of a paged call: its first new token among all, new tokens, tokens in all
-// (of which the page table has a place); off: position of the first new one, in trees
-// whether or not that is past the page table.
-struct Span { int c0, n, len, off; };
+// (of trees, those past the page table too).
+struct Span { int c0, n, len; };
+__device__ __forceinline__ int table_end(const AF& p) { return p.max_pages << p.shift; }
 template <bool TREE> __device__ __forceinline__ Span span_of(const AF& p, int b) {
   Span s;
   s.c0 = b * p.T;
@@ -146,9 +146,7 @@ template <bool TREE> __device__ __forceinline__ Span span_of(const AF& p, int b)
     s.c0 = min(max(p.cu[b], 0), p.N);
     s.n = min(max(p.cu[b + 1], s.c0), p.N) - s.c0;
   }
-  const int len = max(p.lens[b], 0);
-  s.len = min(len, p.max_pages << p.shift);
-  s.off = (TREE ? min(len, kMostIndex) : s.len) - s.n;
+  s.len = min(max(p.lens[b], 0), TREE ? kMostIndex : table_end(p));
   return s;
 }
 
@@ -184,7 +182,7 @@ template <int D, class T, bool PAGED> __device__ __forceinline__ bool has_large(
 
 // Drafted trees.  A new token sees the keys in front of its sequence's new tokens, the
 // window aside, and of those the ones whose bit is set in its words: key `off` is new
-// token 0.  Tokens that the page table has no place for (from s.len on) are seen by none.
+// token 0.  Tokens that the page table has no place for are seen by none.
 // low: the first key that a window of all that it sees leaves (at least 64
 // words of it, so that no new token falls out).
 __device__ __forceinline__ const uint64_t* tree_words(const AF& p, int token) { return p.vis + (int64_t)token * p.words; }
@@ -203,9 +201,10 @@ __device__ __forceinline__ int tree_low(const AF& p, const uint64_t* w, int off,
   return p.window ? max(off + tree_count(p, w, off, n) - p.window, 0) : 0;
 }
 __device__ __forceinline__ bool tree_empty(const AF& p, int token, const Span& s) {
-  if (s.off > 0 && s.off <= s.len) return false;   // (a window is wider than its words)
+  const int off = s.len - s.n, len = min(s.len, table_end(p));
+  if (off > 0 && off <= len) return false;   // (a window is wider than its words)
   const uint64_t* w = tree_words(p, token);
-  return tree_low(p, w, s.off, s.n) >= min(s.off, s.len) && (s.len <= s.off || tree_count(p, w, s.off, min(s.n, s.len - s.off)) == 0);
+  return tree_low(p, w, off, s.n) >= min(off, len) && (len <= off || tree_count(p, w, off, len - off) == 0);
 }
 // Which of the 32 keys from key0 on it sees.
 __device__ __forceinline__ uint32_t tree_bits(const AF& p, const uint64_t* w, int off, int len, int low, int key0) {
@@ -230,7 +229,8 @@ __device__ __forceinline__ uint32_t tree_bits(const AF& p, const uint64_t* w, in
 // Keys [lo, hi) that rows [row0, row1) of a sequence see between them, in units.
 template <bool TREE = false>
 __device__ __forceinline__ void units_of(const AF& p, const Span& s, int row0, int row1, int unit, int& u0, int& u1) {
-  const int off = s.off, p0 = TREE ? off - 1 : off + over_g(p, row0), p1 = TREE ? s.len - 1 : off + over_g(p, row1 - 1);
+  const int off = s.len - s.n, p0 = TREE ? off - 1 : off + over_g(p, row0);
+  const int p1 = TREE ? min(s.len, table_end(p)) - 1 : off + over_g(p, row1 - 1);
   u0 = first_key(p, p0) / unit;
   u1 = p1 < 0 ? u0 : p1 / unit + 1;
   u1 = max(u1, u0 + 1);   // a tile without keys is work too: it writes zeros
@@ -276,7 +276,7 @@ template <bool TREE> struct PlanOf {
   }
   __device__ __forceinline__ void load(int b0, Span& s, int& mine) const {
     const int b = b0 + lane_id();
-    s = {0, 0, 0, 0};
+    s = {0, 0, 0};
     mine = 0;
     if (b >= p.B) return;
     s = span_of<TREE>(p, b);
@@ -312,7 +312,6 @@ template <bool TREE> struct PlanOf {
         t.s.c0 = __builtin_amdgcn_readfirstlane(__shfl(s.c0, w));
         t.s.n = __builtin_amdgcn_readfirstlane(__shfl(s.n, w));
         t.s.len = __builtin_amdgcn_readfirstlane(__shfl(s.len, w));
-        t.s.off = TREE ? __builtin_amdgcn_readfirstlane(__shfl(s.off, w)) : t.s.len - t.s.n;
         per = __builtin_amdgcn_readfirstlane(__shfl(mine, w)) / p.Hkv;
         t.first = before + __builtin_amdgcn_readfirstlane(__shfl(sum - mine, w));
         return true;
@@ -358,7 +357,7 @@ template <bool TREE> struct PlanOf {
         const int w = __builtin_ctzll(in);
         auto of = [&](int y) { return __builtin_amdgcn_readfirstlane(__shfl(y, w)); };
         t.b = b0 + w;
-        t.s = {of(s.c0), of(s.n), of(s.len), of(s.off)};
+        t.s = {of(s.c0), of(s.n), of(s.len)};
         const int n = of(tasks), tiles = n / p.Hkv;
         x -= before + of(ts) - n;
         t.units = of(mine) / n;

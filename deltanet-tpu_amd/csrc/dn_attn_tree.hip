@@ -59,13 +59,15 @@ __global__ __launch_bounds__(64 * NW, 2 * ST * BN * D * (int)sizeof(T) <= 80 * 1
   while (u < uend) {
     Task t;
     if (!plan.of_unit(u, t)) break;
-    const int rows = t.s.n * p.G, row0 = t.m * BM, off = t.s.off, last = max(t.s.len - 1, 0);
-    const int front = min(off, t.s.len);   // keys that every row sees, but for the window
+    const int rows = t.s.n * p.G, row0 = t.m * BM;
+    // off: keys that every row sees, but for the window; the new tokens are behind them, if
+    // the page table has a place for any
+    const int first = t.s.len - t.s.n, len = min(t.s.len, table_end(p)), off = min(first, len), last = max(len - 1, 0);
     int k0, k1;
     units_of<true>(p, t.s, 0, 1, BN, k0, k1);
     const int skip = u - t.first, take = min(t.units - skip, uend - u);
     const int j0 = k0 + skip, j1 = j0 + take;
-    const int lo1 = p.window ? max(off + min(t.s.n, 64 * p.words) - p.window, 0) : 0;   // no row's first key is later
+    const int lo1 = p.window ? max(first + min(t.s.n, 64 * p.words) - p.window, 0) : 0;   // no row's first key is later
 
     F qf[NQ][NS];
     int token[NQ], low[NQ];
@@ -80,7 +82,7 @@ __global__ __launch_bounds__(64 * NW, 2 * ST * BN * D * (int)sizeof(T) <= 80 * 1
 #pragma unroll
         for (int c = 0; c < NS; ++c) qf[i][c] = minus8<T>(qf[i][c]);
       token[i] = t.s.c0 + tk;
-      low[i] = tree_low(p, tree_words(p, token[i]), off, t.s.n);
+      low[i] = tree_low(p, tree_words(p, token[i]), first, t.s.n);
     }
     Rows<T, true> vr;   // (for the values that are not finite)
     vr.base = (const T*)p.v + t.h * p.vs[2];
@@ -141,8 +143,8 @@ __global__ __launch_bounds__(64 * NW, 2 * ST * BN * D * (int)sizeof(T) <= 80 * 1
     // with the values left the range all the same (values from 2^68 on) goes that way too.
     // float16 has no such range, its rows are raised on the way.  (The tile that begins with the last of the
     // windows' first keys is the first of which that row sees any: it is LEARN too.)
-    auto hides = [&](int key0) { return key0 + 32 > front || key0 < lo1; };   // some row must not see some of 32 keys
-    auto learns = [&](int j) { return j == j0 || (j + 1) * BN > front || j * BN <= lo1; };
+    auto hides = [&](int key0) { return key0 + 32 > off || key0 < lo1; };   // some row must not see some of 32 keys
+    auto learns = [&](int j) { return j == j0 || (j + 1) * BN > off || j * BN <= lo1; };
     constexpr bool AHEAD = D == 256 && sizeof(T) == 2;
     constexpr int VB = AHEAD ? 4 : 1, NB = NC / VB;
     auto in_order = [] {
@@ -177,7 +179,7 @@ __global__ __launch_bounds__(64 * NW, 2 * ST * BN * D * (int)sizeof(T) <= 80 * 1
 #pragma unroll
       for (int i = 0; i < NQ; ++i) {
         if (LEARN && masked) {
-          const uint32_t bits = tree_bits(p, tree_words(p, token[i]), off, t.s.len, low[i], key0) >> (4 * q);
+          const uint32_t bits = tree_bits(p, tree_words(p, token[i]), off, len, low[i], key0) >> (4 * q);
 #pragma unroll
           for (int e = 0; e < 2; ++e)
 #pragma unroll
@@ -285,7 +287,7 @@ __global__ __launch_bounds__(64 * NW, 2 * ST * BN * D * (int)sizeof(T) <= 80 * 1
       }
       if (__builtin_expect(!__syncthreads_or(over || out), 1)) break;
       // (values that are not finite: once more as it was, to the same bits)
-      const bool raise = __syncthreads_or(over) || has_large<D>(vr, j0 * BN, min(j1 * BN, t.s.len));
+      const bool raise = __syncthreads_or(over) || has_large<D>(vr, j0 * BN, min(j1 * BN, len));
 #pragma unroll
       for (int i = 0; i < NQ; ++i) mx[i] = raise ? fmaxf(top[i], mx[i]) : -INFINITY;
     }
@@ -295,8 +297,8 @@ __global__ __launch_bounds__(64 * NW, 2 * ST * BN * D * (int)sizeof(T) <= 80 * 1
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
 #pragma unroll 1
-          for (int key = j0 * BN; key < min(j1 * BN, t.s.len); ++key) {
-            if (!hides(key & ~31) || !(tree_bits(p, tree_words(p, token[i]), off, t.s.len, low[i], key & ~31) >> (key & 31) & 1)) continue;
+          for (int key = j0 * BN; key < min(j1 * BN, len); ++key) {
+            if (!hides(key & ~31) || !(tree_bits(p, tree_words(p, token[i]), off, len, low[i], key & ~31) >> (key & 31) & 1)) continue;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const float y = (float)vr(key)[16 * c + 4 * q + e];
