@@ -12,8 +12,13 @@
 // exchange a head's sums in registers.  The angles and the weights are read once for
 // the heads of a thread.
 // Measured on inputs that no cache holds: queries and keys of 2 x 4096 tokens (168 MB in
-// and out) 42 us, their gradients (252 MB) 58 + 4.5 us; prompts of 16384 tokens stored
-// (227 MB) 49 us, 4.6 TB/s; a token of 64 sequences 4.5 us, launch and chain of loads.
+// and out) 44 us, their gradients (252 MB) 58.5 + 4.5 us; prompts of 9040 tokens stored
+// (227 MB) 50 us, 4.5 TB/s; a token of 64 sequences 4.7 us, launch and chain of loads.
+// Other sizes and alignments take a wave a head, bound by its own chain: 8192 tokens, 32 + 8
+// heads of 80 (105 MB) 191 us, of 128 off 16 bytes (168 MB) 201, their gradients 580 and 674;
+// 2048 tokens, heads of 640 (210 MB) 138 and 705.
+#include <type_traits>
+
 #include "dn_attn.h"
 #include "dn_host.h"
 
@@ -463,10 +468,11 @@ __global__ __launch_bounds__(64) void k_heads_grad_any(const HP p, const GP g) {
     const T* s = (const T*)p.x[side] + b * p.xs[side][0] + l * p.xs[side][1] + h * p.xs[side][2];
     const T* z = (const T*)g.dz[side] + b * g.zs[side][0] + l * g.zs[side][1] + h * g.zs[side][2];
     T* d = (T*)g.dx[side] + row * p.D;
+    const bool wanted = g.dx[side] != nullptr;
     const int64_t pos = p.R ? pos_of(p, b, l) : 0;
     const bool in = pos >= 0 && pos < p.rows;
     float r = 1.f, k = 0.f, xx = 0.f, hx = 0.f, by = 1.f;
-    for (int pass = 0; pass < 2; ++pass) {
+    auto pass = [&](auto sums) {
       for (int i = lane_id(); i < p.D - (p.R >> 1); i += 64) {
         int ca, cb;
         pair_of(i, p.R, p.inter, ca, cb);
@@ -480,30 +486,30 @@ __global__ __launch_bounds__(64) void k_heads_grad_any(const HP p, const GP g) {
           gx = a * c + e * sn;
           gy = e * c - a * sn;
         }
-        if (pass == 0) {
+        if constexpr (decltype(sums)::value) {
           xx += x * x + y * y;
           hx += gx * wx * x + gy * wy * y;
         } else {
-          if (g.dx[side]) d[ca] = (T)(r * (gx * wx - x * k) * by);
+          if (wanted) d[ca] = (T)(r * (gx * wx - x * k) * by);
           part[ca] += gx * x * r;
           if (cb >= 0) {
-            if (g.dx[side]) d[cb] = (T)(r * (gy * wy - y * k) * by);
+            if (wanted) d[cb] = (T)(r * (gy * wy - y * k) * by);
             part[cb] += gy * y * r;
           }
         }
       }
-      if (pass == 0) {
-        const float a = sum_lanes<64>(xx) * over + p.eps * by * by;
-        if (by == 1.f && far_off(a)) {   // once more
-          by = scale_of(a);
-          xx = hx = 0.f;
-          pass = -1;
-          continue;
-        }
-        r = rsqrt32(a);
-        k = sum_lanes<64>(hx) * over * r * r;
-      }
+    };
+    pass(std::true_type{});
+    float a = sum_lanes<64>(xx) * over + p.eps;
+    if (far_off(a)) {   // once more
+      by = scale_of(a);
+      xx = hx = 0.f;
+      pass(std::true_type{});
+      a = sum_lanes<64>(xx) * over + p.eps * by * by;
     }
+    r = rsqrt32(a);
+    k = sum_lanes<64>(hx) * over * r * r;
+    pass(std::false_type{});
   }
 }
 
@@ -557,9 +563,15 @@ constexpr int kMostTokens = 0x7fffffff, kMostBlocks = 0xffffff;   // a launch ha
 
 // Threads of one head each that fill the card a few times over; from there on a thread
 // takes two heads and stores past the caches, and in serving, where no gradient reads
-// them again, loads past them too (16384 tokens of prompts, 227 MB, that no cache holds:
+// them again, loads past them too (9040 tokens of prompts, 227 MB, that no cache holds:
 // 49 us, stores alone past them 51, neither 52; blocks of one chunk of heads for all
-// tokens before the next 56).
+// tokens before the next 56).  us of launches in a loop, one head a thread / two, queries and
+// keys normed and, behind the comma, stored with values: bf16 of 32 + 8 heads of 128, 1024
+// tokens (0.3 M threads of one head) 7.7 / 8.2, 11.0 / 9.6; 4096 25.1 / 29.0, 30.7 / 31.4;
+// 16384 89 / 93, 101 / 110; of 64, 8192 tokens (1.25 M) 29.4 / 27.6, 32.2 / 37.7; 16 + 4 heads
+// of 256, 1024 tokens (0.3 M) 7.7 / 6.7, 11.1 / 9.0; 4096 24.8 / 19.7, 30.8 / 24.5; float32 of
+// 256, 512 tokens (0.3 M) 7.1 / 6.3, 9.5 / 8.3; 2048 22.6 / 18.4, 27.7 / 21.9.  Neither side
+// wins for all heads: at 256 channels two heads would pay from the smallest sizes on.
 constexpr int64_t kManyThreads = 1 << 20;
 
 // the checks that the entries share; NULL if all is well
