@@ -7,11 +7,15 @@
 // of is joined by a second launch.  Only the last keys, the trees' own, are masked.
 //
 // Up to 64 rows it is bound by reading the keys once: 64 x 4 tokens over 4096 (1.08 GB, D =
-// 128) 193 us, 5.6 TB/s, where a copy of 4 GB reaches 4.8.  Trees of up to 64 over up to
-// 16384 (0.58 GB, some of it read for two tiles of 128 rows) 150 + 16 us, of up to 25 over
-// up to 4096 (D = 256, float16, 0.29 GB) 72 + 12.  With more rows the LDS reads bound it, as
-// in the kernel of whole rows: 64 x 64 over 2000 203 us, 680 TFLOP/s.  16 tokens over 1000:
-// 13 + 5 us, the chain of lengths, page table, keys, products and the join.
+// 128) 188 us and 4 for the join, 5.6 TB/s, where a copy of 4 GB reaches 4.8.  Ragged trees
+// of up to 64 nodes, 18 on average, over up to 16384 tokens (0.58 GB, some of it read for two
+// tiles of 128 rows) 153 to 162 + 14 us, of up to 25 over up to 4096 (D = 256, float16, 0.29
+// GB) 73 to 81 + 12.  With more rows the products, the exponentials and the waits between
+// them: 64 x 64 over 2000 204 us, 680 TFLOP/s; 16 x 64 over 16384 369 + 15 us, 716 TFLOP/s,
+// where the matrix units are busy 39 % of the time, vector instructions are issued 49 %, LDS
+// is read 19 % without a conflict, and waves wait 40 % of theirs.  float32 is bound by its
+// matrix instruction, busy 70 % (8 x 16 over 8192, 180 us) to 76 % (8 x 64, 619 us).  16 tokens
+// over 1000: 13 + 4 us, the chain of lengths, page table, keys, products and the join.
 #include <type_traits>
 
 #include "dn_attn_split.h"

@@ -4,8 +4,8 @@
 // Nothing here computes: bound by the launch and a chain of two or three dependent
 // loads (lengths, page table, store) at a token or two per sequence, 2.7 us a launch, by
 // the stores in long queues of prompts: 5.6 million tokens' positions and slots (67 MB)
-// 15.4 us.  Accepted tokens of 64 sequences in 12 layers (13 MB) move in 6.7 us, one
-// user's in 4.9.
+// 15 us.  Accepted tokens of 64 sequences in 12 layers (13 MB) move in 7 us, one
+// user's in 4.7.
 #include <atomic>
 
 #include "dn_common.h"

@@ -563,7 +563,8 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, *, cu_seqlens=Non
     h // (Hq // Hkv).  A query at position p sees positions 0 .. p, or the last
     ``window`` of them.  scale: any finite number, 1 / sqrt(D) unless given.  Sums and
     softmax statistics in float32 (which the sums stay within as long as the largest value
-    times the tokens that a query sees is below 2^120).  A query without a key gets zeros (lse -inf), and
+    times the tokens that a query sees is below 2^120); probabilities of 16-bit types are
+    rounded to the type once before their product with the values.  A query without a key gets zeros (lse -inf), and
     so do tokens in front of cu_seqlens[0] and from cu_seqlens[-1] on (a batch of fixed
     size that is not full); in between cu_seqlens must not fall.  Returns the output in
     q's shape and type, and with ``return_lse`` also the log of the sum of exponentials

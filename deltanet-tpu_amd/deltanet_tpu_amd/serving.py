@@ -285,7 +285,9 @@ def paged_tree_attention(q, k_cache, v_cache, page_table, seq_lens, visible, *, 
     new tokens mean nothing).  window: at least 64 words; the last ``window`` of the
     tokens that a token sees.  A token that sees nothing gets zeros (lse -inf).  Tokens
     that the page table has no place for (seq_lens past it) are seen by none; the others
-    keep their positions.  Returns as ``paged_attention`` does.
+    keep their positions.  As there, bfloat16 and float16 probabilities are rounded to the
+    type once before their product with the values (their sum is not).  Returns as
+    ``paged_attention`` does.
     """
     cs, qs, ct = k_cache.shape, q.shape, k_cache.dtype
     kcs, vcs, qt = k_cache.stride(), v_cache.stride(), q.stride()
