@@ -5,7 +5,7 @@ and the accepted tokens moved to the front.  A step that verifies drafts:
 
     short = paged_reserve(pool, page_table, held, lens, page_size=P)
     positions, slots, visible = paged_slots(page_table, lens, N, page_size=P, cu_seqlens=cu, held=held, parents=parents, nodes=T)
-    # in every layer:
+    # in every softmax-attention layer:
     q = paged_qkv_append(q, k, v, k_cache, v_cache, slots, positions, q_weight=wq, k_weight=wk, table=table)
     out = paged_tree_attention(q, k_cache, v_cache, page_table, lens, visible, cu_seqlens=cu)
     # the drafts that the model agrees with, ``kept``:

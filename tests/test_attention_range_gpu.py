@@ -6,10 +6,11 @@ import math
 import pytest
 import torch
 
-from deltanet_tpu_amd import causal_attention, paged_attention
+from deltanet_tpu_amd import causal_attention, paged_attention, paged_tree_attention
 from tests import attn_ref as A
+from tests import serving_ref as S
 from tests.test_attention_gpu import _rows
-from tests.test_tree_attention_pieces_gpu import _masks, _run, _same
+from tests.test_tree_attention_pieces_gpu import HEADS, _masks, _run, _same
 
 pytestmark = pytest.mark.gpu
 
@@ -63,3 +64,31 @@ def test_trees_over_large_values(dev, dt, D, n):
         q[..., 0] = 1.0
         for B, lens in ((64, [1024]), (41, [length, 777])):
             _run(dev, dt, q, k, v, 64, B, lens, _masks("tree", n), scale=1.0, tag=f"{peak} {last}")
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("D,n", [(64, 8), (64, 64), (128, 16), (128, 32), (256, 16), (256, 64)])
+def test_a_value_that_is_none_leaves_the_other_channels(dev, dt, D, n):
+    """Seen by all, in the middle of long walks: its channel is not finite, the others keep
+    their bits, also where the keys behind it score higher than those in front of it."""
+    B, length, page, G = 41, 1024, 64, 4
+    q, k, v = _rows(8, n, G, D, dt=dt, scale=0.1), _rows(9, length, D, dt=dt), _rows(10, length, D, dt=dt)
+    q[..., 0] = 1.0
+    for odd in (math.nan, math.inf):
+        for last in (0.0, 25.0):
+            k[:, 0] = 0.0
+            k[900:, 0] = last
+            outs = []
+            for x in (0.0, odd):
+                w = v.clone()
+                w[500, 9] = x
+                cache = lambda y: y.view(length // page, page, 1, D).expand(length // page, page, HEADS, D).to(dev)
+                words = S.words([_masks("tree", n)], 1).repeat(B, 1).to(dev)
+                pt = torch.arange(length // page, dtype=torch.int32, device=dev).expand(B, -1)
+                qd = q[None, :, None].expand(B, n, HEADS, G, D).reshape(B, n, HEADS * G, D).to(dev)
+                lens = torch.full((B,), length, dtype=torch.int32, device=dev)
+                outs.append(paged_tree_attention(qd, cache(k), cache(w), pt, lens, words, scale=1.0))
+            base, out = outs
+            assert torch.isfinite(base).all() and not torch.isfinite(out[..., 9]).any()
+            rest = [c for c in range(D) if c != 9]
+            assert torch.equal(out[..., rest], base[..., rest]), (odd, last)
