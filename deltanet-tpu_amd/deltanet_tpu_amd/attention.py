@@ -561,7 +561,7 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, *, cu_seqlens=Non
     sequence, or (B, T, Hq, D); D 64, 128 or 256; the cache's type.  Caches,
     page_table and seq_lens as in ``paged_kv_append``; query head h reads key head
     h // (Hq // Hkv).  A query at position p sees positions 0 .. p, or the last
-    ``window`` of them.  scale: any finite number, 1 / sqrt(D) unless given.  Sums and
+    ``window`` of them; a length past the page table counts as the table's end.  scale: any finite number, 1 / sqrt(D) unless given.  Sums and
     softmax statistics in float32 (which the sums stay within as long as the largest value
     times the tokens that a query sees is below 2^120); probabilities of 16-bit types are
     rounded to the type once before their product with the values.  A query without a key gets zeros (lse -inf), and

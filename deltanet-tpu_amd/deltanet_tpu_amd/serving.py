@@ -15,7 +15,8 @@ and the accepted tokens moved to the front.  A step that verifies drafts:
 Nothing here reads a device tensor on the host; all of it can be captured in a graph.  A
 step goes on where the pool runs short: with ``held``, tokens behind the pages that their
 sequence has get no slot, are not stored and not kept, whatever ``kept`` says, and what
-attention returns for them means nothing; the others' results are right.  (Behind them
+attention returns for them means nothing; the others' results are right (for chains by
+``paged_attention`` only as long as no length passes the page table).  (Behind them
 the page table holds numbers of pages that may be another sequence's by now: leave
 ``held`` out only where no sequence is ever short.)
 """
